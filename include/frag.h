@@ -473,6 +473,62 @@ FRAG_API int frag_rope(const frag_rope_tensor* tensors, int num_tensors, int64_t
               int64_t freqs_stride, int64_t freqs_rows, float theta, int layout,
               int inverse, frag_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * Rotary positions with the caller's frequencies, on the first `rot` of the D
+ * elements of each head (the others pass through), forward and gradient.
+ *   angle_j = 2 pi * turns[j] * pos,  j < rot/2
+ *   (a, b) -> factor * (a cos - b sin, b cos + a sin), rounded once to bf16
+ * turns: HOST array of rot/2 doubles (read during the call): a plan's
+ *   frequencies in turns per position, however they were scaled for a longer
+ *   context; p * turns[j] is reduced to a fraction of a turn in 64 bits.
+ * backward != 0 applies the transpose (sin negated, the same factor).
+ * tensors: bf16 in and out only (in_dtype, out_dtype 0).  out may be x itself
+ *   with the same strides; other overlap is not allowed.  rot even, <= 512.
+ * Layouts and positions as in frag_rope.  No counterpart in the reference,
+ * whose RoPE rotates whole heads by a caller's table.
+ * ------------------------------------------------------------------------- */
+FRAG_API int frag_rope_scaled(const frag_rope_tensor* tensors, int num_tensors, int64_t B, int64_t S,
+                     int64_t D, int64_t rot, const void* pos, int pos_dtype,
+                     int64_t pos_stride_b, int64_t pos_stride_s, const double* turns,
+                     float factor, int layout, int backward, frag_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * (Residual add +) RMSNorm forward with its output in 8 bits and scales.
+ *   h     = bf16(res + x), or x when res is NULL
+ *   rstd  = 1 / sqrt(mean_n(h^2) + eps)
+ *   y     = h * rstd * w                      (fp32, not rounded)
+ *   scale = max|y| / fmax over a row (group 0) or over each `group` of its
+ *           values (32, 64 or 128; the last group of a row may be cut); 1
+ *           where all are zero, at least 2^-126; with scale_e8m0 the power of
+ *           two at or above that, stored as its biased exponent byte
+ *   q     = fp8(y / scale), round to nearest even; fmax 448 (E4M3), 57344 (E5M2)
+ * A row that holds inf or NaN gives NaN there and a scale of inf or NaN.
+ * x, res: bf16 [M, N] with row strides in elements; q: [M, N] bytes; scale:
+ * fp32 or bytes [M, ceil(N / group)] ([M] for group 0); h: bf16 [M, N] or NULL
+ * (only with res); rstd: fp32 [M] or NULL.  No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+enum frag_fp8_format { FRAG_FP8_E4M3 = 0, FRAG_FP8_E5M2 = 1 };
+
+FRAG_API int frag_rmsnorm_quant_fwd(const void* x, int64_t x_stride, const void* res, int64_t res_stride,
+                     const void* w, void* q, void* scale, void* h, float* rstd, int64_t M, int64_t N,
+                     float eps, int format, int64_t group, int scale_e8m0, frag_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * The gradient of (residual add +) RMSNorm, also in 8 bits and scales: what
+ * the projection below the residual reads.  xhat = x * rstd, g = dy * w:
+ *   dx = dres + (g - xhat * mean(xhat * g)) * rstd   (fp32; dres optional)
+ *   dx_out = bf16(dx) or NULL; q, scale of dx as in frag_rmsnorm_quant_fwd
+ *   dw[n]  = sum_m dy * xhat (fp32, fixed order), or NULL
+ * x: the normalised input (h of the forward), rstd: the saved fp32 [M].
+ * Unlike frag_rmsnorm_bwd nothing is rounded before dres is added.  Workspace:
+ * frag_rmsnorm_quant_bwd_workspace_bytes(M, N), 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+FRAG_API size_t frag_rmsnorm_quant_bwd_workspace_bytes(int64_t M, int64_t N);
+FRAG_API int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                     const float* rstd, const void* w, const void* dres, int64_t dres_stride, void* dx,
+                     void* q, void* scale, float* dw, int64_t M, int64_t N, int format, int64_t group,
+                     int scale_e8m0, void* workspace, size_t workspace_bytes, frag_stream_t stream);
+
 /* Self-test of the bounded waits: one thread waits limit_cycles
  * (0 < limit_cycles <= 4e9) on an mbarrier that nothing arrives on, with the
  * same wait every TMA kernel here uses.  The wait gives up and sets

@@ -33,6 +33,8 @@ FRAG_ROPE_IN_BF16 = 0
 FRAG_ROPE_IN_F32 = 1
 FRAG_ROPE_NEOX = 0
 FRAG_ROPE_INTERLEAVED = 1
+FRAG_FP8_E4M3 = 0
+FRAG_FP8_E5M2 = 1
 FRAG_POS_NONE = 0
 FRAG_POS_I32 = 1
 FRAG_POS_I64 = 2
@@ -141,6 +143,17 @@ SIGNATURES: dict[str, tuple] = {
         [C.POINTER(RopeTensor), _int, _i64, _i64, _i64, _vp, _int, _i64, _i64, _vp, _i64, _i64,
          _f32, _int, _int, _vp],
     ),
+    "frag_rope_scaled": (
+        _int,
+        [C.POINTER(RopeTensor), _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, C.POINTER(C.c_double),
+         _f32, _int, _int, _vp],
+    ),
+    "frag_rmsnorm_quant_fwd": (
+        _int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _int, _i64, _int, _vp]),
+    "frag_rmsnorm_quant_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "frag_rmsnorm_quant_bwd": (
+        _int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _int, _i64, _int,
+               _vp, _sz, _vp]),
 }
 
 _lock = threading.Lock()

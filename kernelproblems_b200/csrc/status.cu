@@ -59,13 +59,13 @@ int* device_error_word() {
 bool allow_dynamic_smem(const void* kernel, int bytes) {
   // Largest dynamic shared memory size set so far, per device and kernel.
   static std::mutex mu;
-  static const void* kern[64][32] = {};
-  static int set_bytes[64][32] = {};
+  static const void* kern[64][128] = {};
+  static int set_bytes[64][128] = {};
   const int d = current_device();
   if (d < 0 || d >= 64) return false;
   std::lock_guard<std::mutex> lk(mu);
   int slot = -1;
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < 128; ++i) {
     if (kern[d][i] == kernel) {
       if (set_bytes[d][i] >= bytes) return true;
       slot = i;

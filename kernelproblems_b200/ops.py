@@ -13,6 +13,7 @@ after every embedding call (what torch's device-side assert would catch).
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from contextlib import contextmanager
 
@@ -39,6 +40,10 @@ __all__ = [
     "convert",
     "rope",
     "rope_complex",
+    "RopeFrequencies",
+    "rope_scaled",
+    "rmsnorm_quant_fwd",
+    "rmsnorm_quant_bwd",
     "check_status",
     "reset_status",
 ]
@@ -744,3 +749,289 @@ def rope(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor
         _lib.call("frag_rope", arr, len(descs), B, S, D, pos_ptr, pos_dtype, psb, pss, fptr,
                   fstride, frows, theta_v, _LAYOUTS[layout], int(bool(inverse)), _stream(dev))
     return oq, ok
+
+
+class RopeFrequencies:
+    """The frequencies of a rotary embedding, computed once in 64 bits and kept
+    on the host: pass it to rope_scaled.
+
+    head_dim       elements of a head; rotary_dim (default all) of them, the
+                   first, are rotated, the others pass through
+    theta          base: pair j turns by theta^(-2j / rotary_dim) a position
+    scaling        how the frequencies f are slowed for contexts `factor` times
+                   original_context long:
+      "none"       not at all
+      "linear"     f / factor (positions are interpolated)
+      "base"       theta * factor^(rotary_dim / (rotary_dim - 2)): the last
+                   pair is slowed by the factor, the first not at all
+      "smooth"     by the turns a pair makes in original_context: fewer than
+                   low_turns f / factor, more than high_turns f, between them
+                   a linear blend
+      "parts"      a blend linear in the pair's index, f up to the pair that
+                   makes fast_turns in original_context, f / factor from the
+                   one that makes slow_turns; rotated values are multiplied by
+                   0.1 ln(factor) + 1
+    attention_factor  replaces that multiplier (1 for the other scalings)
+
+    `turns` (float64 tensor [rotary_dim / 2]) holds f / (2 pi)."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, theta: float = 500000.0,
+                 scaling: str = "none", factor: float = 1.0, original_context: int = 8192,
+                 low_turns: float = 1.0, high_turns: float = 4.0, fast_turns: float = 32.0,
+                 slow_turns: float = 1.0, attention_factor: float | None = None):
+        rot = head_dim if rotary_dim is None else rotary_dim
+        if rot <= 0 or rot % 2 or rot > head_dim:
+            raise ValueError(f"rotary_dim must be even and in (0, {head_dim}], got {rot}")
+        if rot > 512:
+            raise ValueError(f"rotary_dim must be at most 512, got {rot}")
+        if not theta > 1 or not math.isfinite(theta):
+            raise ValueError("theta must be finite and above 1")
+        if scaling not in ("none", "linear", "base", "smooth", "parts"):
+            raise ValueError(f"unknown scaling {scaling!r}")
+        if not factor >= 1 or not math.isfinite(factor):
+            raise ValueError("factor must be finite and at least 1")
+        if original_context <= 0:
+            raise ValueError("original_context must be positive")
+        if not high_turns > low_turns > 0 or not fast_turns > slow_turns > 0:
+            raise ValueError("high_turns must be above low_turns, and fast_turns above slow_turns, all positive")
+        self.head_dim, self.rotary_dim = head_dim, rot
+        if scaling == "base":
+            if rot < 4:
+                raise ValueError("scaling 'base' needs a rotary_dim of at least 4")
+            theta = theta * factor ** (rot / (rot - 2))
+        j = torch.arange(rot // 2, dtype=torch.float64)
+        turns = theta ** (-2.0 * j / rot) / (2 * math.pi)
+        self.attention_factor = 1.0
+        if scaling == "linear":
+            turns = turns / factor
+        elif scaling == "smooth":
+            keep = ((turns * original_context - low_turns) / (high_turns - low_turns)).clamp(0, 1)
+            turns = turns * (keep + (1 - keep) / factor)
+        elif scaling == "parts":
+            def pair(n):  # the (fractional) pair that makes n turns in the original context
+                return rot * math.log(original_context / (2 * math.pi * n)) / (2 * math.log(theta))
+            first, last = max(math.floor(pair(fast_turns)), 0), min(math.ceil(pair(slow_turns)), rot - 1)
+            slowed = ((j - first) / max(last - first, 1e-3)).clamp(0, 1)
+            turns = turns * (1 - slowed + slowed / factor)
+            self.attention_factor = 0.1 * math.log(factor) + 1.0
+        if attention_factor is not None:
+            self.attention_factor = float(attention_factor)
+        self.turns = turns
+        self._turns = (C.c_double * (rot // 2))(*turns.tolist())
+
+
+def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    end = lambda t: t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def _check_rope_out(x: torch.Tensor, out: torch.Tensor, name: str) -> None:
+    if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.device != x.device:
+        raise TypeError(f"{name}: the output must be a bfloat16 tensor on {x.device}")
+    if out.shape != x.shape:
+        raise ValueError(f"{name}: output shape {tuple(out.shape)} != {tuple(x.shape)}")
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{name}: the output must not repeat elements (an expanded view)")
+    same = out.data_ptr() == x.data_ptr() and all(
+        n <= 1 or a == b for n, a, b in zip(x.shape, x.stride(), out.stride()))
+    if not same and _overlaps(x, out):
+        raise ValueError(f"{name}: the output overlaps the input without being the same view")
+
+
+def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None, *,
+                freqs: RopeFrequencies, layout: str = "neox", backward: bool = False,
+                out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None,
+                out_layout: str = "bshd"):
+    """Rotary embedding of bf16 q (and k), [B, S, H, D] views of any strides
+    with a contiguous head dimension, by a RopeFrequencies plan: the first
+    freqs.rotary_dim elements of every head are rotated (pairs (j, j +
+    rotary_dim/2) for layout "neox", (2j, 2j+1) for "interleaved"), the others
+    pass through.  Returns (out_q, out_k), new contiguous tensors or the given
+    out_q / out_k, which may be q and k themselves (in place).
+
+    positions: int32/int64 [B, S] or [S], or None for position = s.  A product
+    of position and frequency is taken in 64 bits, so a long context's last
+    token is as exact as its first; rotated values are rounded once.
+    backward=True gives the gradient: the transposed rotation, with the same
+    attention factor.  out_layout as in rope."""
+    _need(q, "q", torch.bfloat16)
+    dev = q.device
+    if not isinstance(freqs, RopeFrequencies):
+        raise TypeError("freqs must be a RopeFrequencies")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
+    if q.dim() != 4:
+        raise ValueError("q must be [B, S, H, D] (any strides, last dim contiguous)")
+    B, S, _, D = q.shape
+    if D != freqs.head_dim:
+        raise ValueError(f"q has heads of {D} elements, the plan is for {freqs.head_dim}")
+    oq = _new_out(q, out_layout) if out_q is None else out_q
+    _check_rope_out(q, oq, "q")
+    descs = [_rope_desc(q, oq, "q")]
+    ok = None
+    if k is not None:
+        _need(k, "k", torch.bfloat16, dev)
+        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
+            raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+        ok = _new_out(k, out_layout) if out_k is None else out_k
+        _check_rope_out(k, ok, "k")
+        if _overlaps(oq, ok) and (out_q is not None or out_k is not None) and not _interleaved(oq, ok):
+            raise ValueError("out_q and out_k overlap")
+        descs.append(_rope_desc(k, ok, "k"))
+    pos_ptr, pos_dtype, psb, pss = _rope_positions(positions, B, S, dev)
+    arr = (_lib.RopeTensor * len(descs))(*descs)
+    with _on_device(dev):
+        _lib.call("frag_rope_scaled", arr, len(descs), B, S, D, freqs.rotary_dim, pos_ptr, pos_dtype, psb, pss,
+                  freqs._turns, freqs.attention_factor, _LAYOUTS[layout], int(bool(backward)), _stream(dev))
+    return oq, ok
+
+
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two overlapping ranges are disjoint head slices of one packed
+    tensor: the same batch and sequence strides, heads that do not meet."""
+    if a.stride()[:2] != b.stride()[:2] or min(a.stride(1), b.stride(1)) <= 0:
+        return False
+    lo, hi = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
+    gap = (hi.data_ptr() - lo.data_ptr()) // lo.element_size()
+    span = lambda t: (t.shape[2] - 1) * t.stride(2) + t.shape[3]
+    return gap >= span(lo) and gap + span(hi) <= lo.stride(1)
+
+
+def _rope_positions(positions, B: int, S: int, dev: torch.device):
+    """(pointer, dtype code, batch stride, sequence stride) of a position tensor."""
+    if positions is None:
+        return None, _lib.FRAG_POS_NONE, 0, 0
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 tensor")
+    if positions.device != dev:
+        raise ValueError("positions must be on the same device as q")
+    code = _lib.FRAG_POS_I64 if positions.dtype == torch.int64 else _lib.FRAG_POS_I32
+    if positions.dim() == 1 and positions.shape[0] == S:
+        return C.c_void_p(positions.data_ptr()), code, 0, positions.stride(0)
+    if positions.dim() == 2 and tuple(positions.shape) == (B, S):
+        return C.c_void_p(positions.data_ptr()), code, positions.stride(0), positions.stride(1)
+    raise ValueError(f"positions must be [B, S] or [S], got {tuple(positions.shape)}")
+
+
+# ------------------------------------------------- RMSNorm in 8 bits and scales
+
+_FP8 = {torch.float8_e4m3fn: _lib.FRAG_FP8_E4M3, torch.float8_e5m2: _lib.FRAG_FP8_E5M2}
+_GROUPS = (0, 32, 64, 128)
+
+
+def _strided_rows(t: torch.Tensor, name: str, N: int, dev: torch.device, shape=None):
+    """(the tensor, row stride) of a bf16 tensor whose rows of N are
+    contiguous and whose leading dimensions collapse into one row stride."""
+    _need(t, name, torch.bfloat16, dev)
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} {tuple(t.shape)} and x {tuple(shape)} differ")
+    if t.dim() < 1 or t.shape[-1] != N:
+        raise ValueError(f"{name}: last dim of {tuple(t.shape)} != normalized size {N}")
+    if t.is_contiguous():
+        return t, N
+    try:
+        rows = t.view(-1, N) if t.numel() else t
+    except RuntimeError:
+        raise ValueError(f"{name}'s leading dimensions must collapse into one row stride") from None
+    if N > 1 and rows.stride(-1) != 1:
+        raise ValueError(f"{name}'s rows must be contiguous")
+    return rows, rows.stride(0) if rows.dim() == 2 else N
+
+
+def _quant_out(x: torch.Tensor, N: int, dtype, group: int, scale_dtype, dev):
+    if dtype not in _FP8:
+        raise TypeError("dtype must be float8_e4m3fn or float8_e5m2")
+    if group not in _GROUPS:
+        raise ValueError(f"group must be one of {_GROUPS} (0: one scale for a row)")
+    if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
+        raise TypeError("scale_dtype must be float32 or float8_e8m0fnu")
+    q = torch.empty(x.shape, dtype=dtype, device=dev)
+    shape = x.shape[:-1] + (-(-N // group),) if group else x.shape[:-1]
+    return q, torch.empty(shape, dtype=scale_dtype, device=dev)
+
+
+def _workspace(given: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor:
+    """The caller's workspace where it is large enough, or a new one."""
+    if given is not None:
+        if not isinstance(given, torch.Tensor) or given.device != dev or not given.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        if given.numel() * given.element_size() >= need and given.data_ptr() % 256 == 0:
+            return given
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+
+
+def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
+                      residual: torch.Tensor | None = None, dtype: torch.dtype = torch.float8_e4m3fn,
+                      group: int = 0, scale_dtype: torch.dtype = torch.float32, write_h: bool = True,
+                      save_rstd: bool = True):
+    """(Residual add +) RMSNorm with its output in 8 bits and scales, in one
+    pass.  Returns (q, scale, h, rstd): y = rmsnorm(h) * w is q * scale.
+
+    h      bf16(residual + x): the new residual stream, which the backward
+           (rmsnorm_quant_bwd, rmsnorm_bwd) takes as its x; None without a
+           residual or with write_h=False
+    q      float8_e4m3fn or float8_e5m2, shaped like x, rounded from 32 bits
+    scale  max |y| / the format's largest value, for each row (group=0, shaped
+           x.shape[:-1]) or each `group` of its values (x.shape[:-1] +
+           [ceil(N / group)], the last one of a row may be cut); 1 where all
+           are zero.  scale_dtype=float8_e8m0fnu rounds it up to a power of two
+    rstd   fp32 x.shape[:-1], or None
+
+    x and residual: rows of weight.numel() contiguous values, any row stride."""
+    _need(x, "x", torch.bfloat16)
+    dev = x.device
+    _need(weight, "weight", torch.bfloat16, dev)
+    N = weight.numel()
+    x2, xs = _strided_rows(x, "x", N, dev)
+    r2, rs = (None, 0) if residual is None else _strided_rows(residual, "residual", N, dev, x.shape)
+    q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
+    h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if residual is not None and write_h else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if save_rstd else None
+    wc = weight.contiguous()
+    with _on_device(dev):
+        _lib.call("frag_rmsnorm_quant_fwd", _ptr(x2), xs, _ptr(r2), rs, _ptr(wc), _ptr(q), _ptr(scale), _ptr(h),
+                  _ptr(rstd), x.numel() // N if N else 0, N, float(eps), _FP8[dtype], group,
+                  int(scale_dtype != torch.float32), _stream(dev))
+    return q, scale, h, rstd
+
+
+def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, *,
+                      dres: torch.Tensor | None = None, dtype: torch.dtype = torch.float8_e5m2, group: int = 0,
+                      scale_dtype: torch.dtype = torch.float32, write_dx: bool = True, compute_dw: bool = True,
+                      workspace: torch.Tensor | None = None):
+    """The gradient of (residual add +) RMSNorm in bf16 and, for the
+    projection below the residual, in 8 bits and scales, in one pass.
+    Returns (dx, q, scale, dw).
+
+    dy     gradient of the norm's output (the 8-bit rounding passes it through)
+    x      the normalised input (h of rmsnorm_quant_fwd), rstd its saved fp32
+    dres   the residual stream's own gradient, added to dx
+    dx     bf16(dres + RMSNorm backward), rounded once, or None; q and scale
+           are of the same 32-bit values, as in rmsnorm_quant_fwd
+    dw     fp32 [N] summed in a fixed order, or None"""
+    _need(x, "x", torch.bfloat16)
+    dev = x.device
+    _need(weight, "weight", torch.bfloat16, dev)
+    N = weight.numel()
+    x2, xs = _strided_rows(x, "x", N, dev)
+    y2, ys = _strided_rows(dy, "dy", N, dev, x.shape)
+    r2, rs = (None, 0) if dres is None else _strided_rows(dres, "dres", N, dev, x.shape)
+    M = x.numel() // N if N else 0
+    _need(rstd, "rstd", torch.float32, dev)
+    if rstd.numel() != M or not rstd.is_contiguous():
+        raise ValueError(f"rstd must be contiguous with {M} elements")
+    q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
+    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if write_dx else None
+    dw = torch.empty(N, dtype=torch.float32, device=dev) if compute_dw else None
+    wc = weight.contiguous()
+    with _on_device(dev):
+        need = int(_lib.load().frag_rmsnorm_quant_bwd_workspace_bytes(M, N))
+        workspace = _workspace(workspace, need, dev)
+        _lib.call("frag_rmsnorm_quant_bwd", _ptr(y2), ys, _ptr(x2), xs, _ptr(rstd), _ptr(wc), _ptr(r2), rs,
+                  _ptr(dx), _ptr(q), _ptr(scale), _ptr(dw), M, N, _FP8[dtype], group,
+                  int(scale_dtype != torch.float32), _ptr(workspace),
+                  workspace.numel() * workspace.element_size(), _stream(dev))
+    return dx, q, scale, dw

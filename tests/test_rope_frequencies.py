@@ -1,0 +1,89 @@
+"""RopeFrequencies on the CPU: the scaling rules at their ends, and refusals."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from kernelproblems_b200 import _lib, ops
+
+
+def freq(plan):
+    return plan.turns * 2 * math.pi
+
+
+def plain(rot, theta=500000.0):
+    return theta ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+
+
+def test_unscaled_and_linear():
+    assert torch.allclose(freq(ops.RopeFrequencies(128)), plain(128), rtol=1e-14)
+    p = ops.RopeFrequencies(128, rotary_dim=64, scaling="linear", factor=4.0)
+    assert p.rotary_dim == 64 and torch.allclose(freq(p), plain(64) / 4, rtol=1e-14)
+    assert p.attention_factor == 1.0
+
+
+def test_base_slows_the_last_pair_by_the_factor():
+    f, g = plain(128), freq(ops.RopeFrequencies(128, scaling="base", factor=8.0))
+    assert g[0] == pytest.approx(1.0) and (f[-1] / g[-1]).item() == pytest.approx(8.0, rel=1e-12)
+
+
+def test_smooth_keeps_short_waves_and_slows_long_ones():
+    f = plain(128)
+    g = freq(ops.RopeFrequencies(128, scaling="smooth", factor=8.0, original_context=8192))
+    turns = 8192 * f / (2 * math.pi)
+    assert torch.allclose(g[turns >= 4], f[turns >= 4], rtol=1e-14)
+    assert torch.allclose(g[turns <= 1], f[turns <= 1] / 8, rtol=1e-14)
+    mid = (turns > 1) & (turns < 4)
+    assert mid.any() and bool(((g < f) & (g > f / 8))[mid].all())
+
+
+def test_parts_keeps_the_first_pairs_and_slows_the_last():
+    f, p = plain(128), ops.RopeFrequencies(128, scaling="parts", factor=4.0, original_context=4096)
+    g = freq(p)
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.allclose(g[turns > 34], f[turns > 34], rtol=1e-14)
+    assert torch.allclose(g[turns < 0.7], f[turns < 0.7] / 4, rtol=1e-14)
+    assert p.attention_factor == pytest.approx(0.1 * math.log(4) + 1)
+    assert ops.RopeFrequencies(128, scaling="parts", factor=4.0, attention_factor=0.5).attention_factor == 0.5
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=130), dict(rotary_dim=63), dict(rotary_dim=0), dict(theta=0.0),
+                                dict(theta=float("nan")), dict(scaling="other"), dict(factor=0.5),
+                                dict(factor=float("inf")), dict(original_context=0), dict(high_turns=1.0),
+                                dict(slow_turns=40.0), dict(low_turns=-1.0),
+                                dict(scaling="base", rotary_dim=2)])
+def test_plan_refusals(kw):
+    with pytest.raises(ValueError):
+        ops.RopeFrequencies(128, **kw)
+
+
+def test_rot_limit():
+    with pytest.raises(ValueError):
+        ops.RopeFrequencies(1024)
+    assert ops.RopeFrequencies(1024, rotary_dim=512).turns.numel() == 256
+
+
+def test_entry_points_reject_bad_arguments_on_the_host():
+    lib = _lib.load()
+    turns = (C.c_double * 64)()
+    t = (_lib.RopeTensor * 1)(_lib.RopeTensor(None, None, 2, 0, 0, 0, 0, 0, 0, 0, 0))
+    rope = lambda t, n, B, S, D, rot, lay=0, tu=turns: lib.frag_rope_scaled(  # noqa: E731
+        t, n, B, S, D, rot, None, 0, 0, 0, tu, 1.0, lay, 0, None)
+    assert rope(None, 1, 1, 1, 128, 128) == 1
+    assert rope(t, 3, 1, 1, 128, 128) == 1
+    assert rope(t, 1, -1, 1, 128, 128) == 1
+    assert rope(t, 1, 1, 1, 128, 128, lay=2) == 1
+    assert rope(t, 1, 1, 1, 128, 128, tu=None) == 1
+    assert rope(t, 1, 1, 1, 128, 130) == 2
+    assert rope(t, 1, 1, 1, 128, 127) == 2
+    assert rope(t, 1, 1, 1, 128, 128) == 1   # null tensors
+    assert rope(t, 1, 0, 1, 128, 128) == 0   # nothing to do
+    fwd = lambda M, N, fmt=0, group=0: lib.frag_rmsnorm_quant_fwd(  # noqa: E731
+        None, N, None, 0, None, None, None, None, None, M, N, 1e-5, fmt, group, 0, None)
+    assert fwd(4, 64) == 1 and fwd(-1, 64) == 1 and fwd(4, 64, fmt=2) == 1
+    assert fwd(4, 64, group=48) == 2 and fwd(4, 0) == 2 and fwd(0, 64) == 0
+    bwd = lambda M, N, fmt=1, group=0: lib.frag_rmsnorm_quant_bwd(  # noqa: E731
+        None, N, None, N, None, None, None, 0, None, None, None, None, M, N, fmt, group, 0, None, 0, None)
+    assert bwd(4, 64) == 1 and bwd(-1, 64) == 1 and bwd(4, 64, fmt=7) == 1
+    assert bwd(4, 64, group=1) == 2 and bwd(0, 64) == 0
