@@ -529,6 +529,37 @@ FRAG_API int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const voi
                      void* q, void* scale, float* dw, int64_t M, int64_t N, int format, int64_t group,
                      int scale_e8m0, void* workspace, size_t workspace_bytes, frag_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * Newton-Schulz orthogonalisation of E matrices [m, n], and the weight update
+ * made of it.  With s = min(m, n) and X = G / (|G|_F + eps), `steps` times:
+ *   A = X X' (s x s; X'X for m > n),  B = b A + c A A,  X <- a X + B X (X B)
+ * coefficients: HOST array of `steps` triples (a, b, c).
+ * frag_orthogonalize: out[e] = bf16(X), contiguous [E, m, n].
+ * frag_muon_update:
+ *   m' = mu m + (1 - mu) g;  u = nesterov ? mu m' + (1 - mu) g : m'
+ *   p' = (1 - lr weight_decay) p - lr scale O(u)
+ *   param_out, momentum_out: contiguous [E, m, n] of param's and momentum's
+ *   types; they may be param and momentum themselves when those are contiguous.
+ * Matrices are bf16 or fp32 with any strides (in elements).  Products have
+ * fp16 operands and fp32 accumulators; X is held in 22 bits.  Workspace:
+ * frag_orthogonalize_workspace_bytes(E, m, n), 16-byte aligned.  No
+ * counterpart in the reference, whose graphs end at the weights' gradients.
+ * ------------------------------------------------------------------------- */
+typedef struct frag_matrix {
+  void* data;
+  int64_t stride_batch, stride_row, stride_col;
+  int32_t dtype; /* FRAG_DT_BF16 or FRAG_DT_F32 */
+} frag_matrix;
+
+FRAG_API size_t frag_orthogonalize_workspace_bytes(int64_t E, int64_t m, int64_t n);
+FRAG_API int frag_orthogonalize(const frag_matrix* g, void* out, int64_t E, int64_t m, int64_t n, int steps,
+                     const float* coefficients, float eps, void* workspace, size_t workspace_bytes,
+                     frag_stream_t stream);
+FRAG_API int frag_muon_update(const frag_matrix* param, const frag_matrix* grad, const frag_matrix* momentum,
+                     void* param_out, void* momentum_out, int64_t E, int64_t m, int64_t n, float lr, float mu,
+                     int nesterov, float weight_decay, float scale, int steps, const float* coefficients, float eps,
+                     void* workspace, size_t workspace_bytes, frag_stream_t stream);
+
 /* Self-test of the bounded waits: one thread waits limit_cycles
  * (0 < limit_cycles <= 4e9) on an mbarrier that nothing arrives on, with the
  * same wait every TMA kernel here uses.  The wait gives up and sets

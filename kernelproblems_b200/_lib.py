@@ -71,6 +71,16 @@ class RopeTensor(C.Structure):
     ]
 
 
+class Matrix(C.Structure):
+    _fields_ = [
+        ("data", _vp),
+        ("stride_batch", _i64),
+        ("stride_row", _i64),
+        ("stride_col", _i64),
+        ("dtype", C.c_int32),  # FRAG_DT_BF16 / FRAG_DT_F32
+    ]
+
+
 FRAG_COPY_MAX_SEGMENTS = 16
 FRAG_PEER_MAX_RANKS = 8
 FRAG_IPC_HANDLE_BYTES = 64
@@ -154,6 +164,12 @@ SIGNATURES: dict[str, tuple] = {
     "frag_rmsnorm_quant_bwd": (
         _int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _int, _i64, _int,
                _vp, _sz, _vp]),
+    "frag_orthogonalize_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "frag_orthogonalize": (
+        _int, [C.POINTER(Matrix), _vp, _i64, _i64, _i64, _int, C.POINTER(_f32), _f32, _vp, _sz, _vp]),
+    "frag_muon_update": (
+        _int, [C.POINTER(Matrix), C.POINTER(Matrix), C.POINTER(Matrix), _vp, _vp, _i64, _i64, _i64, _f32, _f32,
+               _int, _f32, _f32, _int, C.POINTER(_f32), _f32, _vp, _sz, _vp]),
 }
 
 _lock = threading.Lock()

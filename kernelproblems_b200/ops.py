@@ -44,6 +44,9 @@ __all__ = [
     "rope_scaled",
     "rmsnorm_quant_fwd",
     "rmsnorm_quant_bwd",
+    "orthogonalize",
+    "muon_update",
+    "orthogonalize_workspace_bytes",
     "check_status",
     "reset_status",
 ]
@@ -1035,3 +1038,134 @@ def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
                   int(scale_dtype != torch.float32), _ptr(workspace),
                   workspace.numel() * workspace.element_size(), _stream(dev))
     return dx, q, scale, dw
+
+
+# --------------------------------------------- orthogonalised weight updates
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def _matrices(t: torch.Tensor, name: str, dev: torch.device | None = None, shape=None):
+    """(E, m, n, descriptor) of a bf16 or fp32 [..., m, n] tensor whose
+    leading dimensions collapse into one stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in _DT:
+        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} {tuple(t.shape)} != {tuple(shape)}")
+    if t.dim() < 2:
+        raise ValueError(f"{name} must be [..., m, n], got {tuple(t.shape)}")
+    m, n = t.shape[-2:]
+    E = 1
+    for d in t.shape[:-2]:
+        E *= d
+    sb = 0
+    if t.dim() > 2 and E > 0:
+        # a stride for the leading dimensions together
+        for size, stride in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+            if size == 1:
+                continue
+            if sb == 0:
+                sb, span = stride, size * stride
+            elif stride != span:
+                raise ValueError(f"{name}'s leading dimensions must collapse into one stride")
+            else:
+                span *= size
+    return E, m, n, _lib.Matrix(t.data_ptr(), sb, t.stride(-2), t.stride(-1), _DT[t.dtype])
+
+
+def _schedule(steps: int, coefficients):
+    """The C array of `steps` triples: one triple for all, or one for each."""
+    if not isinstance(steps, int) or steps < 1:
+        raise ValueError("steps must be a positive integer")
+    rows = list(coefficients)
+    if len(rows) == 3 and all(isinstance(c, (int, float)) for c in rows):
+        rows = [rows] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("coefficients must be a triple (a, b, c) or one for each step")
+    flat = [float(c) for r in rows for c in r]
+    if not all(math.isfinite(c) for c in flat):
+        raise ValueError("coefficients must be finite")
+    return (C.c_float * len(flat))(*flat)
+
+
+def orthogonalize_workspace_bytes(E: int, m: int, n: int) -> int:
+    return int(_lib.load().frag_orthogonalize_workspace_bytes(E, m, n))
+
+
+def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7,
+                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of each matrix of g [..., m, n] (bf16 or
+    fp32, any strides): X = g / (|g|_F + eps), then `steps` times
+    X <- a X + (b A + c A A) X with A = X X' (on the smaller side).  Returns
+    bf16 X, contiguous, shaped like g (or `out`).
+
+    coefficients: a triple (a, b, c) for all steps, or one for each.  They have
+    to keep |X| within a few units (as the default and all schedules that
+    converge do): X is held in 22 bits around 1, and its products have fp16
+    operands and fp32 accumulators."""
+    E, m, n, desc = _matrices(g, "g")
+    dev = g.device
+    if out is None:
+        out = torch.empty(g.shape, dtype=torch.bfloat16, device=dev)
+    else:
+        _check_out(out, "out", torch.bfloat16, dev, shape=g.shape)
+    co = _schedule(steps, coefficients)
+    with _on_device(dev):
+        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), dev)
+        _lib.call("frag_orthogonalize", C.byref(desc), _ptr(out), E, m, n, steps, co, float(eps), _ptr(workspace),
+                  workspace.numel() * workspace.element_size(), _stream(dev))
+    return out
+
+
+def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.Tensor, *, lr: float,
+                momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, scale: float = 1.0,
+                steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7,
+                param_out: torch.Tensor | None = None, momentum_out: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None):
+    """One weight update along the orthogonalised momentum of [..., m, n]
+    matrices.  Returns (param', momentum'):
+
+    momentum'  momentum * momentum_buffer + (1 - momentum) * grad
+    u          momentum * momentum' + (1 - momentum) * grad (nesterov), or momentum'
+    param'     (1 - lr * weight_decay) * param - lr * scale * orthogonalize(u)
+
+    param, grad and momentum_buffer are bf16 or fp32, each its own; outputs are
+    new contiguous tensors of param's and momentum_buffer's types, or the given
+    param_out / momentum_out, which may be param and momentum_buffer themselves
+    (an update in place).  steps, coefficients, eps as in orthogonalize."""
+    E, m, n, dp = _matrices(param, "param")
+    dev = param.device
+    dg = _matrices(grad, "grad", dev, param.shape)[3]
+    dm = _matrices(momentum_buffer, "momentum_buffer", dev, param.shape)[3]
+    for v, name in ((lr, "lr"), (weight_decay, "weight_decay"), (scale, "scale"), (eps, "eps")):
+        if not math.isfinite(v):
+            raise ValueError(f"{name} must be finite")
+    if not 0 <= momentum <= 1:
+        raise ValueError("momentum must be in [0, 1]")
+    outs = []
+    for name, given, like in (("param_out", param_out, param), ("momentum_out", momentum_out, momentum_buffer)):
+        if given is None:
+            given = torch.empty(like.shape, dtype=like.dtype, device=dev)
+        else:
+            _check_out(given, name, like.dtype, dev, shape=like.shape)
+            for other in (param, grad, momentum_buffer):
+                # element by element in place is fine, any other overlap is not
+                if _overlaps(given, other) and not (other is like and given.data_ptr() == other.data_ptr()
+                                                    and other.is_contiguous()):
+                    raise ValueError(f"{name} overlaps an input that it does not replace")
+        outs.append(given)
+    if _overlaps(*outs):
+        raise ValueError("param_out and momentum_out overlap")
+    co = _schedule(steps, coefficients)
+    with _on_device(dev):
+        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), dev)
+        _lib.call("frag_muon_update", C.byref(dp), C.byref(dg), C.byref(dm), _ptr(outs[0]), _ptr(outs[1]), E, m, n,
+                  float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), steps, co,
+                  float(eps), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(dev))
+    return outs[0], outs[1]
