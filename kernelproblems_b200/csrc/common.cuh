@@ -50,6 +50,11 @@ bool allow_dynamic_smem(const void* kernel, int bytes);
 // Current device ordinal or -1.
 int current_device();
 
+// dw[n] = sum over the G rows of partials [G, N], in a fixed order (the second
+// pass of the RMSNorm backwards); `dependent`: the kernel before it on the
+// stream lets its dependents launch early.
+int dw_reduce_after(const float* partials, int64_t G, int64_t N, float* dw, bool dependent, cudaStream_t s);
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 

@@ -1041,6 +1041,11 @@ int launch_bwd_t(const BwdPlan& pl, BwdIn p, int64_t M, int64_t N, float eps, cu
 }
 
 }  // namespace
+
+int dw_reduce_after(const float* partials, int64_t G, int64_t N, float* dw, bool dependent, cudaStream_t s) {
+  return launch_dw_reduce(partials, G, N, dw, nullptr, s, dependent);
+}
+
 }  // namespace frag
 
 using namespace frag;

@@ -17,6 +17,29 @@
 namespace frag {
 namespace {
 
+// Which kernel takes rows of N values: chunks of eight in registers (a warp or
+// a block a row), single values in registers where rows are not aligned, or
+// the row read again from L2 where it does not fit in registers.
+enum RowKind { ROW_WARP, ROW_BLOCK, ROW_ODD_WARP, ROW_ODD, ROW_ANY };
+struct RowShape {
+  RowKind kind;
+  int K, threads;  // chunks (or four single values) a thread, threads of a block
+};
+// Rows of up to so many values are a warp's; the gradient keeps twice the
+// values of the forward in registers.
+constexpr int kWarpRowFwd = 1024, kWarpRowBwd = 512;
+RowShape row_shape(int64_t N, bool aligned, int warp_row) {
+  if (N > 16384) return {ROW_ANY, 0, 256};
+  if (!aligned || N % 8 != 0) {
+    if (N <= warp_row) return {ROW_ODD_WARP, N <= 256 ? 2 : N <= 512 ? 4 : 8, 256};
+    const int K = N <= 8192 ? 4 : 8;
+    return {ROW_ODD, K, static_cast<int>(ceil_div(N, 128 * K) * 32)};
+  }
+  if (N <= warp_row) return {ROW_WARP, N <= 256 ? 1 : N <= 512 ? 2 : 4, 256};
+  // four chunks a thread and few threads, so that more rows are in flight
+  return {ROW_BLOCK, 4, static_cast<int>(ceil_div(N, 32 * 32) * 32)};
+}
+
 struct QuantFwdP {
   const uint16_t* x;
   const uint16_t* res;
@@ -71,6 +94,90 @@ __device__ __forceinline__ void quant_row(const QuantOut& o, int64_t row, int64_
   }
 }
 
+// Quantise the K chunks of eight values that each of a row's T threads holds;
+// `most` is each chunk's largest magnitude.
+template <int K, bool WARP, bool E5M2, bool E8M0>
+__device__ __forceinline__ void quant_chunks(const QuantOut& o, int64_t row, int64_t N, int group, int t, int T,
+                                             int chunks, const float (&y)[K][8], uint32_t (&most)[K],
+                                             uint32_t (*slots)[32], int parity) {
+  float inv = 0.f, s;
+  uint8_t byte = 0;
+  if (group == 0) {
+    uint32_t m = most[0];
+#pragma unroll
+    for (int k = 1; k < K; ++k) m = max(m, most[k]);
+    m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, slots, parity);
+    s = quant_scale<E5M2, E8M0>(m, inv, byte);
+    if (t == 0) store_scale<E8M0>(o, row, s, byte);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = t + k * T;
+    if (group) {
+      uint32_t m = most[k];
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if (group >= 64) m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      if (group >= 128) m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      s = quant_scale<E5M2, E8M0>(m, inv, byte);
+      const int lanes = group >> 3;
+      if ((c & (lanes - 1)) == 0 && c < chunks) store_scale<E8M0>(o, row * o.groups + c / lanes, s, byte);
+    }
+    if (c < chunks) {
+      uint2 q;
+      q.x = to_fp8x2<E5M2>(y[k][0] * inv, y[k][1] * inv) |
+            static_cast<uint32_t>(to_fp8x2<E5M2>(y[k][2] * inv, y[k][3] * inv)) << 16;
+      q.y = to_fp8x2<E5M2>(y[k][4] * inv, y[k][5] * inv) |
+            static_cast<uint32_t>(to_fp8x2<E5M2>(y[k][6] * inv, y[k][7] * inv)) << 16;
+      *reinterpret_cast<uint2*>(o.q + row * N + static_cast<int64_t>(c) * 8) = q;
+    }
+  }
+}
+
+// Quantise values that lie 32 apart, 4 K of them a thread (zeros past the
+// row): value i of round k is number first + k step + 32 i.
+template <int K, bool WARP, bool E5M2, bool E8M0>
+__device__ __forceinline__ void quant_lanes(const QuantOut& o, int64_t row, int N, int group, int first, int step,
+                                            const float (&y)[K][4], uint32_t (*slots)[32], int parity) {
+  uint8_t* q = o.q + row * N;
+  const int lane = threadIdx.x & 31;
+  float inv = 0.f, s;
+  uint8_t byte = 0;
+  if (group == 0) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, mag_bits(y[k][i]));
+    m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, slots, parity);
+    s = quant_scale<E5M2, E8M0>(m, inv, byte);
+    if (WARP ? lane == 0 : threadIdx.x == 0) store_scale<E8M0>(o, row, s, byte);
+  }
+  const int per = group >> 5;  // 1, 2 or 4 lane rows a group
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    uint32_t m[4];
+    if (group) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = __reduce_max_sync(0xffffffffu, mag_bits(y[k][i]));
+      if (per >= 2) {
+        m[0] = m[1] = max(m[0], m[1]);
+        m[2] = m[3] = max(m[2], m[3]);
+      }
+      if (per == 4) m[0] = m[1] = m[2] = m[3] = max(m[0], m[2]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = first + k * step + 32 * i;
+      if (group) {
+        s = quant_scale<E5M2, E8M0>(m[i], inv, byte);
+        if (lane == 0 && (i & (per - 1)) == 0 && n < N) store_scale<E8M0>(o, row * o.groups + n / group, s, byte);
+      }
+      if (n < N) q[n] = to_fp8<E5M2>(y[k][i] * inv);
+    }
+  }
+}
+
 // Any width, any alignment: one CTA per row, the row read once for each pass
 // (the later passes from L2).
 template <bool E5M2, bool E8M0>
@@ -96,6 +203,123 @@ __global__ void __launch_bounds__(256) quant_fwd_any(const QuantFwdP p) {
                         mslots);
 }
 
+// Rows of 16-byte chunks, the row in registers: thread t of the row's threads
+// owns the chunks t, t + T, ... (K of them); T is the block, or with WARP a
+// warp of it (rows of up to 1024 values: eight rows a block, no barrier).
+// A group of 32, 64 or 128 values is 4, 8 or 16 neighbouring lanes.
+template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(512) quant_fwd_vec(const QuantFwdP p, int64_t M) {
+  __shared__ float slots[2][32];
+  __shared__ uint32_t mslots[2][32];
+  const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= M) return;
+  const int chunks = static_cast<int>(p.N >> 3);
+  const uint16_t* x = p.x + row * p.xs;
+  uint4 xv[K], rv[K], wv[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = t + k * T;
+    xv[k] = rv[k] = wv[k] = make_uint4(0, 0, 0, 0);
+    if (c < chunks) {
+      xv[k] = HAS_RES ? ld_plain(x + c * 8) : ld_stream(x + c * 8);
+      if (HAS_RES) rv[k] = ld_plain(p.res + row * p.rs + c * 8);
+      wv[k] = ld_cached(p.w + c * 8);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (HAS_RES) {
+      xv[k] = add_bf16x8(rv[k], xv[k]);
+      const int c = t + k * T;
+      if (p.h && c < chunks) st_global(p.h + row * p.N + c * 8, xv[k]);
+    }
+    float v[8];
+    unpack8(xv[k], v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+  }
+  ss = WARP ? warp_sum(ss) : block_sum(ss, slots, 0);
+  const float r = rsqrtf(ss / static_cast<float>(p.N) + p.eps);
+  if (p.rstd && t == 0) p.rstd[row] = r;
+  float y[K][8];
+  uint32_t most[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float v[8], wf[8];
+    unpack8(xv[k], v);
+    unpack8(wv[k], wf);
+    most[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[k][i] = (v[i] * r) * wf[i];
+      // chunks past the row are zeros, but 0 * inf is NaN
+      most[k] = max(most[k], t + k * T < chunks ? mag_bits(y[k][i]) : 0u);
+    }
+  }
+  quant_chunks<K, WARP, E5M2, E8M0>(p.o, row, p.N, p.group, t, T, chunks, y, most, mslots, 0);
+}
+
+// Rows without that alignment, up to 16384 values in registers: warp w of the
+// row's W owns 128 neighbouring values at a time, lane l every 32nd of them, so
+// a group of 32, 64 or 128 lies within a warp.  WARP: a warp a row (W = 1).
+template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(512) quant_fwd_odd(const QuantFwdP p, int64_t M) {
+  __shared__ float slots[2][32];
+  __shared__ uint32_t mslots[2][32];
+  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= M) return;
+  const bool lead = WARP ? (threadIdx.x & 31) == 0 : threadIdx.x == 0;
+  const int N = static_cast<int>(p.N);
+  const uint16_t* x = p.x + row * p.xs;
+  const uint16_t* res = HAS_RES ? p.res + row * p.rs : nullptr;
+  const int first = (WARP ? 0 : (threadIdx.x >> 5) * 128) + (threadIdx.x & 31), step = WARP ? 128 : blockDim.x * 4;
+  float y[K][4];
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = first + k * step + 32 * i;
+      y[k][i] = n < N ? bf16_to_f(x[n]) : 0.f;
+    }
+  if (HAS_RES) {
+    float rf[K][4];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = first + k * step + 32 * i;
+        rf[k][i] = n < N ? bf16_to_f(res[n]) : 0.f;
+      }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = first + k * step + 32 * i;
+        const uint16_t h = f_to_bf16(rf[k][i] + y[k][i]);
+        if (p.h && n < N) p.h[row * p.N + n] = h;
+        y[k][i] = bf16_to_f(h);
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = fmaf(y[k][i], y[k][i], ss);
+  ss = WARP ? warp_sum(ss) : block_sum(ss, slots, 0);
+  const float r = rsqrtf(ss / static_cast<float>(N) + p.eps);
+  if (p.rstd && lead) p.rstd[row] = r;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = first + k * step + 32 * i;
+      y[k][i] = n < N ? (y[k][i] * r) * bf16_to_f(p.w[n]) : 0.f;
+    }
+  quant_lanes<K, WARP, E5M2, E8M0>(p.o, row, N, p.group, first, step, y, mslots, 0);
+}
+
 struct QuantBwdP {
   const uint16_t* dy;
   const uint16_t* x;
@@ -109,6 +333,268 @@ struct QuantBwdP {
   int64_t N;
   int group;
 };
+
+// The sums of dweight that each of a block's warps holds for its own rows,
+// added in warp order into the block's partials: value(n) of warp w at
+// acc[w * N + n] of shared memory.
+__device__ __forceinline__ void store_partials(const QuantBwdP& p, const float* acc) {
+  __syncthreads();
+  for (int n = threadIdx.x; n < p.N; n += blockDim.x) {
+    float t = 0.f;
+    for (int w = 0; w < blockDim.x >> 5; ++w) t += acc[w * p.N + n];
+    p.partials[static_cast<int64_t>(blockIdx.x) * p.N + n] = t;
+  }
+}
+
+// dx of one value, in 32 bits.
+__device__ __forceinline__ float grad_of(float g, float xhat, float mean, float r) { return (g - xhat * mean) * r; }
+
+// Rows of up to 512 values in 16-byte chunks, a warp a row: a block's warps
+// take rows_per_block rows in turn.
+template <int K, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t M, int64_t rows_per_block) {
+  extern __shared__ float sacc[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = static_cast<int>(p.N >> 3);
+  uint4 wv[K];
+  float acc[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = lane + 32 * k;
+    wv[k] = c < chunks ? ld_cached(p.w + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+  }
+  const int64_t r1 = min(M, (static_cast<int64_t>(blockIdx.x) + 1) * rows_per_block);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block + warp; row < r1; row += blockDim.x >> 5) {
+    uint4 yv[K], xv[K], rv[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = lane + 32 * k;
+      yv[k] = xv[k] = rv[k] = make_uint4(0, 0, 0, 0);
+      if (c < chunks) {
+        yv[k] = ld_stream(p.dy + row * p.ys + c * 8);
+        xv[k] = ld_stream(p.x + row * p.xs + c * 8);
+        if (HAS_RES) rv[k] = ld_stream(p.dres + row * p.rs + c * 8);
+      }
+    }
+    const float r = __ldg(p.rstd + row);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float yf[8], xf[8], wf[8];
+      unpack8(yv[k], yf);
+      unpack8(xv[k], xf);
+      unpack8(wv[k], wf);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(xf[i] * r, yf[i] * wf[i], sum);
+    }
+    const float mean = warp_sum(sum) / static_cast<float>(p.N);
+    float d[K][8];
+    uint32_t most[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = lane + 32 * k;
+      float yf[8], xf[8], wf[8], rf[8];
+      unpack8(yv[k], yf);
+      unpack8(xv[k], xf);
+      unpack8(wv[k], wf);
+      if (HAS_RES) unpack8(rv[k], rf);
+      most[k] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float xhat = xf[i] * r;
+        acc[k][i] = fmaf(yf[i], xhat, acc[k][i]);
+        d[k][i] = grad_of(yf[i] * wf[i], xhat, mean, r);
+        if (HAS_RES) d[k][i] += rf[i];
+        most[k] = max(most[k], c < chunks ? mag_bits(d[k][i]) : 0u);
+      }
+      if (p.dx && c < chunks) st_global(p.dx + row * p.N + c * 8, pack8(d[k]));
+    }
+    quant_chunks<K, true, E5M2, E8M0>(p.o, row, p.N, p.group, lane, 32, chunks, d, most, nullptr, 0);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = lane + 32 * k;
+    if (c < chunks) {
+      float4* o = reinterpret_cast<float4*>(sacc + warp * p.N + c * 8);
+      o[0] = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+      o[1] = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+    }
+  }
+  if (p.partials) store_partials(p, sacc);
+}
+
+// Longer rows in 16-byte chunks, a block a row: thread 0 streams the rows of
+// the block (dy, x, dres) into a ring of S stages by bulk copies, S rows ahead
+// of the arithmetic; dweight sums stay in registers, thread-owned columns.
+template <int K, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(512)
+quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int* err) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float slots[2][32];
+  __shared__ uint32_t mslots[2][32];
+  __shared__ int s_abort;
+  constexpr int NIN = HAS_RES ? 3 : 2;
+  const int N = static_cast<int>(p.N), chunks = N >> 3, row_bytes = N * 2, stage_bytes = NIN * row_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(S) * stage_bytes);
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
+  const int rows = static_cast<int>(min(M - r0, rows_per_block));
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
+    mbar_init_fence();
+  }
+  __syncthreads();
+  int issued = 0;
+  auto issue = [&](int i) {
+    if (i >= rows) return;
+    unsigned char* st = smem + static_cast<size_t>(i % S) * stage_bytes;
+    mbar_arrive_expect_tx(&bars[i % S], stage_bytes);
+    bulk_g2s(st, p.dy + (r0 + i) * p.ys, row_bytes, &bars[i % S]);
+    bulk_g2s(st + row_bytes, p.x + (r0 + i) * p.xs, row_bytes, &bars[i % S]);
+    if (HAS_RES) bulk_g2s(st + 2 * row_bytes, p.dres + (r0 + i) * p.rs, row_bytes, &bars[i % S]);
+    issued = i + 1;
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < S; ++i) issue(i);
+  uint4 wv[K];
+  float acc[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    wv[k] = c < chunks ? ld_cached(p.w + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+  }
+  int i = 0;
+  for (; i < rows; ++i) {
+    const int64_t row = r0 + i;
+    const float r = __ldg(p.rstd + row);
+    const unsigned char* st = smem + static_cast<size_t>(i % S) * stage_bytes;
+    if (!mbar_wait(&bars[i % S], (i / S) & 1, err)) s_abort = 1;
+    uint4 yv[K], xv[K], rv[K];
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      yv[k] = xv[k] = rv[k] = make_uint4(0, 0, 0, 0);
+      if (c < chunks) {
+        yv[k] = *reinterpret_cast<const uint4*>(st + c * 16);
+        xv[k] = *reinterpret_cast<const uint4*>(st + row_bytes + c * 16);
+        if (HAS_RES) rv[k] = *reinterpret_cast<const uint4*>(st + 2 * row_bytes + c * 16);
+      }
+      float yf[8], xf[8], wf[8];
+      unpack8(yv[k], yf);
+      unpack8(xv[k], xf);
+      unpack8(wv[k], wf);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(xf[e] * r, yf[e] * wf[e], sum);
+    }
+    const float mean = block_sum(sum, slots, i & 1) / static_cast<float>(N);
+    if (s_abort) break;
+    if (threadIdx.x == 0) issue(i + S);  // every thread has read stage i % S
+    float d[K][8];
+    uint32_t most[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      float yf[8], xf[8], wf[8], rf[8];
+      unpack8(yv[k], yf);
+      unpack8(xv[k], xf);
+      unpack8(wv[k], wf);
+      if (HAS_RES) unpack8(rv[k], rf);
+      most[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xhat = xf[e] * r;
+        acc[k][e] = fmaf(yf[e], xhat, acc[k][e]);
+        d[k][e] = grad_of(yf[e] * wf[e], xhat, mean, r);
+        if (HAS_RES) d[k][e] += rf[e];
+        most[k] = max(most[k], c < chunks ? mag_bits(d[k][e]) : 0u);
+      }
+      if (p.dx && c < chunks) st_global(p.dx + row * N + c * 8, pack8(d[k]));
+    }
+    quant_chunks<K, false, E5M2, E8M0>(p.o, row, N, p.group, threadIdx.x, blockDim.x, chunks, d, most, mslots, i & 1);
+  }
+  if (threadIdx.x == 0 && s_abort)
+    for (int j = i; j < issued; ++j) mbar_wait(&bars[j % S], (j / S) & 1, nullptr);
+  if (!p.partials) return;
+  float* part = p.partials + static_cast<int64_t>(blockIdx.x) * N;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    if (c < chunks) {
+      *reinterpret_cast<float4*>(part + c * 8) = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+      *reinterpret_cast<float4*>(part + c * 8 + 4) = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+    }
+  }
+}
+
+// Rows without that alignment, up to 16384 values, single values in registers
+// (the layout of quant_fwd_odd); WARP: a warp a row.
+template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(512) quant_bwd_odd(const QuantBwdP p, int64_t M, int64_t rows_per_block) {
+  extern __shared__ float sacc[];  // WARP
+  __shared__ float slots[2][32];
+  __shared__ uint32_t mslots[2][32];
+  const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = (WARP ? 0 : warp * 128) + lane, step = WARP ? 128 : blockDim.x * 4;
+  float acc[K][4];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[k][i] = 0.f;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows_per_block, r1 = min(M, r0 + rows_per_block);
+  int parity = 0;
+  for (int64_t row = r0 + (WARP ? warp : 0); row < r1; row += WARP ? blockDim.x >> 5 : 1, parity ^= 1) {
+    const uint16_t* dy = p.dy + row * p.ys;
+    const uint16_t* x = p.x + row * p.xs;
+    const uint16_t* dres = HAS_RES ? p.dres + row * p.rs : nullptr;
+    const float r = __ldg(p.rstd + row);
+    float g[K][4], xh[K][4], d[K][4];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = first + k * step + 32 * i;
+        g[k][i] = n < N ? bf16_to_f(dy[n]) : 0.f;
+        xh[k][i] = n < N ? bf16_to_f(x[n]) : 0.f;
+        d[k][i] = HAS_RES && n < N ? bf16_to_f(dres[n]) : 0.f;
+      }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = first + k * step + 32 * i;
+        xh[k][i] *= r;
+        acc[k][i] = fmaf(g[k][i], xh[k][i], acc[k][i]);
+        g[k][i] *= n < N ? bf16_to_f(__ldg(p.w + n)) : 0.f;
+        sum = fmaf(xh[k][i], g[k][i], sum);
+      }
+    const float mean = (WARP ? warp_sum(sum) : block_sum(sum, slots, parity)) / static_cast<float>(N);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = first + k * step + 32 * i;
+        d[k][i] = n < N ? d[k][i] + grad_of(g[k][i], xh[k][i], mean, r) : 0.f;
+        if (p.dx && n < N) p.dx[row * N + n] = f_to_bf16(d[k][i]);
+      }
+    quant_lanes<K, WARP, E5M2, E8M0>(p.o, row, N, p.group, first, step, d, mslots, parity);
+  }
+  if (!p.partials) return;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = first + k * step + 32 * i;
+      if (n < N) (WARP ? sacc + warp * N : p.partials + static_cast<int64_t>(blockIdx.x) * N)[n] = acc[k][i];
+    }
+  if (WARP) store_partials(p, sacc);
+}
 
 template <bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(256) quant_bwd_any(const QuantBwdP p) {
@@ -145,16 +631,87 @@ __global__ void __launch_bounds__(256) quant_bwd_any_dw(const QuantBwdP p, int64
   p.partials[static_cast<int64_t>(blockIdx.y) * p.N + col] = acc;
 }
 
-// Row blocks of the dweight partials: the same for every call of M rows.
+// Row blocks of the dweight partials: the same for every call of M rows of N.
 struct QuantBwdPlan {
   int64_t G, rows_per_block;
 };
-QuantBwdPlan quant_bwd_plan(int64_t M) {
+// Threads of a row's block (two or four chunks each), and blocks of an SM.
+int ring_threads(int64_t N) { return static_cast<int>(std::min<int64_t>(512, ceil_div(N, N <= 8192 ? 512 : 1024) * 32)); }
+int ring_blocks(int threads) { return std::max(1, std::min(4, 512 / threads)); }
+
+QuantBwdPlan quant_bwd_plan(int64_t M, int64_t N) {
   int sms = sm_count();
   if (sms <= 0) sms = 148;
-  const int64_t target = std::max<int64_t>(1, std::min<int64_t>(M, 2 * sms));
-  const int64_t rows = ceil_div(M, target);
+  // a warp a row: two blocks of eight an SM; a block a row: 512 threads an SM
+  const int64_t blocks = N <= kWarpRowBwd ? std::min<int64_t>(ceil_div(M, 8), 2 * sms)
+                                          : std::min<int64_t>(M, ring_blocks(ring_threads(N)) * sms);
+  const int64_t rows = ceil_div(M, std::max<int64_t>(1, blocks));
   return {ceil_div(M, rows), rows};
+}
+
+template <int K, bool HAS_RES, bool E5M2, bool E8M0>
+int launch_bwd_ring(const QuantBwdP& p, int64_t M, const QuantBwdPlan& pl, cudaStream_t s) {
+  const int stage_bytes = (HAS_RES ? 3 : 2) * static_cast<int>(p.N) * 2;
+  const int threads = ring_threads(p.N), cps = ring_blocks(threads);
+  const int S = std::min(8, (220 * 1024 / cps - 1024) / (stage_bytes + 8));
+  const int smem = S * (stage_bytes + 8);
+  auto kern = quant_bwd_ring<K, HAS_RES, E5M2, E8M0>;
+  if (!allow_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return FRAG_ERR_CUDA;
+  kern<<<static_cast<unsigned>(pl.G), threads, smem, s>>>(p, M, pl.rows_per_block, S, device_error_word());
+  return check_launch();
+}
+
+template <bool HAS_RES, bool E5M2, bool E8M0>
+int launch_bwd(const QuantBwdP& p, int64_t M, const QuantBwdPlan& pl, const RowShape& r, cudaStream_t s) {
+  const unsigned G = static_cast<unsigned>(pl.G);
+  const int wsmem = static_cast<int>(8 * p.N * sizeof(float));  // the warps' dweight sums (up to 16 KB)
+  switch (r.kind) {
+    case ROW_WARP:
+      if (r.K == 1) quant_bwd_warp<1, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
+      else quant_bwd_warp<2, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
+      return check_launch();
+    case ROW_BLOCK:
+      return p.N <= 8192 ? launch_bwd_ring<2, HAS_RES, E5M2, E8M0>(p, M, pl, s)
+                         : launch_bwd_ring<4, HAS_RES, E5M2, E8M0>(p, M, pl, s);
+    case ROW_ODD_WARP:
+      if (r.K == 2) quant_bwd_odd<2, true, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
+      else quant_bwd_odd<4, true, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
+      return check_launch();
+    case ROW_ODD:
+      if (r.K == 4) quant_bwd_odd<4, false, HAS_RES, E5M2, E8M0><<<G, r.threads, 0, s>>>(p, M, pl.rows_per_block);
+      else quant_bwd_odd<8, false, HAS_RES, E5M2, E8M0><<<G, r.threads, 0, s>>>(p, M, pl.rows_per_block);
+      return check_launch();
+    default: break;
+  }
+  quant_bwd_any<E5M2, E8M0><<<static_cast<unsigned>(M), 256, 0, s>>>(p);
+  int st = check_launch();
+  if (st != FRAG_OK || !p.partials) return st;
+  quant_bwd_any_dw<<<dim3(static_cast<unsigned>(ceil_div(p.N, 256)), G), 256, 0, s>>>(p, M, pl.rows_per_block);
+  return check_launch();
+}
+
+template <bool HAS_RES, bool E5M2, bool E8M0>
+int launch_fwd(const QuantFwdP& p, int64_t M, const RowShape& r, cudaStream_t s) {
+  const unsigned rows = static_cast<unsigned>(M), warps = static_cast<unsigned>(ceil_div(M, r.threads / 32));
+  switch (r.kind) {
+    case ROW_WARP:
+      if (r.K == 1) quant_fwd_vec<1, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      else if (r.K == 2) quant_fwd_vec<2, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      else quant_fwd_vec<4, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      break;
+    case ROW_BLOCK: quant_fwd_vec<4, false, HAS_RES, E5M2, E8M0><<<rows, r.threads, 0, s>>>(p, M); break;
+    case ROW_ODD_WARP:
+      if (r.K == 2) quant_fwd_odd<2, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      else if (r.K == 4) quant_fwd_odd<4, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      else quant_fwd_odd<8, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
+      break;
+    case ROW_ODD:
+      if (r.K == 4) quant_fwd_odd<4, false, HAS_RES, E5M2, E8M0><<<rows, r.threads, 0, s>>>(p, M);
+      else quant_fwd_odd<8, false, HAS_RES, E5M2, E8M0><<<rows, r.threads, 0, s>>>(p, M);
+      break;
+    default: quant_fwd_any<E5M2, E8M0><<<rows, 256, 0, s>>>(p);
+  }
+  return check_launch();
 }
 
 template <class F>
@@ -197,16 +754,20 @@ int frag_rmsnorm_quant_fwd(const void* x, int64_t x_stride, const void* res, int
   p.N = N;
   p.group = static_cast<int>(group);
   p.eps = eps;
+  const RowShape shape = row_shape(N, aligned16(x) && aligned16(w) && (!res || aligned16(res)) &&
+                                          (!h || aligned16(h)) && aligned16(q) && (M == 1 || x_stride % 8 == 0) &&
+                                          (M == 1 || !res || res_stride % 8 == 0),
+                                   kWarpRowFwd);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return by_format(format, scale_e8m0, [&](auto e5m2, auto e8m0) {
-    quant_fwd_any<decltype(e5m2)::value, decltype(e8m0)::value><<<static_cast<unsigned>(M), 256, 0, s>>>(p);
-    return check_launch();
+    return res ? launch_fwd<true, decltype(e5m2)::value, decltype(e8m0)::value>(p, M, shape, s)
+               : launch_fwd<false, decltype(e5m2)::value, decltype(e8m0)::value>(p, M, shape, s);
   });
 }
 
 size_t frag_rmsnorm_quant_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
-  return align_up(static_cast<size_t>(quant_bwd_plan(M).G) * N * sizeof(float), 256);
+  return align_up(static_cast<size_t>(quant_bwd_plan(M, N).G) * N * sizeof(float), 256);
 }
 
 int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* rstd,
@@ -218,7 +779,7 @@ int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const void* x, int
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (M == 0) return dw ? cuda_status(cudaMemsetAsync(dw, 0, N * sizeof(float), s)) : FRAG_OK;
   if (!dy || !x || !rstd || !w || !q || !scale) return FRAG_ERR_INVALID_ARG;
-  const QuantBwdPlan pl = quant_bwd_plan(M);
+  const QuantBwdPlan pl = quant_bwd_plan(M, N);
   if (!workspace || workspace_bytes < frag_rmsnorm_quant_bwd_workspace_bytes(M, N)) return FRAG_ERR_WORKSPACE;
   if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
   QuantBwdP p;
@@ -228,22 +789,24 @@ int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const void* x, int
   p.w = static_cast<const uint16_t*>(w);
   p.dres = static_cast<const uint16_t*>(dres);
   p.dx = static_cast<uint16_t*>(dx);
-  p.partials = static_cast<float*>(workspace);
+  p.partials = dw ? static_cast<float*>(workspace) : nullptr;
   p.ys = dy_stride;
   p.xs = x_stride;
   p.rs = dres_stride;
   p.o = QuantOut{static_cast<uint8_t*>(q), scale, group ? ceil_div(N, group) : 1};
   p.N = N;
   p.group = static_cast<int>(group);
-  int st = by_format(format, scale_e8m0, [&](auto e5m2, auto e8m0) {
-    quant_bwd_any<decltype(e5m2)::value, decltype(e8m0)::value><<<static_cast<unsigned>(M), 256, 0, s>>>(p);
-    return check_launch();
+  const RowShape shape =
+      row_shape(N, aligned16(dy) && aligned16(x) && aligned16(w) && (!dres || aligned16(dres)) &&
+                       (!dx || aligned16(dx)) && aligned16(q) && (M == 1 || (dy_stride % 8 == 0 && x_stride % 8 == 0)) &&
+                       (M == 1 || !dres || dres_stride % 8 == 0),
+                kWarpRowBwd);
+  const int st = by_format(format, scale_e8m0, [&](auto e5m2, auto e8m0) {
+    return dres ? launch_bwd<true, decltype(e5m2)::value, decltype(e8m0)::value>(p, M, pl, shape, s)
+                : launch_bwd<false, decltype(e5m2)::value, decltype(e8m0)::value>(p, M, pl, shape, s);
   });
   if (st != FRAG_OK || !dw) return st;
-  const dim3 grid(static_cast<unsigned>(ceil_div(N, 256)), static_cast<unsigned>(pl.G));
-  quant_bwd_any_dw<<<grid, 256, 0, s>>>(p, M, pl.rows_per_block);
-  st = check_launch();
-  return st != FRAG_OK ? st : frag_dw_reduce(p.partials, pl.G, N, dw, nullptr, stream);
+  return dw_reduce_after(p.partials, pl.G, N, dw, shape.kind == ROW_BLOCK, s);
 }
 
 }  // extern "C"

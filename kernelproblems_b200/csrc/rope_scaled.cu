@@ -61,6 +61,164 @@ __device__ __forceinline__ void turn(double turns, double p, const ScaledP& P, f
   s = sv * P.sin_factor;
 }
 
+// CH bf16 values that one access moves.
+template <int CH> struct Chunk;
+template <> struct Chunk<8> { typedef uint4 T; };
+template <> struct Chunk<4> { typedef uint2 T; };
+template <> struct Chunk<2> { typedef uint32_t T; };
+
+template <int CH>
+__device__ __forceinline__ void widen(const typename Chunk<CH>::T& v, float (&f)[CH]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < CH / 2; ++i) {
+    f[2 * i] = bf16lo(w[i]);
+    f[2 * i + 1] = bf16hi(w[i]);
+  }
+}
+template <int CH>
+__device__ __forceinline__ typename Chunk<CH>::T narrow(const float (&f)[CH]) {
+  typename Chunk<CH>::T v;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < CH / 2; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+// rot a multiple of 2 CH, heads and strides of CH elements.  A warp takes one
+// token and a run of `span` head groups, q's and then k's; L = rot / (2 CH)
+// lanes share a head, and lane j of it owns the chunks at CH j and rot/2 + CH j:
+// whole pairs in either layout, the same frequencies in every head, so its CH
+// sines and cosines are made once.  The passed elements follow, chunk by chunk.
+template <int CH, bool NEOX>
+__global__ void __launch_bounds__(256, 3) rope_scaled_vec(const __grid_constant__ ScaledP p, int splits, int span) {
+  typedef typename Chunk<CH>::T V;
+  constexpr int UNR = 4;
+  __shared__ double turns[kMaxPairs];
+  const int half = p.rot >> 1;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) turns[i] = p.turns[i];
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t tok = w / splits;
+  if (tok >= p.B * p.S) return;
+  const int first = static_cast<int>(w - tok * splits) * span;
+  const int64_t b = tok / p.S, s = tok - b * p.S;
+  const double pos = static_cast<double>(token_pos(p, b, s));
+  const int L = half / CH, HPG = 32 / L;  // lanes of a head, heads of a group
+  const int j = lane % L, hs = lane / L;
+  float cs[CH], sn[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int f = NEOX ? CH * j + i : (i < CH / 2 ? CH / 2 * j + i : (half >> 1) + CH / 2 * j + i - CH / 2);
+    turn(turns[f], pos, p, cs[i], sn[i]);
+  }
+  const int rest = (p.D - p.rot) / CH;
+  const int gq = (p.t[0].H + HPG - 1) / HPG;
+  int base = 0;  // the tensor's first head group
+#pragma unroll
+  for (int ti = 0; ti < 2; ++ti) {
+    if (ti >= p.nt) break;
+    const ScaledT& T = p.t[ti];
+    const int groups = ti == 0 ? gq : (T.H + HPG - 1) / HPG;
+    const int g0 = max(first - base, 0), g1 = min(first + span - base, groups);
+    base += groups;
+    if (g0 >= g1) continue;
+    const uint16_t* x = T.x + b * T.xsb + s * T.xss;
+    uint16_t* out = T.out + b * T.osb + s * T.oss;
+    const int h1 = min(T.H, g1 * HPG);
+    for (int h0 = g0 * HPG + hs; hs < HPG && h0 < h1; h0 += HPG * UNR) {
+      V va[UNR], vb[UNR];
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        const int h = h0 + u * HPG;
+        if (h < h1) {
+          va[u] = *reinterpret_cast<const V*>(x + h * T.xsh + CH * j);
+          vb[u] = *reinterpret_cast<const V*>(x + h * T.xsh + half + CH * j);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        const int h = h0 + u * HPG;
+        if (h < h1) {
+          float fa[CH], fb[CH], ra[CH], rb[CH];
+          widen<CH>(va[u], fa);
+          widen<CH>(vb[u], fb);
+          if (NEOX) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+              ra[i] = fa[i] * cs[i] - fb[i] * sn[i];
+              rb[i] = fb[i] * cs[i] + fa[i] * sn[i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {
+              ra[2 * i] = fa[2 * i] * cs[i] - fa[2 * i + 1] * sn[i];
+              ra[2 * i + 1] = fa[2 * i + 1] * cs[i] + fa[2 * i] * sn[i];
+              rb[2 * i] = fb[2 * i] * cs[CH / 2 + i] - fb[2 * i + 1] * sn[CH / 2 + i];
+              rb[2 * i + 1] = fb[2 * i + 1] * cs[CH / 2 + i] + fb[2 * i] * sn[CH / 2 + i];
+            }
+          }
+          *reinterpret_cast<V*>(out + h * T.osh + CH * j) = narrow<CH>(ra);
+          *reinterpret_cast<V*>(out + h * T.osh + half + CH * j) = narrow<CH>(rb);
+        }
+      }
+    }
+    if (T.copy_rest && rest > 0) {
+      const int hf = g0 * HPG, n = (h1 - hf) * rest;
+      for (int i0 = lane; i0 < n; i0 += 32 * UNR) {
+        V v[UNR];
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+          const int i = i0 + 32 * u, h = i / rest;
+          if (i < n) v[u] = *reinterpret_cast<const V*>(x + (hf + h) * T.xsh + p.rot + CH * (i - h * rest));
+        }
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+          const int i = i0 + 32 * u, h = i / rest;
+          if (i < n) *reinterpret_cast<V*>(out + (hf + h) * T.osh + p.rot + CH * (i - h * rest)) = v[u];
+        }
+      }
+    }
+  }
+}
+
+// Whether every head of the call divides into chunks of CH elements.
+bool fits(const ScaledP& p, int CH) {
+  if (p.rot % (2 * CH) != 0 || p.D % CH != 0 || p.rot / (2 * CH) > 32) return false;
+  for (int i = 0; i < p.nt; ++i) {
+    const ScaledT& t = p.t[i];
+    const int64_t st[6] = {t.xsb, t.xss, t.xsh, t.osb, t.oss, t.osh};
+    for (int64_t v : st)
+      if (v % CH != 0) return false;
+    if ((reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.out)) % (2 * CH) != 0) return false;
+  }
+  return true;
+}
+
+template <int CH>
+int launch_vec(const ScaledP& p, bool neox, cudaStream_t s) {
+  const int HPG = 32 / (p.rot / (2 * CH));
+  int64_t groups = 0;
+  for (int i = 0; i < p.nt; ++i) groups += ceil_div(p.t[i].H, HPG);
+  const int64_t tokens = p.B * p.S;
+  int sms = sm_count();
+  if (sms <= 0) sms = 148;
+  // A token's sines cost as much as a few head groups, so a warp takes the
+  // whole token while there are enough of them to fill the machine (16 warps
+  // an SM), and the heads are split over more warps when there are not.
+  const int64_t splits = std::max<int64_t>(1, std::min(groups, ceil_div(16LL * sms, tokens)));
+  const int64_t span = ceil_div(groups, splits);
+  const int64_t warps = tokens * ceil_div(groups, span);
+  const int per = warps >= 8LL * sms ? 8 : 2;  // warps of a block
+  const int64_t grid = ceil_div(warps, per);
+  if (grid > 0x7fffffffLL) return FRAG_ERR_SHAPE;
+  auto kern = neox ? rope_scaled_vec<CH, true> : rope_scaled_vec<CH, false>;
+  kern<<<static_cast<unsigned>(grid), 32 * per, 0, s>>>(p, static_cast<int>(ceil_div(groups, span)),
+                                                        static_cast<int>(span));
+  return check_launch();
+}
+
 // Any even rot, any strides: one CTA per token, one thread per pair or passed
 // element, the token's sines and cosines in shared memory.
 template <bool NEOX>
@@ -139,12 +297,20 @@ extern "C" int frag_rope_scaled(const frag_rope_tensor* tensors, int num_tensors
     p.t[i] = ScaledT{static_cast<const uint16_t*>(t.x), static_cast<uint16_t*>(t.out), static_cast<int>(t.H),
                      in_place ? 0 : 1, t.x_stride_b, t.x_stride_s, t.x_stride_h, t.out_stride_b,
                      t.out_stride_s, t.out_stride_h};
+    // a dimension of one element has no stride to respect
+    if (B == 1) p.t[i].xsb = p.t[i].osb = 0;
+    if (S == 1) p.t[i].xss = p.t[i].oss = 0;
+    if (t.H == 1) p.t[i].xsh = p.t[i].osh = 0;
     any = any || t.H > 0;
   }
   if (!any) return FRAG_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool neox = layout == FRAG_ROPE_NEOX;
+  if (fits(p, 8)) return launch_vec<8>(p, neox, s);
+  if (fits(p, 4)) return launch_vec<4>(p, neox, s);
+  if (fits(p, 2)) return launch_vec<2>(p, neox, s);
   const unsigned grid = static_cast<unsigned>(B * S);
-  if (layout == FRAG_ROPE_NEOX) rope_scaled_any<true><<<grid, 256, 0, s>>>(p);
+  if (neox) rope_scaled_any<true><<<grid, 256, 0, s>>>(p);
   else rope_scaled_any<false><<<grid, 256, 0, s>>>(p);
   return check_launch();
 }
