@@ -72,14 +72,20 @@ bool make_map_3d(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64
 
 namespace {
 
-constexpr float kXScale = 256.0f;  // X is kept times 2^8
+constexpr float kXScale = 256.0f;   // X is kept times 2^8
 constexpr float kAScale = 1024.0f;  // A and B times 2^10
-constexpr int kT = 128;             // tile side
-constexpr int kStages = 6;
-constexpr int kStageBytes = 2 * kT * kTileK * 2;
-constexpr int kThreads = 192;  // a loading warp, an issuing warp, four for the epilogue
-constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kRows = 128;          // rows of C a block holds
+constexpr int kChunk = 64;          // columns the epilogue takes at a time
+constexpr int kOperand = 128 * kTileK * 2;  // bytes of one operand of a stage
+constexpr int kStageBytes = 2 * kOperand;
+constexpr int kStages = 4;
+constexpr int kSet = 2 * kRows * kChunk * 2;  // two 16-bit chunks
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // a loading warp, an issuing warp, the epilogue
+constexpr int kSmem = kStages * kStageBytes + 2 * kSet + 1024;
 
+// GRAM A = X X', POLY B = b A + c A A, STEP X <- a X + B X; the last step's
+// STEP writes the result (LAST) or the weights (UPDATE) instead of X.
 enum Mode { GRAM = 0, POLY = 1, STEP = 2, LAST = 3, UPDATE = 4 };
 
 struct Elem {  // a tensor of bf16 or fp32 elements with strides
@@ -95,28 +101,23 @@ __device__ __forceinline__ void store_elem(const Elem& e, int64_t i, float v) {
   else static_cast<uint16_t*>(e.p)[i] = f_to_bf16(v);
 }
 
-struct ProductP {
-  CUtensorMap mp, mq;  // operands: C[i, j] = sum_k P[i, k] Q[j, k]
-  int I, J, K, E;
-  int tall;
-  // GRAM and POLY write A / B here, POLY reads A
-  __half* c;
-  const __half* a;
-  int64_t ldc;      // row stride; a batch is I rows
-  float2* diag;     // [E, s] B's diagonal in 32 bits and its rounding residual
-  // STEP, LAST, UPDATE
-  const __half* hi;
-  __half* hi_out;
-  __half* lo;
-  int64_t ldx;
-  float ca, cb, cc;   // the step's coefficients
-  float lo_factor;    // 1 in the last two steps: the diagonal's product with lo
-  Elem out, par;      // LAST, UPDATE; UPDATE also reads par
-  float keep, rate;   // p' = keep p - rate O
+constexpr int kMaxSteps = 32;
+
+struct ChainP {
+  // X's two buffers by 64 columns x 128 rows and by 64 x 64, lo, A and B
+  CUtensorMap xk[2], xm[2], lo, ak, bk, a64, b64;
+  int m, n, s, l, E, tall, steps, split;
+  float2* diag;        // [E, s] B's diagonal in 32 bits and its rounding residual
+  float* partials;     // split GRAM sums
+  unsigned* counters;  // grid barrier, abort, and an arrival count for each split tile
+  int last;            // LAST or UPDATE
+  Elem out, par;
+  float keep, rate;  // p' = keep p - rate O
   int* err;
+  float co[3 * kMaxSteps];
 };
 
-__device__ __forceinline__ void unpack_h8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack_h8(const uint4& v, float* f) {
   const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -125,232 +126,503 @@ __device__ __forceinline__ void unpack_h8(const uint4& v, float (&f)[8]) {
     f[2 * i + 1] = t.y;
   }
 }
-__device__ __forceinline__ uint4 pack_h8(const float (&f)[8]) {
+__device__ __forceinline__ uint4 pack_h8(const float* f) {
   uint4 v;
   __half2* h = reinterpret_cast<__half2*>(&v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
   return v;
 }
-
-// Tile t of a batch: (row tile, column tile).  Symmetric products take the
-// tiles on and below the diagonal.
-template <bool SYM>
-__device__ __forceinline__ void tile_at(int t, int tj_count, int& ti, int& tj) {
-  if (SYM) {
-    ti = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-    while (ti * (ti + 1) / 2 > t) --ti;
-    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-    tj = t - ti * (ti + 1) / 2;
-  } else {
-    ti = t / tj_count;
-    tj = t - ti * tj_count;
-  }
+__device__ __forceinline__ uint4 ld_shared(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
 }
+__device__ __forceinline__ void st_shared(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float ld_shared_f(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void st_shared_h(uint32_t a, __half v) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory");
+}
+// 16-byte unit u of row r of a chunk (128-byte rows under the 128-byte swizzle).
+__device__ __forceinline__ uint32_t unit(uint32_t base, int r, int u) { return base + r * 128 + ((u ^ (r & 7)) << 4); }
 
-// Eight values of row i (< I) from column j on: what the tile's accumulator
-// becomes.  Rows of the working buffers are padded to eight elements, so a
-// group that is cut by the matrix's edge is still read and written whole.
+// One phase's product C[i, j] = sum_k P[i, k] Q[j, k] as a list of work items.
+template <int CG>
+struct Work {
+  static constexpr int TM = kRows * CG, TN = 128 * CG;
+  int I, J, ks, split, ti_count, tj_count, per, items, E;
+  bool sym, cols_fast;
+  __device__ Work(const ChainP& p, int mode) {
+    sym = mode == GRAM || mode == POLY;
+    I = sym ? p.s : p.m;
+    J = sym ? p.s : p.n;
+    E = p.E;
+    ks = ((mode == GRAM ? p.l : p.s) + kTileK - 1) / kTileK;
+    split = mode == GRAM ? p.split : 1;
+    ti_count = (I + TM - 1) / TM;
+    tj_count = (J + TN - 1) / TN;
+    per = sym ? ti_count * (ti_count + 1) / 2 : ti_count * tj_count;
+    items = per * E * split;
+    // the long side's tiles go last, so that blocks at work share the operands
+    cols_fast = p.tall;
+  }
+  // Item w: batch, tile and part of k.  Parts of a tile are neighbours.
+  __device__ void at(int w, int& e, int& ti, int& tj, int& z) const {
+    int t = w / split;
+    z = w - t * split;
+    e = t / per;
+    t -= e * per;
+    if (sym) {
+      ti = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+      while (ti * (ti + 1) / 2 > t) --ti;
+      while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+      tj = t - ti * (ti + 1) / 2;
+    } else if (cols_fast) {
+      ti = t / tj_count;
+      tj = t - ti * tj_count;
+    } else {
+      tj = t / ti_count;
+      ti = t - tj * ti_count;
+    }
+  }
+  __device__ int k_begin(int z) const { return static_cast<int>(static_cast<int64_t>(ks) * z / split); }
+};
+
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory"); }
+
+struct Shared {
+  uint64_t full[kStages], empty[kStages], done[2], freed[2], aux[2], drain;
+  int64_t aux_issued[2];  // the last chunk prepared in each set, plus one
+  uint32_t tmem;
+  int abort;
+};
+constexpr int kLead = 64;  // the epilogue's thread that moves chunks
+
+// The epilogue's view: what it does with 32 accumulator columns of one row of
+// a chunk.  `set` is the chunk's 32 KB of shared memory: hi and lo (STEP), A
+// (POLY), overwritten by the results that a bulk store then takes.
 template <int MODE>
-__device__ __forceinline__ void finish8(const ProductP& p, int e, int i, int j, float (&v)[8], bool mirror) {
+__device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set, int e, int i, int j, int r, int half,
+                                         bool mirror, float2 dr, float (&v)[32]) {
+  const uint32_t lo = set + kSet / 2;
   if (MODE == GRAM || MODE == POLY) {
-    const int64_t at = (static_cast<int64_t>(e) * p.I + i) * p.ldc + j;
     if (MODE == GRAM) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= kAScale / (kXScale * kXScale);
+      for (int k = 0; k < 32; ++k) v[k] *= kAScale / (kXScale * kXScale);
     } else {
-      float a[8];
-      unpack_h8(*reinterpret_cast<const uint4*>(p.a + at), a);
+      const float cb = p.co[3 * step + 1], cc = p.co[3 * step + 2] / kAScale;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = p.cb * a[k] + (p.cc / kAScale) * v[k];
-        if (j + k == i) p.diag[static_cast<int64_t>(e) * p.I + i] = make_float2(v[k], v[k] - __half2float(__float2half_rn(v[k])));
+      for (int u = 0; u < 4; ++u) {
+        float a[8];
+        unpack_h8(ld_shared(unit(set, r, half * 4 + u)), a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[8 * u + k] = cb * a[k] + cc * v[8 * u + k];
+      }
+      if (i >= j && i < j + 32 && i < p.s) {
+        float d = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) d = j + k == i ? v[k] : d;
+        p.diag[static_cast<int64_t>(e) * p.s + i] = make_float2(d, d - __half2float(__float2half_rn(d)));
       }
     }
-    *reinterpret_cast<uint4*>(p.c + at) = pack_h8(v);
-    if (mirror) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (j + k < p.J) p.c[(static_cast<int64_t>(e) * p.I + j + k) * p.ldc + i] = __float2half_rn(v[k]);
+    for (int u = 0; u < 4; ++u) st_shared(unit(set, r, half * 4 + u), pack_h8(v + 8 * u));
+    if (mirror) {
+      // the transposed chunk, 64 rows of 128: two boxes of 64 columns
+      const uint32_t box = lo + (r >> 6) * (kChunk * 128);
+      const int c = r & 63;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int jr = half * 32 + k;
+        st_shared_h(unit(box, jr, c >> 3) + (c & 7) * 2, __float2half_rn(v[k]));
+      }
     }
     return;
   }
-  const int64_t at = (static_cast<int64_t>(e) * p.I + i) * p.ldx + j;
-  float h[8], l[8];
-  unpack_h8(*reinterpret_cast<const uint4*>(p.hi + at), h);
-  unpack_h8(*reinterpret_cast<const uint4*>(p.lo + at), l);
-  const float2* diag = p.diag + static_cast<int64_t>(e) * (p.tall ? p.J : p.I);
-  const float2 dr = p.tall ? make_float2(0.f, 0.f) : diag[i];
+  const float ca = p.co[3 * step];
+  const float lf = step >= p.steps - 2 ? 1.0f / kAScale : 0.0f;  // the diagonal's product with lo
+  float2 dc = dr;
+  if (p.tall) {  // column j + lane's, handed round below
+    const int col = j + (threadIdx.x & 31);
+    dc = col < p.n ? __ldcg(p.diag + static_cast<int64_t>(e) * p.s + col) : make_float2(0.f, 0.f);
+  }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float2 d = p.tall ? (j + k < p.J ? diag[j + k] : make_float2(0.f, 0.f)) : dr;
-    v[k] = p.ca * (h[k] + l[k]) + (v[k] + d.y * h[k] + p.lo_factor * d.x * l[k]) * (1.0f / kAScale);
+  for (int u = 0; u < 4; ++u) {
+    float h[8], l[8];
+    unpack_h8(ld_shared(unit(set, r, half * 4 + u)), h);
+    unpack_h8(ld_shared(unit(lo, r, half * 4 + u)), l);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float2 d = dr;
+      if (p.tall) {
+        d.x = __shfl_sync(0xffffffffu, dc.x, 8 * u + k);
+        d.y = __shfl_sync(0xffffffffu, dc.y, 8 * u + k);
+      }
+      v[8 * u + k] = ca * (h[k] + l[k]) + (v[8 * u + k] + d.y * h[k]) * (1.0f / kAScale) + lf * (d.x * l[k]);
+    }
   }
   if (MODE == STEP) {
-    *reinterpret_cast<uint4*>(p.hi_out + at) = pack_h8(v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
-    *reinterpret_cast<uint4*>(p.lo + at) = pack_h8(v);
-    return;
-  }
-  const int64_t o = static_cast<int64_t>(e) * p.out.sb + i * p.out.sr + j;
+    for (int u = 0; u < 4; ++u) {
+      st_shared(unit(set, r, half * 4 + u), pack_h8(v + 8 * u));
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (j + k >= p.J) break;
-    float r = v[k] * (1.0f / kXScale);
-    if (MODE == UPDATE)
-      r = p.keep * load_elem(p.par, static_cast<int64_t>(e) * p.par.sb + i * p.par.sr + (j + k) * p.par.sc) - p.rate * r;
-    store_elem(p.out, o + k, r);
+      for (int k = 0; k < 8; ++k) v[8 * u + k] -= __half2float(__float2half_rn(v[8 * u + k]));
+      st_shared(unit(lo, r, half * 4 + u), pack_h8(v + 8 * u));
+    }
+  } else {
+    // 32 floats in the place of this thread's hi and lo
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint4 w = make_uint4(__float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]), __float_as_uint(v[4 * u + 2]),
+                                 __float_as_uint(v[4 * u + 3]));
+      st_shared(unit(u < 4 ? set : lo, r, half * 4 + (u & 3)), w);
+    }
   }
 }
 
-// C = P Q' tile by tile: one CTA per SM walks 128 x 128 tiles; a thread loads
-// k-slices of both operands by TMA into a ring, a thread issues the matrix
-// instructions into one of two accumulators, four warps finish the other.
-template <bool P_MN, bool Q_MN, int MODE>
-__global__ void __launch_bounds__(kThreads, 1) product(const __grid_constant__ ProductP p) {
-  constexpr bool SYM = MODE == GRAM || MODE == POLY;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done[2], freed[2], drain;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int s_abort;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5;
-  const int ti_count = (p.I + kT - 1) / kT, tj_count = (p.J + kT - 1) / kT;
-  const int per = SYM ? ti_count * (ti_count + 1) / 2 : ti_count * tj_count;
-  const int64_t tiles = static_cast<int64_t>(per) * p.E;
-  const int ks = (p.K + kTileK - 1) / kTileK;
+// The last step's chunk, 32 floats a thread in shared memory, to the caller's
+// tensors: a warp a row, lanes along it.
+template <int MODE>
+__device__ __forceinline__ void write_out(const ChainP& p, uint32_t set, int e, int i0, int j0, int warp) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int r = warp; r < kRows; r += kEpiWarps) {
+    const int i = i0 + r;
+    if (i >= p.m) break;
+    const int64_t o = static_cast<int64_t>(e) * p.out.sb + static_cast<int64_t>(i) * p.out.sr;
+    const int64_t q = static_cast<int64_t>(e) * p.par.sb + static_cast<int64_t>(i) * p.par.sr;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = j0 + 32 * h + lane;
+      if (j >= p.n) continue;
+      float v = ld_shared_f(unit(lane < 16 ? set : set + kSet / 2, r, h * 4 + ((lane & 15) >> 2)) + (lane & 3) * 4);
+      v *= 1.0f / kXScale;
+      if (MODE == UPDATE) v = p.keep * load_elem(p.par, q + static_cast<int64_t>(j) * p.par.sc) - p.rate * v;
+      store_elem(p.out, o + j, v);
+    }
+  }
+}
 
+// Every wait below is bounded (mbar_wait); after one runs out the block's
+// roles leave their loops, and so do the other blocks at the grid barrier.
+
+// The loading thread: both operands' k-slices of every work item, in order.
+template <int CG>
+__device__ __forceinline__ bool load_phase(const ChainP& p, Shared& sh, uint32_t smem, int mode, int cur, int rank,
+                                           int64_t& n) {
+  const Work<CG> w(p, mode);
+  const bool p_mn = mode == GRAM && p.tall, q_mn = mode == GRAM ? p.tall : mode >= STEP && !p.tall;
+  const CUtensorMap* mp = mode == GRAM ? (p.tall ? &p.xm[cur] : &p.xk[cur])
+                          : mode == POLY ? &p.ak : p.tall ? &p.xk[cur] : &p.bk;
+  const CUtensorMap* mq = mode == GRAM ? mp : mode == POLY ? &p.ak : p.tall ? &p.bk : &p.xm[cur];
+  volatile int* const abort_flag = &sh.abort;
+  for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG) {
+    int e, ti, tj, z;
+    w.at(t, e, ti, tj, z);
+    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.TN + rank * 128;
+    for (int k = w.k_begin(z); k < w.k_begin(z + 1); ++k, ++n) {
+      const int st = static_cast<int>(n % kStages);
+      if (n >= kStages && !mbar_wait(&sh.empty[st], static_cast<uint32_t>(n / kStages - 1) & 1, p.err)) return false;
+      if (*abort_flag) return false;
+      const uint32_t sp = smem + st * kStageBytes, sq = sp + kOperand;
+      if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], CG * kStageBytes);
+      if (p_mn) {
+        tma_load_3d<CG>(sp, mp, &sh.full[st], i0, k * kTileK, e);
+        tma_load_3d<CG>(sp + kOperand / 2, mp, &sh.full[st], i0 + 64, k * kTileK, e);
+      } else {
+        tma_load_3d<CG>(sp, mp, &sh.full[st], k * kTileK, i0, e);
+      }
+      if (q_mn) {
+        tma_load_3d<CG>(sq, mq, &sh.full[st], j0, k * kTileK, e);
+        tma_load_3d<CG>(sq + kOperand / 2, mq, &sh.full[st], j0 + 64, k * kTileK, e);
+      } else {
+        tma_load_3d<CG>(sq, mq, &sh.full[st], k * kTileK, j0, e);
+      }
+    }
+  }
+  return true;
+}
+
+// The issuing thread (of a pair's first block): a work item's products into
+// one of two accumulators.
+template <int CG>
+__device__ __forceinline__ bool issue_phase(const ChainP& p, Shared& sh, uint32_t smem, uint32_t tmem, int mode,
+                                            int64_t& n, int64_t& c) {
+  const Work<CG> w(p, mode);
+  const bool p_mn = mode == GRAM && p.tall, q_mn = mode == GRAM ? p.tall : mode >= STEP && !p.tall;
+  const uint32_t idesc = instr_desc_f16(w.TM, w.TN, p_mn, q_mn);
+  const uint64_t ka = desc_k16(p_mn), kb = desc_k16(q_mn);
+  volatile int* const abort_flag = &sh.abort;
+  for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG, ++c) {
+    int e, ti, tj, z;
+    w.at(t, e, ti, tj, z);
+    const int acc = static_cast<int>(c & 1);
+    if (c >= 2 && !mbar_wait(&sh.freed[acc], static_cast<uint32_t>(c / 2 - 1) & 1, p.err)) return false;
+    tc_fence_after();
+    const uint32_t d = tmem + acc * w.TN;
+    const int k0 = w.k_begin(z), k1 = w.k_begin(z + 1);
+    for (int k = k0; k < k1; ++k, ++n) {
+      const int st = static_cast<int>(n % kStages);
+      if (*abort_flag || !mbar_wait(&sh.full[st], static_cast<uint32_t>(n / kStages) & 1, p.err)) return false;
+      tc_fence_after();
+      const uint32_t sp = smem + st * kStageBytes;
+      const uint64_t da = smem_desc(sp, p_mn), db = smem_desc(sp + kOperand, q_mn);
+#pragma unroll
+      for (int kk = 0; kk < kTileK / 16; ++kk)
+        mma_f16<CG>(d, da + kk * ka, db + kk * kb, idesc, k > k0 || kk > 0);
+      mma_commit<CG>(&sh.empty[st]);
+    }
+    mma_commit<CG>(&sh.done[acc]);
+  }
+  return true;
+}
+
+// A bounded wait that gives the block up when it runs out.  The epilogue's
+// warps never leave their loops early (they meet at barriers): once the block
+// is given up they run through them without waiting.
+__device__ __forceinline__ void wait_or_abort(uint64_t* bar, uint32_t parity, Shared& sh, int* err) {
+  volatile int* const abort_flag = &sh.abort;
+  if (!*abort_flag && !mbar_wait(bar, parity, err)) *abort_flag = 1;
+  __syncwarp();
+}
+
+// Wait until *count reaches `target` (bounded), or the call is given up.
+__device__ __forceinline__ bool wait_count(const ChainP& p, volatile unsigned* count, unsigned target) {
+  volatile unsigned* const given_up = p.counters + 1;
+  const long long t0 = clock64();
+  while (*count < target) {
+    if (*given_up) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      if (p.err) atomicOr(p.err, FRAG_DEVFLAG_WAIT_TIMEOUT);
+      atomicExch(p.counters + 1, 1u);
+      return false;
+    }
+  }
+  __threadfence();
+  return true;
+}
+
+// The epilogue warps.  `c` counts accumulators, `u` chunks (of shared memory).
+template <int CG, int MODE>
+__device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32_t sets, uint32_t tmem, int step,
+                                             int cur, int rank, int64_t& c, int64_t& u) {
+  const Work<CG> w(p, MODE);
+  const int ew = (threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
+  const int quad = (threadIdx.x >> 5) & 3, half = ew >> 2;  // accumulator lanes of this warp; columns of a chunk
+  const int r = quad * 32 + lane;
+  const bool lead = threadIdx.x == kLead;
+  volatile int* const abort_flag = &sh.abort;
+  // chunk v, columns j.. of rows i0.. of batch e: its set is free (the store
+  // of two chunks ago has read it) and its inputs are on their way
+  auto prepare = [&](int64_t v, int e, int i0, int j) {
+    const int b = static_cast<int>(v & 1);
+    const uint32_t set = sets + b * kSet;
+    if (*abort_flag) return;
+    if (MODE == GRAM) {
+      bulk_wait_read<1>();
+      mbar_arrive(&sh.aux[b]);
+    } else {
+      bulk_wait_read<0>();
+      mbar_arrive_expect_tx(&sh.aux[b], MODE == POLY ? kSet / 2 : kSet);
+      if (MODE == POLY) {
+        tma_load_3d<1>(set, &p.ak, &sh.aux[b], j, i0, e);
+      } else {
+        tma_load_3d<1>(set, &p.xk[cur], &sh.aux[b], j, i0, e);
+        tma_load_3d<1>(set + kSet / 2, &p.lo, &sh.aux[b], j, i0, e);
+      }
+    }
+    sh.aux_issued[b] = v + 1;
+  };
+  auto release = [&](int acc) {  // the accumulator is read: the next item's products may overwrite it
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) CG == 1 ? mbar_arrive(&sh.freed[acc]) : mbar_arrive_first(&sh.freed[acc]);
+  };
+  for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG, ++c) {
+    int e, ti, tj, z;
+    w.at(t, e, ti, tj, z);
+    const int acc = static_cast<int>(c & 1);
+    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.TN, i = i0 + r;
+    const int chunks = i0 < w.I ? min(w.TN / kChunk, (w.J - j0 + kChunk - 1) / kChunk) : 0;
+    const bool mirror = w.sym && ti != tj;
+    const uint32_t ta = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * w.TN + half * 32;
+    if (MODE != GRAM && lead && chunks > 0) prepare(u, e, i0, j0);
+    wait_or_abort(&sh.done[acc], static_cast<uint32_t>(c / 2) & 1, sh, p.err);
+    tc_fence_after();
+    const bool parts = MODE == GRAM && w.split > 1;
+    const float* part = nullptr;
+    if (parts) {
+      // This part's sums go out as columns of 128 rows; when all parts of the
+      // tile have arrived, each of its blocks finishes some of the chunks,
+      // adding the parts in order.
+      const int64_t tile = static_cast<int64_t>(t / w.split) * CG + rank;
+      part = p.partials + tile * w.split * (kRows * w.TN);
+      float* mine = p.partials + (tile * w.split + z) * (kRows * w.TN);
+      for (int g = 0; g < chunks; ++g) {
+        float v[32];
+        tmem_load32(ta + g * kChunk, v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) __stcg(mine + (g * kChunk + half * 32 + k) * kRows + r, v[k]);
+      }
+      release(acc);
+      __threadfence();
+      epi_sync();
+      if (lead) {
+        atomicAdd(p.counters + 2 + tile, 1u);
+        if (!wait_count(p, p.counters + 2 + tile, static_cast<unsigned>(w.split) * (step + 1))) *abort_flag = 1;
+      }
+      epi_sync();
+    }
+    const float2 dr = MODE >= STEP && !p.tall && i < p.m ? __ldcg(p.diag + static_cast<int64_t>(e) * p.s + i)
+                                                         : make_float2(0.f, 0.f);
+    for (int g = parts ? z : 0; g < chunks; g += parts ? w.split : 1, ++u) {
+      const int b = static_cast<int>(u & 1), j = j0 + g * kChunk;
+      const uint32_t set = sets + b * kSet;
+      if (lead) {
+        if (MODE == GRAM) prepare(u, e, i0, j);
+        else if (g + 1 < chunks) prepare(u + 1, e, i0, j + kChunk);
+      }
+      float v[32];
+      if (parts) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+        for (int q = 0; q < w.split; ++q) {
+          const float* from = part + (static_cast<int64_t>(q) * w.TN + g * kChunk + half * 32) * kRows + r;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] += __ldcg(from + k * kRows);
+        }
+      } else {
+        tmem_load32(ta + g * kChunk, v);
+        if (g == chunks - 1) release(acc);
+      }
+      wait_or_abort(&sh.aux[b], static_cast<uint32_t>(u / 2) & 1, sh, p.err);
+      finish32<MODE>(p, step, set, e, i, j + half * 32, r, half, mirror, dr, v);
+      if (MODE <= STEP) {
+        proxy_fence();
+        epi_sync();
+        if (lead) {
+          if (MODE == STEP) {
+            tma_store_3d(&p.xk[cur ^ 1], set, j, i0, e);
+            tma_store_3d(&p.lo, set + kSet / 2, j, i0, e);
+          } else {
+            tma_store_3d(MODE == GRAM ? &p.ak : &p.bk, set, j, i0, e);
+            if (mirror) {
+              const CUtensorMap* to = MODE == GRAM ? &p.a64 : &p.b64;
+              tma_store_3d(to, set + kSet / 2, i0, j, e);
+              if (i0 + 64 < w.I) tma_store_3d(to, set + kSet / 2 + kChunk * 128, i0 + 64, j, e);
+            }
+          }
+          bulk_commit();
+        }
+      } else {
+        epi_sync();
+        write_out<MODE>(p, set, e, i0, j, ew);
+        epi_sync();
+      }
+    }
+    if (chunks == 0 && !parts) release(acc);
+  }
+}
+
+// All steps in one launch: every block walks each phase's work items (A, then
+// B, then X), with a grid barrier between phases.  One block per SM; CG = 2:
+// pairs of blocks share 256 x 256 tiles, each holding half of the operands.
+template <int CG>
+__global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ ChainP p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) Shared sh;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sets = smem + kStages * kStageBytes;
+  const int warp = threadIdx.x >> 5;
+  const int rank = CG == 1 ? 0 : static_cast<int>(cluster_rank());
+  constexpr int kColumns = 2 * 128 * CG;
   if (threadIdx.x == 0) {
-    s_abort = 0;
+    sh.abort = 0;
+    sh.aux_issued[0] = sh.aux_issued[1] = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&done[i], 1);
-      mbar_init(&freed[i], 4);
+      mbar_init(&sh.done[i], 1);
+      mbar_init(&sh.freed[i], CG * kEpiWarps);
+      mbar_init(&sh.aux[i], 1);
     }
-    mbar_init(&drain, 1);
+    mbar_init(&sh.drain, 1);
     mbar_init_fence();
-    tma_prefetch_map(&p.mp);
-    tma_prefetch_map(&p.mq);
   }
-  if (warp == 1) tmem_alloc(&tmem_slot, 2 * kT);
+  if (warp == 1) tmem_alloc<CG>(&sh.tmem, kColumns);
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  volatile int* const abort_flag = &s_abort;
-
-  if (warp == 0) {
-    if (elect_one()) {
-      int64_t n = 0;  // k-slices issued
-      bool ok = true;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const int e = static_cast<int>(t / per);
-        int ti, tj;
-        tile_at<SYM>(static_cast<int>(t - static_cast<int64_t>(e) * per), tj_count, ti, tj);
-        for (int k = 0; k < ks; ++k, ++n) {
-          const int st = static_cast<int>(n % kStages);
-          if (n >= kStages && !mbar_wait(&empty[st], static_cast<uint32_t>(n / kStages - 1) & 1, p.err)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          if (*abort_flag) {
-            ok = false;
-            break;
-          }
-          const uint32_t sp = smem + st * kStageBytes, sq = sp + kStageBytes / 2;
-          mbar_arrive_expect_tx(&full[st], kStageBytes);
-          if (P_MN) {
-            tma_load_3d(sp, &p.mp, &full[st], ti * kT, k * kTileK, e);
-            tma_load_3d(sp + 64 * kTileK * 2, &p.mp, &full[st], ti * kT + 64, k * kTileK, e);
-          } else {
-            tma_load_3d(sp, &p.mp, &full[st], k * kTileK, ti * kT, e);
-          }
-          if (Q_MN) {
-            tma_load_3d(sq, &p.mq, &full[st], tj * kT, k * kTileK, e);
-            tma_load_3d(sq + 64 * kTileK * 2, &p.mq, &full[st], tj * kT + 64, k * kTileK, e);
-          } else {
-            tma_load_3d(sq, &p.mq, &full[st], k * kTileK, tj * kT, e);
-          }
+  const uint32_t tmem = sh.tmem;
+  volatile int* const abort_flag = &sh.abort;
+  const bool loads = warp == 0 && elect_one(), issues = warp == 1 && rank == 0 && elect_one();
+  int64_t n = 0, c = 0, u = 0;
+  unsigned phase = 0;
+  bool ok = true;
+  for (int step = 0; step < p.steps && ok; ++step) {
+    const int cur = step & 1;
+    for (int ph = 0; ph < 3; ++ph) {
+      const int mode = ph < STEP ? ph : step + 1 < p.steps ? static_cast<int>(STEP) : p.last;
+      bool good = true;
+      if (warp == 0) {
+        if (loads) good = load_phase<CG>(p, sh, smem, mode, cur, rank, n);
+      } else if (warp == 1) {
+        if (issues) good = issue_phase<CG>(p, sh, smem, tmem, mode, n, c);
+      } else {
+        switch (mode) {
+          case GRAM: finish_phase<CG, GRAM>(p, sh, sets, tmem, step, cur, rank, c, u); break;
+          case POLY: finish_phase<CG, POLY>(p, sh, sets, tmem, step, cur, rank, c, u); break;
+          case STEP: finish_phase<CG, STEP>(p, sh, sets, tmem, step, cur, rank, c, u); break;
+          case LAST: finish_phase<CG, LAST>(p, sh, sets, tmem, step, cur, rank, c, u); break;
+          default: finish_phase<CG, UPDATE>(p, sh, sets, tmem, step, cur, rank, c, u);
         }
+        if (threadIdx.x == kLead) bulk_wait<0>();  // this phase's stores are written
+        proxy_fence();
+        __threadfence();
       }
-      // every copy has landed before the block may end
-      for (int64_t i = n > kStages ? n - kStages : 0; i < n; ++i)
-        mbar_wait(&full[i % kStages], static_cast<uint32_t>(i / kStages) & 1, nullptr);
-    }
-  } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = instr_desc_f16(kT, kT, P_MN, Q_MN);
-      int64_t n = 0, c = 0;  // k-slices, tiles
-      bool ok = true;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++c) {
-        const int acc = static_cast<int>(c & 1);
-        if (c >= 2 && !mbar_wait(&freed[acc], static_cast<uint32_t>(c / 2 - 1) & 1, p.err)) ok = false;
-        tc_fence_after();
-        const uint32_t d = tmem + acc * kT;
-        for (int k = 0; k < ks && ok; ++k, ++n) {
-          const int st = static_cast<int>(n % kStages);
-          if (*abort_flag || !mbar_wait(&full[st], static_cast<uint32_t>(n / kStages) & 1, p.err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sp = smem + st * kStageBytes;
-          const uint64_t da = smem_desc<P_MN>(sp), db = smem_desc<Q_MN>(sp + kStageBytes / 2);
-#pragma unroll
-          for (int kk = 0; kk < kTileK / 16; ++kk)
-            mma_f16(d, da + kk * desc_k16<P_MN>(), db + kk * desc_k16<Q_MN>(), idesc, k > 0 || kk > 0);
-          mma_commit(&empty[st]);
-        }
-        if (ok) mma_commit(&done[acc]);
+      if (!good) *abort_flag = 1;
+      __syncthreads();
+      if (step + 1 == p.steps && ph == 2) break;
+      if (threadIdx.x == 0) {
+        // every block has finished the phase
+        ++phase;
+        if (*abort_flag) atomicExch(p.counters + 1, 1u);
+        __threadfence();
+        atomicAdd(p.counters, 1u);
+        if (!wait_count(p, p.counters, phase * gridDim.x)) *abort_flag = 1;
       }
-      if (!ok) *abort_flag = 1;
-      mma_commit(&drain);  // nothing is in flight when the accumulators are freed
-      mbar_wait(&drain, 0, p.err);
-    }
-  } else {
-    const int quad = warp & 3, lane = threadIdx.x & 31;
-    int64_t c = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++c) {
-      const int e = static_cast<int>(t / per);
-      int ti, tj;
-      tile_at<SYM>(static_cast<int>(t - static_cast<int64_t>(e) * per), tj_count, ti, tj);
-      const int acc = static_cast<int>(c & 1);
-      const bool ok = !*abort_flag && mbar_wait(&done[acc], static_cast<uint32_t>(c / 2) & 1, p.err);
-      if (!__all_sync(0xffffffffu, ok)) {
-        *abort_flag = 1;
+      __syncthreads();
+      proxy_fence();
+      if (*abort_flag) {
+        ok = false;
         break;
       }
-      tc_fence_after();
-      const int i = ti * kT + quad * 32 + lane;
-      for (int j0 = 0; j0 < kT; j0 += 32) {
-        float v[32];
-        tmem_load32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * kT + j0, v);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int j = tj * kT + j0 + 8 * g;
-          float u[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) u[k] = v[8 * g + k];
-          if (i < p.I && j < p.J) finish8<MODE>(p, e, i, j, u, SYM && tj < ti);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&freed[acc]);
     }
   }
+  // nothing is in flight when shared memory and accumulators are given up
+  if (loads)
+    for (int64_t i = n > kStages ? n - kStages : 0; i < n && rank == 0; ++i)
+      mbar_wait(&sh.full[i % kStages], static_cast<uint32_t>(i / kStages) & 1, nullptr);
+  if (threadIdx.x == kLead && *abort_flag)
+    for (int b = 0; b < 2; ++b)
+      if (sh.aux_issued[b]) mbar_wait(&sh.aux[b], static_cast<uint32_t>((sh.aux_issued[b] - 1) / 2) & 1, nullptr);
+  if (issues) mma_commit<CG>(&sh.drain);
+  if (warp == 1 && (rank == 0 ? issues : elect_one())) mbar_wait(&sh.drain, 0, p.err);
   __syncthreads();
+  if (CG == 2) cluster_sync();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_free(tmem, 2 * kT);
+    tmem_free<CG>(tmem, kColumns);
   }
 }
 
@@ -365,6 +637,8 @@ struct PrepP {
   __half* hi;
   __half* lo;
   float* partials;  // [E, blocks]
+  unsigned* counters;
+  int count;  // of them, cleared for the chain of products
 };
 
 // The matrix to be orthogonalised at (r, c): the gradient or the momentum's
@@ -380,6 +654,8 @@ __device__ __forceinline__ float prep_value(const PrepP& p, int64_t e, int64_t r
 __global__ void __launch_bounds__(256) prep_norm(const PrepP p) {
   __shared__ float slots[2][32];
   const int64_t e = blockIdx.y, total = p.rows * p.cols;
+  if (blockIdx.x == 0 && e == 0)
+    for (int i = threadIdx.x; i < p.count; i += blockDim.x) p.counters[i] = 0;
   float ss = 0.f;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -415,10 +691,44 @@ __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
 // -------------------------------------------------------------------- host
 
 struct Plan {
-  int64_t s, l, ldx, lds;
-  size_t hi0, hi1, lo, a, b, diag, partials, bytes;
-  int blocks;
+  int64_t s, l, ldx, lds, tiles;
+  size_t hi0, hi1, lo, a, b, diag, partials, sums, counters, bytes;
+  int blocks, pairs, groups, split, count;
 };
+
+// Blocks (or pairs of them) that are resident at once, one per SM.
+int resident(bool pairs) {
+  static std::mutex mu;
+  static int cache[64][2] = {};
+  const int d = current_device();
+  if (d < 0 || d >= 64) return 0;
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = cache[d][pairs];
+  if (n) return n;
+  if (!pairs) return n = sm_count();
+  if (!allow_dynamic_smem(reinterpret_cast<const void*>(chain<2>), kSmem)) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sm_count());
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, chain<2>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n = std::min(clusters, sm_count() / 2);
+}
+
+int64_t chain_tiles(int64_t E, int64_t rows, int64_t cols, int64_t side, bool sym) {
+  const int64_t ti = ceil_div(rows, side), tj = ceil_div(cols, side);
+  return E * (sym ? ti * (ti + 1) / 2 : ti * tj);
+}
 
 Plan make_plan(int64_t E, int64_t m, int64_t n) {
   Plan q;
@@ -426,9 +736,20 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.l = std::max(m, n);
   q.ldx = ceil_div(n, 8) * 8;
   q.lds = ceil_div(q.s, 8) * 8;
+  // Pairs of blocks and 256 x 256 tiles where X has enough of them to keep the
+  // pairs busy; single blocks and 128 x 128 tiles below.
+  q.pairs = resident(true) > 0 && chain_tiles(E, m, n, 256, false) >= resident(true) / 2;
+  q.groups = resident(q.pairs);
+  const int64_t side = q.pairs ? 256 : 128;
+  q.tiles = chain_tiles(E, q.s, q.s, side, true);
+  // A's few tiles with a long k: each in `split` parts of at least four
+  // k-slices, one work item a group.
+  const int64_t ks = ceil_div(q.l, kTileK);
+  q.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({q.groups / std::max<int64_t>(1, q.tiles), ks / 4, 8})));
   const size_t x = align_up(static_cast<size_t>(E) * m * q.ldx * 2, 256);
   const size_t a = align_up(static_cast<size_t>(E) * q.s * q.lds * 2, 256);
   q.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(1024, ceil_div(m * n, 4096))));
+  q.count = 2 + (q.split > 1 ? static_cast<int>(q.tiles) * (q.pairs ? 2 : 1) : 0);
   q.hi0 = 0;
   q.hi1 = x;
   q.lo = 2 * x;
@@ -436,107 +757,89 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.b = q.a + a;
   q.diag = q.b + a;
   q.partials = q.diag + align_up(static_cast<size_t>(E) * q.s * sizeof(float2), 256);
-  q.bytes = q.partials + align_up(static_cast<size_t>(E) * q.blocks * sizeof(float), 256);
+  q.counters = q.partials + align_up(static_cast<size_t>(E) * q.blocks * sizeof(float), 256);
+  q.sums = q.counters + align_up(static_cast<size_t>(q.count) * sizeof(unsigned), 256);
+  q.bytes = q.sums + (q.split > 1 ? static_cast<size_t>(q.tiles) * q.split * side * side * sizeof(float) : 0);
   return q;
 }
 
-template <bool P_MN, bool Q_MN, int MODE>
-int launch_product(const ProductP& p, cudaStream_t s) {
-  auto kern = product<P_MN, Q_MN, MODE>;
+template <int CG>
+int launch_chain(const ChainP& p, int groups, cudaStream_t s) {
+  auto kern = chain<CG>;
   if (!allow_dynamic_smem(reinterpret_cast<const void*>(kern), kSmem)) return FRAG_ERR_CUDA;
-  const int64_t ti = ceil_div(p.I, kT), tj = ceil_div(p.J, kT);
-  const int64_t tiles = p.E * ((MODE == GRAM || MODE == POLY) ? ti * (ti + 1) / 2 : ti * tj);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, std::max(1, sm_count()))));
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * CG));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeCooperative;  // the grid barrier needs every block resident
+  attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = CG == 1 ? 1 : 2;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_t n, int steps, const float* co,
                   Elem out, const Elem* par, float keep, float rate, unsigned char* ws, cudaStream_t s) {
+  if (q.groups <= 0) return FRAG_ERR_NO_DEVICE;
   PrepP pp = prep;
   pp.hi = reinterpret_cast<__half*>(ws + q.hi0);
   pp.lo = reinterpret_cast<__half*>(ws + q.lo);
   pp.partials = reinterpret_cast<float*>(ws + q.partials);
-  const dim3 grid(static_cast<unsigned>(q.blocks), static_cast<unsigned>(E));
-  prep_norm<<<grid, 256, 0, s>>>(pp);
-  prep_scale<<<grid, 256, 0, s>>>(pp, q.blocks);
-  int st = check_launch();
-  if (st != FRAG_OK) return st;
-
-  const bool tall = m > n;
-  __half* hi[2] = {reinterpret_cast<__half*>(ws + q.hi0), reinterpret_cast<__half*>(ws + q.hi1)};
+  pp.counters = reinterpret_cast<unsigned*>(ws + q.counters);
+  pp.count = q.count;
+  ChainP p = {};
+  __half* hi[2] = {pp.hi, reinterpret_cast<__half*>(ws + q.hi1)};
   __half* A = reinterpret_cast<__half*>(ws + q.a);
   __half* B = reinterpret_cast<__half*>(ws + q.b);
-  CUtensorMap xk[2], xm[2], ak, bk;  // X along its rows, X across them, A, B
+  bool maps = make_map_3d(&p.lo, pp.lo, n, m, E, q.ldx, m * q.ldx, kChunk, kRows);
   for (int i = 0; i < 2; ++i)
-    if (!make_map_3d(&xk[i], hi[i], n, m, E, q.ldx, m * q.ldx, kTileK, kT) ||
-        !make_map_3d(&xm[i], hi[i], n, m, E, q.ldx, m * q.ldx, 64, kTileK))
-      return FRAG_ERR_CUDA;
-  if (!make_map_3d(&ak, A, q.s, q.s, E, q.lds, q.s * q.lds, kTileK, kT) ||
-      !make_map_3d(&bk, B, q.s, q.s, E, q.lds, q.s * q.lds, kTileK, kT))
-    return FRAG_ERR_CUDA;
-
-  ProductP p = {};
+    maps = maps && make_map_3d(&p.xk[i], hi[i], n, m, E, q.ldx, m * q.ldx, kTileK, kRows) &&
+           make_map_3d(&p.xm[i], hi[i], n, m, E, q.ldx, m * q.ldx, 64, kTileK);
+  maps = maps && make_map_3d(&p.ak, A, q.s, q.s, E, q.lds, q.s * q.lds, kTileK, kRows) &&
+         make_map_3d(&p.bk, B, q.s, q.s, E, q.lds, q.s * q.lds, kTileK, kRows) &&
+         make_map_3d(&p.a64, A, q.s, q.s, E, q.lds, q.s * q.lds, 64, 64) &&
+         make_map_3d(&p.b64, B, q.s, q.s, E, q.lds, q.s * q.lds, 64, 64);
+  if (!maps) return FRAG_ERR_CUDA;
+  p.m = static_cast<int>(m);
+  p.n = static_cast<int>(n);
+  p.s = static_cast<int>(q.s);
+  p.l = static_cast<int>(q.l);
   p.E = static_cast<int>(E);
-  p.tall = tall;
-  p.ldc = q.lds;
-  p.ldx = q.ldx;
-  p.a = A;
+  p.tall = m > n;
+  p.steps = steps;
+  p.split = q.split;
   p.diag = reinterpret_cast<float2*>(ws + q.diag);
-  p.lo = pp.lo;
+  p.partials = reinterpret_cast<float*>(ws + q.sums);
+  p.counters = pp.counters;
+  p.last = par ? UPDATE : LAST;
   p.out = out;
   if (par) p.par = *par;
   p.keep = keep;
   p.rate = rate;
   p.err = device_error_word();
-  for (int k = 0; k < steps; ++k) {
-    const int cur = k & 1;
-    p.ca = co[3 * k];
-    p.cb = co[3 * k + 1];
-    p.cc = co[3 * k + 2];
-    p.lo_factor = k >= steps - 2 ? 1.0f : 0.0f;
-    p.I = p.J = static_cast<int>(q.s);
-    p.K = static_cast<int>(q.l);
-    p.c = A;
-    p.mp = p.mq = tall ? xm[cur] : xk[cur];
-    st = tall ? launch_product<true, true, GRAM>(p, s) : launch_product<false, false, GRAM>(p, s);
-    if (st != FRAG_OK) return st;
-    p.K = static_cast<int>(q.s);
-    p.c = B;
-    p.mp = p.mq = ak;
-    st = launch_product<false, false, POLY>(p, s);
-    if (st != FRAG_OK) return st;
-    p.I = static_cast<int>(m);
-    p.J = static_cast<int>(n);
-    p.hi = hi[cur];
-    p.hi_out = hi[cur ^ 1];
-    p.mp = tall ? xk[cur] : bk;
-    p.mq = tall ? bk : xm[cur];
-    const int mode = k + 1 < steps ? STEP : par ? UPDATE : LAST;
-    if (tall)
-      st = mode == STEP ? launch_product<false, false, STEP>(p, s)
-           : mode == LAST ? launch_product<false, false, LAST>(p, s)
-                          : launch_product<false, false, UPDATE>(p, s);
-    else
-      st = mode == STEP ? launch_product<false, true, STEP>(p, s)
-           : mode == LAST ? launch_product<false, true, LAST>(p, s)
-                          : launch_product<false, true, UPDATE>(p, s);
-    if (st != FRAG_OK) return st;
-  }
-  return FRAG_OK;
+  for (int i = 0; i < 3 * steps; ++i) p.co[i] = co[i];
+
+  const dim3 grid(static_cast<unsigned>(q.blocks), static_cast<unsigned>(E));
+  prep_norm<<<grid, 256, 0, s>>>(pp);
+  prep_scale<<<grid, 256, 0, s>>>(pp, q.blocks);
+  const int st = check_launch();
+  if (st != FRAG_OK) return st;
+  // no more groups than the busiest phase has items
+  const int64_t side = q.pairs ? 256 : 128;
+  const int64_t most = std::max<int64_t>(q.tiles * q.split, chain_tiles(E, m, n, side, false));
+  const int groups = static_cast<int>(std::min<int64_t>(q.groups, most));
+  return q.pairs ? launch_chain<2>(p, groups, s) : launch_chain<1>(p, groups, s);
 }
 
 int check_sizes(int64_t E, int64_t m, int64_t n, int steps, const float* co) {
   if (E < 0 || m < 0 || n < 0 || steps < 1 || !co) return FRAG_ERR_INVALID_ARG;
-  if (m > (1 << 30) || n > (1 << 30) || E > 65535) return FRAG_ERR_SHAPE;
+  if (m > (1 << 24) || n > (1 << 24) || E > 65535 || steps > kMaxSteps) return FRAG_ERR_SHAPE;
+  if (m > 0 && n > 0 && chain_tiles(E, m, n, 128, false) > (1 << 24)) return FRAG_ERR_SHAPE;
   return FRAG_OK;
 }
 

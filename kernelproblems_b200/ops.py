@@ -1081,8 +1081,8 @@ def _matrices(t: torch.Tensor, name: str, dev: torch.device | None = None, shape
 
 def _schedule(steps: int, coefficients):
     """The C array of `steps` triples: one triple for all, or one for each."""
-    if not isinstance(steps, int) or steps < 1:
-        raise ValueError("steps must be a positive integer")
+    if not isinstance(steps, int) or not 1 <= steps <= 32:
+        raise ValueError("steps must be an integer from 1 to 32")
     rows = list(coefficients)
     if len(rows) == 3 and all(isinstance(c, (int, float)) for c in rows):
         rows = [rows] * steps
