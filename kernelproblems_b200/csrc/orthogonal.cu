@@ -80,9 +80,10 @@ constexpr int kOperand = 128 * kTileK * 2;  // bytes of one operand of a stage
 constexpr int kStageBytes = 2 * kOperand;
 constexpr int kStages = 4;
 constexpr int kSet = 2 * kRows * kChunk * 2;  // two 16-bit chunks
+constexpr int kSets = 3;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;  // a loading warp, an issuing warp, the epilogue
-constexpr int kSmem = kStages * kStageBytes + 2 * kSet + 1024;
+// a loading warp, an issuing warp, the epilogue, and a warp that moves its chunks
+constexpr int kThreads = 64 + 32 * kEpiWarps + 32;
 
 // GRAM A = X X', POLY B = b A + c A A, STEP X <- a X + B X; the last step's
 // STEP writes the result (LAST) or the weights (UPDATE) instead of X.
@@ -117,15 +118,6 @@ struct ChainP {
   float co[3 * kMaxSteps];
 };
 
-__device__ __forceinline__ void unpack_h8(const uint4& v, float* f) {
-  const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = __half22float2(h[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
 __device__ __forceinline__ uint4 pack_h8(const float* f) {
   uint4 v;
   __half2* h = reinterpret_cast<__half2*>(&v);
@@ -191,91 +183,109 @@ struct Work {
       ti = t - tj * ti_count;
     }
   }
+  // Chunks of the block's rows from i0 on in the tile's columns from j0 on.
+  __device__ int chunks(int i0, int j0) const {
+    return i0 < I ? min(TN / kChunk, (J - j0 + kChunk - 1) / kChunk) : 0;
+  }
   __device__ int k_begin(int z) const { return static_cast<int>(static_cast<int64_t>(ks) * z / split); }
 };
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory"); }
 
-struct Shared {
-  uint64_t full[kStages], empty[kStages], done[2], freed[2], aux[2], drain;
-  int64_t aux_issued[2];  // the last chunk prepared in each set, plus one
+struct __align__(16) Shared {
+  uint64_t full[kStages], empty[kStages], done[2], freed[2], aux[kSets], written[kSets], drain;
+  alignas(16) float2 cols[kEpiWarps][32];  // a tall matrix's factors of a warp's 32 columns
   uint32_t tmem;
   int abort;
 };
-constexpr int kLead = 64;  // the epilogue's thread that moves chunks
+constexpr int kSmem = kStages * kStageBytes + kSets * kSet + sizeof(Shared);
+static_assert(kSmem <= 227 * 1024, "a block's shared memory");
+constexpr int kLead = 64;  // the epilogue's first thread
 
 // The epilogue's view: what it does with 32 accumulator columns of one row of
 // a chunk.  `set` is the chunk's 32 KB of shared memory: hi and lo (STEP), A
 // (POLY), overwritten by the results that a bulk store then takes.
+//
+// X's element becomes  ca (hi + lo) + (acc + d_res hi + f d lo) / 2^10
+//                    = acc / 2^10 + hi (ca + d_res / 2^10) + lo (ca + f d / 2^10):
+// two factors for a row (`coef`), or for a column when the matrix is tall
+// (`cols`, this warp's 32 of them in shared memory).
 template <int MODE>
 __device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set, int e, int i, int j, int r, int half,
-                                         bool mirror, float2 dr, float (&v)[32]) {
+                                         bool mirror, float2 coef, const float4* cols, float (&v)[32]) {
   const uint32_t lo = set + kSet / 2;
   if (MODE == GRAM || MODE == POLY) {
     if (MODE == GRAM) {
 #pragma unroll
       for (int k = 0; k < 32; ++k) v[k] *= kAScale / (kXScale * kXScale);
     } else {
-      const float cb = p.co[3 * step + 1], cc = p.co[3 * step + 2] / kAScale;
+      const float2 cb = make_float2(p.co[3 * step + 1], p.co[3 * step + 1]);
+      const float2 cc = make_float2(p.co[3 * step + 2] / kAScale, p.co[3 * step + 2] / kAScale);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        float a[8];
-        unpack_h8(ld_shared(unit(set, r, half * 4 + u)), a);
+        const uint4 a = ld_shared(unit(set, r, half * 4 + u));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[8 * u + k] = cb * a[k] + cc * v[8 * u + k];
+        for (int q = 0; q < 4; ++q) {
+          float2* f = reinterpret_cast<float2*>(v + 8 * u + 2 * q);
+          const uint32_t w = u4_word(a, q);
+          *f = __ffma2_rn(*f, cc, __fmul2_rn(cb, __half22float2(*reinterpret_cast<const __half2*>(&w))));
+        }
       }
       if (i >= j && i < j + 32 && i < p.s) {
         float d = 0.f;
 #pragma unroll
         for (int k = 0; k < 32; ++k) d = j + k == i ? v[k] : d;
         p.diag[static_cast<int64_t>(e) * p.s + i] = make_float2(d, d - __half2float(__float2half_rn(d)));
+        __threadfence();
       }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) st_shared(unit(set, r, half * 4 + u), pack_h8(v + 8 * u));
     if (mirror) {
       // the transposed chunk, 64 rows of 128: two boxes of 64 columns
-      const uint32_t box = lo + (r >> 6) * (kChunk * 128);
-      const int c = r & 63;
+      const uint32_t box = lo + (r >> 6) * (kChunk * 128) + half * 32 * 128 + (r & 7) * 2;
+      const int c = (r & 63) >> 3;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const int jr = half * 32 + k;
-        st_shared_h(unit(box, jr, c >> 3) + (c & 7) * 2, __float2half_rn(v[k]));
-      }
+      for (int k = 0; k < 32; ++k) st_shared_h(unit(box, k, c), __float2half_rn(v[k]));
     }
     return;
   }
-  const float ca = p.co[3 * step];
-  const float lf = step >= p.steps - 2 ? 1.0f / kAScale : 0.0f;  // the diagonal's product with lo
-  float2 dc = dr;
-  if (p.tall) {  // column j + lane's, handed round below
-    const int col = j + (threadIdx.x & 31);
-    dc = col < p.n ? __ldcg(p.diag + static_cast<int64_t>(e) * p.s + col) : make_float2(0.f, 0.f);
-  }
+  const float2 scale = make_float2(1.0f / kAScale, 1.0f / kAScale);
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    float h[8], l[8];
-    unpack_h8(ld_shared(unit(set, r, half * 4 + u)), h);
-    unpack_h8(ld_shared(unit(lo, r, half * 4 + u)), l);
+    const uint32_t ah = unit(set, r, half * 4 + u), al = unit(lo, r, half * 4 + u);
+    const uint4 h = ld_shared(ah), l = ld_shared(al);
+    uint4 oh, ol;
+    uint32_t* const wh = reinterpret_cast<uint32_t*>(&oh);
+    uint32_t* const wl = reinterpret_cast<uint32_t*>(&ol);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float2 d = dr;
+    for (int q = 0; q < 4; ++q) {
+      float2 ch = make_float2(coef.x, coef.x), cl = make_float2(coef.y, coef.y);
       if (p.tall) {
-        d.x = __shfl_sync(0xffffffffu, dc.x, 8 * u + k);
-        d.y = __shfl_sync(0xffffffffu, dc.y, 8 * u + k);
+        const float4 t = cols[4 * u + q];
+        ch = make_float2(t.x, t.z);
+        cl = make_float2(t.y, t.w);
       }
-      v[8 * u + k] = ca * (h[k] + l[k]) + (v[8 * u + k] + d.y * h[k]) * (1.0f / kAScale) + lf * (d.x * l[k]);
+      const uint32_t hw = u4_word(h, q), lw = u4_word(l, q);
+      float2* f = reinterpret_cast<float2*>(v + 8 * u + 2 * q);
+      float2 y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hw)), ch, __fmul2_rn(*f, scale));
+      y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lw)), cl, y);
+      if (MODE == STEP) {
+        const __half2 hi = __float22half2_rn(y);
+        const float2 back = __half22float2(hi);
+        const __half2 rest = __float22half2_rn(make_float2(y.x - back.x, y.y - back.y));
+        wh[q] = *reinterpret_cast<const uint32_t*>(&hi);
+        wl[q] = *reinterpret_cast<const uint32_t*>(&rest);
+      } else {
+        *f = y;
+      }
+    }
+    if (MODE == STEP) {
+      st_shared(ah, oh);
+      st_shared(al, ol);
     }
   }
-  if (MODE == STEP) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      st_shared(unit(set, r, half * 4 + u), pack_h8(v + 8 * u));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[8 * u + k] -= __half2float(__float2half_rn(v[8 * u + k]));
-      st_shared(unit(lo, r, half * 4 + u), pack_h8(v + 8 * u));
-    }
-  } else {
+  if (MODE != STEP) {
     // 32 floats in the place of this thread's hi and lo
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -286,26 +296,22 @@ __device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set
   }
 }
 
-// The last step's chunk, 32 floats a thread in shared memory, to the caller's
-// tensors: a warp a row, lanes along it.
+// The last step's 32 rows and 32 columns of a warp, 32 floats a thread in
+// shared memory, to the caller's tensors: row by row, lanes along it.
 template <int MODE>
-__device__ __forceinline__ void write_out(const ChainP& p, uint32_t set, int e, int i0, int j0, int warp) {
+__device__ __forceinline__ void write_out(const ChainP& p, uint32_t set, int e, int i0, int j, int r0, int half) {
   const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int r = warp; r < kRows; r += kEpiWarps) {
-    const int i = i0 + r;
-    if (i >= p.m) break;
-    const int64_t o = static_cast<int64_t>(e) * p.out.sb + static_cast<int64_t>(i) * p.out.sr;
-    const int64_t q = static_cast<int64_t>(e) * p.par.sb + static_cast<int64_t>(i) * p.par.sr;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = j0 + 32 * h + lane;
-      if (j >= p.n) continue;
-      float v = ld_shared_f(unit(lane < 16 ? set : set + kSet / 2, r, h * 4 + ((lane & 15) >> 2)) + (lane & 3) * 4);
-      v *= 1.0f / kXScale;
-      if (MODE == UPDATE) v = p.keep * load_elem(p.par, q + static_cast<int64_t>(j) * p.par.sc) - p.rate * v;
-      store_elem(p.out, o + j, v);
-    }
+  const int col = j + lane, rows = min(32, p.m - i0);
+  if (col >= p.n) return;
+  const uint32_t from = lane < 16 ? set : set + kSet / 2;
+  const int64_t o = static_cast<int64_t>(e) * p.out.sb + static_cast<int64_t>(i0) * p.out.sr + col;
+  const int64_t q = static_cast<int64_t>(e) * p.par.sb + static_cast<int64_t>(i0) * p.par.sr +
+                    static_cast<int64_t>(col) * p.par.sc;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    float v = ld_shared_f(unit(from, r0 + r, half * 4 + ((lane & 15) >> 2)) + (lane & 3) * 4) * (1.0f / kXScale);
+    if (MODE == UPDATE) v = p.keep * load_elem(p.par, q + r * p.par.sr) - p.rate * v;
+    store_elem(p.out, o + r * p.out.sr, v);
   }
 }
 
@@ -408,51 +414,119 @@ __device__ __forceinline__ bool wait_count(const ChainP& p, volatile unsigned* c
   return true;
 }
 
-// The epilogue warps.  `c` counts accumulators, `u` chunks (of shared memory).
+// Walks the chunks that this block finishes in a phase, in the order of its
+// work items.
+template <int CG>
+struct Cursor {
+  const Work<CG>& w;
+  const int rank;
+  int t, g, step, chunks, e, i0, j0;
+  bool mirror;
+  __device__ Cursor(const Work<CG>& w_, int rank_) : w(w_), rank(rank_), t(blockIdx.x / CG) { item(); }
+  __device__ void item() {
+    for (; t < w.items; t += gridDim.x / CG) {
+      int ti, tj, z;
+      w.at(t, e, ti, tj, z);
+      i0 = ti * w.TM + rank * kRows;
+      j0 = tj * w.TN;
+      chunks = w.chunks(i0, j0);
+      mirror = w.sym && ti != tj;
+      g = w.split > 1 ? z : 0;  // a tile in parts: each of its blocks finishes some chunks
+      step = w.split;
+      if (g < chunks) return;
+    }
+  }
+  __device__ bool valid() const { return t < w.items; }
+  __device__ void next() {
+    g += step;
+    if (g < chunks) return;
+    t += gridDim.x / CG;
+    item();
+  }
+  __device__ int col() const { return j0 + g * kChunk; }
+};
+
+// The moving thread: brings each chunk's inputs into one of three sets, two
+// chunks ahead of the epilogue, and stores its results.  `v` counts chunks.
+template <int CG>
+__device__ __forceinline__ void move_phase(const ChainP& p, Shared& sh, uint32_t sets, int mode, int cur, int rank,
+                                           int64_t& v) {
+  const Work<CG> w(p, mode);
+  volatile int* const abort_flag = &sh.abort;
+  int64_t ahead = v;
+  Cursor<CG> in(w, rank), out(w, rank);
+  auto bring = [&]() {
+    if (!in.valid() || *abort_flag) return;
+    uint64_t* const bar = &sh.aux[ahead % kSets];
+    const uint32_t set = sets + static_cast<uint32_t>(ahead % kSets) * kSet;
+    if (mode == GRAM) {
+      mbar_arrive(bar);  // nothing to bring: the set is free
+    } else {
+      mbar_arrive_expect_tx(bar, mode == POLY ? kSet / 2 : kSet);
+      tma_load_3d<1>(set, mode == POLY ? &p.ak : &p.xk[cur], bar, in.col(), in.i0, in.e);
+      if (mode != POLY) tma_load_3d<1>(set + kSet / 2, &p.lo, bar, in.col(), in.i0, in.e);
+    }
+    ++ahead;
+    in.next();
+  };
+  bring();
+  bring();
+  for (; out.valid(); ++v, out.next()) {
+    const uint32_t set = sets + static_cast<uint32_t>(v % kSets) * kSet;
+    if (*abort_flag || !mbar_wait(&sh.written[v % kSets], static_cast<uint32_t>(v / kSets) & 1, p.err)) {
+      *abort_flag = 1;
+      break;
+    }
+    if (mode == STEP) {
+      tma_store_3d(&p.xk[cur ^ 1], set, out.col(), out.i0, out.e);
+      tma_store_3d(&p.lo, set + kSet / 2, out.col(), out.i0, out.e);
+    } else if (mode < STEP) {
+      tma_store_3d(mode == GRAM ? &p.ak : &p.bk, set, out.col(), out.i0, out.e);
+      if (out.mirror) {
+        const CUtensorMap* to = mode == GRAM ? &p.a64 : &p.b64;
+        tma_store_3d(to, set + kSet / 2, out.i0, out.col(), out.e);
+        if (out.i0 + 64 < w.I) tma_store_3d(to, set + kSet / 2 + kChunk * 128, out.i0 + 64, out.col(), out.e);
+      }
+    }
+    bulk_commit();
+    bulk_wait_read<1>();  // the chunk before this one is out of its set
+    bring();
+  }
+  bulk_wait<0>();  // the phase's results are written
+  if (*abort_flag)  // no copy is left on its way into this block
+    for (int64_t i = ahead > kSets ? ahead - kSets : 0; i < ahead; ++i)
+      mbar_wait(&sh.aux[i % kSets], static_cast<uint32_t>(i / kSets) & 1, nullptr);
+}
+
+// The epilogue warps.  `c` counts accumulators, `u` chunks.
 template <int CG, int MODE>
 __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32_t sets, uint32_t tmem, int step,
-                                             int cur, int rank, int64_t& c, int64_t& u) {
+                                             int rank, int64_t& c, int64_t& u) {
   const Work<CG> w(p, MODE);
   const int ew = (threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
   const int quad = (threadIdx.x >> 5) & 3, half = ew >> 2;  // accumulator lanes of this warp; columns of a chunk
   const int r = quad * 32 + lane;
-  const bool lead = threadIdx.x == kLead;
   volatile int* const abort_flag = &sh.abort;
-  // chunk v, columns j.. of rows i0.. of batch e: its set is free (the store
-  // of two chunks ago has read it) and its inputs are on their way
-  auto prepare = [&](int64_t v, int e, int i0, int j) {
-    const int b = static_cast<int>(v & 1);
-    const uint32_t set = sets + b * kSet;
-    if (*abort_flag) return;
-    if (MODE == GRAM) {
-      bulk_wait_read<1>();
-      mbar_arrive(&sh.aux[b]);
-    } else {
-      bulk_wait_read<0>();
-      mbar_arrive_expect_tx(&sh.aux[b], MODE == POLY ? kSet / 2 : kSet);
-      if (MODE == POLY) {
-        tma_load_3d<1>(set, &p.ak, &sh.aux[b], j, i0, e);
-      } else {
-        tma_load_3d<1>(set, &p.xk[cur], &sh.aux[b], j, i0, e);
-        tma_load_3d<1>(set + kSet / 2, &p.lo, &sh.aux[b], j, i0, e);
-      }
-    }
-    sh.aux_issued[b] = v + 1;
-  };
   auto release = [&](int acc) {  // the accumulator is read: the next item's products may overwrite it
     tc_fence_before();
     __syncwarp();
     if (lane == 0) CG == 1 ? mbar_arrive(&sh.freed[acc]) : mbar_arrive_first(&sh.freed[acc]);
+  };
+  // hi's and lo's factors in row (or column) d of batch e; lo's meets the
+  // diagonal in the last two steps only
+  auto factors = [&](int e, int d) {
+    const float2 v = __ldcg(p.diag + static_cast<int64_t>(e) * p.s + d);
+    const float ca = p.co[3 * step];
+    return make_float2(ca + v.y * (1.0f / kAScale), step >= p.steps - 2 ? ca + v.x * (1.0f / kAScale) : ca);
   };
   for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG, ++c) {
     int e, ti, tj, z;
     w.at(t, e, ti, tj, z);
     const int acc = static_cast<int>(c & 1);
     const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.TN, i = i0 + r;
-    const int chunks = i0 < w.I ? min(w.TN / kChunk, (w.J - j0 + kChunk - 1) / kChunk) : 0;
+    const int chunks = w.chunks(i0, j0);
     const bool mirror = w.sym && ti != tj;
     const uint32_t ta = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * w.TN + half * 32;
-    if (MODE != GRAM && lead && chunks > 0) prepare(u, e, i0, j0);
     wait_or_abort(&sh.done[acc], static_cast<uint32_t>(c / 2) & 1, sh, p.err);
     tc_fence_after();
     const bool parts = MODE == GRAM && w.split > 1;
@@ -473,58 +547,58 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
       release(acc);
       __threadfence();
       epi_sync();
-      if (lead) {
+      if (threadIdx.x == kLead) {
         atomicAdd(p.counters + 2 + tile, 1u);
         if (!wait_count(p, p.counters + 2 + tile, static_cast<unsigned>(w.split) * (step + 1))) *abort_flag = 1;
       }
       epi_sync();
     }
-    const float2 dr = MODE >= STEP && !p.tall && i < p.m ? __ldcg(p.diag + static_cast<int64_t>(e) * p.s + i)
-                                                         : make_float2(0.f, 0.f);
+    float2 coef = make_float2(0.f, 0.f);
+    if (MODE >= STEP && !p.tall && i < p.m) coef = factors(e, i);
     for (int g = parts ? z : 0; g < chunks; g += parts ? w.split : 1, ++u) {
-      const int b = static_cast<int>(u & 1), j = j0 + g * kChunk;
+      const int b = static_cast<int>(u % kSets), j = j0 + g * kChunk;
       const uint32_t set = sets + b * kSet;
-      if (lead) {
-        if (MODE == GRAM) prepare(u, e, i0, j);
-        else if (g + 1 < chunks) prepare(u + 1, e, i0, j + kChunk);
-      }
       float v[32];
       if (parts) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = 0.f;
-        for (int q = 0; q < w.split; ++q) {
-          const float* from = part + (static_cast<int64_t>(q) * w.TN + g * kChunk + half * 32) * kRows + r;
+        const float* from = part + (g * kChunk + half * 32) * kRows + r;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] += __ldcg(from + k * kRows);
-        }
+        for (int k0 = 0; k0 < 32; k0 += 16)
+          for (int q0 = 0; q0 < w.split; q0 += 4) {
+            float f[4][16];  // loads of four parts in flight
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                f[q][k] = q0 + q < w.split
+                              ? __ldcg(from + (static_cast<int64_t>(q0 + q) * w.TN + k0 + k) * kRows) : 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int k = 0; k < 16; ++k) v[k0 + k] += f[q][k];
+          }
       } else {
         tmem_load32(ta + g * kChunk, v);
         if (g == chunks - 1) release(acc);
       }
-      wait_or_abort(&sh.aux[b], static_cast<uint32_t>(u / 2) & 1, sh, p.err);
-      finish32<MODE>(p, step, set, e, i, j + half * 32, r, half, mirror, dr, v);
-      if (MODE <= STEP) {
-        proxy_fence();
-        epi_sync();
-        if (lead) {
-          if (MODE == STEP) {
-            tma_store_3d(&p.xk[cur ^ 1], set, j, i0, e);
-            tma_store_3d(&p.lo, set + kSet / 2, j, i0, e);
-          } else {
-            tma_store_3d(MODE == GRAM ? &p.ak : &p.bk, set, j, i0, e);
-            if (mirror) {
-              const CUtensorMap* to = MODE == GRAM ? &p.a64 : &p.b64;
-              tma_store_3d(to, set + kSet / 2, i0, j, e);
-              if (i0 + 64 < w.I) tma_store_3d(to, set + kSet / 2 + kChunk * 128, i0 + 64, j, e);
-            }
-          }
-          bulk_commit();
-        }
-      } else {
-        epi_sync();
-        write_out<MODE>(p, set, e, i0, j, ew);
-        epi_sync();
+      if (MODE >= STEP && p.tall) {
+        const int col = j + half * 32 + lane;
+        __syncwarp();
+        sh.cols[ew][lane] = col < p.n ? factors(e, col) : coef;
+        __syncwarp();
       }
+      wait_or_abort(&sh.aux[b], static_cast<uint32_t>(u / kSets) & 1, sh, p.err);
+      finish32<MODE>(p, step, set, e, i, j + half * 32, r, half, mirror, coef,
+                     reinterpret_cast<const float4*>(sh.cols[ew]), v);
+      if (MODE <= STEP) {
+        proxy_fence_shared();
+      } else {
+        __syncwarp();
+        write_out<MODE>(p, set, e, i0 + quad * 32, j + half * 32, quad * 32, half);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.written[b]);
     }
     if (chunks == 0 && !parts) release(acc);
   }
@@ -535,16 +609,17 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
 // pairs of blocks share 256 x 256 tiles, each holding half of the operands.
 template <int CG>
 __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ ChainP p) {
+  // stages, sets, and the rest behind them: no static shared memory, so that
+  // the stages start on the swizzle's 1024 bytes
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ __align__(8) Shared sh;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  Shared& sh = *reinterpret_cast<Shared*>(smem_raw + kStages * kStageBytes + kSets * kSet);
+  const uint32_t smem = smem_u32(smem_raw);
   const uint32_t sets = smem + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5;
   const int rank = CG == 1 ? 0 : static_cast<int>(cluster_rank());
   constexpr int kColumns = 2 * 128 * CG;
   if (threadIdx.x == 0) {
     sh.abort = 0;
-    sh.aux_issued[0] = sh.aux_issued[1] = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
@@ -552,7 +627,10 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.done[i], 1);
       mbar_init(&sh.freed[i], CG * kEpiWarps);
+    }
+    for (int i = 0; i < kSets; ++i) {
       mbar_init(&sh.aux[i], 1);
+      mbar_init(&sh.written[i], kEpiWarps);
     }
     mbar_init(&sh.drain, 1);
     mbar_init_fence();
@@ -565,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
   const uint32_t tmem = sh.tmem;
   volatile int* const abort_flag = &sh.abort;
   const bool loads = warp == 0 && elect_one(), issues = warp == 1 && rank == 0 && elect_one();
-  int64_t n = 0, c = 0, u = 0;
+  const bool moves = warp == 2 + kEpiWarps && elect_one();
+  int64_t n = 0, c = 0, u = 0;  // k-slices, accumulators, chunks so far
   unsigned phase = 0;
   bool ok = true;
   for (int step = 0; step < p.steps && ok; ++step) {
@@ -577,17 +656,16 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
         if (loads) good = load_phase<CG>(p, sh, smem, mode, cur, rank, n);
       } else if (warp == 1) {
         if (issues) good = issue_phase<CG>(p, sh, smem, tmem, mode, n, c);
+      } else if (warp == 2 + kEpiWarps) {
+        if (moves) move_phase<CG>(p, sh, sets, mode, cur, rank, u);
       } else {
         switch (mode) {
-          case GRAM: finish_phase<CG, GRAM>(p, sh, sets, tmem, step, cur, rank, c, u); break;
-          case POLY: finish_phase<CG, POLY>(p, sh, sets, tmem, step, cur, rank, c, u); break;
-          case STEP: finish_phase<CG, STEP>(p, sh, sets, tmem, step, cur, rank, c, u); break;
-          case LAST: finish_phase<CG, LAST>(p, sh, sets, tmem, step, cur, rank, c, u); break;
-          default: finish_phase<CG, UPDATE>(p, sh, sets, tmem, step, cur, rank, c, u);
+          case GRAM: finish_phase<CG, GRAM>(p, sh, sets, tmem, step, rank, c, u); break;
+          case POLY: finish_phase<CG, POLY>(p, sh, sets, tmem, step, rank, c, u); break;
+          case STEP: finish_phase<CG, STEP>(p, sh, sets, tmem, step, rank, c, u); break;
+          case LAST: finish_phase<CG, LAST>(p, sh, sets, tmem, step, rank, c, u); break;
+          default: finish_phase<CG, UPDATE>(p, sh, sets, tmem, step, rank, c, u);
         }
-        if (threadIdx.x == kLead) bulk_wait<0>();  // this phase's stores are written
-        proxy_fence();
-        __threadfence();
       }
       if (!good) *abort_flag = 1;
       __syncthreads();
@@ -601,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
         if (!wait_count(p, p.counters, phase * gridDim.x)) *abort_flag = 1;
       }
       __syncthreads();
-      proxy_fence();
+      if (loads || moves) proxy_fence();
       if (*abort_flag) {
         ok = false;
         break;
@@ -612,9 +690,6 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
   if (loads)
     for (int64_t i = n > kStages ? n - kStages : 0; i < n && rank == 0; ++i)
       mbar_wait(&sh.full[i % kStages], static_cast<uint32_t>(i / kStages) & 1, nullptr);
-  if (threadIdx.x == kLead && *abort_flag)
-    for (int b = 0; b < 2; ++b)
-      if (sh.aux_issued[b]) mbar_wait(&sh.aux[b], static_cast<uint32_t>((sh.aux_issued[b] - 1) / 2) & 1, nullptr);
   if (issues) mma_commit<CG>(&sh.drain);
   if (warp == 1 && (rank == 0 ? issues : elect_one())) mbar_wait(&sh.drain, 0, p.err);
   __syncthreads();
@@ -641,51 +716,115 @@ struct PrepP {
   int count;  // of them, cleared for the chain of products
 };
 
+// V neighbouring elements of a row (V = 8: one 16- or two 16-byte accesses).
+template <int V>
+__device__ __forceinline__ void load_elems(const Elem& e, int64_t i, float (&f)[V]) {
+  if (V == 8 && e.f32) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(e.p) + i));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(e.p) + i) + 1);
+    f[0] = a.x, f[1 % V] = a.y, f[2 % V] = a.z, f[3 % V] = a.w, f[4 % V] = b.x, f[5 % V] = b.y, f[6 % V] = b.z, f[7 % V] = b.w;
+  } else if (V == 8) {
+    const uint4 u = ld_cached(static_cast<const uint16_t*>(e.p) + i);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) f[2 * k] = bf16lo(u4_word(u, k)), f[(2 * k + 1) % V] = bf16hi(u4_word(u, k));
+  } else {
+    f[0] = load_elem(e, i);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_elems(const Elem& e, int64_t i, const float (&f)[V]) {
+  if (V == 8 && e.f32) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(e.p) + i);
+    o[0] = make_float4(f[0], f[1 % V], f[2 % V], f[3 % V]);
+    o[1] = make_float4(f[4 % V], f[5 % V], f[6 % V], f[7 % V]);
+  } else if (V == 8) {
+    uint4 u;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) w[k] = pack_bf16x2(f[2 * k], f[(2 * k + 1) % V]);
+    st_global(static_cast<uint16_t*>(e.p) + i, u);
+  } else {
+    store_elem(e, i, f[0]);
+  }
+}
+
 // The matrix to be orthogonalised at (r, c): the gradient or the momentum's
 // look-ahead; m' in `m`.
-__device__ __forceinline__ float prep_value(const PrepP& p, int64_t e, int64_t r, int64_t c, float& m) {
-  const float g = load_elem(p.g, e * p.g.sb + r * p.g.sr + c * p.g.sc);
-  if (!p.has_mom) return g;
-  m = p.mu * load_elem(p.mom, e * p.mom.sb + r * p.mom.sr + c * p.mom.sc) + (1.0f - p.mu) * g;
-  return p.nesterov ? p.mu * m + (1.0f - p.mu) * g : m;
+template <int V>
+__device__ __forceinline__ void prep_value(const PrepP& p, int64_t e, int64_t r, int64_t c, float (&u)[V],
+                                           float (&m)[V]) {
+  load_elems<V>(p.g, e * p.g.sb + r * p.g.sr + c * p.g.sc, u);
+  if (!p.has_mom) return;
+  load_elems<V>(p.mom, e * p.mom.sb + r * p.mom.sr + c * p.mom.sc, m);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const float g = (1.0f - p.mu) * u[k];
+    m[k] = p.mu * m[k] + g;
+    u[k] = p.nesterov ? p.mu * m[k] + g : m[k];
+  }
 }
 
 // Sums of squares, a block's in a fixed order.
+template <int V>
 __global__ void __launch_bounds__(256) prep_norm(const PrepP p) {
   __shared__ float slots[2][32];
-  const int64_t e = blockIdx.y, total = p.rows * p.cols;
+  const int64_t e = blockIdx.y;
+  const uint32_t per = static_cast<uint32_t>(p.cols / V);
+  const uint32_t total = static_cast<uint32_t>(p.rows * per), stride = gridDim.x * blockDim.x;
   if (blockIdx.x == 0 && e == 0)
     for (int i = threadIdx.x; i < p.count; i += blockDim.x) p.counters[i] = 0;
   float ss = 0.f;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / p.cols;
-    float m;
-    const float u = prep_value(p, e, r, i - r * p.cols, m);
-    ss = fmaf(u, u, ss);
+#pragma unroll 4
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const uint32_t r = i / per;
+    float u[V], m[V];
+    prep_value<V>(p, e, r, (i - r * per) * V, u, m);
+#pragma unroll
+    for (int k = 0; k < V; ++k) ss = fmaf(u[k], u[k], ss);
   }
   ss = block_sum(ss, slots, 0);
   if (threadIdx.x == 0) p.partials[e * gridDim.x + blockIdx.x] = ss;
 }
 
 // X = u / (|u| + eps) as hi + lo, and the new momentum.
+template <int V>
 __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
   __shared__ float slots[2][32];
-  const int64_t e = blockIdx.y, total = p.rows * p.cols;
+  const int64_t e = blockIdx.y;
+  const uint32_t per = static_cast<uint32_t>(p.cols / V);
+  const uint32_t total = static_cast<uint32_t>(p.rows * per), stride = gridDim.x * blockDim.x;
   float ss = 0.f;
   for (int i = threadIdx.x; i < blocks; i += blockDim.x) ss += p.partials[e * blocks + i];
   const float f = kXScale / (sqrtf(block_sum(ss, slots, 0)) + p.eps);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / p.cols, c = i - r * p.cols;
-    float m;
-    const float x = prep_value(p, e, r, c, m) * f;
-    if (p.has_mom) store_elem(p.mom_out, (e * p.rows + r) * p.cols + c, m);
-    const __half h = __float2half_rn(x);
+#pragma unroll 4
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const uint32_t r = i / per, c = (i - r * per) * V;
+    float u[V], m[V];
+    prep_value<V>(p, e, r, c, u, m);
+    if (p.has_mom) store_elems<V>(p.mom_out, (e * p.rows + r) * p.cols + c, m);
     const int64_t o = (e * p.rows + r) * p.ldx + c;
-    p.hi[o] = h;
-    p.lo[o] = __float2half_rn(x - __half2float(h));
+    if (V == 8) {
+      float l[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float x = u[k % V] * f;
+        u[k % V] = x;
+        l[k] = x - __half2float(__float2half_rn(x));
+      }
+      *reinterpret_cast<uint4*>(p.hi + o) = pack_h8(u);
+      *reinterpret_cast<uint4*>(p.lo + o) = pack_h8(l);
+    } else {
+      const float x = u[0] * f;
+      const __half h = __float2half_rn(x);
+      p.hi[o] = h;
+      p.lo[o] = __float2half_rn(x - __half2float(h));
+    }
   }
+}
+
+// Rows of whole 8-element chunks, aligned for 16-byte accesses.
+bool chunked(const Elem& e, int64_t E, int64_t rows, int64_t cols) {
+  return cols % 8 == 0 && e.sc == 1 && (rows == 1 || e.sr % 8 == 0) && (E == 1 || e.sb % 8 == 0) && aligned16(e.p);
 }
 
 // -------------------------------------------------------------------- host
@@ -736,19 +875,22 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.l = std::max(m, n);
   q.ldx = ceil_div(n, 8) * 8;
   q.lds = ceil_div(q.s, 8) * 8;
-  // Pairs of blocks and 256 x 256 tiles where X has enough of them to keep the
-  // pairs busy; single blocks and 128 x 128 tiles below.
-  q.pairs = resident(true) > 0 && chain_tiles(E, m, n, 256, false) >= resident(true) / 2;
+  // Pairs of blocks and 256 x 256 tiles where X has enough of them to keep three
+  // quarters of the pairs busy, single blocks and 128 x 128 tiles below.  A
+  // step, single against pairs: 1536 x 1536 (36 tiles) 46 and 53 us, 2048 x
+  // 2048 (64) 70 and 63, 4096 x 4096 405 and 270.
+  q.pairs = resident(true) > 0 && 4 * chain_tiles(E, m, n, 256, false) >= 3 * resident(true);
   q.groups = resident(q.pairs);
   const int64_t side = q.pairs ? 256 : 128;
   q.tiles = chain_tiles(E, q.s, q.s, side, true);
-  // A's few tiles with a long k: each in `split` parts of at least four
-  // k-slices, one work item a group.
+  // A's few tiles with a long k: each in up to four parts of at least four
+  // k-slices, one work item a group.  A step of 1024 x 4096 in 1, 2, 4 and 8
+  // parts: 63, 55, 49 and 49 us.
   const int64_t ks = ceil_div(q.l, kTileK);
-  q.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({q.groups / std::max<int64_t>(1, q.tiles), ks / 4, 8})));
+  q.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({q.groups / std::max<int64_t>(1, q.tiles), ks / 4, 4})));
   const size_t x = align_up(static_cast<size_t>(E) * m * q.ldx * 2, 256);
   const size_t a = align_up(static_cast<size_t>(E) * q.s * q.lds * 2, 256);
-  q.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(1024, ceil_div(m * n, 4096))));
+  q.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(1184, ceil_div(m * n, 2048))));
   q.count = 2 + (q.split > 1 ? static_cast<int>(q.tiles) * (q.pairs ? 2 : 1) : 0);
   q.hi0 = 0;
   q.hi1 = x;
@@ -825,8 +967,13 @@ int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_
   for (int i = 0; i < 3 * steps; ++i) p.co[i] = co[i];
 
   const dim3 grid(static_cast<unsigned>(q.blocks), static_cast<unsigned>(E));
-  prep_norm<<<grid, 256, 0, s>>>(pp);
-  prep_scale<<<grid, 256, 0, s>>>(pp, q.blocks);
+  if (chunked(pp.g, E, m, n) && (!pp.has_mom || (chunked(pp.mom, E, m, n) && chunked(pp.mom_out, E, m, n)))) {
+    prep_norm<8><<<grid, 256, 0, s>>>(pp);
+    prep_scale<8><<<grid, 256, 0, s>>>(pp, q.blocks);
+  } else {
+    prep_norm<1><<<grid, 256, 0, s>>>(pp);
+    prep_scale<1><<<grid, 256, 0, s>>>(pp, q.blocks);
+  }
   const int st = check_launch();
   if (st != FRAG_OK) return st;
   // no more groups than the busiest phase has items
@@ -839,7 +986,7 @@ int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_
 int check_sizes(int64_t E, int64_t m, int64_t n, int steps, const float* co) {
   if (E < 0 || m < 0 || n < 0 || steps < 1 || !co) return FRAG_ERR_INVALID_ARG;
   if (m > (1 << 24) || n > (1 << 24) || E > 65535 || steps > kMaxSteps) return FRAG_ERR_SHAPE;
-  if (m > 0 && n > 0 && chain_tiles(E, m, n, 128, false) > (1 << 24)) return FRAG_ERR_SHAPE;
+  if (m > 0 && n > 0 && (chain_tiles(E, m, n, 128, false) > (1 << 24) || m * n > 0x7fffffffLL)) return FRAG_ERR_SHAPE;
   return FRAG_OK;
 }
 
