@@ -23,13 +23,12 @@
 //    carries most of B's rounding error: its residual is kept in 32 bits and
 //    added in the epilogue, as is the diagonal's product with lo in the last
 //    two steps (earlier, lo along small directions would be amplified).
-#include <cuda_fp16.h>
 #include <math.h>
 
 #include <algorithm>
 #include <mutex>
 
-#include "tc.cuh"
+#include "orthogonal.cuh"
 
 namespace frag {
 
@@ -72,8 +71,6 @@ bool make_map_3d(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64
 
 namespace {
 
-constexpr float kXScale = 256.0f;   // X is kept times 2^8
-constexpr float kAScale = 1024.0f;  // A and B times 2^10
 constexpr int kRows = 128;          // rows of C a block holds
 constexpr int kChunk = 64;          // columns the epilogue takes at a time
 constexpr int kOperand = 128 * kTileK * 2;  // bytes of one operand of a stage
@@ -85,25 +82,6 @@ constexpr int kEpiWarps = 8;
 // a loading warp, an issuing warp, the epilogue, and a warp that moves its chunks
 constexpr int kThreads = 64 + 32 * kEpiWarps + 32;
 
-// GRAM A = X X', POLY B = b A + c A A, STEP X <- a X + B X; the last step's
-// STEP writes the result (LAST) or the weights (UPDATE) instead of X.
-enum Mode { GRAM = 0, POLY = 1, STEP = 2, LAST = 3, UPDATE = 4 };
-
-struct Elem {  // a tensor of bf16 or fp32 elements with strides
-  void* p;
-  int f32;
-  int64_t sb, sr, sc;
-};
-__device__ __forceinline__ float load_elem(const Elem& e, int64_t i) {
-  return e.f32 ? static_cast<const float*>(e.p)[i] : bf16_to_f(static_cast<const uint16_t*>(e.p)[i]);
-}
-__device__ __forceinline__ void store_elem(const Elem& e, int64_t i, float v) {
-  if (e.f32) static_cast<float*>(e.p)[i] = v;
-  else static_cast<uint16_t*>(e.p)[i] = f_to_bf16(v);
-}
-
-constexpr int kMaxSteps = 32;
-
 struct ChainP {
   // X's two buffers by 64 columns x 128 rows and by 64 x 64, lo, A and B
   CUtensorMap xk[2], xm[2], lo, ak, bk, a64, b64;
@@ -111,38 +89,10 @@ struct ChainP {
   float2* diag;        // [E, s] B's diagonal in 32 bits and its rounding residual
   float* partials;     // split GRAM sums
   unsigned* counters;  // grid barrier, abort, and an arrival count for each split tile
-  int last;            // LAST or UPDATE
-  Elem out, par;
-  float keep, rate;  // p' = keep p - rate O
+  ResultP res;
   int* err;
   float co[3 * kMaxSteps];
 };
-
-__device__ __forceinline__ uint4 pack_h8(const float* f) {
-  uint4 v;
-  __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-  return v;
-}
-__device__ __forceinline__ uint4 ld_shared(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void st_shared(uint32_t a, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ float ld_shared_f(uint32_t a) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void st_shared_h(uint32_t a, __half v) {
-  asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory");
-}
-// 16-byte unit u of row r of a chunk (128-byte rows under the 128-byte swizzle).
-__device__ __forceinline__ uint32_t unit(uint32_t base, int r, int u) { return base + r * 128 + ((u ^ (r & 7)) << 4); }
 
 // One phase's product C[i, j] = sum_k P[i, k] Q[j, k] as a list of work items.
 template <int CG>
@@ -304,14 +254,14 @@ __device__ __forceinline__ void write_out(const ChainP& p, uint32_t set, int e, 
   const int col = j + lane, rows = min(32, p.m - i0);
   if (col >= p.n) return;
   const uint32_t from = lane < 16 ? set : set + kSet / 2;
-  const int64_t o = static_cast<int64_t>(e) * p.out.sb + static_cast<int64_t>(i0) * p.out.sr + col;
-  const int64_t q = static_cast<int64_t>(e) * p.par.sb + static_cast<int64_t>(i0) * p.par.sr +
-                    static_cast<int64_t>(col) * p.par.sc;
+  const int64_t o = static_cast<int64_t>(e) * p.res.out.sb + static_cast<int64_t>(i0) * p.res.out.sr + col;
+  const int64_t q = static_cast<int64_t>(e) * p.res.par.sb + static_cast<int64_t>(i0) * p.res.par.sr +
+                    static_cast<int64_t>(col) * p.res.par.sc;
 #pragma unroll 8
   for (int r = 0; r < rows; ++r) {
     float v = ld_shared_f(unit(from, r0 + r, half * 4 + ((lane & 15) >> 2)) + (lane & 3) * 4) * (1.0f / kXScale);
-    if (MODE == UPDATE) v = p.keep * load_elem(p.par, q + r * p.par.sr) - p.rate * v;
-    store_elem(p.out, o + r * p.out.sr, v);
+    if (MODE == UPDATE) v = p.res.keep * load_elem(p.res.par, q + r * p.res.par.sr) - p.res.rate * v;
+    store_elem(p.res.out, o + r * p.res.out.sr, v);
   }
 }
 
@@ -650,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
   for (int step = 0; step < p.steps && ok; ++step) {
     const int cur = step & 1;
     for (int ph = 0; ph < 3; ++ph) {
-      const int mode = ph < STEP ? ph : step + 1 < p.steps ? static_cast<int>(STEP) : p.last;
+      const int mode = ph < STEP ? ph : step + 1 < p.steps ? static_cast<int>(STEP) : p.res.last;
       bool good = true;
       if (warp == 0) {
         if (loads) good = load_phase<CG>(p, sh, smem, mode, cur, rank, n);
@@ -702,19 +652,6 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
 }
 
 // ------------------------------------------------------------- preparation
-
-struct PrepP {
-  Elem g, mom, mom_out;
-  int has_mom, nesterov;
-  float mu;
-  int64_t rows, cols, ldx;  // of one matrix
-  float eps;
-  __half* hi;
-  __half* lo;
-  float* partials;  // [E, blocks]
-  unsigned* counters;
-  int count;  // of them, cleared for the chain of products
-};
 
 // V neighbouring elements of a row (V = 8: one 16- or two 16-byte accesses).
 template <int V>
@@ -927,6 +864,9 @@ int launch_chain(const ChainP& p, int groups, cudaStream_t s) {
 
 int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_t n, int steps, const float* co,
                   Elem out, const Elem* par, float keep, float rate, unsigned char* ws, cudaStream_t s) {
+  const ResultP res = {par ? UPDATE : LAST, out, par ? *par : Elem{}, keep, rate};
+  const int small = orthogonalise_small(prep, E, steps, co, res, s);
+  if (small != -1) return small;
   if (q.groups <= 0) return FRAG_ERR_NO_DEVICE;
   PrepP pp = prep;
   pp.hi = reinterpret_cast<__half*>(ws + q.hi0);
@@ -958,11 +898,7 @@ int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_
   p.diag = reinterpret_cast<float2*>(ws + q.diag);
   p.partials = reinterpret_cast<float*>(ws + q.sums);
   p.counters = pp.counters;
-  p.last = par ? UPDATE : LAST;
-  p.out = out;
-  if (par) p.par = *par;
-  p.keep = keep;
-  p.rate = rate;
+  p.res = res;
   p.err = device_error_word();
   for (int i = 0; i < 3 * steps; ++i) p.co[i] = co[i];
 

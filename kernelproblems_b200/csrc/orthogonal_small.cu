@@ -1,0 +1,385 @@
+// orthogonal_small.cu — the Newton-Schulz chain of matrices with a side of at
+// most 128, one cluster of blocks a matrix, in one launch.
+//
+// Block c of the cluster holds up to 256 columns of X (taken as s <= 128 rows
+// of the long side l; a tall matrix is read transposed) as hi and lo in shared
+// memory, from the first step to the last:
+//   A  each block multiplies its columns into a partial X X' (tensor memory ->
+//      shared memory), sums every C-th column of all blocks' partials in block
+//      order over the cluster, and writes it, a row of the symmetric A, to all
+//   B  every block makes b A + c A A for itself, in A's place
+//   X  every block updates its own columns where they are
+// Only A crosses blocks: two cluster barriers a step, nothing in global memory.
+//
+// The same 64-column block of X is A's K-major operand (rows of k) and X's
+// MN-major one (rows across k), so it is stored once.  Bound: latency, about
+// 40 dependent tensor and barrier steps.
+#include <algorithm>
+#include <mutex>
+
+#include "orthogonal.cuh"
+
+namespace frag {
+namespace {
+
+constexpr int kSide = 128;
+constexpr int kMaxBlocks = 4;                 // of 64 columns a block holds
+constexpr int kBlock = kSide * 64 * 2;        // bytes of one, 16 bits
+constexpr int kPart = kSide * kSide * 4;      // partial A, columns of 128 rows
+constexpr int kASize = kSide * kSide * 2;     // A, then B: two 64-column blocks
+constexpr int kSmallThreads = 256;
+constexpr int kMaxCluster = 16;
+
+struct SmallP {
+  PrepP prep;
+  ResultP res;
+  int s, l, tall, blocks, steps;  // blocks: of 64 columns in each block of the cluster
+  int* err;
+  float co[3 * kMaxSteps];
+};
+
+struct SmallShared {
+  uint64_t bar;
+  uint32_t tmem;
+  int abort;
+  float slots[2][32];
+  float sum;             // of this block's squares
+  float2 coef[kSide];    // hi's and lo's factors by row
+};
+
+__device__ __forceinline__ uint32_t small_tail(int blocks) { return 2 * blocks * kBlock + kPart + kASize; }
+
+template <int MODE>
+__device__ __forceinline__ void small_out(const SmallP& p, uint32_t hi, uint32_t lo, int e, int c0, int cols) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const ResultP& q = p.res;
+  auto put = [&](int i, int j) {
+    // the first four floats of an 8-column unit lie in hi's place, the others in lo's
+    const uint32_t a = unit((j & 4 ? lo : hi) + (j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 3) * 4;
+    const int64_t row = p.tall ? c0 + j : i, col = p.tall ? i : c0 + j;
+    float v = ld_shared_f(a) * (1.0f / kXScale);
+    if (MODE == UPDATE) v = q.keep * load_elem(q.par, e * q.par.sb + row * q.par.sr + col * q.par.sc) - q.rate * v;
+    store_elem(q.out, e * q.out.sb + row * q.out.sr + col, v);
+  };
+  if (p.tall) {
+    for (int j = warp; j < cols; j += kSmallThreads / 32)
+      for (int i = lane; i < p.s; i += 32) put(i, j);
+  } else {
+    for (int i = warp; i < p.s; i += kSmallThreads / 32)
+#pragma unroll 4
+      for (int j = lane; j < cols; j += 32) put(i, j);
+  }
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_constant__ SmallP p, int C) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t hi = smem_u32(smem_raw), lo = hi + p.blocks * kBlock, part = lo + p.blocks * kBlock;
+  const uint32_t am = part + kPart;
+  SmallShared& sh = *reinterpret_cast<SmallShared*>(smem_raw + small_tail(p.blocks));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+  const int c = static_cast<int>(blockIdx.x) % C, e = static_cast<int>(blockIdx.x) / C;
+  const int c0 = c * p.blocks * 64, cols = max(0, min(p.blocks * 64, p.l - c0));
+  volatile int* const abort_flag = &sh.abort;
+
+  if (threadIdx.x == 0) {
+    sh.abort = 0;
+    mbar_init(&sh.bar, 1);
+    mbar_init_fence();
+  }
+  if (warp == 0) tmem_alloc<1>(&sh.tmem, 512);
+  // zeros past the matrix's rows and columns
+  const int words = (2 * p.blocks * kBlock + kPart + kASize) / 16;
+  for (int i = threadIdx.x; i < words; i += kSmallThreads)
+    if (i < 2 * p.blocks * (kBlock / 16) || i >= (2 * p.blocks * kBlock + kPart) / 16)
+      st_shared(hi + i * 16, make_uint4(0, 0, 0, 0));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  // The matrix and its sum of squares; a value's 32 bits wait in hi's and lo's
+  // places until the norm is known.
+  float ss = 0.f;
+  auto take = [&](int i, int j) {
+    const PrepP& q = p.prep;
+    const int64_t row = p.tall ? c0 + j : i, col = p.tall ? i : c0 + j;
+    float v = load_elem(q.g, e * q.g.sb + row * q.g.sr + col * q.g.sc);
+    if (q.has_mom) {
+      const float g = (1.0f - q.mu) * v;
+      const float m = q.mu * load_elem(q.mom, e * q.mom.sb + row * q.mom.sr + col * q.mom.sc) + g;
+      store_elem(q.mom_out, e * q.mom_out.sb + row * q.mom_out.sr + col, m);
+      v = q.nesterov ? q.mu * m + g : m;
+    }
+    ss = fmaf(v, v, ss);
+    const uint32_t o = unit((j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 7) * 2, bits = __float_as_uint(v);
+    st_shared_h(hi + o, __ushort_as_half(static_cast<unsigned short>(bits >> 16)));
+    st_shared_h(lo + o, __ushort_as_half(static_cast<unsigned short>(bits)));
+  };
+  if (p.tall) {
+    for (int j = warp; j < cols; j += kSmallThreads / 32)
+#pragma unroll 4
+      for (int i = lane; i < p.s; i += 32) take(i, j);
+  } else {
+    for (int i = warp; i < p.s; i += kSmallThreads / 32)
+#pragma unroll 8
+      for (int j = lane; j < cols; j += 32) take(i, j);
+  }
+  ss = block_sum(ss, sh.slots, 0);
+  if (threadIdx.x == 0) sh.sum = ss;
+  cluster_sync();
+  if (C > 1) {
+    ss = 0.f;
+    for (int q = 0; q < C; ++q) ss += ld_cluster_f(cluster_address(smem_u32(&sh.sum), q));
+  }
+  const float f = kXScale / (sqrtf(ss) + p.prep.eps);
+  for (int i = threadIdx.x; i < p.blocks * (kBlock / 16); i += kSmallThreads) {
+    const uint4 a = ld_shared(hi + i * 16), b = ld_shared(lo + i * 16);
+    uint4 oh, ol;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t aw = u4_word(a, w), bw = u4_word(b, w);
+      const float x0 = __uint_as_float(aw << 16 | (bw & 0xffffu)) * f;
+      const float x1 = __uint_as_float((aw & 0xffff0000u) | bw >> 16) * f;
+      const __half2 h = __floats2half2_rn(x0, x1);
+      const float2 back = __half22float2(h);
+      const __half2 rest = __floats2half2_rn(x0 - back.x, x1 - back.y);
+      reinterpret_cast<uint32_t*>(&oh)[w] = *reinterpret_cast<const uint32_t*>(&h);
+      reinterpret_cast<uint32_t*>(&ol)[w] = *reinterpret_cast<const uint32_t*>(&rest);
+    }
+    st_shared(hi + i * 16, oh);
+    st_shared(lo + i * 16, ol);
+  }
+
+  uint32_t phase = 0;
+  // what the block has written to shared memory is seen by thread 0's products
+  auto publish = [&]() {
+    proxy_fence_shared();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  auto wait = [&]() {  // the products are done (bounded; after that the block only keeps step with the others)
+    if (!*abort_flag && !mbar_wait(&sh.bar, phase, p.err)) *abort_flag = 1;
+    phase ^= 1;
+    __syncwarp();
+    tc_fence_after();
+  };
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  const int k16 = (p.s + 15) / 16;
+
+  for (int step = 0; step < p.steps; ++step) {
+    const float ca = p.co[3 * step], cb = p.co[3 * step + 1], cc = p.co[3 * step + 2] / kAScale;
+    // ---- A = X X'
+    publish();
+    if (threadIdx.x == 0) {
+      for (int b = 0; b < p.blocks; ++b) {
+        const uint64_t d = smem_desc(hi + b * kBlock, false);
+        for (int k = 0; k < 4; ++k)
+          mma_f16<1>(tmem, d + k * desc_k16(false), d + k * desc_k16(false), instr_desc_f16(kSide, kSide, false, false),
+                     b + k > 0);
+      }
+      mma_commit<1>(&sh.bar);
+    }
+    wait();
+    if (C == 1) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float v[32];
+        tmem_load32(lanes + half * 64 + g * 32, v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= kAScale / (kXScale * kXScale);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) st_shared(unit(am + half * kBlock, r, g * 4 + u), pack_h8(v + 8 * u));
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float v[32];
+        tmem_load32(lanes + half * 64 + g * 32, v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + ((half * 64 + g * 32 + k) * kSide + r) * 4), "f"(v[k])
+                       : "memory");
+      }
+      cluster_sync();
+      // columns c, c + C, ... of all partials: row j of A
+      for (int j = c + C * warp; j < p.s; j += C * (kSmallThreads / 32)) {
+        const uint32_t from = part + (j * kSide + 4 * lane) * 4;
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q0 = 0; q0 < C; q0 += 8) {
+          float4 x[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            x[q] = q0 + q < C ? ld_cluster_f4(cluster_address(from, q0 + q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) t.x += x[q].x, t.y += x[q].y, t.z += x[q].z, t.w += x[q].w;
+        }
+        constexpr float scale = kAScale / (kXScale * kXScale);
+        const __half2 a = __floats2half2_rn(t.x * scale, t.y * scale), b = __floats2half2_rn(t.z * scale, t.w * scale);
+        const uint32_t to = unit(am + (lane >> 4) * kBlock, j, (lane & 15) >> 1) + (lane & 1) * 8;
+        for (int q = 0; q < C; ++q)
+          st_cluster_u2(cluster_address(to, q), *reinterpret_cast<const uint32_t*>(&a),
+                        *reinterpret_cast<const uint32_t*>(&b));
+      }
+      proxy_fence();
+      cluster_sync();
+    }
+    // ---- B = b A + c A A
+    publish();
+    if (threadIdx.x == 0) {
+      const uint32_t id = instr_desc_f16(kSide, kSide, false, false);
+      for (int k = 0; k < k16; ++k) {
+        const uint64_t d = smem_desc(am + (k >> 2) * kBlock, false) + (k & 3) * desc_k16(false);
+        mma_f16<1>(tmem + kSide, d, d, id, k > 0);
+      }
+      mma_commit<1>(&sh.bar);
+    }
+    wait();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float v[32];
+      tmem_load32(lanes + kSide + half * 64 + g * 32, v);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t at = unit(am + half * kBlock, r, g * 4 + u);
+        const uint4 a = ld_shared(at);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t w = u4_word(a, q);
+          const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w));
+          v[8 * u + 2 * q] = fmaf(v[8 * u + 2 * q], cc, cb * t.x);
+          v[8 * u + 2 * q + 1] = fmaf(v[8 * u + 2 * q + 1], cc, cb * t.y);
+        }
+        st_shared(at, pack_h8(v + 8 * u));
+      }
+      const int j = half * 64 + g * 32;
+      if (r >= j && r < j + 32) {
+        float d = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) d = j + k == r ? v[k] : d;
+        const float rest = d - __half2float(__float2half_rn(d));
+        sh.coef[r] = make_float2(ca + rest * (1.0f / kAScale), step >= p.steps - 2 ? ca + d * (1.0f / kAScale) : ca);
+      }
+    }
+    // ---- X = a X + B X
+    publish();
+    if (threadIdx.x == 0) {
+      const uint32_t id = instr_desc_f16(kSide, 64 * p.blocks, false, true);
+      for (int k = 0; k < k16; ++k)
+        mma_f16<1>(tmem + 2 * kSide, smem_desc(am + (k >> 2) * kBlock, false) + (k & 3) * desc_k16(false),
+                   smem_desc(hi, true, kBlock) + k * desc_k16(true), id, k > 0);
+      mma_commit<1>(&sh.bar);
+    }
+    wait();
+    const float2 coef = sh.coef[r];
+    const bool last = step + 1 == p.steps;
+    for (int b = 0; b < p.blocks; ++b) {
+      float v[32];
+      tmem_load32(lanes + 2 * kSide + b * 64 + half * 32, v);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t ah = unit(hi + b * kBlock, r, half * 4 + u), al = unit(lo + b * kBlock, r, half * 4 + u);
+        const uint4 h = ld_shared(ah), l = ld_shared(al);
+        uint4 oh, ol;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t hw = u4_word(h, q), lw = u4_word(l, q);
+          float2* y = reinterpret_cast<float2*>(v + 8 * u + 2 * q);
+          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hw)), make_float2(coef.x, coef.x),
+                          __fmul2_rn(*y, make_float2(1.0f / kAScale, 1.0f / kAScale)));
+          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lw)), make_float2(coef.y, coef.y), *y);
+          const __half2 t = __float22half2_rn(*y);
+          const float2 back = __half22float2(t);
+          const __half2 rest = __floats2half2_rn(y->x - back.x, y->y - back.y);
+          reinterpret_cast<uint32_t*>(&oh)[q] = *reinterpret_cast<const uint32_t*>(&t);
+          reinterpret_cast<uint32_t*>(&ol)[q] = *reinterpret_cast<const uint32_t*>(&rest);
+        }
+        if (last) {  // 32 bits a value: four in each place
+          const float* y = v + 8 * u;
+          oh = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+          ol = make_uint4(__float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7]));
+        }
+        st_shared(ah, oh);
+        st_shared(al, ol);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (p.res.last == UPDATE) small_out<UPDATE>(p, hi, lo, e, c0, cols);
+  else small_out<LAST>(p, hi, lo, e, c0, cols);
+  if (warp == 0) {
+    __syncwarp();
+    tmem_free<1>(tmem, 512);
+  }
+  cluster_sync();  // no block leaves while another may still read its shared memory
+}
+
+int small_smem(int blocks) { return 2 * blocks * kBlock + kPart + kASize + static_cast<int>(sizeof(SmallShared)); }
+
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int grid, int C, int smem, cudaStream_t s) {
+  cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(C);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+}
+
+// Whether a cluster of C blocks fits on the device (asked once for each C).
+bool cluster_fits(int C) {
+  static std::mutex mu;
+  static int known[64][kMaxCluster + 1] = {};  // 1: no, 2: yes
+  const int d = current_device();
+  if (d < 0 || d >= 64) return false;
+  std::lock_guard<std::mutex> lk(mu);
+  if (known[d][C]) return known[d][C] == 2;
+  const void* kern = reinterpret_cast<const void*>(small_chain);
+  if (!allow_dynamic_smem(kern, small_smem(kMaxBlocks))) return false;
+  if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  cluster_config(cfg, attr, C, C, small_smem(kMaxBlocks), nullptr);
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, small_chain, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  known[d][C] = n > 0 ? 2 : 1;
+  return n > 0;
+}
+
+}  // namespace
+
+int orthogonalise_small(const PrepP& prep, int64_t E, int steps, const float* co, const ResultP& res, cudaStream_t s) {
+  const int64_t small = std::min(prep.rows, prep.cols), longer = std::max(prep.rows, prep.cols);
+  if (small > kSide || longer > static_cast<int64_t>(kMaxCluster) * kMaxBlocks * 64) return -1;
+  const int64_t blocks64 = ceil_div(longer, 64);
+  int C = static_cast<int>(ceil_div(blocks64, kMaxBlocks));
+  if (!cluster_fits(C)) return -1;
+  SmallP p = {};
+  p.prep = prep;
+  p.res = res;
+  p.s = static_cast<int>(small);
+  p.l = static_cast<int>(longer);
+  p.tall = prep.rows > prep.cols;
+  p.blocks = static_cast<int>(ceil_div(blocks64, C));
+  p.steps = steps;
+  p.err = device_error_word();
+  for (int i = 0; i < 3 * steps; ++i) p.co[i] = co[i];
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  cluster_config(cfg, attr, static_cast<int>(E) * C, C, small_smem(p.blocks), s);
+  return cuda_status(cudaLaunchKernelEx(&cfg, small_chain, p, C));
+}
+
+}  // namespace frag

@@ -86,10 +86,10 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // Shared-memory operand descriptor (128-byte swizzle).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn) {
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn, uint32_t lbo = 64 * kTileK * 2) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((addr & 0x3ffff) >> 4);
-  d |= static_cast<uint64_t>(mn ? (64 * kTileK * 2) >> 4 : 1) << 16;  // LBO
+  d |= static_cast<uint64_t>(mn ? lbo >> 4 : 1) << 16;                // LBO
   d |= static_cast<uint64_t>(1024 >> 4) << 32;                        // SBO
   d |= 1ull << 46;                                                    // descriptor version of sm_100
   d |= 2ull << 61;                                                    // 128-byte swizzle
@@ -144,7 +144,26 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void st_cluster_u2(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 }
 

@@ -15,7 +15,6 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
-from contextlib import contextmanager
 
 import torch
 
@@ -55,24 +54,38 @@ _SYNC_CHECK = os.environ.get("FRAG_SYNC_CHECK", "0") not in ("", "0")
 _status_words: dict[int, torch.Tensor] = {}
 
 
+# These helpers run in every call, and a small call's time is the host's: a raw
+# stream handle takes 0.1 us where a Stream object takes 2.5, a plain class
+# 0.5 us where a generator context takes 1.3.
+
 def _ptr(t: torch.Tensor | None):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _stream(dev: torch.device):
-    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
-@contextmanager
-def _on_device(dev: torch.device):
-    if dev.type != "cuda":
-        raise ValueError(f"kernelproblems_b200 ops need CUDA tensors, got device {dev}")
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    if torch.cuda.current_device() == idx:
-        yield
-    else:
-        with torch.cuda.device(idx):
-            yield
+class _on_device:
+    """Makes `dev` the current CUDA device for a with block."""
+
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, dev: torch.device):
+        if dev.type != "cuda":
+            raise ValueError(f"kernelproblems_b200 ops need CUDA tensors, got device {dev}")
+        self.idx = dev.index
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        self.prev = None
+        if self.idx is not None and self.idx != cur:
+            self.prev = cur
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device | None = None):
@@ -871,25 +884,40 @@ def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch
     B, S, _, D = q.shape
     if D != freqs.head_dim:
         raise ValueError(f"q has heads of {D} elements, the plan is for {freqs.head_dim}")
-    oq = _new_out(q, out_layout) if out_q is None else out_q
-    _check_rope_out(q, oq, "q")
-    descs = [_rope_desc(q, oq, "q")]
+    oq, dq = _rope_pair(q, out_q, out_layout, "q")
     ok = None
-    if k is not None:
+    if k is None:
+        arr = (_lib.RopeTensor * 1)(dq)
+    else:
         _need(k, "k", torch.bfloat16, dev)
         if k.dim() != 4 or k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
             raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
-        ok = _new_out(k, out_layout) if out_k is None else out_k
-        _check_rope_out(k, ok, "k")
-        if _overlaps(oq, ok) and (out_q is not None or out_k is not None) and not _interleaved(oq, ok):
+        ok, dk = _rope_pair(k, out_k, out_layout, "k")
+        if (out_q is not None or out_k is not None) and _overlaps(oq, ok) and not _interleaved(oq, ok):
             raise ValueError("out_q and out_k overlap")
-        descs.append(_rope_desc(k, ok, "k"))
+        arr = (_lib.RopeTensor * 2)(dq, dk)
     pos_ptr, pos_dtype, psb, pss = _rope_positions(positions, B, S, dev)
-    arr = (_lib.RopeTensor * len(descs))(*descs)
     with _on_device(dev):
-        _lib.call("frag_rope_scaled", arr, len(descs), B, S, D, freqs.rotary_dim, pos_ptr, pos_dtype, psb, pss,
-                  freqs._turns, freqs.attention_factor, _LAYOUTS[layout], int(bool(backward)), _stream(dev))
+        _lib.call("frag_rope_scaled", arr, 1 if k is None else 2, B, S, D, freqs.rotary_dim, pos_ptr, pos_dtype, psb,
+                  pss, freqs._turns, freqs.attention_factor, _LAYOUTS[layout], 1 if backward else 0, _stream(dev))
     return oq, ok
+
+
+def _rope_pair(x: torch.Tensor, out: torch.Tensor | None, out_layout: str, name: str):
+    """x's output, checked or new, and the descriptor of the two."""
+    if x.stride(-1) != 1:
+        raise ValueError(f"{name}: the head dimension must be contiguous")
+    if out is not None:
+        _check_rope_out(x, out, name)
+        if out.stride(-1) != 1:
+            raise ValueError(f"{name}: the output's head dimension must be contiguous")
+    elif out_layout == "bshd":
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
+        out = _new_out(x, out_layout)
+    xs, os_ = x.stride(), out.stride()
+    return out, _lib.RopeTensor(x.data_ptr(), out.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], os_[0], os_[1], os_[2],
+                                _lib.FRAG_ROPE_OUT_BF16, _lib.FRAG_ROPE_IN_BF16)
 
 
 def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -913,9 +941,9 @@ def _rope_positions(positions, B: int, S: int, dev: torch.device):
         raise ValueError("positions must be on the same device as q")
     code = _lib.FRAG_POS_I64 if positions.dtype == torch.int64 else _lib.FRAG_POS_I32
     if positions.dim() == 1 and positions.shape[0] == S:
-        return C.c_void_p(positions.data_ptr()), code, 0, positions.stride(0)
+        return positions.data_ptr(), code, 0, positions.stride(0)
     if positions.dim() == 2 and tuple(positions.shape) == (B, S):
-        return C.c_void_p(positions.data_ptr()), code, positions.stride(0), positions.stride(1)
+        return positions.data_ptr(), code, positions.stride(0), positions.stride(1)
     raise ValueError(f"positions must be [B, S] or [S], got {tuple(positions.shape)}")
 
 
@@ -951,9 +979,9 @@ def _quant_out(x: torch.Tensor, N: int, dtype, group: int, scale_dtype, dev):
         raise ValueError(f"group must be one of {_GROUPS} (0: one scale for a row)")
     if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
         raise TypeError("scale_dtype must be float32 or float8_e8m0fnu")
-    q = torch.empty(x.shape, dtype=dtype, device=dev)
+    q = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     shape = x.shape[:-1] + (-(-N // group),) if group else x.shape[:-1]
-    return q, torch.empty(shape, dtype=scale_dtype, device=dev)
+    return q, x.new_empty(shape, dtype=scale_dtype)
 
 
 def _workspace(given: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor:
@@ -991,8 +1019,10 @@ def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, 
     x2, xs = _strided_rows(x, "x", N, dev)
     r2, rs = (None, 0) if residual is None else _strided_rows(residual, "residual", N, dev, x.shape)
     q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
-    h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if residual is not None and write_h else None
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if save_rstd else None
+    h = None
+    if residual is not None and write_h:
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32) if save_rstd else None
     wc = weight.contiguous()
     with _on_device(dev):
         _lib.call("frag_rmsnorm_quant_fwd", _ptr(x2), xs, _ptr(r2), rs, _ptr(wc), _ptr(q), _ptr(scale), _ptr(h),
@@ -1027,8 +1057,8 @@ def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
     if rstd.numel() != M or not rstd.is_contiguous():
         raise ValueError(f"rstd must be contiguous with {M} elements")
     q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
-    dx = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if write_dx else None
-    dw = torch.empty(N, dtype=torch.float32, device=dev) if compute_dw else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if write_dx else None
+    dw = weight.new_empty((N,), dtype=torch.float32) if compute_dw else None
     wc = weight.contiguous()
     with _on_device(dev):
         need = int(_lib.load().frag_rmsnorm_quant_bwd_workspace_bytes(M, N))
