@@ -653,54 +653,6 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
 
 // ------------------------------------------------------------- preparation
 
-// V neighbouring elements of a row (V = 8: one 16- or two 16-byte accesses).
-template <int V>
-__device__ __forceinline__ void load_elems(const Elem& e, int64_t i, float (&f)[V]) {
-  if (V == 8 && e.f32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(e.p) + i));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(e.p) + i) + 1);
-    f[0] = a.x, f[1 % V] = a.y, f[2 % V] = a.z, f[3 % V] = a.w, f[4 % V] = b.x, f[5 % V] = b.y, f[6 % V] = b.z, f[7 % V] = b.w;
-  } else if (V == 8) {
-    const uint4 u = ld_cached(static_cast<const uint16_t*>(e.p) + i);
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) f[2 * k] = bf16lo(u4_word(u, k)), f[(2 * k + 1) % V] = bf16hi(u4_word(u, k));
-  } else {
-    f[0] = load_elem(e, i);
-  }
-}
-template <int V>
-__device__ __forceinline__ void store_elems(const Elem& e, int64_t i, const float (&f)[V]) {
-  if (V == 8 && e.f32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(e.p) + i);
-    o[0] = make_float4(f[0], f[1 % V], f[2 % V], f[3 % V]);
-    o[1] = make_float4(f[4 % V], f[5 % V], f[6 % V], f[7 % V]);
-  } else if (V == 8) {
-    uint4 u;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) w[k] = pack_bf16x2(f[2 * k], f[(2 * k + 1) % V]);
-    st_global(static_cast<uint16_t*>(e.p) + i, u);
-  } else {
-    store_elem(e, i, f[0]);
-  }
-}
-
-// The matrix to be orthogonalised at (r, c): the gradient or the momentum's
-// look-ahead; m' in `m`.
-template <int V>
-__device__ __forceinline__ void prep_value(const PrepP& p, int64_t e, int64_t r, int64_t c, float (&u)[V],
-                                           float (&m)[V]) {
-  load_elems<V>(p.g, e * p.g.sb + r * p.g.sr + c * p.g.sc, u);
-  if (!p.has_mom) return;
-  load_elems<V>(p.mom, e * p.mom.sb + r * p.mom.sr + c * p.mom.sc, m);
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const float g = (1.0f - p.mu) * u[k];
-    m[k] = p.mu * m[k] + g;
-    u[k] = p.nesterov ? p.mu * m[k] + g : m[k];
-  }
-}
-
 // Sums of squares, a block's in a fixed order.
 template <int V>
 __global__ void __launch_bounds__(256) prep_norm(const PrepP p) {
@@ -757,11 +709,6 @@ __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
       p.lo[o] = __float2half_rn(x - __half2float(h));
     }
   }
-}
-
-// Rows of whole 8-element chunks, aligned for 16-byte accesses.
-bool chunked(const Elem& e, int64_t E, int64_t rows, int64_t cols) {
-  return cols % 8 == 0 && e.sc == 1 && (rows == 1 || e.sr % 8 == 0) && (E == 1 || e.sb % 8 == 0) && aligned16(e.p);
 }
 
 // -------------------------------------------------------------------- host

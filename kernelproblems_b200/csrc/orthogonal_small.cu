@@ -49,28 +49,121 @@ struct SmallShared {
 
 __device__ __forceinline__ uint32_t small_tail(int blocks) { return 2 * blocks * kBlock + kPart + kASize; }
 
-template <int MODE>
+// How a block's threads walk its part of the matrix in memory order: lines
+// (matrix rows) over warps, V neighbouring elements a lane, N pieces of work
+// in flight a thread.  A line is a row of X, or a column when it is tall.
+template <int V>
+struct Walk {
+  static constexpr int kLines = V == 8 ? 8 : 2, kSteps = V == 8 ? 1 : 8;
+  int lines, length, per, first;  // per: lines of a warp's pass
+  __device__ Walk(const SmallP& p, int cols) {
+    lines = p.tall ? cols : p.s;
+    length = p.tall ? p.s : cols;
+    per = V == 8 && p.tall ? 2 : 1;  // 128 elements are half a warp's
+    first = (threadIdx.x >> 5) * per + (per == 2 ? (threadIdx.x & 31) >> 4 : 0);
+  }
+  __device__ int stride() const { return per * (kSmallThreads / 32); }
+  __device__ int pos(int b) const { return (per == 2 ? threadIdx.x & 15 : (threadIdx.x & 31) + 32 * b) * V; }
+};
+
+// Place of X's element (i, j) in hi's (or lo's) columns.
+__device__ __forceinline__ uint32_t place(int i, int j) { return unit((j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 7) * 2; }
+
+template <int V, int MODE>
 __device__ __forceinline__ void small_out(const SmallP& p, uint32_t hi, uint32_t lo, int e, int c0, int cols) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const ResultP& q = p.res;
-  auto put = [&](int i, int j) {
-    // the first four floats of an 8-column unit lie in hi's place, the others in lo's
-    const uint32_t a = unit((j & 4 ? lo : hi) + (j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 3) * 4;
-    const int64_t row = p.tall ? c0 + j : i, col = p.tall ? i : c0 + j;
-    float v = ld_shared_f(a) * (1.0f / kXScale);
-    if (MODE == UPDATE) v = q.keep * load_elem(q.par, e * q.par.sb + row * q.par.sr + col * q.par.sc) - q.rate * v;
-    store_elem(q.out, e * q.out.sb + row * q.out.sr + col, v);
-  };
-  if (p.tall) {
-    for (int j = warp; j < cols; j += kSmallThreads / 32)
-      for (int i = lane; i < p.s; i += 32) put(i, j);
-  } else {
-    for (int i = warp; i < p.s; i += kSmallThreads / 32)
-#pragma unroll 4
-      for (int j = lane; j < cols; j += 32) put(i, j);
+  const Walk<V> w(p, cols);
+  for (int l0 = w.first; l0 - w.first < w.lines; l0 += w.kLines * w.stride()) {
+    float old[w.kLines][w.kSteps][V];
+    if (MODE == UPDATE) {
+#pragma unroll
+      for (int a = 0; a < w.kLines; ++a)
+#pragma unroll
+        for (int b = 0; b < w.kSteps; ++b) {
+          const int line = l0 + a * w.stride(), pos = w.pos(b);
+          if (line < w.lines && pos < w.length)
+            load_elems<V>(q.par, e * q.par.sb + static_cast<int64_t>(p.tall ? c0 + line : line) * q.par.sr +
+                                     static_cast<int64_t>(p.tall ? pos : c0 + pos) * q.par.sc, old[a][b]);
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < w.kLines; ++a)
+#pragma unroll
+      for (int b = 0; b < w.kSteps; ++b) {
+        const int line = l0 + a * w.stride(), pos = w.pos(b);
+        if (line >= w.lines || pos >= w.length) continue;
+        float v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          // the first four floats of an 8-column unit lie in hi's place, the others in lo's
+          const int i = p.tall ? pos + k : line, j = p.tall ? line : pos + k;
+          v[k] = ld_shared_f(unit((j & 4 ? lo : hi) + (j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 3) * 4) *
+                 (1.0f / kXScale);
+          if (MODE == UPDATE) v[k] = q.keep * old[a][b][k] - q.rate * v[k];
+        }
+        store_elems<V>(q.out, e * q.out.sb + static_cast<int64_t>(p.tall ? c0 + line : line) * q.out.sr +
+                                  (p.tall ? pos : c0 + pos), v);
+      }
   }
 }
 
+// Reads the block's part of the matrix (and makes the new momentum), returns
+// this thread's sum of squares; a value's 32 bits wait in hi's and lo's places
+// until the norm is known.
+template <int V>
+__device__ __forceinline__ float small_in(const SmallP& p, uint32_t hi, uint32_t lo, int e, int c0, int cols) {
+  const PrepP& q = p.prep;
+  const Walk<V> w(p, cols);
+  float ss = 0.f;
+  for (int l0 = w.first; l0 - w.first < w.lines; l0 += w.kLines * w.stride()) {
+    float v[w.kLines][w.kSteps][V], m[w.kLines][w.kSteps][V];
+#pragma unroll
+    for (int a = 0; a < w.kLines; ++a)
+#pragma unroll
+      for (int b = 0; b < w.kSteps; ++b) {
+        const int line = l0 + a * w.stride(), pos = w.pos(b);
+        if (line < w.lines && pos < w.length)
+          prep_value<V>(q, e, p.tall ? c0 + line : line, p.tall ? pos : c0 + pos, v[a][b], m[a][b]);
+      }
+#pragma unroll
+    for (int a = 0; a < w.kLines; ++a)
+#pragma unroll
+      for (int b = 0; b < w.kSteps; ++b) {
+        const int line = l0 + a * w.stride(), pos = w.pos(b);
+        if (line >= w.lines || pos >= w.length) continue;
+        if (q.has_mom)
+          store_elems<V>(q.mom_out, e * q.mom_out.sb + static_cast<int64_t>(p.tall ? c0 + line : line) * q.mom_out.sr +
+                                        (p.tall ? pos : c0 + pos), m[a][b]);
+        uint32_t bits[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          ss = fmaf(v[a][b][k], v[a][b][k], ss);
+          bits[k] = __float_as_uint(v[a][b][k]);
+        }
+        if (V == 8 && !p.tall) {
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t x = bits[(2 * k) % V], y = bits[(2 * k + 1) % V];
+            h[k] = x >> 16 | (y & 0xffff0000u);
+            l[k] = (x & 0xffffu) | y << 16;
+          }
+          st_shared(hi + place(line, pos), make_uint4(h[0], h[1], h[2], h[3]));
+          st_shared(lo + place(line, pos), make_uint4(l[0], l[1], l[2], l[3]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const uint32_t o = p.tall ? place(pos + k, line) : place(line, pos + k);
+            st_shared_h(hi + o, __ushort_as_half(static_cast<unsigned short>(bits[k] >> 16)));
+            st_shared_h(lo + o, __ushort_as_half(static_cast<unsigned short>(bits[k])));
+          }
+        }
+      }
+  }
+  return ss;
+}
+
+template <int V>
 __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_constant__ SmallP p, int C) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t hi = smem_u32(smem_raw), lo = hi + p.blocks * kBlock, part = lo + p.blocks * kBlock;
@@ -98,33 +191,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  // The matrix and its sum of squares; a value's 32 bits wait in hi's and lo's
-  // places until the norm is known.
-  float ss = 0.f;
-  auto take = [&](int i, int j) {
-    const PrepP& q = p.prep;
-    const int64_t row = p.tall ? c0 + j : i, col = p.tall ? i : c0 + j;
-    float v = load_elem(q.g, e * q.g.sb + row * q.g.sr + col * q.g.sc);
-    if (q.has_mom) {
-      const float g = (1.0f - q.mu) * v;
-      const float m = q.mu * load_elem(q.mom, e * q.mom.sb + row * q.mom.sr + col * q.mom.sc) + g;
-      store_elem(q.mom_out, e * q.mom_out.sb + row * q.mom_out.sr + col, m);
-      v = q.nesterov ? q.mu * m + g : m;
-    }
-    ss = fmaf(v, v, ss);
-    const uint32_t o = unit((j >> 6) * kBlock, i, (j & 63) >> 3) + (j & 7) * 2, bits = __float_as_uint(v);
-    st_shared_h(hi + o, __ushort_as_half(static_cast<unsigned short>(bits >> 16)));
-    st_shared_h(lo + o, __ushort_as_half(static_cast<unsigned short>(bits)));
-  };
-  if (p.tall) {
-    for (int j = warp; j < cols; j += kSmallThreads / 32)
-#pragma unroll 4
-      for (int i = lane; i < p.s; i += 32) take(i, j);
-  } else {
-    for (int i = warp; i < p.s; i += kSmallThreads / 32)
-#pragma unroll 8
-      for (int j = lane; j < cols; j += 32) take(i, j);
-  }
+  float ss = small_in<V>(p, hi, lo, e, c0, cols);
   ss = block_sum(ss, sh.slots, 0);
   if (threadIdx.x == 0) sh.sum = ss;
   cluster_sync();
@@ -308,8 +375,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (p.res.last == UPDATE) small_out<UPDATE>(p, hi, lo, e, c0, cols);
-  else small_out<LAST>(p, hi, lo, e, c0, cols);
+  if (p.res.last == UPDATE) small_out<V, UPDATE>(p, hi, lo, e, c0, cols);
+  else small_out<V, LAST>(p, hi, lo, e, c0, cols);
   if (warp == 0) {
     __syncwarp();
     tmem_free<1>(tmem, 512);
@@ -340,17 +407,18 @@ bool cluster_fits(int C) {
   if (d < 0 || d >= 64) return false;
   std::lock_guard<std::mutex> lk(mu);
   if (known[d][C]) return known[d][C] == 2;
-  const void* kern = reinterpret_cast<const void*>(small_chain);
-  if (!allow_dynamic_smem(kern, small_smem(kMaxBlocks))) return false;
-  if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
+  for (const void* kern : {reinterpret_cast<const void*>(small_chain<1>), reinterpret_cast<const void*>(small_chain<8>)}) {
+    if (!allow_dynamic_smem(kern, small_smem(kMaxBlocks))) return false;
+    if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
   }
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
   cluster_config(cfg, attr, C, C, small_smem(kMaxBlocks), nullptr);
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, small_chain, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, small_chain<8>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
@@ -379,7 +447,11 @@ int orthogonalise_small(const PrepP& prep, int64_t E, int steps, const float* co
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
   cluster_config(cfg, attr, static_cast<int>(E) * C, C, small_smem(p.blocks), s);
-  return cuda_status(cudaLaunchKernelEx(&cfg, small_chain, p, C));
+  const int64_t m = prep.rows, n = prep.cols;
+  const bool wide_access = chunked(prep.g, E, m, n) && chunked(res.out, E, m, n) &&
+                           (res.last != UPDATE || chunked(res.par, E, m, n)) &&
+                           (!prep.has_mom || (chunked(prep.mom, E, m, n) && chunked(prep.mom_out, E, m, n)));
+  return cuda_status(cudaLaunchKernelEx(&cfg, wide_access ? small_chain<8> : small_chain<1>, p, C));
 }
 
 }  // namespace frag
