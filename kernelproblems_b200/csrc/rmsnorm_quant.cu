@@ -36,8 +36,10 @@ RowShape row_shape(int64_t N, bool aligned, int warp_row) {
     return {ROW_ODD, K, static_cast<int>(ceil_div(N, 128 * K) * 32)};
   }
   if (N <= warp_row) return {ROW_WARP, N <= 256 ? 1 : N <= 512 ? 2 : 4, 256};
-  // four chunks a thread and few threads, so that more rows are in flight
-  return {ROW_BLOCK, 4, static_cast<int>(ceil_div(N, 32 * 32) * 32)};
+  // Two chunks a thread up to 512 threads, four beyond (16384 rows of 4096 with
+  // the residual: two 72 us, four 76, one 86).
+  const int K = N <= 8192 ? 2 : 4;
+  return {ROW_BLOCK, K, static_cast<int>(ceil_div(N, 256 * K) * 32)};
 }
 
 struct QuantFwdP {
@@ -57,12 +59,12 @@ struct QuantFwdP {
 // the row, or a warp for each group in turn.
 template <bool E5M2, bool E8M0, class F>
 __device__ __forceinline__ void quant_row(const QuantOut& o, int64_t row, int64_t N, int group, F value,
-                                          uint32_t (*slots)[32]) {
+                                          float (*slots)[32]) {
   uint8_t* q = o.q + row * N;
   if (group == 0) {
-    uint32_t most = 0;
-    for (int64_t n = threadIdx.x; n < N; n += blockDim.x) most = max(most, mag_bits(value(n)));
-    most = block_umax(most, slots, 0);
+    float most = 0.f;
+    for (int64_t n = threadIdx.x; n < N; n += blockDim.x) most = max_mag(most, value(n));
+    most = block_max_mag(most, slots, 0);
     float inv;
     uint8_t byte = 0;
     const float s = quant_scale<E5M2, E8M0>(most, inv, byte);
@@ -74,14 +76,14 @@ __device__ __forceinline__ void quant_row(const QuantOut& o, int64_t row, int64_
   for (int64_t g = threadIdx.x >> 5; g < o.groups; g += blockDim.x >> 5) {
     const int64_t n0 = g * group, n1 = min(N, n0 + group);
     float v[4];
-    uint32_t most = 0;
+    float most = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t n = n0 + lane + 32 * i;
       v[i] = n < n1 ? value(n) : 0.f;
-      most = max(most, mag_bits(v[i]));
+      most = max_mag(most, v[i]);
     }
-    most = __reduce_max_sync(0xffffffffu, most);
+    most = warp_max_mag(most);
     float inv;
     uint8_t byte = 0;
     const float s = quant_scale<E5M2, E8M0>(most, inv, byte);
@@ -98,15 +100,15 @@ __device__ __forceinline__ void quant_row(const QuantOut& o, int64_t row, int64_
 // `most` is each chunk's largest magnitude.
 template <int K, bool WARP, bool E5M2, bool E8M0>
 __device__ __forceinline__ void quant_chunks(const QuantOut& o, int64_t row, int64_t N, int group, int t, int T,
-                                             int chunks, const float (&y)[K][8], uint32_t (&most)[K],
-                                             uint32_t (*slots)[32], int parity) {
+                                             int chunks, const float2 (&y)[K][4], const float (&most)[K],
+                                             float (*slots)[32], int parity) {
   float inv = 0.f, s;
   uint8_t byte = 0;
   if (group == 0) {
-    uint32_t m = most[0];
+    float m = most[0];
 #pragma unroll
-    for (int k = 1; k < K; ++k) m = max(m, most[k]);
-    m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, slots, parity);
+    for (int k = 1; k < K; ++k) m = max_mag(m, most[k]);
+    m = WARP ? warp_max_mag(m) : block_max_mag(m, slots, parity);
     s = quant_scale<E5M2, E8M0>(m, inv, byte);
     if (t == 0) store_scale<E8M0>(o, row, s, byte);
   }
@@ -114,21 +116,24 @@ __device__ __forceinline__ void quant_chunks(const QuantOut& o, int64_t row, int
   for (int k = 0; k < K; ++k) {
     const int c = t + k * T;
     if (group) {
-      uint32_t m = most[k];
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      if (group >= 64) m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-      if (group >= 128) m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      float m = most[k];
+      m = max_mag(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max_mag(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if (group >= 64) m = max_mag(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      if (group >= 128) m = max_mag(m, __shfl_xor_sync(0xffffffffu, m, 8));
       s = quant_scale<E5M2, E8M0>(m, inv, byte);
       const int lanes = group >> 3;
       if ((c & (lanes - 1)) == 0 && c < chunks) store_scale<E8M0>(o, row * o.groups + c / lanes, s, byte);
     }
     if (c < chunks) {
-      uint2 q;
-      q.x = to_fp8x2<E5M2>(y[k][0] * inv, y[k][1] * inv) |
-            static_cast<uint32_t>(to_fp8x2<E5M2>(y[k][2] * inv, y[k][3] * inv)) << 16;
-      q.y = to_fp8x2<E5M2>(y[k][4] * inv, y[k][5] * inv) |
-            static_cast<uint32_t>(to_fp8x2<E5M2>(y[k][6] * inv, y[k][7] * inv)) << 16;
+      const float2 f = make_float2(inv, inv);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = __fmul2_rn(y[k][i], f);
+        w[i] = to_fp8x2<E5M2>(v.x, v.y);
+      }
+      const uint2 q = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
       *reinterpret_cast<uint2*>(o.q + row * N + static_cast<int64_t>(c) * 8) = q;
     }
   }
@@ -138,33 +143,33 @@ __device__ __forceinline__ void quant_chunks(const QuantOut& o, int64_t row, int
 // row): value i of round k is number first + k step + 32 i.
 template <int K, bool WARP, bool E5M2, bool E8M0>
 __device__ __forceinline__ void quant_lanes(const QuantOut& o, int64_t row, int N, int group, int first, int step,
-                                            const float (&y)[K][4], uint32_t (*slots)[32], int parity) {
+                                            const float (&y)[K][4], float (*slots)[32], int parity) {
   uint8_t* q = o.q + row * N;
   const int lane = threadIdx.x & 31;
   float inv = 0.f, s;
   uint8_t byte = 0;
   if (group == 0) {
-    uint32_t m = 0;
+    float m = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, mag_bits(y[k][i]));
-    m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, slots, parity);
+      for (int i = 0; i < 4; ++i) m = max_mag(m, y[k][i]);
+    m = WARP ? warp_max_mag(m) : block_max_mag(m, slots, parity);
     s = quant_scale<E5M2, E8M0>(m, inv, byte);
     if (WARP ? lane == 0 : threadIdx.x == 0) store_scale<E8M0>(o, row, s, byte);
   }
   const int per = group >> 5;  // 1, 2 or 4 lane rows a group
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    uint32_t m[4];
+    float m[4];
     if (group) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = __reduce_max_sync(0xffffffffu, mag_bits(y[k][i]));
+      for (int i = 0; i < 4; ++i) m[i] = warp_max_mag(fabsf(y[k][i]));
       if (per >= 2) {
-        m[0] = m[1] = max(m[0], m[1]);
-        m[2] = m[3] = max(m[2], m[3]);
+        m[0] = m[1] = max_mag(m[0], m[1]);
+        m[2] = m[3] = max_mag(m[2], m[3]);
       }
-      if (per == 4) m[0] = m[1] = m[2] = m[3] = max(m[0], m[2]);
+      if (per == 4) m[0] = m[1] = m[2] = m[3] = max_mag(m[0], m[2]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -183,7 +188,7 @@ __device__ __forceinline__ void quant_lanes(const QuantOut& o, int64_t row, int 
 template <bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(256) quant_fwd_any(const QuantFwdP p) {
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   const int64_t row = blockIdx.x;
   const uint16_t* x = p.x + row * p.xs;
   const uint16_t* res = p.res ? p.res + row * p.rs : nullptr;
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(256) quant_fwd_any(const QuantFwdP p) {
     if (p.h) p.h[row * p.N + n] = f_to_bf16(v);
     ss = fmaf(v, v, ss);
   }
-  const float r = rsqrtf(block_sum(ss, slots, 0) / static_cast<float>(p.N) + p.eps);
+  const float r = rsqrtf(block_sum_lanes(ss, slots, 0) / static_cast<float>(p.N) + p.eps);
   if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
   quant_row<E5M2, E8M0>(p.o, row, p.N, p.group, [&](int64_t n) { return (h(n) * r) * bf16_to_f(p.w[n]); },
                         mslots);
@@ -205,60 +210,74 @@ __global__ void __launch_bounds__(256) quant_fwd_any(const QuantFwdP p) {
 
 // Rows of 16-byte chunks, the row in registers: thread t of the row's threads
 // owns the chunks t, t + T, ... (K of them); T is the block, or with WARP a
-// warp of it (rows of up to 1024 values: eight rows a block, no barrier).
-// A group of 32, 64 or 128 values is 4, 8 or 16 neighbouring lanes.
-template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
-__global__ void __launch_bounds__(512) quant_fwd_vec(const QuantFwdP p, int64_t M) {
+// warp of it (rows of up to 1024 values, no barrier).  A group of 32, 64 or 128
+// values is 4, 8 or 16 neighbouring lanes.  A block (or warp) stays for R rows,
+// with the weights in registers and the next row's loads in flight while this
+// one is reduced (without AHEAD, where registers run out, not).
+template <int K, bool WARP, bool AHEAD, bool HAS_RES, bool E5M2, bool E8M0>
+__global__ void __launch_bounds__(512) quant_fwd_vec(const QuantFwdP p, int64_t M, int R) {
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= M) return;
+  const int per = WARP ? blockDim.x >> 5 : 1;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * per * R + (WARP ? threadIdx.x >> 5 : 0);
+  const int64_t end = min(M, static_cast<int64_t>(blockIdx.x + 1) * per * R);
   const int chunks = static_cast<int>(p.N >> 3);
-  const uint16_t* x = p.x + row * p.xs;
   uint4 xv[K], rv[K], wv[K];
+  auto load = [&](int64_t n) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = t + k * T;
+      if (n < end && c < chunks) {
+        xv[k] = HAS_RES ? ld_plain(p.x + n * p.xs + c * 8) : ld_stream(p.x + n * p.xs + c * 8);
+        if (HAS_RES) rv[k] = ld_plain(p.res + n * p.rs + c * 8);
+      }
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k) xv[k] = rv[k] = make_uint4(0, 0, 0, 0);
+  load(row);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = t + k * T;
-    xv[k] = rv[k] = wv[k] = make_uint4(0, 0, 0, 0);
-    if (c < chunks) {
-      xv[k] = HAS_RES ? ld_plain(x + c * 8) : ld_stream(x + c * 8);
-      if (HAS_RES) rv[k] = ld_plain(p.res + row * p.rs + c * 8);
-      wv[k] = ld_cached(p.w + c * 8);
-    }
+    wv[k] = c < chunks ? ld_cached(p.w + c * 8) : make_uint4(0, 0, 0, 0);
   }
-  float ss = 0.f;
+  for (int parity = 0; row < end; row += per, parity ^= 1) {
+    uint4 hv[K];
+    float ss = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (HAS_RES) {
-      xv[k] = add_bf16x8(rv[k], xv[k]);
+    for (int k = 0; k < K; ++k) {
       const int c = t + k * T;
-      if (p.h && c < chunks) st_global(p.h + row * p.N + c * 8, xv[k]);
+      hv[k] = HAS_RES ? add_bf16x8(rv[k], xv[k]) : xv[k];
+      if (HAS_RES && p.h && c < chunks) st_global(p.h + row * p.N + c * 8, hv[k]);
+      float2 sq = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = bf16x2_to_f2(u4_word(hv[k], i));
+        sq = __ffma2_rn(v, v, sq);
+      }
+      ss += sq.x + sq.y;
     }
-    float v[8];
-    unpack8(xv[k], v);
+    if (AHEAD) load(row + per);
+    ss = WARP ? warp_sum(ss) : block_sum_lanes(ss, slots, parity);
+    const float r = rsqrtf(ss / static_cast<float>(p.N) + p.eps);
+    if (p.rstd && t == 0) p.rstd[row] = r;
+    float2 y[K][4];
+    float most[K];
+    const float2 r2 = make_float2(r, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-  }
-  ss = WARP ? warp_sum(ss) : block_sum(ss, slots, 0);
-  const float r = rsqrtf(ss / static_cast<float>(p.N) + p.eps);
-  if (p.rstd && t == 0) p.rstd[row] = r;
-  float y[K][8];
-  uint32_t most[K];
+    for (int k = 0; k < K; ++k) {
+      most[k] = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float v[8], wf[8];
-    unpack8(xv[k], v);
-    unpack8(wv[k], wf);
-    most[k] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[k][i] = (v[i] * r) * wf[i];
-      // chunks past the row are zeros, but 0 * inf is NaN
-      most[k] = max(most[k], t + k * T < chunks ? mag_bits(y[k][i]) : 0u);
+      for (int i = 0; i < 4; ++i) {
+        y[k][i] = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(u4_word(hv[k], i)), r2), bf16x2_to_f2(u4_word(wv[k], i)));
+        most[k] = max_mag2(most[k], y[k][i]);
+      }
+      if (t + k * T >= chunks) most[k] = 0.f;  // (past the row there are zeros, but 0 * inf is NaN)
     }
+    quant_chunks<K, WARP, E5M2, E8M0>(p.o, row, p.N, p.group, t, T, chunks, y, most, mslots, parity);
+    if (!AHEAD) load(row + per);
   }
-  quant_chunks<K, WARP, E5M2, E8M0>(p.o, row, p.N, p.group, t, T, chunks, y, most, mslots, 0);
 }
 
 // Rows without that alignment, up to 16384 values in registers: warp w of the
@@ -267,7 +286,7 @@ __global__ void __launch_bounds__(512) quant_fwd_vec(const QuantFwdP p, int64_t 
 template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(512) quant_fwd_odd(const QuantFwdP p, int64_t M) {
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP && row >= M) return;
   const bool lead = WARP ? (threadIdx.x & 31) == 0 : threadIdx.x == 0;
@@ -307,7 +326,7 @@ __global__ void __launch_bounds__(512) quant_fwd_odd(const QuantFwdP p, int64_t 
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) ss = fmaf(y[k][i], y[k][i], ss);
-  ss = WARP ? warp_sum(ss) : block_sum(ss, slots, 0);
+  ss = WARP ? warp_sum(ss) : block_sum_lanes(ss, slots, 0);
   const float r = rsqrtf(ss / static_cast<float>(N) + p.eps);
   if (p.rstd && lead) p.rstd[row] = r;
 #pragma unroll
@@ -349,6 +368,36 @@ __device__ __forceinline__ void store_partials(const QuantBwdP& p, const float* 
 // dx of one value, in 32 bits.
 __device__ __forceinline__ float grad_of(float g, float xhat, float mean, float r) { return (g - xhat * mean) * r; }
 
+// The gradient's arithmetic on a chunk of eight, in pairs (one instruction for
+// two columns): the chunk's part of sum(x g), g = dy w ...
+__device__ __forceinline__ float chunk_dot(const uint4& y, const uint4& x, const uint4& w) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    s = __ffma2_rn(bf16x2_to_f2(u4_word(x, i)), __fmul2_rn(bf16x2_to_f2(u4_word(y, i)), bf16x2_to_f2(u4_word(w, i))), s);
+  return s.x + s.y;
+}
+// ... and d = dres + (g - xhat mean) r, dweight += dy xhat, the largest |d|.
+template <bool HAS_RES>
+__device__ __forceinline__ float chunk_grad(const uint4& y, const uint4& x, const uint4& w, const uint4& res, float mean,
+                                            float r, float2 (&acc)[4], float2 (&d)[4]) {
+  const float2 r2 = make_float2(r, r), m2 = make_float2(-mean, -mean);
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 dy = bf16x2_to_f2(u4_word(y, i));
+    const float2 xhat = __fmul2_rn(bf16x2_to_f2(u4_word(x, i)), r2);
+    acc[i] = __ffma2_rn(dy, xhat, acc[i]);
+    const float2 t = __ffma2_rn(xhat, m2, __fmul2_rn(dy, bf16x2_to_f2(u4_word(w, i))));
+    d[i] = HAS_RES ? __ffma2_rn(t, r2, bf16x2_to_f2(u4_word(res, i))) : __fmul2_rn(t, r2);
+    most = max_mag2(most, d[i]);
+  }
+  return most;
+}
+__device__ __forceinline__ uint4 pack_pairs(const float2 (&d)[4]) {
+  return make_uint4(f2_to_bf16x2(d[0]), f2_to_bf16x2(d[1]), f2_to_bf16x2(d[2]), f2_to_bf16x2(d[3]));
+}
+
 // Rows of up to 512 values in 16-byte chunks, a warp a row: a block's warps
 // take rows_per_block rows in turn.
 template <int K, bool HAS_RES, bool E5M2, bool E8M0>
@@ -357,13 +406,13 @@ __global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunks = static_cast<int>(p.N >> 3);
   uint4 wv[K];
-  float acc[K][8];
+  float2 acc[K][4];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = lane + 32 * k;
     wv[k] = c < chunks ? ld_cached(p.w + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+    for (int i = 0; i < 4; ++i) acc[k][i] = make_float2(0.f, 0.f);
   }
   const int64_t r1 = min(M, (static_cast<int64_t>(blockIdx.x) + 1) * rows_per_block);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block + warp; row < r1; row += blockDim.x >> 5) {
@@ -381,35 +430,16 @@ __global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t
     const float r = __ldg(p.rstd + row);
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float yf[8], xf[8], wf[8];
-      unpack8(yv[k], yf);
-      unpack8(xv[k], xf);
-      unpack8(wv[k], wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(xf[i] * r, yf[i] * wf[i], sum);
-    }
-    const float mean = warp_sum(sum) / static_cast<float>(p.N);
-    float d[K][8];
-    uint32_t most[K];
+    for (int k = 0; k < K; ++k) sum += chunk_dot(yv[k], xv[k], wv[k]);
+    const float mean = r * warp_sum(sum) / static_cast<float>(p.N);
+    float2 d[K][4];
+    float most[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = lane + 32 * k;
-      float yf[8], xf[8], wf[8], rf[8];
-      unpack8(yv[k], yf);
-      unpack8(xv[k], xf);
-      unpack8(wv[k], wf);
-      if (HAS_RES) unpack8(rv[k], rf);
-      most[k] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float xhat = xf[i] * r;
-        acc[k][i] = fmaf(yf[i], xhat, acc[k][i]);
-        d[k][i] = grad_of(yf[i] * wf[i], xhat, mean, r);
-        if (HAS_RES) d[k][i] += rf[i];
-        most[k] = max(most[k], c < chunks ? mag_bits(d[k][i]) : 0u);
-      }
-      if (p.dx && c < chunks) st_global(p.dx + row * p.N + c * 8, pack8(d[k]));
+      most[k] = chunk_grad<HAS_RES>(yv[k], xv[k], wv[k], rv[k], mean, r, acc[k], d[k]);
+      if (c >= chunks) most[k] = 0.f;
+      if (p.dx && c < chunks) st_global(p.dx + row * p.N + c * 8, pack_pairs(d[k]));
     }
     quant_chunks<K, true, E5M2, E8M0>(p.o, row, p.N, p.group, lane, 32, chunks, d, most, nullptr, 0);
   }
@@ -418,8 +448,8 @@ __global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t
     const int c = lane + 32 * k;
     if (c < chunks) {
       float4* o = reinterpret_cast<float4*>(sacc + warp * p.N + c * 8);
-      o[0] = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
-      o[1] = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+      o[0] = make_float4(acc[k][0].x, acc[k][0].y, acc[k][1].x, acc[k][1].y);
+      o[1] = make_float4(acc[k][2].x, acc[k][2].y, acc[k][3].x, acc[k][3].y);
     }
   }
   if (p.partials) store_partials(p, sacc);
@@ -434,7 +464,7 @@ quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int*
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   __shared__ int s_abort;
   constexpr int NIN = HAS_RES ? 3 : 2;
   const int N = static_cast<int>(p.N), chunks = N >> 3, row_bytes = N * 2, stage_bytes = NIN * row_bytes;
@@ -452,21 +482,22 @@ quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int*
     if (i >= rows) return;
     unsigned char* st = smem + static_cast<size_t>(i % S) * stage_bytes;
     mbar_arrive_expect_tx(&bars[i % S], stage_bytes);
-    bulk_g2s(st, p.dy + (r0 + i) * p.ys, row_bytes, &bars[i % S]);
-    bulk_g2s(st + row_bytes, p.x + (r0 + i) * p.xs, row_bytes, &bars[i % S]);
-    if (HAS_RES) bulk_g2s(st + 2 * row_bytes, p.dres + (r0 + i) * p.rs, row_bytes, &bars[i % S]);
+    const uint64_t pol = l2_policy_evict_first();
+    bulk_g2s_hint(st, p.dy + (r0 + i) * p.ys, row_bytes, &bars[i % S], pol);
+    bulk_g2s_hint(st + row_bytes, p.x + (r0 + i) * p.xs, row_bytes, &bars[i % S], pol);
+    if (HAS_RES) bulk_g2s_hint(st + 2 * row_bytes, p.dres + (r0 + i) * p.rs, row_bytes, &bars[i % S], pol);
     issued = i + 1;
   };
   if (threadIdx.x == 0)
     for (int i = 0; i < S; ++i) issue(i);
   uint4 wv[K];
-  float acc[K][8];
+  float2 acc[K][4];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = threadIdx.x + k * blockDim.x;
     wv[k] = c < chunks ? ld_cached(p.w + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[k][i] = 0.f;
+    for (int i = 0; i < 4; ++i) acc[k][i] = make_float2(0.f, 0.f);
   }
   int i = 0;
   for (; i < rows; ++i) {
@@ -485,36 +516,19 @@ quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int*
         xv[k] = *reinterpret_cast<const uint4*>(st + row_bytes + c * 16);
         if (HAS_RES) rv[k] = *reinterpret_cast<const uint4*>(st + 2 * row_bytes + c * 16);
       }
-      float yf[8], xf[8], wf[8];
-      unpack8(yv[k], yf);
-      unpack8(xv[k], xf);
-      unpack8(wv[k], wf);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(xf[e] * r, yf[e] * wf[e], sum);
+      sum += chunk_dot(yv[k], xv[k], wv[k]);
     }
-    const float mean = block_sum(sum, slots, i & 1) / static_cast<float>(N);
+    const float mean = r * block_sum_lanes(sum, slots, i & 1) / static_cast<float>(N);
     if (s_abort) break;
     if (threadIdx.x == 0) issue(i + S);  // every thread has read stage i % S
-    float d[K][8];
-    uint32_t most[K];
+    float2 d[K][4];
+    float most[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = threadIdx.x + k * blockDim.x;
-      float yf[8], xf[8], wf[8], rf[8];
-      unpack8(yv[k], yf);
-      unpack8(xv[k], xf);
-      unpack8(wv[k], wf);
-      if (HAS_RES) unpack8(rv[k], rf);
-      most[k] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float xhat = xf[e] * r;
-        acc[k][e] = fmaf(yf[e], xhat, acc[k][e]);
-        d[k][e] = grad_of(yf[e] * wf[e], xhat, mean, r);
-        if (HAS_RES) d[k][e] += rf[e];
-        most[k] = max(most[k], c < chunks ? mag_bits(d[k][e]) : 0u);
-      }
-      if (p.dx && c < chunks) st_global(p.dx + row * N + c * 8, pack8(d[k]));
+      most[k] = chunk_grad<HAS_RES>(yv[k], xv[k], wv[k], rv[k], mean, r, acc[k], d[k]);
+      if (c >= chunks) most[k] = 0.f;
+      if (p.dx && c < chunks) st_stream(p.dx + row * N + c * 8, pack_pairs(d[k]));
     }
     quant_chunks<K, false, E5M2, E8M0>(p.o, row, N, p.group, threadIdx.x, blockDim.x, chunks, d, most, mslots, i & 1);
   }
@@ -526,8 +540,8 @@ quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int*
   for (int k = 0; k < K; ++k) {
     const int c = threadIdx.x + k * blockDim.x;
     if (c < chunks) {
-      *reinterpret_cast<float4*>(part + c * 8) = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
-      *reinterpret_cast<float4*>(part + c * 8 + 4) = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+      *reinterpret_cast<float4*>(part + c * 8) = make_float4(acc[k][0].x, acc[k][0].y, acc[k][1].x, acc[k][1].y);
+      *reinterpret_cast<float4*>(part + c * 8 + 4) = make_float4(acc[k][2].x, acc[k][2].y, acc[k][3].x, acc[k][3].y);
     }
   }
 }
@@ -538,7 +552,7 @@ template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(512) quant_bwd_odd(const QuantBwdP p, int64_t M, int64_t rows_per_block) {
   extern __shared__ float sacc[];  // WARP
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = (WARP ? 0 : warp * 128) + lane, step = WARP ? 128 : blockDim.x * 4;
   float acc[K][4];
@@ -574,7 +588,7 @@ __global__ void __launch_bounds__(512) quant_bwd_odd(const QuantBwdP p, int64_t 
         g[k][i] *= n < N ? bf16_to_f(__ldg(p.w + n)) : 0.f;
         sum = fmaf(xh[k][i], g[k][i], sum);
       }
-    const float mean = (WARP ? warp_sum(sum) : block_sum(sum, slots, parity)) / static_cast<float>(N);
+    const float mean = (WARP ? warp_sum(sum) : block_sum_lanes(sum, slots, parity)) / static_cast<float>(N);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -599,7 +613,7 @@ __global__ void __launch_bounds__(512) quant_bwd_odd(const QuantBwdP p, int64_t 
 template <bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(256) quant_bwd_any(const QuantBwdP p) {
   __shared__ float slots[2][32];
-  __shared__ uint32_t mslots[2][32];
+  __shared__ float mslots[2][32];
   const int64_t row = blockIdx.x;
   const uint16_t* dy = p.dy + row * p.ys;
   const uint16_t* x = p.x + row * p.xs;
@@ -608,7 +622,7 @@ __global__ void __launch_bounds__(256) quant_bwd_any(const QuantBwdP p) {
   float sum = 0.f;
   for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x)
     sum = fmaf(bf16_to_f(x[n]) * r, bf16_to_f(dy[n]) * bf16_to_f(p.w[n]), sum);
-  const float mean = block_sum(sum, slots, 0) / static_cast<float>(p.N);
+  const float mean = block_sum_lanes(sum, slots, 0) / static_cast<float>(p.N);
   auto dx = [&](int64_t n) {
     const float xhat = bf16_to_f(x[n]) * r;
     const float d = (bf16_to_f(dy[n]) * bf16_to_f(p.w[n]) - xhat * mean) * r;
@@ -690,16 +704,36 @@ int launch_bwd(const QuantBwdP& p, int64_t M, const QuantBwdPlan& pl, const RowS
   return check_launch();
 }
 
+// `units` rows (or eights of rows) over blocks that stay for R of them.  With
+// the residual, R = 4 as far as that leaves two blocks for every place on the
+// device: 32768 rows of 8192, group 128, 284 us against 357 for one and 326
+// for as many blocks as are resident; 16384 rows of 4096 75, 89 and 88.
+// Without, as many blocks as are resident: 16384 rows of 4096 40, 61 for one.
+template <class Kern>
+int launch_stay(Kern kern, int64_t units, bool has_res, int threads, const QuantFwdP& p, int64_t M, cudaStream_t s) {
+  static int per_sm[33] = {};  // by warps of a block; the same on every device of this architecture
+  int& n = per_sm[threads / 32];
+  if (n == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n == 0)) {
+    cudaGetLastError();
+    n = 1;
+  }
+  const int64_t places = static_cast<int64_t>(n) * std::max(1, sm_count());
+  const int64_t R = has_res ? std::max<int64_t>(1, std::min<int64_t>(4, units / (2 * places))) : ceil_div(units, places);
+  kern<<<static_cast<unsigned>(ceil_div(units, R)), threads, 0, s>>>(p, M, static_cast<int>(R));
+  return check_launch();
+}
+
 template <bool HAS_RES, bool E5M2, bool E8M0>
 int launch_fwd(const QuantFwdP& p, int64_t M, const RowShape& r, cudaStream_t s) {
   const unsigned rows = static_cast<unsigned>(M), warps = static_cast<unsigned>(ceil_div(M, r.threads / 32));
   switch (r.kind) {
     case ROW_WARP:
-      if (r.K == 1) quant_fwd_vec<1, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
-      else if (r.K == 2) quant_fwd_vec<2, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
-      else quant_fwd_vec<4, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
-      break;
-    case ROW_BLOCK: quant_fwd_vec<4, false, HAS_RES, E5M2, E8M0><<<rows, r.threads, 0, s>>>(p, M); break;
+      if (r.K == 1) return launch_stay(quant_fwd_vec<1, true, true, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
+      if (r.K == 2) return launch_stay(quant_fwd_vec<2, true, true, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
+      return launch_stay(quant_fwd_vec<4, true, !HAS_RES, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
+    case ROW_BLOCK:
+      if (r.K == 2) return launch_stay(quant_fwd_vec<2, false, true, HAS_RES, E5M2, E8M0>, rows, HAS_RES, r.threads, p, M, s);
+      return launch_stay(quant_fwd_vec<4, false, !HAS_RES, HAS_RES, E5M2, E8M0>, rows, HAS_RES, r.threads, p, M, s);
     case ROW_ODD_WARP:
       if (r.K == 2) quant_fwd_odd<2, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
       else if (r.K == 4) quant_fwd_odd<4, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
