@@ -75,9 +75,10 @@ constexpr int kRows = 128;          // rows of C a block holds
 constexpr int kChunk = 64;          // columns the epilogue takes at a time
 constexpr int kOperand = 128 * kTileK * 2;  // bytes of one operand of a stage
 constexpr int kStageBytes = 2 * kOperand;
-constexpr int kStages = 4;
 constexpr int kSet = 2 * kRows * kChunk * 2;  // two 16-bit chunks
-constexpr int kSets = 3;
+// Shared memory: stages of operands and sets of chunks.  Five stages and two
+// sets take 7 to 13% longer below 1100 x 1100: chunks then wait for stores.
+constexpr int kStages = 4, kSets = 3;
 constexpr int kEpiWarps = 8;
 // a loading warp, an issuing warp, the epilogue, and a warp that moves its chunks
 constexpr int kThreads = 64 + 32 * kEpiWarps + 32;
@@ -88,7 +89,7 @@ struct ChainP {
   int m, n, s, l, E, tall, steps, split;
   float2* diag;        // [E, s] B's diagonal in 32 bits and its rounding residual
   float* partials;     // split GRAM sums
-  unsigned* counters;  // grid barrier, abort, and an arrival count for each split tile
+  unsigned* counters;  // finished phases of all blocks, abort, and arrived parts of each split tile
   ResultP res;
   int* err;
   float co[3 * kMaxSteps];
@@ -266,7 +267,7 @@ __device__ __forceinline__ void write_out(const ChainP& p, uint32_t set, int e, 
 }
 
 // Every wait below is bounded (mbar_wait); after one runs out the block's
-// roles leave their loops, and so do the other blocks at the grid barrier.
+// roles leave their loops, and so do the other blocks where they wait for phases.
 
 // The loading thread: both operands' k-slices of every work item, in order.
 template <int CG>
@@ -348,20 +349,26 @@ __device__ __forceinline__ void wait_or_abort(uint64_t* bar, uint32_t parity, Sh
   __syncwarp();
 }
 
+// Add to a counter that other blocks wait on: all that this thread has seen
+// written is seen by those that see the sum.
+__device__ __forceinline__ void count_up(unsigned* count) {
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
+}
 // Wait until *count reaches `target` (bounded), or the call is given up.
-__device__ __forceinline__ bool wait_count(const ChainP& p, volatile unsigned* count, unsigned target) {
-  volatile unsigned* const given_up = p.counters + 1;
+__device__ __forceinline__ bool wait_count(const ChainP& p, const unsigned* count, unsigned target) {
   const long long t0 = clock64();
-  while (*count < target) {
-    if (*given_up) return false;
+  for (int i = 0;; ++i) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
+    if (v >= target) return true;
+    if (i & 15) continue;
+    if (*static_cast<volatile unsigned*>(p.counters + 1)) return false;
     if (clock64() - t0 > kWaitCycles) {
       if (p.err) atomicOr(p.err, FRAG_DEVFLAG_WAIT_TIMEOUT);
       atomicExch(p.counters + 1, 1u);
       return false;
     }
   }
-  __threadfence();
-  return true;
 }
 
 // Walks the chunks that this block finishes in a phase, in the order of its
@@ -396,8 +403,8 @@ struct Cursor {
   __device__ int col() const { return j0 + g * kChunk; }
 };
 
-// The moving thread: brings each chunk's inputs into one of three sets, two
-// chunks ahead of the epilogue, and stores its results.  `v` counts chunks.
+// The moving thread: brings each chunk's inputs into a set, all but one of
+// them ahead of the epilogue, and stores its results.  `v` counts chunks.
 template <int CG>
 __device__ __forceinline__ void move_phase(const ChainP& p, Shared& sh, uint32_t sets, int mode, int cur, int rank,
                                            int64_t& v) {
@@ -419,8 +426,7 @@ __device__ __forceinline__ void move_phase(const ChainP& p, Shared& sh, uint32_t
     ++ahead;
     in.next();
   };
-  bring();
-  bring();
+  for (int i = 0; i < kSets - 1; ++i) bring();
   for (; out.valid(); ++v, out.next()) {
     const uint32_t set = sets + static_cast<uint32_t>(v % kSets) * kSet;
     if (*abort_flag || !mbar_wait(&sh.written[v % kSets], static_cast<uint32_t>(v / kSets) & 1, p.err)) {
@@ -498,7 +504,7 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
       __threadfence();
       epi_sync();
       if (threadIdx.x == kLead) {
-        atomicAdd(p.counters + 2 + tile, 1u);
+        count_up(p.counters + 2 + tile);
         if (!wait_count(p, p.counters + 2 + tile, static_cast<unsigned>(w.split) * (step + 1))) *abort_flag = 1;
       }
       epi_sync();
@@ -555,7 +561,7 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
 }
 
 // All steps in one launch: every block walks each phase's work items (A, then
-// B, then X), with a grid barrier between phases.  One block per SM; CG = 2:
+// B, then X), and a count of finished blocks parts the phases.  One block per SM; CG = 2:
 // pairs of blocks share 256 x 256 tiles, each holding half of the operands.
 template <int CG>
 __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ ChainP p) {
@@ -595,47 +601,54 @@ __global__ void __launch_bounds__(kThreads, 1) chain(const __grid_constant__ Cha
   const bool loads = warp == 0 && elect_one(), issues = warp == 1 && rank == 0 && elect_one();
   const bool moves = warp == 2 + kEpiWarps && elect_one();
   int64_t n = 0, c = 0, u = 0;  // k-slices, accumulators, chunks so far
-  unsigned phase = 0;
-  bool ok = true;
-  for (int step = 0; step < p.steps && ok; ++step) {
-    const int cur = step & 1;
-    for (int ph = 0; ph < 3; ++ph) {
+  // Phase f may start when every block's mover has counted phase f - 1.  The
+  // loading thread waits for that; the others follow it from barrier to
+  // barrier, and no part of the block waits for another to end a phase.
+  auto phases = [&](auto body) {
+    for (int f = 0; f < 3 * p.steps; ++f) {
+      const int step = f / 3, ph = f - 3 * step;
       const int mode = ph < STEP ? ph : step + 1 < p.steps ? static_cast<int>(STEP) : p.res.last;
-      bool good = true;
-      if (warp == 0) {
-        if (loads) good = load_phase<CG>(p, sh, smem, mode, cur, rank, n);
-      } else if (warp == 1) {
-        if (issues) good = issue_phase<CG>(p, sh, smem, tmem, mode, n, c);
-      } else if (warp == 2 + kEpiWarps) {
-        if (moves) move_phase<CG>(p, sh, sets, mode, cur, rank, u);
-      } else {
-        switch (mode) {
-          case GRAM: finish_phase<CG, GRAM>(p, sh, sets, tmem, step, rank, c, u); break;
-          case POLY: finish_phase<CG, POLY>(p, sh, sets, tmem, step, rank, c, u); break;
-          case STEP: finish_phase<CG, STEP>(p, sh, sets, tmem, step, rank, c, u); break;
-          case LAST: finish_phase<CG, LAST>(p, sh, sets, tmem, step, rank, c, u); break;
-          default: finish_phase<CG, UPDATE>(p, sh, sets, tmem, step, rank, c, u);
-        }
-      }
-      if (!good) *abort_flag = 1;
-      __syncthreads();
-      if (step + 1 == p.steps && ph == 2) break;
-      if (threadIdx.x == 0) {
-        // every block has finished the phase
-        ++phase;
-        if (*abort_flag) atomicExch(p.counters + 1, 1u);
-        __threadfence();
-        atomicAdd(p.counters, 1u);
-        if (!wait_count(p, p.counters, phase * gridDim.x)) *abort_flag = 1;
-      }
-      __syncthreads();
-      if (loads || moves) proxy_fence();
-      if (*abort_flag) {
-        ok = false;
-        break;
+      if (!body(f, step, mode)) {
+        *abort_flag = 1;
+        atomicExch(p.counters + 1, 1u);
+        return;
       }
     }
+  };
+  auto started = [&](int f) {
+    if (f > 0 && !wait_count(p, p.counters, static_cast<unsigned>(f) * gridDim.x)) return false;
+    proxy_fence();
+    return true;
+  };
+  if (warp == 0) {
+    if (loads)
+      phases([&](int f, int step, int mode) {
+        return started(f) && load_phase<CG>(p, sh, smem, mode, step & 1, rank, n);
+      });
+  } else if (warp == 1) {
+    if (issues) phases([&](int, int, int mode) { return issue_phase<CG>(p, sh, smem, tmem, mode, n, c); });
+  } else if (warp == 2 + kEpiWarps) {
+    if (moves)
+      phases([&](int f, int step, int mode) {
+        // A has to be there; X and lo have been since the phase before A's
+        if (mode == POLY && !started(f)) return false;
+        const int64_t before = u;
+        move_phase<CG>(p, sh, sets, mode, step & 1, rank, u);
+        // a block with nothing to do in a phase may not count ahead of the others
+        if (u == before && !started(f)) return false;
+        count_up(p.counters);
+        return !*abort_flag;
+      });
+  } else {
+    for (int step = 0; step < p.steps; ++step) {
+      finish_phase<CG, GRAM>(p, sh, sets, tmem, step, rank, c, u);
+      finish_phase<CG, POLY>(p, sh, sets, tmem, step, rank, c, u);
+      if (step + 1 < p.steps) finish_phase<CG, STEP>(p, sh, sets, tmem, step, rank, c, u);
+      else if (p.res.last == LAST) finish_phase<CG, LAST>(p, sh, sets, tmem, step, rank, c, u);
+      else finish_phase<CG, UPDATE>(p, sh, sets, tmem, step, rank, c, u);
+    }
   }
+  __syncthreads();
   // nothing is in flight when shared memory and accumulators are given up
   if (loads)
     for (int64_t i = n > kStages ? n - kStages : 0; i < n && rank == 0; ++i)
@@ -767,11 +780,11 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.groups = resident(q.pairs);
   const int64_t side = q.pairs ? 256 : 128;
   q.tiles = chain_tiles(E, q.s, q.s, side, true);
-  // A's few tiles with a long k: each in up to four parts of at least four
-  // k-slices, one work item a group.  A step of 1024 x 4096 in 1, 2, 4 and 8
-  // parts: 63, 55, 49 and 49 us.
+  // A's few tiles with a long k: each in up to four parts of at least six
+  // k-slices (a part costs about 5 us, a slice 0.3), one work item a group.  A
+  // step of 1024 x 4096 in 1, 2, 4 and 8 parts: 63, 55, 49 and 49 us.
   const int64_t ks = ceil_div(q.l, kTileK);
-  q.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({q.groups / std::max<int64_t>(1, q.tiles), ks / 4, 4})));
+  q.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({q.groups / std::max<int64_t>(1, q.tiles), ks / 6, 4})));
   const size_t x = align_up(static_cast<size_t>(E) * m * q.ldx * 2, 256);
   const size_t a = align_up(static_cast<size_t>(E) * q.s * q.lds * 2, 256);
   q.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(1184, ceil_div(m * n, 2048))));
@@ -799,7 +812,7 @@ int launch_chain(const ChainP& p, int groups, cudaStream_t s) {
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeCooperative;  // the grid barrier needs every block resident
+  attr[0].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: every one is resident
   attr[0].val.cooperative = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = CG;
