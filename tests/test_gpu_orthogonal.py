@@ -45,7 +45,8 @@ def tol(g):
 
 
 SIZES = [(1, 1), (1, 7), (5, 1), (3, 200), (16, 16), (96, 160), (127, 129), (128, 128), (160, 96), (129, 1000),
-         (257, 64), (64, 1031), (500, 500), (333, 1025), (1024, 256), (700, 1300)]
+         (257, 64), (64, 1031), (500, 500), (333, 1025), (1024, 256), (700, 1300), (100, 2050), (4096, 128), (16, 4097),
+         (129, 5000), (2049, 1793), (2000, 2312), (1100, 4000)]
 
 
 @pytest.mark.parametrize("m,n", SIZES)
@@ -83,13 +84,18 @@ def test_spectra(m, n, spectrum):
     assert off(small, o.double()) <= 2 * TOL or spectrum == "rank one"
 
 
-@pytest.mark.parametrize("shape", [(3, 100, 60), (2, 2, 33, 140), (5, 128, 256)])
+@pytest.mark.parametrize("shape", [(3, 100, 60), (2, 2, 33, 140), (5, 128, 256), (3, 130, 515)])
 def test_batches(shape):
     g = normal(*shape, seed=4)
     o = ops.orthogonalize(g)
     assert off(o, exact(g)) <= TOL
     for i in range(shape[0]):  # every matrix by itself, to the bit
         assert torch.equal(ops.orthogonalize(g[i]), o[i])
+
+
+def test_batch_of_large_matrices():
+    g = normal(2, 1800, 1810, seed=4)  # (the batch's count may choose another tile: not bit for bit)
+    assert off(ops.orthogonalize(g), exact(g)) <= TOL
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -143,10 +149,11 @@ def test_reproducible_with_buffers_and_on_another_stream():
     assert torch.equal(other, want)
 
 
-def test_in_a_graph():
-    g = normal(200, 100, seed=11)
-    out = torch.empty(200, 100, dtype=torch.bfloat16, device=DEV)
-    ws = torch.empty(ops.orthogonalize_workspace_bytes(1, 200, 100), dtype=torch.uint8, device=DEV)
+@pytest.mark.parametrize("m,n", [(200, 100), (300, 700), (2304, 2304)])  # a cluster, blocks, pairs of blocks
+def test_in_a_graph(m, n):
+    g = normal(m, n, seed=11)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    ws = torch.empty(ops.orthogonalize_workspace_bytes(1, m, n), dtype=torch.uint8, device=DEV)
     want = ops.orthogonalize(g, out=out, workspace=ws).clone()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
@@ -159,7 +166,7 @@ def test_in_a_graph():
 UNIT = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -22}  # fp32: a few roundings
 
 
-@pytest.mark.parametrize("shape", [(96, 160), (2, 200, 77), (1, 5), (512, 1024)])
+@pytest.mark.parametrize("shape", [(96, 160), (2, 200, 77), (1, 5), (512, 1024), (700, 301), (1900, 2100), (120, 2600)])
 @pytest.mark.parametrize("pd,gd,md", [(torch.float32, torch.float32, torch.float32),
                                       (torch.bfloat16, torch.bfloat16, torch.bfloat16),
                                       (torch.float32, torch.bfloat16, torch.float32),
@@ -192,8 +199,26 @@ def test_update_of_strided_tensors():
     assert torch.equal(p1, p2) and torch.equal(m1, m2)
 
 
+def test_calls_on_two_streams_at_once():
+    gs = [normal(700, 900, seed=s) for s in (20, 21)]
+    want = [ops.orthogonalize(g) for g in gs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in gs]
+    got = []
+    for _ in range(3):
+        for g, s in zip(gs, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.orthogonalize(g))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])
+    ops.check_status()
+
+
 def test_refusals():
     g = normal(8, 8)
+    with pytest.raises(ValueError):
+        ops.orthogonalize(g, steps=33)
     with pytest.raises(TypeError):
         ops.orthogonalize(g.half())
     with pytest.raises(ValueError):

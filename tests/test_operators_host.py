@@ -87,3 +87,18 @@ def test_entry_points_reject_bad_arguments_on_the_host():
         None, N, None, N, None, None, None, 0, None, None, None, None, M, N, fmt, group, 0, None, 0, None)
     assert bwd(4, 64) == 1 and bwd(-1, 64) == 1 and bwd(4, 64, fmt=7) == 1
     assert bwd(4, 64, group=1) == 2 and bwd(0, 64) == 0
+
+
+def test_orthogonalize_rejects_bad_arguments_on_the_host():
+    lib = _lib.load()
+    co = (C.c_float * 15)(*([3.4, -4.8, 2.0] * 5))
+    none = _lib.Matrix(None, 0, 8, 1, 0)
+    orth = lambda E, m, n, steps=5, c=co, g=none: lib.frag_orthogonalize(  # noqa: E731
+        C.byref(g), None, E, m, n, steps, c, 1e-7, None, 0, None)
+    assert orth(1, 8, 8) == 1 and orth(-1, 8, 8) == 1 and orth(1, 8, 8, steps=0) == 1 and orth(1, 8, 8, c=None) == 1
+    assert orth(1, 8, 8, steps=33) == 2 and orth(1 << 20, 8, 8) == 2 and orth(1, 1 << 25, 8) == 2
+    assert orth(1, 1 << 16, 1 << 16) == 2  # 2^32 elements
+    assert orth(0, 8, 8) == 0 and orth(1, 0, 8) == 0
+    assert lib.frag_muon_update(C.byref(none), C.byref(none), C.byref(none), None, None, 1, 8, 8, 0.1, 0.9, 1, 0.0, 1.0,
+                                5, co, 1e-7, None, 0, None) == 1
+    assert lib.frag_orthogonalize_workspace_bytes(0, 8, 8) == 0
