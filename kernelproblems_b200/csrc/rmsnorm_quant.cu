@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t
 // the block (dy, x, dres) into a ring of S stages by bulk copies, S rows ahead
 // of the arithmetic; dweight sums stay in registers, thread-owned columns.
 template <int K, bool HAS_RES, bool E5M2, bool E8M0>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(K == 3 ? 256 : 512, K == 3 ? 2 : 1)
 quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int* err) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) unsigned char smem[];
@@ -649,8 +649,12 @@ __global__ void __launch_bounds__(256) quant_bwd_any_dw(const QuantBwdP p, int64
 struct QuantBwdPlan {
   int64_t G, rows_per_block;
 };
-// Threads of a row's block (two or four chunks each), and blocks of an SM.
-int ring_threads(int64_t N) { return static_cast<int>(std::min<int64_t>(512, ceil_div(N, N <= 8192 ? 512 : 1024) * 32)); }
+// Chunks of a thread and threads of a row's block, and blocks of an SM: two
+// chunks, but three just above 4096, where two would leave one block of little
+// more than 256 threads an SM (22686 rows of 4176, group 128: 172 us against
+// 222; from 6160 on two are faster, 8192 rows of 8192 111 against 155 for four).
+int ring_chunks(int64_t N) { return N <= 4096 ? 2 : N <= 6144 ? 3 : N <= 8192 ? 2 : 4; }
+int ring_threads(int64_t N) { return static_cast<int>(ceil_div(N, 256 * ring_chunks(N)) * 32); }
 int ring_blocks(int threads) { return std::max(1, std::min(4, 512 / threads)); }
 
 QuantBwdPlan quant_bwd_plan(int64_t M, int64_t N) {
@@ -685,8 +689,11 @@ int launch_bwd(const QuantBwdP& p, int64_t M, const QuantBwdPlan& pl, const RowS
       else quant_bwd_warp<2, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
       return check_launch();
     case ROW_BLOCK:
-      return p.N <= 8192 ? launch_bwd_ring<2, HAS_RES, E5M2, E8M0>(p, M, pl, s)
-                         : launch_bwd_ring<4, HAS_RES, E5M2, E8M0>(p, M, pl, s);
+      switch (ring_chunks(p.N)) {
+        case 2: return launch_bwd_ring<2, HAS_RES, E5M2, E8M0>(p, M, pl, s);
+        case 3: return launch_bwd_ring<3, HAS_RES, E5M2, E8M0>(p, M, pl, s);
+        default: return launch_bwd_ring<4, HAS_RES, E5M2, E8M0>(p, M, pl, s);
+      }
     case ROW_ODD_WARP:
       if (r.K == 2) quant_bwd_odd<2, true, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
       else quant_bwd_odd<4, true, HAS_RES, E5M2, E8M0><<<G, 256, wsmem, s>>>(p, M, pl.rows_per_block);
