@@ -12,8 +12,12 @@
 // Only A crosses blocks: two cluster barriers a step, nothing in global memory.
 //
 // The same 64-column block of X is A's K-major operand (rows of k) and X's
-// MN-major one (rows across k), so it is stored once.  Bound: latency, about
-// 40 dependent tensor and barrier steps.
+// MN-major one (rows across k), so it is stored once.
+//
+// Bound: latency.  A step takes 4 us in one block (96 x 160: 33 us for five
+// steps and the rest) and 9 over eight (128 x 2048: 59), where the sum of A over
+// the cluster is the larger part; the launch, reading the matrix and writing the
+// result take 13.  The same sizes through orthogonal.cu's chain: 92 and 128.
 #include <algorithm>
 #include <mutex>
 

@@ -10,6 +10,12 @@
 // Gradient: xhat = x rstd, g = dy w,
 //   dx = dres + (g - xhat mean(xhat g)) rstd,  dw = sum over rows of dy xhat
 // rounded once to bf16 and once, from the same 32 bits, to 8.
+//
+// Bound: HBM with the residual (32768 rows of 8192, group 128: 284 us, 6.6 TB/s,
+// the measured copy's rate; scales for whole rows 278), instruction issue
+// without (three bytes a value: 16384 rows of 4096 41 us for a floor of 31, 52
+// with a scale for each 128) and in the gradient (8192 rows of 4096 with the
+// residual 58 us for a floor of 46, 3.5 of them the dweight's second pass).
 #include <algorithm>
 
 #include "quant.cuh"

@@ -1094,19 +1094,18 @@ def _matrices(t: torch.Tensor, name: str, dev: torch.device | None = None, shape
     E = 1
     for d in t.shape[:-2]:
         E *= d
-    sb = 0
-    if t.dim() > 2 and E > 0:
-        # a stride for the leading dimensions together
+    sb = span = None
+    if E > 0:  # one stride for the leading dimensions together
         for size, stride in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
             if size == 1:
                 continue
-            if sb == 0:
+            if sb is None:
                 sb, span = stride, size * stride
             elif stride != span:
                 raise ValueError(f"{name}'s leading dimensions must collapse into one stride")
             else:
                 span *= size
-    return E, m, n, _lib.Matrix(t.data_ptr(), sb, t.stride(-2), t.stride(-1), _DT[t.dtype])
+    return E, m, n, _lib.Matrix(t.data_ptr(), sb or 0, t.stride(-2), t.stride(-1), _DT[t.dtype])
 
 
 def _schedule(steps: int, coefficients):

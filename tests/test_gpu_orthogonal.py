@@ -102,7 +102,7 @@ def test_batch_of_large_matrices():
 def test_strides(dtype):
     base = normal(4, 130, 222, seed=5, dtype=dtype)
     for g in (base[0].t(), base[:, 3:100, 7:201], base[::2, ::2, ::3], base[1:2].expand(3, 130, 222),
-              base.transpose(1, 2), normal(60, 1, seed=6, dtype=dtype).expand(60, 70)[:, :1]):
+              base.transpose(1, 2), base[:1, None].expand(1, 3, 130, 222), normal(60, 1, seed=6, dtype=dtype).expand(60, 70)[:, :1]):
         o = ops.orthogonalize(g)
         assert torch.equal(o, ops.orthogonalize(g.contiguous()))
         assert off(o, exact(g)) <= tol(g)
@@ -235,6 +235,8 @@ def test_refusals():
         ops.orthogonalize(g, out=torch.empty(8, 9, dtype=torch.bfloat16, device=DEV))
     with pytest.raises(ValueError):
         ops.orthogonalize(normal(4, 6, 8, 8)[:, :5])
+    with pytest.raises(ValueError):  # a repeated dimension inside another
+        ops.orthogonalize(normal(4, 1, 8, 8).expand(4, 3, 8, 8))
     with pytest.raises(ValueError):
         ops.muon_update(g, normal(8, 9), g.clone(), lr=0.1)
     with pytest.raises(ValueError):
