@@ -315,6 +315,7 @@ __device__ __forceinline__ bool issue_phase(const ChainP& p, Shared& sh, uint32_
   const bool p_mn = mode == GRAM && p.tall, q_mn = mode == GRAM ? p.tall : mode >= STEP && !p.tall;
   const uint32_t idesc = instr_desc_f16(w.TM, w.TN, p_mn, q_mn);
   const uint64_t ka = desc_k16(p_mn), kb = desc_k16(q_mn);
+  const uint64_t first_a = smem_desc(smem, p_mn), first_b = smem_desc(smem + kOperand, q_mn);
   volatile int* const abort_flag = &sh.abort;
   for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG, ++c) {
     int e, ti, tj, z;
@@ -328,8 +329,7 @@ __device__ __forceinline__ bool issue_phase(const ChainP& p, Shared& sh, uint32_
       const int st = static_cast<int>(n % kStages);
       if (*abort_flag || !mbar_wait(&sh.full[st], static_cast<uint32_t>(n / kStages) & 1, p.err)) return false;
       tc_fence_after();
-      const uint32_t sp = smem + st * kStageBytes;
-      const uint64_t da = smem_desc(sp, p_mn), db = smem_desc(sp + kOperand, q_mn);
+      const uint64_t da = first_a + st * (kStageBytes >> 4), db = first_b + st * (kStageBytes >> 4);
 #pragma unroll
       for (int kk = 0; kk < kTileK / 16; ++kk)
         mma_f16<CG>(d, da + kk * ka, db + kk * kb, idesc, k > k0 || kk > 0);

@@ -9,15 +9,22 @@
 //      order over the cluster, and writes it, a row of the symmetric A, to all
 //   B  every block makes b A + c A A for itself, in A's place
 //   X  every block updates its own columns where they are
-// Only A crosses blocks: two cluster barriers a step, nothing in global memory.
+// Only A crosses blocks: two or three cluster barriers a step, nothing in global
+// memory.
+//
+// Results in bf16 take the chain's arithmetic (single fp16 operands, B's
+// diagonal in 32 bits): an error of 0.6 to 1.5e-3 under a rounding of 1.7e-3.
+// Where the result is stored in 32 bits (FINE), A and B are kept as two fp16
+// numbers like X and each product takes hi hi, hi lo and lo hi: 5e-7 at 64 x
+// 100, for 12 to 25 us more.
 //
 // The same 64-column block of X is A's K-major operand (rows of k) and X's
 // MN-major one (rows across k), so it is stored once.
 //
-// Bound: latency.  A step takes 4 us in one block (96 x 160: 33 us for five
+// Bound: latency.  A step takes 4 us in one block (96 x 160: 31 us for five
 // steps and the rest) and 9 over eight (128 x 2048: 59), where the sum of A over
 // the cluster is the larger part; the launch, reading the matrix and writing the
-// result take 13.  The same sizes through orthogonal.cu's chain: 92 and 128.
+// result take 11 to 15.  The same sizes through orthogonal.cu's chain: 92, 128.
 #include <algorithm>
 #include <mutex>
 
@@ -29,8 +36,8 @@ namespace {
 constexpr int kSide = 128;
 constexpr int kMaxBlocks = 4;                 // of 64 columns a block holds
 constexpr int kBlock = kSide * 64 * 2;        // bytes of one, 16 bits
-constexpr int kPart = kSide * kSide * 4;      // partial A, columns of 128 rows
-constexpr int kASize = kSide * kSide * 2;     // A, then B: two 64-column blocks
+constexpr int kPart = kSide * kSide * 4;      // partial A, columns of 128 rows; then A's (and B's) lo
+constexpr int kASize = kSide * kSide * 2;     // hi of A, then of B: two 64-column blocks
 constexpr int kSmallThreads = 256;
 constexpr int kMaxCluster = 16;
 
@@ -47,8 +54,8 @@ struct SmallShared {
   uint32_t tmem;
   int abort;
   float slots[2][32];
-  float sum;             // of this block's squares
-  float2 coef[kSide];    // hi's and lo's factors by row
+  float sum;           // of this block's squares
+  float2 coef[kSide];  // hi's and lo's factors by row (not FINE)
 };
 
 __device__ __forceinline__ uint32_t small_tail(int blocks) { return 2 * blocks * kBlock + kPart + kASize; }
@@ -167,11 +174,11 @@ __device__ __forceinline__ float small_in(const SmallP& p, uint32_t hi, uint32_t
   return ss;
 }
 
-template <int V>
+template <int V, bool FINE>
 __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_constant__ SmallP p, int C) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t hi = smem_u32(smem_raw), lo = hi + p.blocks * kBlock, part = lo + p.blocks * kBlock;
-  const uint32_t am = part + kPart;
+  const uint32_t am = part + kPart, al = part;  // A's hi and lo
   SmallShared& sh = *reinterpret_cast<SmallShared*>(smem_raw + small_tail(p.blocks));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
@@ -186,10 +193,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   }
   if (warp == 0) tmem_alloc<1>(&sh.tmem, 512);
   // zeros past the matrix's rows and columns
-  const int words = (2 * p.blocks * kBlock + kPart + kASize) / 16;
-  for (int i = threadIdx.x; i < words; i += kSmallThreads)
-    if (i < 2 * p.blocks * (kBlock / 16) || i >= (2 * p.blocks * kBlock + kPart) / 16)
-      st_shared(hi + i * 16, make_uint4(0, 0, 0, 0));
+  for (int i = threadIdx.x; i < static_cast<int>(small_tail(p.blocks)) / 16; i += kSmallThreads)
+    st_shared(hi + i * 16, make_uint4(0, 0, 0, 0));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -238,71 +243,116 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   };
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   const int k16 = (p.s + 15) / 16;
+  // eight values' hi and lo in two units
+  auto split8 = [](const float* v, uint4& oh, uint4& ol) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __half2 t = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
+      const float2 back = __half22float2(t);
+      const __half2 rest = __floats2half2_rn(v[2 * q] - back.x, v[2 * q + 1] - back.y);
+      reinterpret_cast<uint32_t*>(&oh)[q] = *reinterpret_cast<const uint32_t*>(&t);
+      reinterpret_cast<uint32_t*>(&ol)[q] = *reinterpret_cast<const uint32_t*>(&rest);
+    }
+  };
+  constexpr float a_scale = kAScale / (kXScale * kXScale);
+  // operands: X's columns along and across k, A and B (and their lo); a block
+  // of 64 columns further is kBlock / 16 more
+  const uint64_t xh = smem_desc(hi, false), xl = smem_desc(lo, false);
+  const uint64_t yh = smem_desc(hi, true, kBlock), yl = smem_desc(lo, true, kBlock);
+  const uint64_t ah = smem_desc(am, false), ax = smem_desc(al, false);
+  constexpr uint64_t kNext = kBlock >> 4;
+  const uint32_t id_a = instr_desc_f16(kSide, kSide, false, false);
+  const uint32_t id_x = instr_desc_f16(kSide, 64 * p.blocks, false, true);
 
   for (int step = 0; step < p.steps; ++step) {
     const float ca = p.co[3 * step], cb = p.co[3 * step + 1], cc = p.co[3 * step + 2] / kAScale;
     // ---- A = X X'
     publish();
     if (threadIdx.x == 0) {
-      for (int b = 0; b < p.blocks; ++b) {
-        const uint64_t d = smem_desc(hi + b * kBlock, false);
-        for (int k = 0; k < 4; ++k)
-          mma_f16<1>(tmem, d + k * desc_k16(false), d + k * desc_k16(false), instr_desc_f16(kSide, kSide, false, false),
-                     b + k > 0);
-      }
+      uint64_t o = 0;
+      for (int b = 0; b < p.blocks; ++b, o += kNext)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint64_t h = xh + o + 2 * k, l = xl + o + 2 * k;
+          mma_f16<1>(tmem, h, h, id_a, b + k > 0);
+          if (!FINE) continue;
+          mma_f16<1>(tmem, h, l, id_a, true);
+          mma_f16<1>(tmem, l, h, id_a, true);
+        }
       mma_commit<1>(&sh.bar);
     }
     wait();
-    if (C == 1) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float v[32];
-        tmem_load32(lanes + half * 64 + g * 32, v);
+    for (int g = 0; g < 2; ++g) {
+      float v[32];
+      tmem_load32(lanes + half * 64 + g * 32, v);
+      if (C == 1) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= kAScale / (kXScale * kXScale);
+        for (int k = 0; k < 32; ++k) v[k] *= a_scale;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) st_shared(unit(am + half * kBlock, r, g * 4 + u), pack_h8(v + 8 * u));
-      }
-    } else {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float v[32];
-        tmem_load32(lanes + half * 64 + g * 32, v);
+        for (int u = 0; u < 4; ++u) {
+          uint4 oh = pack_h8(v + 8 * u), ol;
+          if (FINE) split8(v + 8 * u, oh, ol);
+          st_shared(unit(am + half * kBlock, r, g * 4 + u), oh);
+          if (FINE) st_shared(unit(al + half * kBlock, r, g * 4 + u), ol);
+        }
+      } else {
 #pragma unroll
         for (int k = 0; k < 32; ++k)
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + ((half * 64 + g * 32 + k) * kSide + r) * 4), "f"(v[k])
                        : "memory");
       }
+    }
+    if (C > 1) {
       cluster_sync();
-      // columns c, c + C, ... of all partials: row j of A
-      for (int j = c + C * warp; j < p.s; j += C * (kSmallThreads / 32)) {
+      // columns c, c + C, ... of all partials, at most eight a warp: rows of A
+      constexpr int kRowsOfWarp = 8;
+      float4 t[kRowsOfWarp];
+#pragma unroll
+      for (int n = 0; n < kRowsOfWarp; ++n) {
+        const int j = c + C * (warp + n * (kSmallThreads / 32));
+        t[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j >= p.s) continue;
         const uint32_t from = part + (j * kSide + 4 * lane) * 4;
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int q0 = 0; q0 < C; q0 += 8) {
           float4 x[8];
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             x[q] = q0 + q < C ? ld_cluster_f4(cluster_address(from, q0 + q)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) t.x += x[q].x, t.y += x[q].y, t.z += x[q].z, t.w += x[q].w;
+          for (int q = 0; q < 8; ++q) t[n].x += x[q].x, t[n].y += x[q].y, t[n].z += x[q].z, t[n].w += x[q].w;
         }
-        constexpr float scale = kAScale / (kXScale * kXScale);
-        const __half2 a = __floats2half2_rn(t.x * scale, t.y * scale), b = __floats2half2_rn(t.z * scale, t.w * scale);
-        const uint32_t to = unit(am + (lane >> 4) * kBlock, j, (lane & 15) >> 1) + (lane & 1) * 8;
-        for (int q = 0; q < C; ++q)
-          st_cluster_u2(cluster_address(to, q), *reinterpret_cast<const uint32_t*>(&a),
-                        *reinterpret_cast<const uint32_t*>(&b));
       }
+      if (FINE) cluster_sync();  // every partial is read: lo takes its place
+#pragma unroll
+      for (int n = 0; n < kRowsOfWarp; ++n) {
+        const int j = c + C * (warp + n * (kSmallThreads / 32));
+        if (j >= p.s) continue;
+        const float v[8] = {t[n].x * a_scale, t[n].y * a_scale, t[n].z * a_scale, t[n].w * a_scale, 0.f, 0.f, 0.f, 0.f};
+        uint4 oh, ol;
+        split8(v, oh, ol);
+        const uint32_t to = unit((lane >> 4) * kBlock, j, (lane & 15) >> 1) + (lane & 1) * 8;
+        for (int q = 0; q < C; ++q) {
+          st_cluster_u2(cluster_address(am + to, q), oh.x, oh.y);
+          if (FINE) st_cluster_u2(cluster_address(al + to, q), ol.x, ol.y);
+        }
+      }
+      // rows past the matrix hold partials where lo has to be zero
+      for (int i = threadIdx.x; FINE && i < 2 * (kSide - p.s) * 8; i += kSmallThreads)
+        st_shared(al + (i / ((kSide - p.s) * 8)) * kBlock + p.s * 128 + (i % ((kSide - p.s) * 8)) * 16,
+                  make_uint4(0, 0, 0, 0));
       proxy_fence();
       cluster_sync();
     }
     // ---- B = b A + c A A
     publish();
     if (threadIdx.x == 0) {
-      const uint32_t id = instr_desc_f16(kSide, kSide, false, false);
       for (int k = 0; k < k16; ++k) {
-        const uint64_t d = smem_desc(am + (k >> 2) * kBlock, false) + (k & 3) * desc_k16(false);
-        mma_f16<1>(tmem + kSide, d, d, id, k > 0);
+        const uint64_t o = (k >> 2) * kNext + (k & 3) * 2;
+        mma_f16<1>(tmem + kSide, ah + o, ah + o, id_a, k > 0);
+        if (!FINE) continue;
+        mma_f16<1>(tmem + kSide, ah + o, ax + o, id_a, true);
+        mma_f16<1>(tmem + kSide, ax + o, ah + o, id_a, true);
       }
       mma_commit<1>(&sh.bar);
     }
@@ -313,19 +363,23 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
       tmem_load32(lanes + kSide + half * 64 + g * 32, v);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint32_t at = unit(am + half * kBlock, r, g * 4 + u);
-        const uint4 a = ld_shared(at);
+        const uint32_t uh = unit(am + half * kBlock, r, g * 4 + u), ul = unit(al + half * kBlock, r, g * 4 + u);
+        const uint4 h = ld_shared(uh), l = FINE ? ld_shared(ul) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t w = u4_word(a, q);
-          const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w));
-          v[8 * u + 2 * q] = fmaf(v[8 * u + 2 * q], cc, cb * t.x);
-          v[8 * u + 2 * q + 1] = fmaf(v[8 * u + 2 * q + 1], cc, cb * t.y);
+          const uint32_t hw = u4_word(h, q), lw = u4_word(l, q);
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lw));
+          v[8 * u + 2 * q] = fmaf(v[8 * u + 2 * q], cc, cb * (FINE ? x.x + y.x : x.x));
+          v[8 * u + 2 * q + 1] = fmaf(v[8 * u + 2 * q + 1], cc, cb * (FINE ? x.y + y.y : x.y));
         }
-        st_shared(at, pack_h8(v + 8 * u));
+        uint4 oh = pack_h8(v + 8 * u), ol;
+        if (FINE) split8(v + 8 * u, oh, ol);
+        st_shared(uh, oh);
+        if (FINE) st_shared(ul, ol);
       }
       const int j = half * 64 + g * 32;
-      if (r >= j && r < j + 32) {
+      if (!FINE && r >= j && r < j + 32) {
         float d = 0.f;
 #pragma unroll
         for (int k = 0; k < 32; ++k) d = j + k == r ? v[k] : d;
@@ -336,43 +390,43 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
     // ---- X = a X + B X
     publish();
     if (threadIdx.x == 0) {
-      const uint32_t id = instr_desc_f16(kSide, 64 * p.blocks, false, true);
-      for (int k = 0; k < k16; ++k)
-        mma_f16<1>(tmem + 2 * kSide, smem_desc(am + (k >> 2) * kBlock, false) + (k & 3) * desc_k16(false),
-                   smem_desc(hi, true, kBlock) + k * desc_k16(true), id, k > 0);
+      for (int k = 0; k < k16; ++k) {
+        const uint64_t o = (k >> 2) * kNext + (k & 3) * 2, ox = static_cast<uint64_t>(k) * 128;
+        mma_f16<1>(tmem + 2 * kSide, ah + o, yh + ox, id_x, k > 0);
+        if (!FINE) continue;
+        mma_f16<1>(tmem + 2 * kSide, ax + o, yh + ox, id_x, true);
+        mma_f16<1>(tmem + 2 * kSide, ah + o, yl + ox, id_x, true);
+      }
       mma_commit<1>(&sh.bar);
     }
     wait();
-    const float2 coef = sh.coef[r];
     const bool last = step + 1 == p.steps;
+    const float2 coef = FINE ? make_float2(ca, ca) : sh.coef[r], k2 = make_float2(1.0f / kAScale, 1.0f / kAScale);
+    const float2 fh = make_float2(coef.x, coef.x), fl = make_float2(coef.y, coef.y);
     for (int b = 0; b < p.blocks; ++b) {
       float v[32];
       tmem_load32(lanes + 2 * kSide + b * 64 + half * 32, v);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint32_t ah = unit(hi + b * kBlock, r, half * 4 + u), al = unit(lo + b * kBlock, r, half * 4 + u);
-        const uint4 h = ld_shared(ah), l = ld_shared(al);
-        uint4 oh, ol;
+        const uint32_t uh = unit(hi + b * kBlock, r, half * 4 + u), ul = unit(lo + b * kBlock, r, half * 4 + u);
+        const uint4 h = ld_shared(uh), l = ld_shared(ul);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t hw = u4_word(h, q), lw = u4_word(l, q);
           float2* y = reinterpret_cast<float2*>(v + 8 * u + 2 * q);
-          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hw)), make_float2(coef.x, coef.x),
-                          __fmul2_rn(*y, make_float2(1.0f / kAScale, 1.0f / kAScale)));
-          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lw)), make_float2(coef.y, coef.y), *y);
-          const __half2 t = __float22half2_rn(*y);
-          const float2 back = __half22float2(t);
-          const __half2 rest = __floats2half2_rn(y->x - back.x, y->y - back.y);
-          reinterpret_cast<uint32_t*>(&oh)[q] = *reinterpret_cast<const uint32_t*>(&t);
-          reinterpret_cast<uint32_t*>(&ol)[q] = *reinterpret_cast<const uint32_t*>(&rest);
+          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lw)), fl, __fmul2_rn(*y, k2));
+          *y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hw)), fh, *y);
         }
+        uint4 oh, ol;
+        const float* y = v + 8 * u;
         if (last) {  // 32 bits a value: four in each place
-          const float* y = v + 8 * u;
           oh = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
           ol = make_uint4(__float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7]));
+        } else {
+          split8(y, oh, ol);
         }
-        st_shared(ah, oh);
-        st_shared(al, ol);
+        st_shared(uh, oh);
+        st_shared(ul, ol);
       }
     }
   }
@@ -411,7 +465,9 @@ bool cluster_fits(int C) {
   if (d < 0 || d >= 64) return false;
   std::lock_guard<std::mutex> lk(mu);
   if (known[d][C]) return known[d][C] == 2;
-  for (const void* kern : {reinterpret_cast<const void*>(small_chain<1>), reinterpret_cast<const void*>(small_chain<8>)}) {
+  for (const void* kern :
+       {reinterpret_cast<const void*>(small_chain<1, false>), reinterpret_cast<const void*>(small_chain<1, true>),
+        reinterpret_cast<const void*>(small_chain<8, false>), reinterpret_cast<const void*>(small_chain<8, true>)}) {
     if (!allow_dynamic_smem(kern, small_smem(kMaxBlocks))) return false;
     if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
       cudaGetLastError();
@@ -422,7 +478,7 @@ bool cluster_fits(int C) {
   cudaLaunchAttribute attr[1];
   cluster_config(cfg, attr, C, C, small_smem(kMaxBlocks), nullptr);
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, small_chain<8>, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, small_chain<8, true>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
@@ -455,7 +511,9 @@ int orthogonalise_small(const PrepP& prep, int64_t E, int steps, const float* co
   const bool wide_access = chunked(prep.g, E, m, n) && chunked(res.out, E, m, n) &&
                            (res.last != UPDATE || chunked(res.par, E, m, n)) &&
                            (!prep.has_mom || (chunked(prep.mom, E, m, n) && chunked(prep.mom_out, E, m, n)));
-  return cuda_status(cudaLaunchKernelEx(&cfg, wide_access ? small_chain<8> : small_chain<1>, p, C));
+  auto kern = res.out.f32 ? (wide_access ? small_chain<8, true> : small_chain<1, true>)
+                          : (wide_access ? small_chain<8, false> : small_chain<1, false>);
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, p, C));
 }
 
 }  // namespace frag

@@ -192,6 +192,19 @@ def test_update(shape, pd, gd, md, nesterov):
     assert torch.equal(q, p1) and torch.equal(n, m1)
 
 
+@pytest.mark.parametrize("m,n", [(24, 100), (96, 160), (128, 700), (1500, 100), (3, 200)])
+def test_short_sided_updates_in_32_bits(m, n):
+    """With a side of at most 128 and weights in 32 bits the products take three
+    terms: 5e-7 in a 64-bit emulation at 24 x 100, accumulators in 32 bits
+    beside it; the step is as large as the weights, so that it shows."""
+    p, g, mom = (normal(m, n, seed=s) for s in (22, 23, 24))
+    p1, _ = ops.muon_update(p, g, mom, lr=1.0, momentum=0.5, nesterov=False, scale=math.sqrt(max(m, n)))
+    o = exact(0.5 * mom.double() + 0.5 * g.double())
+    p64 = p.double() - math.sqrt(max(m, n)) * o
+    err = torch.linalg.vector_norm(p1.double() - p64)
+    assert err <= 1e-5 * math.sqrt(max(m, n)) * torch.linalg.vector_norm(o) + 2.0 ** -22 * torch.linalg.vector_norm(p64)
+
+
 def test_update_of_strided_tensors():
     p, g, m = (normal(130, 90, seed=s).t() for s in (15, 16, 17))
     p1, m1 = ops.muon_update(p, g, m, lr=0.1)
