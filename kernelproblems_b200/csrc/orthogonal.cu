@@ -187,7 +187,6 @@ __device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set
 #pragma unroll
         for (int k = 0; k < 32; ++k) d = j + k == i ? v[k] : d;
         p.diag[static_cast<int64_t>(e) * p.s + i] = make_float2(d, d - __half2float(__float2half_rn(d)));
-        __threadfence();
       }
     }
 #pragma unroll
