@@ -13,6 +13,7 @@ after every embedding call (what torch's device-side assert would catch).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import os
 
@@ -64,6 +65,11 @@ def _ptr(t: torch.Tensor | None):
 
 def _stream(dev: torch.device):
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
+
+
+def _new(like: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+    """A new tensor on like's device (one integer size: 1.6 us, a tuple: 2.5)."""
+    return like.new_empty(shape[0] if len(shape) == 1 else shape, dtype=dtype)
 
 
 class _on_device:
@@ -981,17 +987,17 @@ def _quant_out(x: torch.Tensor, N: int, dtype, group: int, scale_dtype, dev):
         raise TypeError("scale_dtype must be float32 or float8_e8m0fnu")
     q = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     shape = x.shape[:-1] + (-(-N // group),) if group else x.shape[:-1]
-    return q, x.new_empty(shape, dtype=scale_dtype)
+    return q, _new(x, shape, scale_dtype)
 
 
-def _workspace(given: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor:
+def _workspace(given: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
     """The caller's workspace where it is large enough, or a new one."""
     if given is not None:
-        if not isinstance(given, torch.Tensor) or given.device != dev or not given.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        if not isinstance(given, torch.Tensor) or given.device != like.device or not given.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {like.device}")
         if given.numel() * given.element_size() >= need and given.data_ptr() % 256 == 0:
             return given
-    return torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    return like.new_empty(max(need, 16), dtype=torch.uint8)
 
 
 def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
@@ -1022,7 +1028,7 @@ def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, 
     h = None
     if residual is not None and write_h:
         h = torch.empty_like(x, memory_format=torch.contiguous_format)
-    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32) if save_rstd else None
+    rstd = _new(x, x.shape[:-1], torch.float32) if save_rstd else None
     wc = weight.contiguous()
     with _on_device(dev):
         _lib.call("frag_rmsnorm_quant_fwd", _ptr(x2), xs, _ptr(r2), rs, _ptr(wc), _ptr(q), _ptr(scale), _ptr(h),
@@ -1058,11 +1064,11 @@ def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
         raise ValueError(f"rstd must be contiguous with {M} elements")
     q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if write_dx else None
-    dw = weight.new_empty((N,), dtype=torch.float32) if compute_dw else None
+    dw = weight.new_empty(N, dtype=torch.float32) if compute_dw else None
     wc = weight.contiguous()
     with _on_device(dev):
         need = int(_lib.load().frag_rmsnorm_quant_bwd_workspace_bytes(M, N))
-        workspace = _workspace(workspace, need, dev)
+        workspace = _workspace(workspace, need, x)
         _lib.call("frag_rmsnorm_quant_bwd", _ptr(y2), ys, _ptr(x2), xs, _ptr(rstd), _ptr(wc), _ptr(r2), rs,
                   _ptr(dx), _ptr(q), _ptr(scale), _ptr(dw), M, N, _FP8[dtype], group,
                   int(scale_dtype != torch.float32), _ptr(workspace),
@@ -1108,13 +1114,20 @@ def _matrices(t: torch.Tensor, name: str, dev: torch.device | None = None, shape
     return E, m, n, _lib.Matrix(t.data_ptr(), sb or 0, t.stride(-2), t.stride(-1), _DT[t.dtype])
 
 
+@functools.lru_cache(maxsize=64)
+def _repeated(steps: int, a: float, b: float, c: float):
+    return (C.c_float * (3 * steps))(*([a, b, c] * steps))
+
+
 def _schedule(steps: int, coefficients):
     """The C array of `steps` triples: one triple for all, or one for each."""
     if not isinstance(steps, int) or not 1 <= steps <= 32:
         raise ValueError("steps must be an integer from 1 to 32")
     rows = list(coefficients)
     if len(rows) == 3 and all(isinstance(c, (int, float)) for c in rows):
-        rows = [rows] * steps
+        if not all(math.isfinite(c) for c in rows):
+            raise ValueError("coefficients must be finite")
+        return _repeated(steps, *rows)
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError("coefficients must be a triple (a, b, c) or one for each step")
     flat = [float(c) for r in rows for c in r]
@@ -1141,12 +1154,12 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ
     E, m, n, desc = _matrices(g, "g")
     dev = g.device
     if out is None:
-        out = torch.empty(g.shape, dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(g, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
     else:
         _check_out(out, "out", torch.bfloat16, dev, shape=g.shape)
     co = _schedule(steps, coefficients)
     with _on_device(dev):
-        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), dev)
+        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), g)
         _lib.call("frag_orthogonalize", C.byref(desc), _ptr(out), E, m, n, steps, co, float(eps), _ptr(workspace),
                   workspace.numel() * workspace.element_size(), _stream(dev))
     return out
@@ -1180,7 +1193,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
     outs = []
     for name, given, like in (("param_out", param_out, param), ("momentum_out", momentum_out, momentum_buffer)):
         if given is None:
-            given = torch.empty(like.shape, dtype=like.dtype, device=dev)
+            given = torch.empty_like(like, memory_format=torch.contiguous_format)
         else:
             _check_out(given, name, like.dtype, dev, shape=like.shape)
             for other in (param, grad, momentum_buffer):
@@ -1193,7 +1206,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
         raise ValueError("param_out and momentum_out overlap")
     co = _schedule(steps, coefficients)
     with _on_device(dev):
-        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), dev)
+        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), param)
         _lib.call("frag_muon_update", C.byref(dp), C.byref(dg), C.byref(dm), _ptr(outs[0]), _ptr(outs[1]), E, m, n,
                   float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), steps, co,
                   float(eps), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(dev))
