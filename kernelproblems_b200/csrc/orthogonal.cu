@@ -86,7 +86,7 @@ constexpr int kThreads = 64 + 32 * kEpiWarps + 32;
 struct ChainP {
   // X's two buffers by 64 columns x 128 rows and by 64 x 64, lo, A and B
   CUtensorMap xk[2], xm[2], lo, ak, bk, a64, b64;
-  int m, n, s, l, E, tall, steps, split;
+  int m, n, s, l, E, tall, steps, split, narrow;
   float2* diag;        // [E, s] B's diagonal in 32 bits and its rounding residual
   float* partials;     // split GRAM sums
   unsigned* counters;  // finished phases of all blocks, abort, and arrived parts of each split tile
@@ -95,11 +95,14 @@ struct ChainP {
   float co[3 * kMaxSteps];
 };
 
-// One phase's product C[i, j] = sum_k P[i, k] Q[j, k] as a list of work items.
+// One phase's product C[i, j] = sum_k P[i, k] Q[j, k] as a list of work items:
+// tiles of TM rows and `tn` columns.  A symmetric product takes the tiles that
+// reach the diagonal or lie below it; a narrow one (pairs of blocks, 128
+// columns) has twice as many of them.
 template <int CG>
 struct Work {
   static constexpr int TM = kRows * CG, TN = 128 * CG;
-  int I, J, ks, split, ti_count, tj_count, per, items, E;
+  int I, J, ks, split, ti_count, tj_count, per, items, E, tn, ratio;
   bool sym, cols_fast;
   __device__ Work(const ChainP& p, int mode) {
     sym = mode == GRAM || mode == POLY;
@@ -108,9 +111,11 @@ struct Work {
     E = p.E;
     ks = ((mode == GRAM ? p.l : p.s) + kTileK - 1) / kTileK;
     split = mode == GRAM ? p.split : 1;
+    ratio = CG == 2 && sym && p.narrow ? 2 : 1;
+    tn = TN / ratio;
     ti_count = (I + TM - 1) / TM;
-    tj_count = (J + TN - 1) / TN;
-    per = sym ? ti_count * (ti_count + 1) / 2 : ti_count * tj_count;
+    tj_count = (J + tn - 1) / tn;
+    per = sym ? ratio * ti_count * (ti_count - 1) / 2 + tj_count : ti_count * tj_count;
     items = per * E * split;
     // the long side's tiles go last, so that blocks at work share the operands
     cols_fast = p.tall;
@@ -121,11 +126,11 @@ struct Work {
     z = w - t * split;
     e = t / per;
     t -= e * per;
-    if (sym) {
-      ti = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-      while (ti * (ti + 1) / 2 > t) --ti;
-      while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-      tj = t - ti * (ti + 1) / 2;
+    if (sym) {  // row ti has ratio (ti + 1) tiles (the last row tj_count)
+      ti = static_cast<int>((sqrtf(8.0f * t / ratio + 1.0f) - 1.0f) * 0.5f);
+      while (ratio * ti * (ti + 1) / 2 > t) --ti;
+      while (ratio * (ti + 1) * (ti + 2) / 2 <= t) ++ti;
+      tj = t - ratio * ti * (ti + 1) / 2;
     } else if (cols_fast) {
       ti = t / tj_count;
       tj = t - ti * tj_count;
@@ -134,9 +139,11 @@ struct Work {
       ti = t - tj * ti_count;
     }
   }
+  // Whether a tile lies wholly below the diagonal: its transpose is written too.
+  __device__ bool mirrored(int ti, int tj) const { return sym && tj < ratio * ti; }
   // Chunks of the block's rows from i0 on in the tile's columns from j0 on.
   __device__ int chunks(int i0, int j0) const {
-    return i0 < I ? min(TN / kChunk, (J - j0 + kChunk - 1) / kChunk) : 0;
+    return i0 < I ? min(tn / kChunk, (J - j0 + kChunk - 1) / kChunk) : 0;
   }
   __device__ int k_begin(int z) const { return static_cast<int>(static_cast<int64_t>(ks) * z / split); }
 };
@@ -277,17 +284,20 @@ __device__ __forceinline__ bool load_phase(const ChainP& p, Shared& sh, uint32_t
   const CUtensorMap* mp = mode == GRAM ? (p.tall ? &p.xm[cur] : &p.xk[cur])
                           : mode == POLY ? &p.ak : p.tall ? &p.xk[cur] : &p.bk;
   const CUtensorMap* mq = mode == GRAM ? mp : mode == POLY ? &p.ak : p.tall ? &p.bk : &p.xm[cur];
+  const bool half_q = w.ratio == 2;  // a block's 64 rows of Q: the maps by 64 x 64
+  if (half_q) mq = mode == GRAM ? &p.xm[cur] : &p.a64;
+  const uint32_t bytes = CG * (kOperand + kOperand / w.ratio);
   volatile int* const abort_flag = &sh.abort;
   for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG) {
     int e, ti, tj, z;
     w.at(t, e, ti, tj, z);
-    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.TN + rank * 128;
+    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.tn + rank * (w.tn / CG);
     for (int k = w.k_begin(z); k < w.k_begin(z + 1); ++k, ++n) {
       const int st = static_cast<int>(n % kStages);
       if (n >= kStages && !mbar_wait(&sh.empty[st], static_cast<uint32_t>(n / kStages - 1) & 1, p.err)) return false;
       if (*abort_flag) return false;
       const uint32_t sp = smem + st * kStageBytes, sq = sp + kOperand;
-      if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], CG * kStageBytes);
+      if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], bytes);
       if (p_mn) {
         tma_load_3d<CG>(sp, mp, &sh.full[st], i0, k * kTileK, e);
         tma_load_3d<CG>(sp + kOperand / 2, mp, &sh.full[st], i0 + 64, k * kTileK, e);
@@ -296,7 +306,7 @@ __device__ __forceinline__ bool load_phase(const ChainP& p, Shared& sh, uint32_t
       }
       if (q_mn) {
         tma_load_3d<CG>(sq, mq, &sh.full[st], j0, k * kTileK, e);
-        tma_load_3d<CG>(sq + kOperand / 2, mq, &sh.full[st], j0 + 64, k * kTileK, e);
+        if (!half_q) tma_load_3d<CG>(sq + kOperand / 2, mq, &sh.full[st], j0 + 64, k * kTileK, e);
       } else {
         tma_load_3d<CG>(sq, mq, &sh.full[st], k * kTileK, j0, e);
       }
@@ -312,7 +322,7 @@ __device__ __forceinline__ bool issue_phase(const ChainP& p, Shared& sh, uint32_
                                             int64_t& n, int64_t& c) {
   const Work<CG> w(p, mode);
   const bool p_mn = mode == GRAM && p.tall, q_mn = mode == GRAM ? p.tall : mode >= STEP && !p.tall;
-  const uint32_t idesc = instr_desc_f16(w.TM, w.TN, p_mn, q_mn);
+  const uint32_t idesc = instr_desc_f16(w.TM, w.tn, p_mn, q_mn);
   const uint64_t ka = desc_k16(p_mn), kb = desc_k16(q_mn);
   const uint64_t first_a = smem_desc(smem, p_mn), first_b = smem_desc(smem + kOperand, q_mn);
   volatile int* const abort_flag = &sh.abort;
@@ -384,9 +394,9 @@ struct Cursor {
       int ti, tj, z;
       w.at(t, e, ti, tj, z);
       i0 = ti * w.TM + rank * kRows;
-      j0 = tj * w.TN;
+      j0 = tj * w.tn;
       chunks = w.chunks(i0, j0);
-      mirror = w.sym && ti != tj;
+      mirror = w.mirrored(ti, tj);
       g = w.split > 1 ? z : 0;  // a tile in parts: each of its blocks finishes some chunks
       step = w.split;
       if (g < chunks) return;
@@ -478,9 +488,9 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
     int e, ti, tj, z;
     w.at(t, e, ti, tj, z);
     const int acc = static_cast<int>(c & 1);
-    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.TN, i = i0 + r;
+    const int i0 = ti * w.TM + rank * kRows, j0 = tj * w.tn, i = i0 + r;
     const int chunks = w.chunks(i0, j0);
-    const bool mirror = w.sym && ti != tj;
+    const bool mirror = w.mirrored(ti, tj);
     const uint32_t ta = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * w.TN + half * 32;
     wait_or_abort(&sh.done[acc], static_cast<uint32_t>(c / 2) & 1, sh, p.err);
     tc_fence_after();
@@ -491,8 +501,8 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
       // tile have arrived, each of its blocks finishes some of the chunks,
       // adding the parts in order.
       const int64_t tile = static_cast<int64_t>(t / w.split) * CG + rank;
-      part = p.partials + tile * w.split * (kRows * w.TN);
-      float* mine = p.partials + (tile * w.split + z) * (kRows * w.TN);
+      part = p.partials + tile * w.split * (kRows * w.tn);
+      float* mine = p.partials + (tile * w.split + z) * (kRows * w.tn);
       for (int g = 0; g < chunks; ++g) {
         float v[32];
         tmem_load32(ta + g * kChunk, v);
@@ -527,7 +537,7 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
 #pragma unroll
               for (int k = 0; k < 16; ++k)
                 f[q][k] = q0 + q < w.split
-                              ? __ldcg(from + (static_cast<int64_t>(q0 + q) * w.TN + k0 + k) * kRows) : 0.f;
+                              ? __ldcg(from + (static_cast<int64_t>(q0 + q) * w.tn + k0 + k) * kRows) : 0.f;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -737,7 +747,7 @@ __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
 struct Plan {
   int64_t s, l, ldx, lds, tiles;
   size_t hi0, hi1, lo, a, b, diag, partials, sums, counters, bytes;
-  int blocks, pairs, groups, split, count;
+  int blocks, pairs, groups, narrow, split, count;
 };
 
 // Blocks (or pairs of them) that are resident at once, one per SM.
@@ -788,6 +798,9 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.groups = resident(q.pairs);
   const int64_t side = q.pairs ? 256 : 128;
   q.tiles = chain_tiles(E, q.s, q.s, side, true);
+  // A's and B's tiles at half the width where pairs outnumber them two to one
+  q.narrow = q.pairs && 2 * q.tiles <= q.groups;
+  if (q.narrow) q.tiles = E * (ceil_div(q.s, 256) * (ceil_div(q.s, 256) - 1) + ceil_div(q.s, 128));
   // A's few tiles with a long k: each in up to four parts of at least six
   // k-slices (a part costs about 5 us, a slice 0.3), one work item a group.  A
   // step of 1024 x 4096 in 1, 2, 4 and 8 parts: 63, 55, 49 and 49 us.
@@ -806,7 +819,7 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.partials = q.diag + align_up(static_cast<size_t>(E) * q.s * sizeof(float2), 256);
   q.counters = q.partials + align_up(static_cast<size_t>(E) * q.blocks * sizeof(float), 256);
   q.sums = q.counters + align_up(static_cast<size_t>(q.count) * sizeof(unsigned), 256);
-  q.bytes = q.sums + (q.split > 1 ? static_cast<size_t>(q.tiles) * q.split * side * side * sizeof(float) : 0);
+  q.bytes = q.sums + (q.split > 1 ? static_cast<size_t>(q.tiles) * q.split * side * (q.narrow ? 128 : side) * sizeof(float) : 0);
   return q;
 }
 
@@ -863,6 +876,7 @@ int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_
   p.tall = m > n;
   p.steps = steps;
   p.split = q.split;
+  p.narrow = q.narrow;
   p.diag = reinterpret_cast<float2*>(ws + q.diag);
   p.partials = reinterpret_cast<float*>(ws + q.sums);
   p.counters = pp.counters;
