@@ -843,11 +843,42 @@ class RopeFrequencies:
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
+    """Whether two tensors share memory.  Where their address ranges meet, as
+    those of head slices of one packed tensor do, the strides decide: an element
+    of each has the same address where sum(stride * index difference) is the
+    distance of the two, with the index differences of equal strides taken
+    together.  The largest stride goes first, and as soon as the strides left
+    reach every distance within their span the question is answered."""
     if a.numel() == 0 or b.numel() == 0:
         return False
-    end = lambda t: t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    distance = b.data_ptr() - a.data_ptr()
+    reach = {1: [1 - b.element_size(), a.element_size() - 1]}  # stride in bytes: index differences
+    for t, at in ((b, 0), (a, 1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s > 0:
+                r = reach.setdefault(s * t.element_size(), [0, 0])
+                r[at] += n - 1 if at else 1 - n
+    strides = sorted(reach, reverse=True)
+    lo, hi = [0], [0]  # of the strides from i on
+    dense = [True]
+    for s in reversed(strides):
+        dense.insert(0, dense[0] and s <= hi[0] - lo[0] + 1)
+        lo.insert(0, lo[0] + s * reach[s][0])
+        hi.insert(0, hi[0] + s * reach[s][1])
+    left = [4096]  # cases to look at; what is not settled by then counts as shared
+
+    def meet(i: int, d: int) -> bool:
+        if not lo[i] <= d <= hi[i]:
+            return False
+        if dense[i]:
+            return True
+        s = strides[i]
+        for k in range(max(reach[s][0], -((hi[i + 1] - d) // s)), min(reach[s][1], (d - lo[i + 1]) // s) + 1):
+            left[0] -= 1
+            if left[0] < 0 or meet(i + 1, d - k * s):
+                return True
+        return False
+    return meet(0, distance)
 
 
 def _check_rope_out(x: torch.Tensor, out: torch.Tensor, name: str) -> None:
@@ -899,7 +930,7 @@ def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch
         if k.dim() != 4 or k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
             raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         ok, dk = _rope_pair(k, out_k, out_layout, "k")
-        if (out_q is not None or out_k is not None) and _overlaps(oq, ok) and not _interleaved(oq, ok):
+        if (out_q is not None or out_k is not None) and _overlaps(oq, ok):
             raise ValueError("out_q and out_k overlap")
         arr = (_lib.RopeTensor * 2)(dq, dk)
     pos_ptr, pos_dtype, psb, pss = _rope_positions(positions, B, S, dev)
@@ -924,17 +955,6 @@ def _rope_pair(x: torch.Tensor, out: torch.Tensor | None, out_layout: str, name:
     xs, os_ = x.stride(), out.stride()
     return out, _lib.RopeTensor(x.data_ptr(), out.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], os_[0], os_[1], os_[2],
                                 _lib.FRAG_ROPE_OUT_BF16, _lib.FRAG_ROPE_IN_BF16)
-
-
-def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two overlapping ranges are disjoint head slices of one packed
-    tensor: the same batch and sequence strides, heads that do not meet."""
-    if a.stride()[:2] != b.stride()[:2] or min(a.stride(1), b.stride(1)) <= 0:
-        return False
-    lo, hi = (a, b) if a.data_ptr() <= b.data_ptr() else (b, a)
-    gap = (hi.data_ptr() - lo.data_ptr()) // lo.element_size()
-    span = lambda t: (t.shape[2] - 1) * t.stride(2) + t.shape[3]
-    return gap >= span(lo) and gap + span(hi) <= lo.stride(1)
 
 
 def _rope_positions(positions, B: int, S: int, dev: torch.device):

@@ -188,3 +188,25 @@ def test_refusals():
         ops.rope_scaled(q, freqs=plan, out_q=torch.empty(2, 4, 3, 64, device=DEV))
     with pytest.raises(ValueError):
         ops.rope_scaled(rand(2, 4, 64, 3).transpose(2, 3), freqs=plan)
+
+
+@pytest.mark.parametrize("D,rot", [(128, 128), (96, 32), (80, 20)])
+def test_in_place_on_head_major_slices(D, rot):
+    """q and k of one packed [B, H, S, D] tensor."""
+    plan = ops.RopeFrequencies(D, rotary_dim=rot)
+    packed = rand(3, 8, 17, D, seed=15)
+    before = packed.clone().transpose(1, 2)
+    q, k = packed[:, :4].transpose(1, 2), packed[:, 4:6].transpose(1, 2)
+    ops.rope_scaled(q, k, None, freqs=plan, out_q=q, out_k=k)
+    pos = torch.arange(17, device=DEV).expand(3, 17)
+    after = packed.transpose(1, 2)
+    check(after[:, :, :6], before[:, :, :6], pos, plan, "neox")
+    assert torch.equal(after[:, :, 6:], before[:, :, 6:])
+
+
+def test_outputs_that_meet_across_sequences_are_refused():
+    plan = ops.RopeFrequencies(64)
+    y = torch.empty(4, 3, 5, 64, dtype=torch.bfloat16, device=DEV)
+    q, k = rand(2, 4, 5, 64), rand(2, 4, 5, 64, seed=1)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope_scaled(q, k, None, freqs=plan, out_q=y[:, 0:2].transpose(0, 1), out_k=y[:, 1:3].transpose(0, 1))

@@ -102,3 +102,45 @@ def test_orthogonalize_rejects_bad_arguments_on_the_host():
     assert lib.frag_muon_update(C.byref(none), C.byref(none), C.byref(none), None, None, 1, 8, 8, 0.1, 0.9, 1, 0.0, 1.0,
                                 5, co, 1e-7, None, 0, None) == 1
     assert lib.frag_orthogonalize_workspace_bytes(0, 8, 8) == 0
+
+
+def addresses(t):
+    """Every byte of a tensor."""
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * s).reshape(-1)
+    return set((at[:, None] * t.element_size() + t.data_ptr() + torch.arange(t.element_size())).reshape(-1).tolist())
+
+
+def test_overlap_of_packed_slices():
+    packed = torch.empty(2, 5, 8, 16, dtype=torch.bfloat16)  # [B, S, H, D]
+    assert not ops._overlaps(packed[:, :, :4], packed[:, :, 4:6])
+    assert ops._overlaps(packed[:, :, :5], packed[:, :, 4:6])
+    major = torch.empty(2, 8, 5, 16, dtype=torch.bfloat16).transpose(1, 2)  # [B, H, S, D] storage
+    assert not ops._overlaps(major[:, :, :4], major[:, :, 4:6])
+    assert ops._overlaps(major[:, :, :4], major[:, :, 3:6])
+    # sequences that are disjoint row by row, although row 1 of one is row 0 of the other
+    y = torch.empty(4, 3, 5, 8)
+    assert ops._overlaps(y[:, 0:2].transpose(0, 1), y[:, 1:3].transpose(0, 1))
+    assert not ops._overlaps(y[:, 0:1], y[:, 1:3]) and not ops._overlaps(y[:0], y)
+    flat = torch.empty(64)
+    assert not ops._overlaps(flat[::2], flat[1::2]) and ops._overlaps(flat[::2], flat[1::3])
+    assert ops._overlaps(flat[:4], flat.view(torch.bfloat16)[7:]) and not ops._overlaps(flat[:4], flat.view(torch.bfloat16)[8:])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_overlap_against_every_address(seed):
+    import random
+    r = random.Random(seed)
+    buf = torch.empty(4000, dtype=r.choice([torch.bfloat16, torch.float32]))
+    other = buf.view(torch.bfloat16)
+    for _ in range(300):
+        shape = [r.randint(1, 4) for _ in range(r.randint(1, 4))]
+        a = buf.as_strided(shape, [r.choice([0, 1, 2, 3, 4, 6, 8, 12, 16, 24, 40, 64]) for _ in shape], r.randint(0, 60))
+        if r.random() < 0.5:  # the same strides, as of slices
+            b = buf.as_strided([max(1, n + r.choice([-1, 0, 1])) for n in shape], a.stride(), r.randint(0, 60))
+        else:
+            shape = [r.randint(1, 4) for _ in range(r.randint(1, 4))]
+            b = r.choice([buf, other]).as_strided(shape, [r.choice([0, 1, 2, 4, 5, 8, 16, 20, 64]) for _ in shape],
+                                                  r.randint(0, 60))
+        assert ops._overlaps(a, b) == bool(addresses(a) & addresses(b)), (a.shape, a.stride(), b.shape, b.stride())
