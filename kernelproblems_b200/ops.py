@@ -894,6 +894,18 @@ def _check_rope_out(x: torch.Tensor, out: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: the output overlaps the input without being the same view")
 
 
+def _check_rope_outs(q: torch.Tensor, k: torch.Tensor, oq: torch.Tensor, ok: torch.Tensor) -> None:
+    """One launch reads q and k while it writes the outputs, heads of a token
+    by different warps: neither output may share memory with the other input or
+    the other output.  (In place the three questions are one.)"""
+    if _overlaps(oq, ok):
+        raise ValueError("out_q and out_k overlap")
+    if ok is not k and _overlaps(oq, k):
+        raise ValueError("out_q overlaps k")
+    if oq is not q and _overlaps(ok, q):
+        raise ValueError("out_k overlaps q")
+
+
 def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None, *,
                 freqs: RopeFrequencies, layout: str = "neox", backward: bool = False,
                 out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None,
@@ -903,7 +915,10 @@ def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch
     freqs.rotary_dim elements of every head are rotated (pairs (j, j +
     rotary_dim/2) for layout "neox", (2j, 2j+1) for "interleaved"), the others
     pass through.  Returns (out_q, out_k), new contiguous tensors or the given
-    out_q / out_k, which may be q and k themselves (in place).
+    out_q / out_k, which may be q and k themselves (in place); an output must not
+    share memory with its input in any other way, nor with the other input or
+    output (slices of one packed tensor, in either order of heads and tokens,
+    are fine).
 
     positions: int32/int64 [B, S] or [S], or None for position = s.  A product
     of position and frequency is taken in 64 bits, so a long context's last
@@ -930,8 +945,8 @@ def rope_scaled(q: torch.Tensor, k: torch.Tensor | None = None, positions: torch
         if k.dim() != 4 or k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
             raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         ok, dk = _rope_pair(k, out_k, out_layout, "k")
-        if (out_q is not None or out_k is not None) and _overlaps(oq, ok):
-            raise ValueError("out_q and out_k overlap")
+        if out_q is not None or out_k is not None:
+            _check_rope_outs(q, k, oq, ok)
         arr = (_lib.RopeTensor * 2)(dq, dk)
     pos_ptr, pos_dtype, psb, pss = _rope_positions(positions, B, S, dev)
     with _on_device(dev):

@@ -210,3 +210,17 @@ def test_outputs_that_meet_across_sequences_are_refused():
     q, k = rand(2, 4, 5, 64), rand(2, 4, 5, 64, seed=1)
     with pytest.raises(ValueError, match="overlap"):
         ops.rope_scaled(q, k, None, freqs=plan, out_q=y[:, 0:2].transpose(0, 1), out_k=y[:, 1:3].transpose(0, 1))
+
+
+def test_outputs_over_the_other_input_are_refused():
+    plan = ops.RopeFrequencies(64)
+    q, k = rand(1, 3, 4, 64), rand(1, 3, 4, 64, seed=1)
+    before = q.clone(), k.clone()
+    for kw in (dict(out_q=k), dict(out_k=q), dict(out_q=k, out_k=q)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.rope_scaled(q, k, None, freqs=plan, **kw)
+    assert torch.equal(q, before[0]) and torch.equal(k, before[1])
+    out = torch.empty_like(q)  # one output given, the other input in place
+    ops.rope_scaled(q, k, None, freqs=plan, out_q=out, out_k=k)
+    check(out, before[0], torch.arange(3, device=DEV)[None], plan, "neox")
+    check(k, before[1], torch.arange(3, device=DEV)[None], plan, "neox")

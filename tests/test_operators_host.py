@@ -144,3 +144,19 @@ def test_overlap_against_every_address(seed):
             b = r.choice([buf, other]).as_strided(shape, [r.choice([0, 1, 2, 4, 5, 8, 16, 20, 64]) for _ in shape],
                                                   r.randint(0, 60))
         assert ops._overlaps(a, b) == bool(addresses(a) & addresses(b)), (a.shape, a.stride(), b.shape, b.stride())
+
+
+def test_rope_outputs_and_the_other_input():
+    """Strides only: the check runs before anything is launched."""
+    q, k = (torch.empty(2, 3, 4, 16, dtype=torch.bfloat16) for _ in range(2))
+    new = torch.empty_like
+    ops._check_rope_outs(q, k, q, k)
+    ops._check_rope_outs(q, k, q, new(k))
+    ops._check_rope_outs(q, k, new(q), k)
+    packed = torch.empty(2, 3, 6, 16, dtype=torch.bfloat16)
+    ops._check_rope_outs(packed[:, :, :4], packed[:, :, 4:], packed[:, :, :4], packed[:, :, 4:])
+    for oq, ok in ((k, new(k)), (new(q), q), (k, q), (q, q), (k, k)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops._check_rope_outs(q, k, oq, ok)
+    with pytest.raises(ValueError, match="overlap"):  # two heads of k
+        ops._check_rope_outs(packed[:, :, :4], packed[:, :, 4:], packed[:, :, 2:], new(packed[:, :, 4:]))
