@@ -307,16 +307,15 @@ extern "C" int frag_rope_scaled(const frag_rope_tensor* tensors, int num_tensors
     if (t.H > 0 && (!t.x || !t.out)) return FRAG_ERR_INVALID_ARG;
     if (t.in_dtype != FRAG_ROPE_IN_BF16 || t.out_dtype != FRAG_ROPE_OUT_BF16) return FRAG_ERR_INVALID_ARG;
     const bool in_place = t.x == t.out;
-    if (in_place && (t.x_stride_b != t.out_stride_b || t.x_stride_s != t.out_stride_s ||
-                     t.x_stride_h != t.out_stride_h))
-      return FRAG_ERR_INVALID_ARG;
-    p.t[i] = ScaledT{static_cast<const uint16_t*>(t.x), static_cast<uint16_t*>(t.out), static_cast<int>(t.H),
-                     in_place ? 0 : 1, t.x_stride_b, t.x_stride_s, t.x_stride_h, t.out_stride_b,
-                     t.out_stride_s, t.out_stride_h};
+    ScaledT& o = p.t[i];
+    o = ScaledT{static_cast<const uint16_t*>(t.x), static_cast<uint16_t*>(t.out), static_cast<int>(t.H),
+                in_place ? 0 : 1, t.x_stride_b, t.x_stride_s, t.x_stride_h, t.out_stride_b,
+                t.out_stride_s, t.out_stride_h};
     // a dimension of one element has no stride to respect
-    if (B == 1) p.t[i].xsb = p.t[i].osb = 0;
-    if (S == 1) p.t[i].xss = p.t[i].oss = 0;
-    if (t.H == 1) p.t[i].xsh = p.t[i].osh = 0;
+    if (B == 1) o.xsb = o.osb = 0;
+    if (S == 1) o.xss = o.oss = 0;
+    if (t.H == 1) o.xsh = o.osh = 0;
+    if (in_place && (o.xsb != o.osb || o.xss != o.oss || o.xsh != o.osh)) return FRAG_ERR_INVALID_ARG;
     any = any || t.H > 0;
   }
   if (!any) return FRAG_OK;

@@ -224,3 +224,17 @@ def test_outputs_over_the_other_input_are_refused():
     ops.rope_scaled(q, k, None, freqs=plan, out_q=out, out_k=k)
     check(out, before[0], torch.arange(3, device=DEV)[None], plan, "neox")
     check(k, before[1], torch.arange(3, device=DEV)[None], plan, "neox")
+
+
+def test_in_place_with_other_strides_of_single_dimensions():
+    """One token a sequence, one sequence or one head: that dimension's stride
+    says nothing, and views of the same elements may differ in it."""
+    plan = ops.RopeFrequencies(64)
+    for x, view in ((rand(3, 1, 4, 64), lambda t: t.view(3, 4, 1, 64).transpose(1, 2)),
+                    (rand(1, 5, 4, 64), lambda t: t.as_strided(t.shape, (64, 256, 64, 1))),
+                    (rand(2, 5, 1, 64), lambda t: t.as_strided(t.shape, (320, 64, 8, 1)))):
+        before, out = x.clone(), view(x)
+        assert out.data_ptr() == x.data_ptr() and out.stride() != x.stride()
+        got, _ = ops.rope_scaled(x, None, None, freqs=plan, out_q=out)
+        assert got is out
+        check(x, before, torch.arange(x.shape[1], device=DEV).expand(x.shape[:2]), plan, "neox")
