@@ -1149,6 +1149,16 @@ def _matrices(t: torch.Tensor, name: str, dev: torch.device | None = None, shape
     return E, m, n, _lib.Matrix(t.data_ptr(), sb or 0, t.stride(-2), t.stride(-1), _DT[t.dtype])
 
 
+def _check_replaces(out: torch.Tensor, name: str, like: torch.Tensor, inputs) -> None:
+    """A contiguous output may be `like` itself, element by element.  Any other
+    memory shared with an input is refused: a stack's matrices are not written
+    in the order in which they are read."""
+    for t in inputs:
+        if _overlaps(out, t) and not (t is like and out.data_ptr() == t.data_ptr() and t.is_contiguous()
+                                      and out.dtype == t.dtype):
+            raise ValueError(f"{name} overlaps an input that it does not replace")
+
+
 @functools.lru_cache(maxsize=64)
 def _repeated(steps: int, a: float, b: float, c: float):
     return (C.c_float * (3 * steps))(*([a, b, c] * steps))
@@ -1180,7 +1190,8 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ
     """Newton-Schulz orthogonalisation of each matrix of g [..., m, n] (bf16 or
     fp32, any strides): X = g / (|g|_F + eps), then `steps` times
     X <- a X + (b A + c A A) X with A = X X' (on the smaller side).  Returns
-    bf16 X, contiguous, shaped like g (or `out`).
+    bf16 X, contiguous, shaped like g (or `out`, which may be a contiguous bf16 g
+    itself but not overlap it otherwise).
 
     coefficients: a triple (a, b, c) for all steps, or one for each.  They have
     to keep |X| within a few units (as the default and all schedules that
@@ -1192,6 +1203,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ
         out = torch.empty_like(g, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
     else:
         _check_out(out, "out", torch.bfloat16, dev, shape=g.shape)
+        _check_replaces(out, "out", g, (g,))
     co = _schedule(steps, coefficients)
     with _on_device(dev):
         workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), g)
@@ -1231,11 +1243,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
             given = torch.empty_like(like, memory_format=torch.contiguous_format)
         else:
             _check_out(given, name, like.dtype, dev, shape=like.shape)
-            for other in (param, grad, momentum_buffer):
-                # element by element in place is fine, any other overlap is not
-                if _overlaps(given, other) and not (other is like and given.data_ptr() == other.data_ptr()
-                                                    and other.is_contiguous()):
-                    raise ValueError(f"{name} overlaps an input that it does not replace")
+            _check_replaces(given, name, like, (param, grad, momentum_buffer))
         outs.append(given)
     if _overlaps(*outs):
         raise ValueError("param_out and momentum_out overlap")

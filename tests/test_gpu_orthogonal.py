@@ -264,3 +264,20 @@ def test_refusals():
         ops.muon_update(g, g.clone(), g.clone(), lr=0.1, param_out=o, momentum_out=o)
     with pytest.raises(ValueError):
         ops.muon_update(g, g.clone(), g.clone(), lr=0.1, workspace=torch.empty(9, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("shape", [(5, 64, 100), (2, 300, 700), (130, 60)])
+def test_in_place(shape):
+    g = normal(*shape, seed=25, dtype=torch.bfloat16)
+    want = ops.orthogonalize(g)
+    assert ops.orthogonalize(g, out=g) is g and torch.equal(g, want)
+
+
+def test_outputs_over_other_matrices_are_refused():
+    buf = normal(5, 64, 100, seed=26, dtype=torch.bfloat16)
+    before = buf.clone()
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.orthogonalize(buf[:4], out=buf[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.orthogonalize(buf[0, :64, :64].t(), out=buf[0].flatten()[:4096].view(64, 64))
+    assert torch.equal(buf, before)

@@ -160,3 +160,19 @@ def test_rope_outputs_and_the_other_input():
             ops._check_rope_outs(q, k, oq, ok)
     with pytest.raises(ValueError, match="overlap"):  # two heads of k
         ops._check_rope_outs(packed[:, :, :4], packed[:, :, 4:], packed[:, :, 2:], new(packed[:, :, 4:]))
+
+
+def test_matrix_outputs_and_what_they_replace():
+    buf = torch.empty(5, 8, 8, dtype=torch.bfloat16)
+    g, other = buf[:4], torch.empty(4, 8, 8, dtype=torch.bfloat16)
+    ops._check_replaces(torch.empty_like(g), "out", g, (g,))
+    ops._check_replaces(g, "out", g, (g,))
+    ops._check_replaces(buf[:4], "out", g, (g, other))
+    halves = torch.empty(4, 8, 16)[:, :, :8]  # fp32, every second run of 8
+    ops._check_replaces(torch.empty_like(halves, memory_format=torch.contiguous_format), "out", halves, (halves,))
+    wide = torch.empty(4, 8, 8)
+    for out, like, inputs in ((buf[1:], g, (g,)), (g, other, (g, other)),
+                              (wide.view(torch.bfloat16).flatten()[:256].view(4, 8, 8), wide, (wide,)),
+                              (g, buf.as_strided((4, 8, 8), (64, 1, 8)), (buf.as_strided((4, 8, 8), (64, 1, 8)),))):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops._check_replaces(out, "out", like, inputs)
