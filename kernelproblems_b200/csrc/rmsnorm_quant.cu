@@ -17,6 +17,7 @@
 // with a scale for each 128) and in the gradient (8192 rows of 4096 with the
 // residual 58 us for a floor of 46, 3.5 of them the dweight's second pass).
 #include <algorithm>
+#include <atomic>
 
 #include "quant.cuh"
 
@@ -722,13 +723,18 @@ int launch_bwd(const QuantBwdP& p, int64_t M, const QuantBwdPlan& pl, const RowS
 // device: 32768 rows of 8192, group 128, 284 us against 357 for one and 326
 // for as many blocks as are resident; 16384 rows of 4096 75, 89 and 88.
 // Without, as many blocks as are resident: 16384 rows of 4096 40, 61 for one.
-template <class Kern>
-int launch_stay(Kern kern, int64_t units, bool has_res, int threads, const QuantFwdP& p, int64_t M, cudaStream_t s) {
-  static int per_sm[33] = {};  // by warps of a block; the same on every device of this architecture
-  int& n = per_sm[threads / 32];
-  if (n == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n == 0)) {
-    cudaGetLastError();
-    n = 1;
+template <auto kern>  // (a parameter of its own for each kernel: their types are the same)
+int launch_stay(int64_t units, bool has_res, int threads, const QuantFwdP& p, int64_t M, cudaStream_t s) {
+  // this kernel's resident blocks by warps of a block; the same on every device of this architecture
+  static std::atomic<int> per_sm[33];
+  int n = per_sm[threads / 32].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) == cudaSuccess && n > 0) {
+      per_sm[threads / 32].store(n, std::memory_order_relaxed);
+    } else {
+      cudaGetLastError();
+      n = 1;
+    }
   }
   const int64_t places = static_cast<int64_t>(n) * std::max(1, sm_count());
   const int64_t R = has_res ? std::max<int64_t>(1, std::min<int64_t>(4, units / (2 * places))) : ceil_div(units, places);
@@ -741,12 +747,12 @@ int launch_fwd(const QuantFwdP& p, int64_t M, const RowShape& r, cudaStream_t s)
   const unsigned rows = static_cast<unsigned>(M), warps = static_cast<unsigned>(ceil_div(M, r.threads / 32));
   switch (r.kind) {
     case ROW_WARP:
-      if (r.K == 1) return launch_stay(quant_fwd_vec<1, true, true, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
-      if (r.K == 2) return launch_stay(quant_fwd_vec<2, true, true, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
-      return launch_stay(quant_fwd_vec<4, true, !HAS_RES, HAS_RES, E5M2, E8M0>, warps, HAS_RES, r.threads, p, M, s);
+      if (r.K == 1) return launch_stay<quant_fwd_vec<1, true, true, HAS_RES, E5M2, E8M0>>(warps, HAS_RES, r.threads, p, M, s);
+      if (r.K == 2) return launch_stay<quant_fwd_vec<2, true, true, HAS_RES, E5M2, E8M0>>(warps, HAS_RES, r.threads, p, M, s);
+      return launch_stay<quant_fwd_vec<4, true, !HAS_RES, HAS_RES, E5M2, E8M0>>(warps, HAS_RES, r.threads, p, M, s);
     case ROW_BLOCK:
-      if (r.K == 2) return launch_stay(quant_fwd_vec<2, false, true, HAS_RES, E5M2, E8M0>, rows, HAS_RES, r.threads, p, M, s);
-      return launch_stay(quant_fwd_vec<4, false, !HAS_RES, HAS_RES, E5M2, E8M0>, rows, HAS_RES, r.threads, p, M, s);
+      if (r.K == 2) return launch_stay<quant_fwd_vec<2, false, true, HAS_RES, E5M2, E8M0>>(rows, HAS_RES, r.threads, p, M, s);
+      return launch_stay<quant_fwd_vec<4, false, !HAS_RES, HAS_RES, E5M2, E8M0>>(rows, HAS_RES, r.threads, p, M, s);
     case ROW_ODD_WARP:
       if (r.K == 2) quant_fwd_odd<2, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);
       else if (r.K == 4) quant_fwd_odd<4, true, HAS_RES, E5M2, E8M0><<<warps, r.threads, 0, s>>>(p, M);

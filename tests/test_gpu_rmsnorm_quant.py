@@ -257,3 +257,41 @@ def test_refusals():
         ops.rmsnorm_quant_bwd(x, x, r, w, dres=rand(4, 32))
     with pytest.raises(ValueError):
         ops.rmsnorm_quant_bwd(x, x, r, w, workspace=torch.empty(1 << 20, dtype=torch.uint8))
+
+
+GRIDS = """
+import sys
+import torch
+from cuda.bindings import driver
+from kernelproblems_b200 import ops
+order = [(20000, 256, False), (20000, 1024, False), (20000, 4096, True), (20000, 4096, False), (20000, 1000, False)]
+w = {N: torch.ones(N, dtype=torch.bfloat16, device="cuda") for _, N, _ in order}
+grids = []
+for M, N, res in order[::int(sys.argv[1])]:
+    x = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    call = lambda: ops.rmsnorm_quant_fwd(x, w[N], residual=x if res else None)
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    h = driver.CUgraph(graph.raw_cuda_graph())
+    _, _, n = driver.cuGraphGetNodes(h)
+    _, nodes, n = driver.cuGraphGetNodes(h, n)
+    assert n == 1
+    err, p = driver.cuGraphKernelNodeGetParams(nodes[0])
+    assert int(err) == 0
+    grids.append(f"{M}x{N}{res} {p.gridDimX} of {p.blockDimX}")
+print(sorted(grids))
+"""
+
+
+def test_grid_does_not_depend_on_earlier_calls():
+    """Each kernel's resident blocks are its own: the same calls in the other
+    order, in a process of their own, get the same grids."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    runs = [subprocess.run([sys.executable, "-c", GRIDS, step], cwd=Path(__file__).resolve().parent.parent, timeout=300,
+                           capture_output=True, text=True) for step in ("1", "-1")]
+    assert all(r.returncode == 0 for r in runs), runs[0].stderr + runs[1].stderr
+    assert runs[0].stdout == runs[1].stdout
