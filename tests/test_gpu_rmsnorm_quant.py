@@ -295,3 +295,43 @@ def test_grid_does_not_depend_on_earlier_calls():
                            capture_output=True, text=True) for step in ("1", "-1")]
     assert all(r.returncode == 0 for r in runs), runs[0].stderr + runs[1].stderr
     assert runs[0].stdout == runs[1].stdout
+
+
+# Rows enough that blocks and warps take several (the next row's loads ahead,
+# alternating slots, a last block that is cut; the gradient's ring reused, with
+# both parities of its barriers), each width's own kernel.
+LONG = [(40013, 256), (40013, 504), (40013, 1000), (9001, 4096), (3001, 8200), (1501, 16384), (20011, 300), (5003, 1001)]
+
+
+@pytest.mark.parametrize("M,N", LONG)
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_forward_of_many_rows(M, N, group):
+    x, w, res = rand(M, N, seed=31), weight(N), rand(M, N, seed=32)
+    x[5::7] *= 30  # neighbouring rows of one block differ
+    x[3::64] = 0
+    for r in (None, res):
+        check_fwd(x, w, r, ops.rmsnorm_quant_fwd(x, w, EPS, residual=r, group=group), group)
+
+
+@pytest.mark.parametrize("M,N", [(20011, 136), (20011, 512), (12007, 1032), (9001, 4096), (6007, 4104), (3001, 5120),
+                                 (3001, 6144), (3001, 6152), (3001, 8192), (1501, 8200), (1501, 16384), (20011, 300),
+                                 (5003, 1001), (1501, 9001)])
+@pytest.mark.parametrize("group", [0, 128])
+def test_backward_of_many_rows(M, N, group):
+    x, dy, w, dres = rand(M, N, seed=33), rand(M, N, seed=34, std=1e-3), weight(N), rand(M, N, seed=35, std=1e-3)
+    dy[5::7] *= 30
+    x[3::64] = 0
+    rstd = (x.float().square().mean(-1) + EPS).rsqrt()
+    for dr in (None, dres):
+        check_bwd(dy, x, rstd, w, dr, ops.rmsnorm_quant_bwd(dy, x, rstd, w, dres=dr, group=group), group)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("N", [264, 300, 504, 513, 520, 1016, 1032, 4100, 4104, 5120, 6144, 6152, 8191, 8200, 9001, 16383])
+def test_widths_at_the_variants_borders(N):
+    x, dy, w, res = rand(37, N, seed=36), rand(37, N, seed=37), weight(N), rand(37, N, seed=38)
+    rstd = (x.float().square().mean(-1) + EPS).rsqrt()
+    for group in (0, 64):
+        for r in (None, res):
+            check_fwd(x, w, r, ops.rmsnorm_quant_fwd(x, w, EPS, residual=r, group=group, scale_dtype=E8), group)
+            check_bwd(dy, x, rstd, w, r, ops.rmsnorm_quant_bwd(dy, x, rstd, w, dres=r, group=group), group)
