@@ -176,3 +176,12 @@ def test_matrix_outputs_and_what_they_replace():
                               (g, buf.as_strided((4, 8, 8), (64, 1, 8)), (buf.as_strided((4, 8, 8), (64, 1, 8)),))):
         with pytest.raises(ValueError, match="overlaps"):
             ops._check_replaces(out, "out", like, inputs)
+
+
+def test_smoke_has_no_matrix_for_pairs_of_blocks():
+    """Pairs of blocks take over from 56 tiles of 256 x 256 (three quarters of 74 pairs)."""
+    import __graft_entry__ as entry
+    import inspect
+    assert "SMOKE_MATRICES" in inspect.getsource(entry.smoke)
+    for m, n in entry.SMOKE_MATRICES:
+        assert 4 * -(-m // 256) * -(-n // 256) < 3 * 74
