@@ -843,13 +843,17 @@ int launch_chain(const ChainP& p, int groups, cudaStream_t s) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-int orthogonalise(const PrepP& prep, const Plan& q, int64_t E, int64_t m, int64_t n, int steps, const float* co,
-                  Elem out, const Elem* par, float keep, float rate, unsigned char* ws, cudaStream_t s) {
+int orthogonalise(const PrepP& prep, int64_t E, int64_t m, int64_t n, int steps, const float* co, Elem out,
+                  const Elem* par, float keep, float rate, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   const ResultP res = {par ? UPDATE : LAST, out, par ? *par : Elem{}, keep, rate};
-  const int small = orthogonalise_small(prep, E, steps, co, res, s);
-  if (small != -1) return small;
+  if (small_takes(m, n)) return orthogonalise_small(prep, E, steps, co, res, s);
+  const Plan q = make_plan(E, m, n);
+  if (!workspace || workspace_bytes < q.bytes) return FRAG_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
+  unsigned char* const ws = static_cast<unsigned char*>(workspace);
   if (q.groups <= 0) return FRAG_ERR_NO_DEVICE;
   PrepP pp = prep;
+  pp.ldx = q.ldx;
   pp.hi = reinterpret_cast<__half*>(ws + q.hi0);
   pp.lo = reinterpret_cast<__half*>(ws + q.lo);
   pp.partials = reinterpret_cast<float*>(ws + q.partials);
@@ -923,7 +927,7 @@ extern "C" {
 
 size_t frag_orthogonalize_workspace_bytes(int64_t E, int64_t m, int64_t n) {
   if (E <= 0 || m <= 0 || n <= 0) return 0;
-  return make_plan(E, m, n).bytes;
+  return small_takes(m, n) ? 0 : make_plan(E, m, n).bytes;
 }
 
 int frag_orthogonalize(const frag_matrix* g, void* out, int64_t E, int64_t m, int64_t n, int steps,
@@ -934,16 +938,12 @@ int frag_orthogonalize(const frag_matrix* g, void* out, int64_t E, int64_t m, in
   if (E == 0 || m == 0 || n == 0) return FRAG_OK;
   PrepP prep = {};
   if (!elem_of(g, prep.g) || !out) return FRAG_ERR_INVALID_ARG;
-  const Plan q = make_plan(E, m, n);
-  if (!workspace || workspace_bytes < q.bytes) return FRAG_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
   prep.rows = m;
   prep.cols = n;
-  prep.ldx = q.ldx;
   prep.eps = eps;
   const Elem o{out, 0, m * n, n, 1};
-  return orthogonalise(prep, q, E, m, n, steps, coefficients, o, nullptr, 0.f, 0.f,
-                       static_cast<unsigned char*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+  return orthogonalise(prep, E, m, n, steps, coefficients, o, nullptr, 0.f, 0.f,
+                       workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int frag_muon_update(const frag_matrix* param, const frag_matrix* grad, const frag_matrix* momentum, void* param_out,
@@ -957,20 +957,16 @@ int frag_muon_update(const frag_matrix* param, const frag_matrix* grad, const fr
   Elem par;
   if (!elem_of(param, par) || !elem_of(grad, prep.g) || !elem_of(momentum, prep.mom)) return FRAG_ERR_INVALID_ARG;
   if (!param_out || !momentum_out) return FRAG_ERR_INVALID_ARG;
-  const Plan q = make_plan(E, m, n);
-  if (!workspace || workspace_bytes < q.bytes) return FRAG_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
   prep.mom_out = Elem{momentum_out, prep.mom.f32, m * n, n, 1};
   prep.has_mom = 1;
   prep.nesterov = nesterov;
   prep.mu = mu;
   prep.rows = m;
   prep.cols = n;
-  prep.ldx = q.ldx;
   prep.eps = eps;
   const Elem o{param_out, par.f32, m * n, n, 1};
-  return orthogonalise(prep, q, E, m, n, steps, coefficients, o, &par, 1.0f - lr * weight_decay, lr * scale,
-                       static_cast<unsigned char*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+  return orthogonalise(prep, E, m, n, steps, coefficients, o, &par, 1.0f - lr * weight_decay, lr * scale,
+                       workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -131,8 +131,9 @@ struct ResultP {
   float keep, rate;
 };
 
-// Everything in one launch for matrices with a side of at most 128 that fit in
-// a cluster's shared memory; -1 (nothing launched) when they do not.
+// Everything in one launch, without a workspace, for matrices with a side of at
+// most 128 that fit in a cluster's shared memory: whether m x n are such.
+bool small_takes(int64_t m, int64_t n);
 int orthogonalise_small(const PrepP& prep, int64_t E, int steps, const float* co, const ResultP& res, cudaStream_t s);
 
 }  // namespace frag

@@ -486,21 +486,27 @@ bool cluster_fits(int C) {
   return n > 0;
 }
 
+// Blocks of a cluster whose matrix has this long side.
+int cluster_blocks(int64_t longer) { return static_cast<int>(ceil_div(ceil_div(longer, 64), kMaxBlocks)); }
+
 }  // namespace
+
+bool small_takes(int64_t m, int64_t n) {
+  const int64_t longer = std::max(m, n);
+  return std::min(m, n) <= kSide && longer <= static_cast<int64_t>(kMaxCluster) * kMaxBlocks * 64 &&
+         cluster_fits(cluster_blocks(longer));
+}
 
 int orthogonalise_small(const PrepP& prep, int64_t E, int steps, const float* co, const ResultP& res, cudaStream_t s) {
   const int64_t small = std::min(prep.rows, prep.cols), longer = std::max(prep.rows, prep.cols);
-  if (small > kSide || longer > static_cast<int64_t>(kMaxCluster) * kMaxBlocks * 64) return -1;
-  const int64_t blocks64 = ceil_div(longer, 64);
-  int C = static_cast<int>(ceil_div(blocks64, kMaxBlocks));
-  if (!cluster_fits(C)) return -1;
+  const int C = cluster_blocks(longer);
   SmallP p = {};
   p.prep = prep;
   p.res = res;
   p.s = static_cast<int>(small);
   p.l = static_cast<int>(longer);
   p.tall = prep.rows > prep.cols;
-  p.blocks = static_cast<int>(ceil_div(blocks64, C));
+  p.blocks = static_cast<int>(ceil_div(ceil_div(longer, 64), C));
   p.steps = steps;
   p.err = device_error_word();
   for (int i = 0; i < 3 * steps; ++i) p.co[i] = co[i];

@@ -1025,14 +1025,18 @@ def _quant_out(x: torch.Tensor, N: int, dtype, group: int, scale_dtype, dev):
     return q, _new(x, shape, scale_dtype)
 
 
-def _workspace(given: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
-    """The caller's workspace where it is large enough, or a new one."""
+def _workspace(given: torch.Tensor | None, need: int, like: torch.Tensor):
+    """(pointer, bytes, the tensor) of the caller's workspace where it is large
+    enough, or of a new one; nothing where none is needed."""
     if given is not None:
         if not isinstance(given, torch.Tensor) or given.device != like.device or not given.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on {like.device}")
-        if given.numel() * given.element_size() >= need and given.data_ptr() % 256 == 0:
-            return given
-    return like.new_empty(max(need, 16), dtype=torch.uint8)
+        if need and given.numel() * given.element_size() >= need and given.data_ptr() % 256 == 0:
+            return given.data_ptr(), given.numel() * given.element_size(), given
+    if need == 0:
+        return None, 0, None
+    new = like.new_empty(need, dtype=torch.uint8)
+    return new.data_ptr(), need, new
 
 
 def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
@@ -1103,11 +1107,10 @@ def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
     wc = weight.contiguous()
     with _on_device(dev):
         need = int(_lib.load().frag_rmsnorm_quant_bwd_workspace_bytes(M, N))
-        workspace = _workspace(workspace, need, x)
+        ws, ws_bytes, workspace = _workspace(workspace, need, x)
         _lib.call("frag_rmsnorm_quant_bwd", _ptr(y2), ys, _ptr(x2), xs, _ptr(rstd), _ptr(wc), _ptr(r2), rs,
                   _ptr(dx), _ptr(q), _ptr(scale), _ptr(dw), M, N, _FP8[dtype], group,
-                  int(scale_dtype != torch.float32), _ptr(workspace),
-                  workspace.numel() * workspace.element_size(), _stream(dev))
+                  int(scale_dtype != torch.float32), ws, ws_bytes, _stream(dev))
     return dx, q, scale, dw
 
 
@@ -1206,9 +1209,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ
         _check_replaces(out, "out", g, (g,))
     co = _schedule(steps, coefficients)
     with _on_device(dev):
-        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), g)
-        _lib.call("frag_orthogonalize", C.byref(desc), _ptr(out), E, m, n, steps, co, float(eps), _ptr(workspace),
-                  workspace.numel() * workspace.element_size(), _stream(dev))
+        ws, ws_bytes, workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), g)
+        _lib.call("frag_orthogonalize", C.byref(desc), _ptr(out), E, m, n, steps, co, float(eps), ws, ws_bytes,
+                  _stream(dev))
     return out
 
 
@@ -1249,8 +1252,8 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
         raise ValueError("param_out and momentum_out overlap")
     co = _schedule(steps, coefficients)
     with _on_device(dev):
-        workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), param)
+        ws, ws_bytes, workspace = _workspace(workspace, orthogonalize_workspace_bytes(E, m, n), param)
         _lib.call("frag_muon_update", C.byref(dp), C.byref(dg), C.byref(dm), _ptr(outs[0]), _ptr(outs[1]), E, m, n,
                   float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), steps, co,
-                  float(eps), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(dev))
+                  float(eps), ws, ws_bytes, _stream(dev))
     return outs[0], outs[1]

@@ -281,3 +281,19 @@ def test_outputs_over_other_matrices_are_refused():
     with pytest.raises(ValueError, match="overlaps"):
         ops.orthogonalize(buf[0, :64, :64].t(), out=buf[0].flatten()[:4096].view(64, 64))
     assert torch.equal(buf, before)
+
+
+def test_one_cluster_a_matrix_takes_no_workspace():
+    assert all(ops.orthogonalize_workspace_bytes(4000, m, n) == 0 for m, n in ((128, 1024), (4096, 128), (1, 1), (64, 100)))
+    assert ops.orthogonalize_workspace_bytes(1, 128, 4097) > 0 and ops.orthogonalize_workspace_bytes(1, 129, 129) > 0
+    g = normal(600, 128, 1024, seed=27, dtype=torch.bfloat16)  # 157 MB; the other form's workspace is 500
+    out = torch.empty_like(g)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.orthogonalize(g, out=out)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert off(out[::97], exact(g[::97])) <= TOL
+    # the caller's is left alone
+    ws = torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
+    assert torch.equal(ops.orthogonalize(g[:2], workspace=ws), out[:2]) and not bool(ws.any())
