@@ -1013,6 +1013,14 @@ def _strided_rows(t: torch.Tensor, name: str, N: int, dev: torch.device, shape=N
     return rows, rows.stride(0) if rows.dim() == 2 else N
 
 
+def _width(weight: torch.Tensor, x: torch.Tensor) -> int:
+    """Values of a row.  Rows of none have no mean: refused, as by the C entry."""
+    N = weight.numel()
+    if N == 0 and math.prod(x.shape[:-1]):
+        raise ValueError("rows must hold at least one value")
+    return N
+
+
 def _quant_out(x: torch.Tensor, N: int, dtype, group: int, scale_dtype, dev):
     if dtype not in _FP8:
         raise TypeError("dtype must be float8_e4m3fn or float8_e5m2")
@@ -1060,7 +1068,7 @@ def rmsnorm_quant_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, 
     _need(x, "x", torch.bfloat16)
     dev = x.device
     _need(weight, "weight", torch.bfloat16, dev)
-    N = weight.numel()
+    N = _width(weight, x)
     x2, xs = _strided_rows(x, "x", N, dev)
     r2, rs = (None, 0) if residual is None else _strided_rows(residual, "residual", N, dev, x.shape)
     q, scale = _quant_out(x, N, dtype, group, scale_dtype, dev)
@@ -1093,7 +1101,7 @@ def rmsnorm_quant_bwd(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
     _need(x, "x", torch.bfloat16)
     dev = x.device
     _need(weight, "weight", torch.bfloat16, dev)
-    N = weight.numel()
+    N = _width(weight, x)
     x2, xs = _strided_rows(x, "x", N, dev)
     y2, ys = _strided_rows(dy, "dy", N, dev, x.shape)
     r2, rs = (None, 0) if dres is None else _strided_rows(dres, "dres", N, dev, x.shape)

@@ -335,3 +335,15 @@ def test_widths_at_the_variants_borders(N):
         for r in (None, res):
             check_fwd(x, w, r, ops.rmsnorm_quant_fwd(x, w, EPS, residual=r, group=group, scale_dtype=E8), group)
             check_bwd(dy, x, rstd, w, r, ops.rmsnorm_quant_bwd(dy, x, rstd, w, dres=r, group=group), group)
+
+
+def test_rows_of_no_values_are_refused():
+    x, w, r = rand(5, 0), rand(0), torch.ones(5, device=DEV)
+    with pytest.raises(ValueError, match="at least one"):
+        ops.rmsnorm_quant_fwd(x, w)
+    with pytest.raises(ValueError, match="at least one"):
+        ops.rmsnorm_quant_fwd(x, w, residual=x, group=32)
+    with pytest.raises(ValueError, match="at least one"):
+        ops.rmsnorm_quant_bwd(x, x, r, w)
+    q, s, _, rstd = ops.rmsnorm_quant_fwd(rand(0, 0), w)  # no rows either
+    assert q.shape == (0, 0) and s.shape == rstd.shape == (0,)
