@@ -24,10 +24,15 @@ __device__ __forceinline__ uint32_t elect_one() {
   return p;
 }
 
-// CG: blocks that share one tile.  With two, a load reports to the barrier of
-// the pair's first block (the address without the bit that tells them apart).
-constexpr uint32_t kPairMask = 0xFEFFFFFFu;
+// The place of a shared-memory address in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
 
+// CG: blocks that share one tile.  With two, a load reports to the barrier of
+// the pair's first block.
 template <int CG>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y,
                                             int z) {
@@ -41,7 +46,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
         "[%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(map), "r"(smem_u32(bar) & kPairMask), "r"(x), "r"(y), "r"(z)
+        "l"(map), "r"(cluster_address(smem_u32(bar), 0)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
@@ -135,19 +140,13 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 }
 // Arrive on the barrier at `bar`'s place in the pair's first block.
 __device__ __forceinline__ void mbar_arrive_first(uint64_t* bar) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address(smem_u32(bar), 0))
+               : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
-}
-__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
   float4 v;
