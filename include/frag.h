@@ -542,7 +542,9 @@ FRAG_API int frag_rmsnorm_quant_bwd(const void* dy, int64_t dy_stride, const voi
  *   types; they may be param and momentum themselves when those are contiguous.
  * Matrices are bf16 or fp32 with any strides (in elements).  Products have
  * fp16 operands (two for each number where a side is at most 128, the other at
- * most 4096 and the result fp32) and fp32 accumulators; X is held in 22 bits.  m, n <= 2^24,
+ * most 4096 and the result fp32) and fp32 accumulators.  X is held in 22 bits,
+ * elements below 2^-22 to 2^-44 (below 2^-11 to 2^-33 where numbers have two
+ * operands), so that a norm far below eps keeps its digits.  m, n <= 2^24,
  * m n < 2^31, steps <= 32, E <= 65535 (FRAG_ERR_SHAPE beyond).  Workspace:
  * frag_orthogonalize_workspace_bytes(E, m, n), 16-byte aligned; 0 (NULL will
  * do) where one side is at most 128 and the other at most 4096.  No

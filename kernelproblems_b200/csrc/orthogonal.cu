@@ -10,15 +10,18 @@
 //
 // Products run on the tensor cores with fp16 operands and fp32 accumulators.
 // What the 16 bits are, and why it is enough:
-//  - X = hi + lo, two fp16 numbers (22 bits).  a X uses both, B X uses hi: an
-//    error of B X lies along directions that are already large, which later
+//  - X = hi + lo, two fp16 numbers: 22 bits where |x| is above 2^-22, 2^-44
+//    below (an element of the largest matrices is 2^-16).  a X uses both, B X
+//    uses hi: an error of B X lies along directions that are already large, which later
 //    steps do not amplify, while an error of a X is multiplied by a^5 = 485
 //    along small ones.  On a gradient of 16 strong directions and a rest of 2%
 //    (512 x 2048), relative error of the result against 64 bits: bf16
 //    throughout 0.27, one fp16 0.035, hi + lo 0.0003.
 //  - everything is kept times a power of two (X 2^8, A and B 2^10), so that
 //    the first step's small entries (1/sqrt(mn) of a unit norm) stay clear of
-//    fp16's subnormals, and the largest (|B| <= 24 for steep schedules) of 65504.
+//    fp16's subnormals, and the largest (|B| <= 24 for steep schedules) of 65504;
+//    lo times another 2^11.  Where the norm is far below eps, X stays small
+//    through all steps and hi is subnormal; lo carries it then.
 //  - B's diagonal (near -2.7 at the end, against small off-diagonal entries)
 //    carries most of B's rounding error: its residual is kept in 32 bits and
 //    added in the epilogue, as is the diagonal's product with lo in the last
@@ -167,7 +170,8 @@ constexpr int kLead = 64;  // the epilogue's first thread
 // X's element becomes  ca (hi + lo) + (acc + d_res hi + f d lo) / 2^10
 //                    = acc / 2^10 + hi (ca + d_res / 2^10) + lo (ca + f d / 2^10):
 // two factors for a row (`coef`), or for a column when the matrix is tall
-// (`cols`, this warp's 32 of them in shared memory).
+// (`cols`, this warp's 32 of them in shared memory); lo's is made for the
+// stored lo, 2^11 times as large.
 template <int MODE>
 __device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set, int e, int i, int j, int r, int half,
                                          bool mirror, float2 coef, const float4* cols, float (&v)[32]) {
@@ -229,8 +233,9 @@ __device__ __forceinline__ void finish32(const ChainP& p, int step, uint32_t set
       y = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lw)), cl, y);
       if (MODE == STEP) {
         const __half2 hi = __float22half2_rn(y);
-        const float2 back = __half22float2(hi);
-        const __half2 rest = __float22half2_rn(make_float2(y.x - back.x, y.y - back.y));
+        // (y - hi) 2^11, exact before it is rounded
+        const __half2 rest = __float22half2_rn(__ffma2_rn(__half22float2(hi), make_float2(-kLoScale, -kLoScale),
+                                                          __fmul2_rn(y, make_float2(kLoScale, kLoScale))));
         wh[q] = *reinterpret_cast<const uint32_t*>(&hi);
         wl[q] = *reinterpret_cast<const uint32_t*>(&rest);
       } else {
@@ -482,7 +487,8 @@ __device__ __forceinline__ void finish_phase(const ChainP& p, Shared& sh, uint32
   auto factors = [&](int e, int d) {
     const float2 v = __ldcg(p.diag + static_cast<int64_t>(e) * p.s + d);
     const float ca = p.co[3 * step];
-    return make_float2(ca + v.y * (1.0f / kAScale), step >= p.steps - 2 ? ca + v.x * (1.0f / kAScale) : ca);
+    return make_float2(ca + v.y * (1.0f / kAScale),
+                       (step >= p.steps - 2 ? ca + v.x * (1.0f / kAScale) : ca) * (1.0f / kLoScale));
   };
   for (int t = blockIdx.x / CG; t < w.items; t += gridDim.x / CG, ++c) {
     int e, ti, tj, z;
@@ -729,7 +735,7 @@ __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
       for (int k = 0; k < 8; ++k) {
         const float x = u[k % V] * f;
         u[k % V] = x;
-        l[k] = x - __half2float(__float2half_rn(x));
+        l[k] = (x - __half2float(__float2half_rn(x))) * kLoScale;
       }
       *reinterpret_cast<uint4*>(p.hi + o) = pack_h8(u);
       *reinterpret_cast<uint4*>(p.lo + o) = pack_h8(l);
@@ -737,7 +743,7 @@ __global__ void __launch_bounds__(256) prep_scale(const PrepP p, int blocks) {
       const float x = u[0] * f;
       const __half h = __float2half_rn(x);
       p.hi[o] = h;
-      p.lo[o] = __float2half_rn(x - __half2float(h));
+      p.lo[o] = __float2half_rn((x - __half2float(h)) * kLoScale);
     }
   }
 }

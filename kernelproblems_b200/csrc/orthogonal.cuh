@@ -10,6 +10,9 @@ namespace frag {
 
 constexpr float kXScale = 256.0f;   // X is kept times 2^8
 constexpr float kAScale = 1024.0f;  // A and B times 2^10
+// lo, where it is no operand of a product, times another 2^11: as large as hi
+// at most, and clear of fp16's subnormals wherever hi is.
+constexpr float kLoScale = 2048.0f;
 
 // GRAM A = X X', POLY B = b A + c A A, STEP X <- a X + B X; the last step's
 // STEP writes the result (LAST) or the weights (UPDATE) instead of X.

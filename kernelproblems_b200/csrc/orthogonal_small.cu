@@ -16,7 +16,8 @@
 // diagonal in 32 bits): an error of 0.6 to 1.5e-3 under a rounding of 1.7e-3.
 // Where the result is stored in 32 bits (FINE), A and B are kept as two fp16
 // numbers like X and each product takes hi hi, hi lo and lo hi: 5e-7 at 64 x
-// 100, for 12 to 25 us more.
+// 100, for 12 to 25 us more.  X's lo is an operand there and not scaled up: an
+// element of X is off by up to 2^-33, which shows where the norm is far below eps.
 //
 // The same 64-column block of X is A's K-major operand (rows of k) and X's
 // MN-major one (rows across k), so it is stored once.
@@ -182,6 +183,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   SmallShared& sh = *reinterpret_cast<SmallShared*>(smem_raw + small_tail(p.blocks));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+  constexpr float lo_scale = FINE ? 1.0f : kLoScale;  // of X's lo
   const int c = static_cast<int>(blockIdx.x) % C, e = static_cast<int>(blockIdx.x) / C;
   const int c0 = c * p.blocks * 64, cols = max(0, min(p.blocks * 64, p.l - c0));
   volatile int* const abort_flag = &sh.abort;
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
       const float x1 = __uint_as_float((aw & 0xffff0000u) | bw >> 16) * f;
       const __half2 h = __floats2half2_rn(x0, x1);
       const float2 back = __half22float2(h);
-      const __half2 rest = __floats2half2_rn(x0 - back.x, x1 - back.y);
+      const __half2 rest = __floats2half2_rn((x0 - back.x) * lo_scale, (x1 - back.y) * lo_scale);
       reinterpret_cast<uint32_t*>(&oh)[w] = *reinterpret_cast<const uint32_t*>(&h);
       reinterpret_cast<uint32_t*>(&ol)[w] = *reinterpret_cast<const uint32_t*>(&rest);
     }
@@ -243,13 +245,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
   };
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   const int k16 = (p.s + 15) / 16;
-  // eight values' hi and lo in two units
+  // eight values' hi and lo in two units (the lo of A and B is used if FINE)
   auto split8 = [](const float* v, uint4& oh, uint4& ol) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const __half2 t = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
       const float2 back = __half22float2(t);
-      const __half2 rest = __floats2half2_rn(v[2 * q] - back.x, v[2 * q + 1] - back.y);
+      const __half2 rest = __floats2half2_rn((v[2 * q] - back.x) * lo_scale, (v[2 * q + 1] - back.y) * lo_scale);
       reinterpret_cast<uint32_t*>(&oh)[q] = *reinterpret_cast<const uint32_t*>(&t);
       reinterpret_cast<uint32_t*>(&ol)[q] = *reinterpret_cast<const uint32_t*>(&rest);
     }
@@ -384,7 +386,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_chain(const __grid_con
 #pragma unroll
         for (int k = 0; k < 32; ++k) d = j + k == r ? v[k] : d;
         const float rest = d - __half2float(__float2half_rn(d));
-        sh.coef[r] = make_float2(ca + rest * (1.0f / kAScale), step >= p.steps - 2 ? ca + d * (1.0f / kAScale) : ca);
+        sh.coef[r] = make_float2(ca + rest * (1.0f / kAScale),
+                                 (step >= p.steps - 2 ? ca + d * (1.0f / kAScale) : ca) * (1.0f / lo_scale));
       }
     }
     // ---- X = a X + B X

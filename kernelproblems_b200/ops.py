@@ -1206,8 +1206,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ
 
     coefficients: a triple (a, b, c) for all steps, or one for each.  They have
     to keep |X| within a few units (as the default and all schedules that
-    converge do): X is held in 22 bits around 1, and its products have fp16
-    operands and fp32 accumulators."""
+    converge do): X is held in 22 bits, its products have fp16 operands and fp32
+    accumulators, and the result is within about 1e-3 of its definition before it
+    is rounded to bf16.  |g|_F^2 is summed in 32 bits: |g|_F up to 1e19."""
     E, m, n, desc = _matrices(g, "g")
     dev = g.device
     if out is None:

@@ -297,3 +297,30 @@ def test_one_cluster_a_matrix_takes_no_workspace():
     # the caller's is left alone
     ws = torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
     assert torch.equal(ops.orthogonalize(g[:2], workspace=ws), out[:2]) and not bool(ws.any())
+
+
+@pytest.mark.parametrize("m,n", [(100, 128), (128, 2048), (300, 700), (700, 301), (2304, 2304)])
+@pytest.mark.parametrize("norm", [1e-3, 1e-6, 1e-8])
+def test_norm_far_below_eps(m, n, norm):
+    """|G| = norm * eps: X stays small through all steps, which then only
+    multiply it.  hi is off by up to 2^-25 and hi + lo by 2^-36 (of 256 times
+    an element), uniformly: 0.6 * 2^-44 * sqrt(mn) / norm of X, 8e-3 for the
+    largest at 1e-8, and the same again from the steps after (each a third as
+    much); under 1e-3 with the rest of TOL elsewhere."""
+    g = normal(m, n, seed=28)
+    g = g / torch.linalg.matrix_norm(g) * (norm * 1e-2)
+    want = exact(g, eps=1e-2)
+    noise = 0.6 * 2.0 ** -44 * math.sqrt(m * n) / norm * 1.5
+    assert off(ops.orthogonalize(g, eps=1e-2), want) <= TOL + noise
+
+
+@pytest.mark.parametrize("m,n", [(64, 100), (96, 160), (128, 700)])
+@pytest.mark.parametrize("norm", [1e-3, 1e-6])
+def test_short_sided_update_with_a_norm_far_below_eps(m, n, norm):
+    """Weights in 32 bits with a side of at most 128: X is off by up to 2^-33 an
+    element in each step, multiplied by the steps after (3.4445^5 = 485)."""
+    g = normal(m, n, seed=29)
+    g = g / torch.linalg.matrix_norm(g) * (norm * 1e-2)
+    p, mom = torch.zeros_like(g), torch.zeros_like(g)
+    p1, _ = ops.muon_update(p, g, mom, lr=1.0, momentum=0.0, nesterov=False, eps=1e-2)
+    assert bool(((p1.double() + exact(g, eps=1e-2)).abs() <= 485 * 1.5 * 2.0 ** -33 + 1e-5 / math.sqrt(max(m, n)) * norm * 485).all())
