@@ -804,7 +804,10 @@ Plan make_plan(int64_t E, int64_t m, int64_t n) {
   q.groups = resident(q.pairs);
   const int64_t side = q.pairs ? 256 : 128;
   q.tiles = chain_tiles(E, q.s, q.s, side, true);
-  // A's and B's tiles at half the width where pairs outnumber them two to one
+  // A's and B's tiles at half the width where pairs outnumber them two to one.
+  // Five steps, full against half: 1024 x 4096 246 and 240 us, 2048 x 2048 331
+  // and 310, 1536 x 2560 290 and 282; but 1100 x 5000, whose A is then split into
+  // fewer parts, 326 and 340.
   q.narrow = q.pairs && 2 * q.tiles <= q.groups;
   if (q.narrow) q.tiles = E * (ceil_div(q.s, 256) * (ceil_div(q.s, 256) - 1) + ceil_div(q.s, 128));
   // A's few tiles with a long k: each in up to four parts of at least six

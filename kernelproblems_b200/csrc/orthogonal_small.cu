@@ -15,8 +15,8 @@
 // Results in bf16 take the chain's arithmetic (single fp16 operands, B's
 // diagonal in 32 bits): an error of 0.6 to 1.5e-3 under a rounding of 1.7e-3.
 // Where the result is stored in 32 bits (FINE), A and B are kept as two fp16
-// numbers like X and each product takes hi hi, hi lo and lo hi: 5e-7 at 64 x
-// 100, for 12 to 25 us more.  X's lo is an operand there and not scaled up: an
+// numbers like X and each product takes hi hi, hi lo and lo hi: 1.5 to 1.7e-6 of
+// the step at 96 x 160 and 128 x 2048, for 12 to 25 us more.  X's lo is an operand there and not scaled up: an
 // element of X is off by up to 2^-33, which shows where the norm is far below eps.
 //
 // The same 64-column block of X is A's K-major operand (rows of k) and X's

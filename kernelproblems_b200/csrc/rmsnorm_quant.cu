@@ -16,6 +16,10 @@
 // without (three bytes a value: 16384 rows of 4096 41 us for a floor of 31, 52
 // with a scale for each 128) and in the gradient (8192 rows of 4096 with the
 // residual 58 us for a floor of 46, 3.5 of them the dweight's second pass).
+// Further from it: rows above 8192 values (4096 rows of 16384 with the residual
+// 92 us for 72, the gradient 153 for 92), rows that are not aligned (8192 rows of
+// 4097 92 us for 36, the gradient 190 for 46) and rows above 16384 values (4096
+// rows of 20000 373 us for 88, the gradient 523 for 113).
 #include <algorithm>
 #include <atomic>
 
@@ -465,6 +469,8 @@ __global__ void __launch_bounds__(256) quant_bwd_warp(const QuantBwdP p, int64_t
 // Longer rows in 16-byte chunks, a block a row: thread 0 streams the rows of
 // the block (dy, x, dres) into a ring of S stages by bulk copies, S rows ahead
 // of the arithmetic; dweight sums stay in registers, thread-owned columns.
+// Four chunks a thread do not fit in the 128 registers of 512 threads: 276 bytes
+// are spilled with the residual and 200 without (three chunks: 64 and 16).
 template <int K, bool HAS_RES, bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(K == 3 ? 256 : 512, K == 3 ? 2 : 1)
 quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int* err) {
@@ -554,7 +560,9 @@ quant_bwd_ring(const QuantBwdP p, int64_t M, int64_t rows_per_block, int S, int*
 }
 
 // Rows without that alignment, up to 16384 values, single values in registers
-// (the layout of quant_fwd_odd); WARP: a warp a row.
+// (the layout of quant_fwd_odd); WARP: a warp a row.  Eight rounds of values in a
+// block's threads (above 8192) spill 208 to 216 bytes with the residual, 64 to 72
+// without.
 template <int K, bool WARP, bool HAS_RES, bool E5M2, bool E8M0>
 __global__ void __launch_bounds__(512) quant_bwd_odd(const QuantBwdP p, int64_t M, int64_t rows_per_block) {
   extern __shared__ float sacc[];  // WARP

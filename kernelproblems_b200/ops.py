@@ -1239,7 +1239,11 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
     param, grad and momentum_buffer are bf16 or fp32, each its own; outputs are
     new contiguous tensors of param's and momentum_buffer's types, or the given
     param_out / momentum_out, which may be param and momentum_buffer themselves
-    (an update in place).  steps, coefficients, eps as in orthogonalize."""
+    (an update in place).  steps, coefficients, eps as in orthogonalize.
+
+    The step's own error, before param' is rounded: about 5e-4 of it (fp16
+    operands), and 2e-6 where param is fp32, a matrix's one side is at most 128
+    and the other at most 4096 (two fp16 numbers for each operand)."""
     E, m, n, dp = _matrices(param, "param")
     dev = param.device
     dg = _matrices(grad, "grad", dev, param.shape)[3]
