@@ -483,7 +483,7 @@ bool cluster_fits(int C) {
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, small_chain<8, true>, &cfg) != cudaSuccess) {
     cudaGetLastError();
-    n = 0;
+    return false;  // asked again by the next call
   }
   known[d][C] = n > 0 ? 2 : 1;
   return n > 0;
