@@ -565,6 +565,81 @@ FRAG_API int frag_muon_update(const frag_matrix* param, const frag_matrix* grad,
                      int nesterov, float weight_decay, float scale, int steps, const float* coefficients, float eps,
                      void* workspace, size_t workspace_bytes, frag_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * (Residual add +) layer norm, and its gradient.
+ *   h = T(res + x) or x;  mean, rstd = 1 / sqrt(mean((h - mean)^2) + eps) per row
+ *   y = T((h - mean) rstd w + b)
+ *   xhat = (x - mean) rstd;  g = dy w
+ *   dx = T(dres + (g - mean(g) - xhat mean(xhat g)) rstd)     rounded once
+ *   dw[n] = sum_m dy xhat,  db[n] = sum_m dy                  fp32, fixed order
+ * T (dtype): FRAG_DT_BF16 or FRAG_DT_F32, of x, res, h, y, dy, dres and dx alike;
+ * w, b: [N] of wdtype, NULL for 1 and 0.  x, res, dy, dres: rows of N values
+ * *_stride values apart; h, y, dx: dense [M,N].  mean, rstd: fp32 [M].  NULL: res,
+ * h (only with res), mean and rstd of the forward, dres, dw, db.  A row's sums are
+ * taken about its mean, so a mean far from zero costs no digits.  y and h may not
+ * share memory with x or res, nor dx with dy, x or dres.  Workspace:
+ * frag_layernorm_bwd_workspace_bytes(M, N), 16-byte aligned.  The reference's
+ * graphs have RMSNorm only; these stand beside frag_rmsnorm_fwd and
+ * frag_rmsnorm_bwd.
+ * ------------------------------------------------------------------------- */
+FRAG_API int frag_layernorm_fwd(const void* x, int64_t x_stride, const void* res, int64_t res_stride, const void* w,
+                     const void* b, void* y, void* h, float* mean, float* rstd, int64_t M, int64_t N, float eps,
+                     int dtype, int wdtype, frag_stream_t stream);
+FRAG_API size_t frag_layernorm_bwd_workspace_bytes(int64_t M, int64_t N);
+FRAG_API int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
+                     const float* rstd, const void* w, const void* dres, int64_t dres_stride, void* dx, float* dw,
+                     float* db, int64_t M, int64_t N, int dtype, int wdtype, void* workspace, size_t workspace_bytes,
+                     frag_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * The 2-norm of `count` tensors together and the factor that clips it.
+ *   norm = sqrt(sum of all g^2);  scale = max_norm / max(norm, max_norm), or NaN
+ *   where norm is not finite
+ * grads, numel, dtypes: HOST arrays of device pointers, counts and FRAG_DT_BF16 /
+ * FRAG_DT_F32; any alignment of whole values.  norm, scale (or NULL): fp32 device
+ * words.  Squares are added in 32 bits within a thread's 32 values and in 64
+ * beyond, in an order that the sizes fix: |g| up to 1e18.  Workspace:
+ * frag_grad_norm_workspace_bytes(count), 16-byte aligned.  No counterpart in the
+ * reference, whose graphs end at the weights' gradients.
+ * ------------------------------------------------------------------------- */
+FRAG_API size_t frag_grad_norm_workspace_bytes(int64_t count);
+FRAG_API int frag_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int64_t count,
+                     float max_norm, float* norm, float* scale, void* workspace, size_t workspace_bytes,
+                     frag_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * One AdamW step over `count` tensors, in place.
+ *   g' = grad_scale g;  m' = beta1 m + (1 - beta1) g';  v' = beta2 v + (1 - beta2) g'^2
+ *   p' = (1 - l weight_decay) p - l m' / c1 / (sqrt(v' / c2) + eps)
+ *   l = lr lr_scale,  c1 = 1 - beta1^step,  c2 = 1 - beta2^step
+ *   copy = bf16(p'), where a tensor has one
+ * tensors, grads, grad_dtypes: HOST arrays; a NULL gradient leaves its tensor as
+ * it is.  Tensors are dense, bf16 or fp32, of any alignment of whole values, and
+ * none shares memory with another or with a gradient.
+ * States are flat and 16-byte aligned: a tensor's begin at state_offset, a multiple
+ * of 128, and take its numel rounded up to 128; those behind its end are zero
+ * and stay so.  exp_avg_scale, exp_avg_sq_scale NULL: exp_avg = m and exp_avg_sq =
+ * v in fp32.  Given: exp_avg = m and exp_avg_sq = sqrt(v) in E4M3, each 128 values
+ * times the fp32 scale [state / 128]; a scale is the largest magnitude / 448 (1
+ * where all are zero), and what is not zero of sqrt(v) stays at least 2^-9 scale.
+ * step counts from 1; step_device, lr_device (device words) replace step and lr
+ * when given, for steps that are captured once and replayed.  With a grad_scale
+ * (device word, or NULL) or a device lr that is not finite, or a device step below
+ * 1, nothing is changed.  No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+typedef struct frag_adamw_tensor {
+  void* param;
+  void* copy; /* bf16, or NULL */
+  int64_t numel, state_offset;
+  float lr_scale, weight_decay;
+  int32_t param_dtype; /* FRAG_DT_BF16 or FRAG_DT_F32 */
+} frag_adamw_tensor;
+
+FRAG_API int frag_adamw_update(const frag_adamw_tensor* tensors, const void* const* grads, const int32_t* grad_dtypes,
+                     int64_t count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale,
+                     double lr, const float* lr_device, double beta1, double beta2, double eps, int64_t step,
+                     const int64_t* step_device, const float* grad_scale, frag_stream_t stream);
+
 /* Self-test of the bounded waits: one thread waits limit_cycles
  * (0 < limit_cycles <= 4e9) on an mbarrier that nothing arrives on, with the
  * same wait every TMA kernel here uses.  The wait gives up and sets

@@ -81,6 +81,18 @@ class Matrix(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("param", _vp),
+        ("copy", _vp),
+        ("numel", _i64),
+        ("state_offset", _i64),
+        ("lr_scale", _f32),
+        ("weight_decay", _f32),
+        ("param_dtype", C.c_int32),  # FRAG_DT_BF16 / FRAG_DT_F32
+    ]
+
+
 FRAG_COPY_MAX_SEGMENTS = 16
 FRAG_PEER_MAX_RANKS = 8
 FRAG_IPC_HANDLE_BYTES = 64
@@ -170,6 +182,16 @@ SIGNATURES: dict[str, tuple] = {
     "frag_muon_update": (
         _int, [C.POINTER(Matrix), C.POINTER(Matrix), C.POINTER(Matrix), _vp, _vp, _i64, _i64, _i64, _f32, _f32,
                _int, _f32, _f32, _int, C.POINTER(_f32), _f32, _vp, _sz, _vp]),
+    "frag_layernorm_fwd": (
+        _int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _int, _int, _vp]),
+    "frag_layernorm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "frag_layernorm_bwd": (
+        _int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp, _sz, _vp]),
+    "frag_grad_norm_workspace_bytes": (_sz, [_i64]),
+    "frag_grad_norm": (_int, [_vp, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "frag_adamw_update": (
+        _int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, C.c_double, _vp, C.c_double, C.c_double, C.c_double, _i64,
+               _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -15,7 +15,9 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 import os
+from array import array
 
 import torch
 
@@ -47,6 +49,11 @@ __all__ = [
     "orthogonalize",
     "muon_update",
     "orthogonalize_workspace_bytes",
+    "layernorm_fwd",
+    "layernorm_bwd",
+    "grad_norm",
+    "AdamWStates",
+    "adamw_update",
     "check_status",
     "reset_status",
 ]
@@ -994,10 +1001,11 @@ _FP8 = {torch.float8_e4m3fn: _lib.FRAG_FP8_E4M3, torch.float8_e5m2: _lib.FRAG_FP
 _GROUPS = (0, 32, 64, 128)
 
 
-def _strided_rows(t: torch.Tensor, name: str, N: int, dev: torch.device, shape=None):
-    """(the tensor, row stride) of a bf16 tensor whose rows of N are
+def _strided_rows(t: torch.Tensor, name: str, N: int, dev: torch.device, shape=None,
+                  dtype: torch.dtype = torch.bfloat16):
+    """(the tensor, row stride) of a tensor whose rows of N are
     contiguous and whose leading dimensions collapse into one row stride."""
-    _need(t, name, torch.bfloat16, dev)
+    _need(t, name, dtype, dev)
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} {tuple(t.shape)} and x {tuple(shape)} differ")
     if t.dim() < 1 or t.shape[-1] != N:
@@ -1270,3 +1278,394 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
                   float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), steps, co,
                   float(eps), ws, ws_bytes, _stream(dev))
     return outs[0], outs[1]
+
+
+# ------------------------------------------------------------------ layer norm
+
+def _norm_input(x: torch.Tensor, name: str):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype not in _DT:
+        raise TypeError(f"{name} must be bfloat16 or float32, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if x.dim() < 1:
+        raise ValueError(f"{name} must have at least one dimension")
+    return x.shape[-1], x.dtype, x.device
+
+
+def _norm_vectors(N: int, dev: torch.device, **vectors):
+    """The vectors as contiguous [N] tensors or None, and the code of their one type."""
+    out, dtype = [], None
+    for name, v in vectors.items():
+        if v is not None:
+            if not isinstance(v, torch.Tensor) or v.dtype not in _DT or (dtype is not None and v.dtype != dtype):
+                raise TypeError(f"{name} must be bfloat16 or float32, weight and bias of one type")
+            dtype = v.dtype
+            _need(v, name, dtype, dev)
+            if v.numel() != N:
+                raise ValueError(f"{name}: {v.numel()} elements, rows have {N}")
+            v = v.contiguous()
+        out.append(v)
+    return (*out, _DT[dtype or torch.float32])
+
+
+def _row_count(x: torch.Tensor, N: int) -> int:
+    M = math.prod(x.shape[:-1])
+    if N == 0 and M:
+        raise ValueError("rows must hold at least one value")
+    return M
+
+
+def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  eps: float = 1e-5, *, residual: torch.Tensor | None = None, write_h: bool = True,
+                  save_stats: bool = True):
+    """(Residual add +) layer norm over the last dimension, in one pass.
+    Returns (y, h, mean, rstd).
+
+    y      (h - mean) * rstd * weight + bias, rounded once to x's type
+    h      residual + x in x's type: the new residual stream, which the
+           backward takes as its x; None without a residual or with write_h=False
+    mean   fp32 x.shape[:-1], and
+    rstd   1 / sqrt(mean((h - mean)^2) + eps), the same; None with save_stats=False
+
+    x and residual: bf16 or fp32, rows of contiguous values, any row stride.
+    weight, bias: bf16 or fp32 (both the same), or None for 1 and 0."""
+    N, dtype, dev = _norm_input(x, "x")
+    M = _row_count(x, N)
+    x2, xs = _strided_rows(x, "x", N, dev, None, dtype)
+    r2, rs = (None, 0) if residual is None else _strided_rows(residual, "residual", N, dev, x.shape, dtype)
+    w, b, wdt = _norm_vectors(N, dev, weight=weight, bias=bias)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = mean = rstd = None
+    if residual is not None and write_h:
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if save_stats:
+        mean, rstd = _new(x, x.shape[:-1], torch.float32), _new(x, x.shape[:-1], torch.float32)
+    with _on_device(dev):
+        _lib.call("frag_layernorm_fwd", _ptr(x2), xs, _ptr(r2), rs, _ptr(w), _ptr(b), _ptr(y), _ptr(h), _ptr(mean),
+                  _ptr(rstd), M, N, float(eps), _DT[dtype], wdt, _stream(dev))
+    return y, h, mean, rstd
+
+
+def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                  weight: torch.Tensor | None = None, *, dres: torch.Tensor | None = None, compute_dw: bool = True,
+                  compute_db: bool = True, workspace: torch.Tensor | None = None):
+    """The gradient of layernorm_fwd.  Returns (dx, dw, db).
+
+    x      the normalised input (h of layernorm_fwd), mean and rstd its saved fp32
+    dres   the residual stream's own gradient, added to dx
+    dx     dres + the gradient of the norm, rounded once to x's type
+    dw     fp32 [N], sum over the rows of dy * (x - mean) * rstd in a fixed order;
+           None with compute_dw=False or without a weight
+    db     fp32 [N], sum over the rows of dy in a fixed order; None with compute_db=False
+
+    dy, x and dres: of one type, rows of contiguous values, any row stride."""
+    N, dtype, dev = _norm_input(x, "x")
+    M = _row_count(x, N)
+    x2, xs = _strided_rows(x, "x", N, dev, None, dtype)
+    y2, ys = _strided_rows(dy, "dy", N, dev, x.shape, dtype)
+    r2, rs = (None, 0) if dres is None else _strided_rows(dres, "dres", N, dev, x.shape, dtype)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _need(t, name, torch.float32, dev)
+        if t.numel() != M or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with {M} elements")
+    w, wdt = _norm_vectors(N, dev, weight=weight)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dw = x.new_empty(N, dtype=torch.float32) if compute_dw and weight is not None else None
+    db = x.new_empty(N, dtype=torch.float32) if compute_db else None
+    with _on_device(dev):
+        need = int(_lib.load().frag_layernorm_bwd_workspace_bytes(M, N)) if dw is not None or db is not None else 0
+        ws, ws_bytes, workspace = _workspace(workspace, need, x)
+        _lib.call("frag_layernorm_bwd", _ptr(y2), ys, _ptr(x2), xs, _ptr(mean), _ptr(rstd), _ptr(w), _ptr(r2), rs,
+                  _ptr(dx), _ptr(dw), _ptr(db), M, N, _DT[dtype], wdt, ws, ws_bytes, _stream(dev))
+    return dx, dw, db
+
+
+# -------------------------------------------------- many tensors in one launch
+
+# A step's lists have hundreds of tensors: what is asked of each goes through
+# map, 0.05 us a tensor and question where a loop of checks would take 1.
+_dtype_of = operator.attrgetter("dtype")
+_shape_of = operator.attrgetter("shape")
+
+
+def _pointers(tensors) -> array:
+    return array("Q", map(torch.Tensor.data_ptr, tensors))
+
+
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _dense_list(tensors, name: str) -> torch.device:
+    """Checks a list of contiguous bf16 or fp32 tensors on one CUDA device."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
+    dtypes = set(map(_dtype_of, tensors))
+    if not dtypes <= _DT.keys():
+        raise TypeError(f"{name} must be bfloat16 or float32, got {sorted(map(str, dtypes - _DT.keys()))}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError(f"{name} must be contiguous")
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if len(devices) != 1:
+        raise ValueError(f"{name} must be on one device")
+    if devices == {-1}:
+        raise ValueError(f"{name} must be CUDA tensors")
+    return tensors[0].device
+
+
+def _dtype_codes(tensors) -> array:
+    dtypes = list(map(_dtype_of, tensors))
+    first = dtypes[0] if dtypes else None
+    if dtypes.count(first) == len(dtypes):
+        return array("i", [_DT[first]] * len(dtypes)) if dtypes else array("i")
+    return array("i", [_DT[d] for d in dtypes])
+
+
+def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor | None = None):
+    """The 2-norm of a list of gradients together, and the factor that clips it,
+    without a look from the host.  Returns (norm, scale), fp32 tensors of no
+    dimension:
+
+    norm   sqrt(sum of all squares), in an order that the sizes alone decide
+    scale  max_norm / max(norm, max_norm), which adamw_update takes as its
+           grad_scale; NaN where norm is not finite (the update then changes
+           nothing); None without max_norm
+
+    grads: contiguous bf16 and fp32 tensors on one device, |g| up to 1e18; None
+    entries are left out."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise ValueError("grad_norm needs at least one tensor")
+    if max_norm is not None and not (max_norm > 0 and math.isfinite(max_norm)):
+        raise ValueError("max_norm must be positive and finite")
+    dev = _dense_list(grads, "grads")
+    ptrs, numel, codes = _pointers(grads), array("q", map(torch.Tensor.numel, grads)), _dtype_codes(grads)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    scale = None if max_norm is None else torch.empty((), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        need = int(_lib.load().frag_grad_norm_workspace_bytes(len(grads)))
+        ws, ws_bytes, workspace = _workspace(workspace, need, norm)
+        _lib.call("frag_grad_norm", _address(ptrs), _address(numel), _address(codes), len(grads),
+                  1.0 if max_norm is None else float(max_norm), _ptr(norm), _ptr(scale), ws, ws_bytes, _stream(dev))
+    return norm, scale
+
+
+def _each(v, n: int, name: str) -> list[float]:
+    values = [float(v)] * n if isinstance(v, (int, float)) else [float(x) for x in v]
+    if len(values) != n:
+        raise ValueError(f"{name}: {len(values)} values for {n} tensors")
+    if not all(map(math.isfinite, values)):
+        raise ValueError(f"{name} must be finite")
+    return values
+
+
+def _disjoint(tensors, name: str) -> None:
+    """Refuses contiguous tensors that share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise ValueError(f"{name} share memory")
+
+
+class AdamWStates:
+    """The moments of a list of parameters for adamw_update, and what is fixed
+    about each parameter.
+
+    params        contiguous bf16 or fp32 CUDA tensors of one device, updated in place
+    dtype         torch.float32, or torch.float8_e4m3fn: 8 bits and a scale for
+                  each 128 values of a tensor
+    weight_decay  one for all, or one for each (0 for norms and biases)
+    lr_scale      a factor on lr, one for all or one for each
+    copies        bf16 tensors (or None) shaped like the parameters, which receive
+                  the rounded parameter in the same pass: the model's weights where
+                  the parameters are their fp32 masters
+
+    States are flat tensors, zero at first; parameter i's begin at offsets[i] (a
+    multiple of 128), and the values behind its end are zero:
+      exp_avg, exp_avg_sq               fp32: first and second moment
+      exp_avg, exp_avg_scale,           8 bits: the first moment and the root of the
+      exp_avg_sq, exp_avg_sq_scale      second, each value * scale[its index // 128]
+    A tensor's place in memory is looked up in every call, so a parameter whose data
+    was replaced (by one of the same shape and type) is found again."""
+
+    GROUP = 128
+
+    def __init__(self, params, *, dtype: torch.dtype = torch.float32, weight_decay=0.0, lr_scale=1.0, copies=None):
+        self.params = list(params)
+        n = len(self.params)
+        if not n:
+            raise ValueError("AdamWStates needs at least one parameter")
+        if dtype not in (torch.float32, torch.float8_e4m3fn):
+            raise TypeError("dtype must be float32 or float8_e4m3fn")
+        decay, lr_scale = _each(weight_decay, n, "weight_decay"), _each(lr_scale, n, "lr_scale")
+        self.device = _dense_list(self.params, "params")
+        self.copies = [None] * n if copies is None else list(copies)
+        if len(self.copies) != n:
+            raise ValueError(f"copies: {len(self.copies)} for {n} parameters")
+        for p, c in zip(self.params, self.copies):
+            if c is not None:
+                _check_out(c, "a copy", torch.bfloat16, self.device, shape=p.shape)
+        self.dtype = dtype
+        self._shapes = list(map(_shape_of, self.params))
+        self._written = self.params + [c for c in self.copies if c is not None]
+        self._kinds = list(map(_dtype_of, self._written))
+        self._numel = list(map(torch.Tensor.numel, self._written))
+        _disjoint(self._written, "parameters and copies")
+        self.offsets, total = [], 0
+        for numel in self._numel[:n]:
+            self.offsets.append(total)
+            total += -(-numel // self.GROUP) * self.GROUP
+        self._total = total
+        self.exp_avg = torch.zeros(total, dtype=dtype, device=self.device)
+        self.exp_avg_sq = torch.zeros(total, dtype=dtype, device=self.device)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if dtype != torch.float32:
+            self.exp_avg_scale = torch.ones(total // self.GROUP, dtype=torch.float32, device=self.device)
+            self.exp_avg_sq_scale = torch.ones_like(self.exp_avg_scale)
+        self._table = (_lib.AdamWTensor * n)()
+        for i, e in enumerate(self._table):
+            e.numel, e.state_offset = self._numel[i], self.offsets[i]
+            e.lr_scale, e.weight_decay, e.param_dtype = lr_scale[i], decay[i], _DT[self._kinds[i]]
+        self._places = None
+        self._place()
+
+    def _place(self) -> None:
+        """The table's addresses, looked up again; checked where any has changed."""
+        written = self._written
+        if (list(map(_dtype_of, written)) != self._kinds or list(map(torch.Tensor.numel, written)) != self._numel
+                or not all(map(torch.Tensor.is_contiguous, written))):
+            raise ValueError("a parameter or copy has another type or shape than the states were made for")
+        places = _pointers(written)
+        if places == self._places:
+            return
+        if _dense_list(written, "params") != self.device:
+            raise ValueError(f"parameters are no longer on {self.device}")
+        if list(map(_shape_of, self.params)) != self._shapes:
+            raise ValueError("a parameter has another shape than the states were made for")
+        _disjoint(written, "parameters and copies")
+        at = len(self.params)
+        for i, e in enumerate(self._table):
+            e.param, e.copy = places[i], None
+            if self.copies[i] is not None:
+                e.copy = places[at]
+                at += 1
+        self._places = places
+
+    def _held(self):
+        """The states' addresses; refused where one is not what it was made as."""
+        total, out = self._total, []
+        for k, dtype, numel in (("exp_avg", self.dtype, total), ("exp_avg_sq", self.dtype, total),
+                                ("exp_avg_scale", torch.float32, total // self.GROUP),
+                                ("exp_avg_sq_scale", torch.float32, total // self.GROUP)):
+            t = getattr(self, k)
+            if k.endswith("scale") and self.dtype == torch.float32:
+                out.append(None)
+            else:
+                out.append(_check_out(t, k, dtype, self.device, numel=numel).data_ptr())
+        return out
+
+    def moments(self, i: int):
+        """Parameter i's first and second moment, new fp32 tensors of its shape."""
+        a, n, shape = self.offsets[i], self._numel[i], self._shapes[i]
+        held = slice(a, a + -(-n // self.GROUP) * self.GROUP)
+        m, v = self.exp_avg[held].float(), self.exp_avg_sq[held].float()
+        if self.dtype != torch.float32:
+            at = slice(held.start // self.GROUP, held.stop // self.GROUP)
+            m = (m.view(-1, self.GROUP) * self.exp_avg_scale[at, None]).view(-1)
+            v = (v.view(-1, self.GROUP) * self.exp_avg_sq_scale[at, None]).view(-1).square()
+        return m[:n].clone().view(shape), v[:n].clone().view(shape)
+
+    _NAMES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+
+    def state_dict(self) -> dict:
+        """The states themselves (not copies), by name, and the sizes they are for."""
+        d = {k: getattr(self, k) for k in self._NAMES if getattr(self, k) is not None}
+        return {"numel": self._numel[:len(self.params)], **d}
+
+    def load_state_dict(self, d: dict) -> None:
+        if list(d["numel"]) != self._numel[:len(self.params)]:
+            raise ValueError("the states are of parameters of other sizes")
+        held = [k for k in self._NAMES if getattr(self, k) is not None]
+        if {k for k in self._NAMES if d.get(k) is not None} != set(held) or any(
+                d[k].dtype != getattr(self, k).dtype or d[k].shape != getattr(self, k).shape for k in held):
+            raise ValueError("the states are of another type or shape")
+        for k in held:
+            getattr(self, k).copy_(d[k])
+
+
+def _device_word(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device) -> int:
+    _need(t, name, dtype, dev)
+    if t.numel() != 1:
+        raise ValueError(f"{name} must have one element")
+    return t.data_ptr()
+
+
+def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps: float = 1e-8,
+                 grad_scale: torch.Tensor | None = None) -> None:
+    """One AdamW step over all parameters of `states` in one launch, in place
+    (parameters, their bf16 copies, and states):
+
+      g  grad_scale * grad
+      m  beta1 * m + (1 - beta1) * g,   v  beta2 * v + (1 - beta2) * g^2
+      p  (1 - l * weight_decay) * p - l * m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps)
+         with l = lr * lr_scale
+
+    grads       a tensor for each parameter, of its shape, contiguous, bf16 or fp32;
+                None leaves that parameter and its states as they are
+    lr          a number, or a one-element fp32 CUDA tensor
+    step        counts from 1: an int, or a one-element int64 CUDA tensor, which a
+                captured call reads anew in every replay (an int and a float lr
+                are what they were at capture)
+    grad_scale  one-element fp32 CUDA tensor (grad_norm's scale), or None
+
+    Where grad_scale or a device lr is not finite, or a device step below 1, nothing
+    is changed.  Parameters are rounded to nearest: bf16 ones do not move by less than
+    2^-9 of their value, for which there are fp32 parameters with bf16 copies.  With
+    states in 8 bits a gradient that is not finite makes its whole group of 128 NaN.
+    Gradients must not share memory with parameters, copies or states."""
+    if not isinstance(states, AdamWStates):
+        raise TypeError("states must be an AdamWStates")
+    dev = states.device
+    n = len(states.params)
+    grads = list(grads)
+    if len(grads) != n:
+        raise ValueError(f"{len(grads)} gradients for {n} parameters")
+    b1, b2 = betas
+    if not (0 <= b1 < 1 and 0 <= b2 < 1):
+        raise ValueError("betas must be in [0, 1)")
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and not negative")
+    lr_ptr = step_ptr = None
+    if isinstance(lr, torch.Tensor):
+        lr_ptr, lr = _device_word(lr, "lr", torch.float32, dev), 0.0
+    elif not math.isfinite(lr):
+        raise ValueError("lr must be finite")
+    if isinstance(step, torch.Tensor):
+        step_ptr, step = _device_word(step, "step", torch.int64, dev), 0
+    elif not isinstance(step, int) or step < 1:
+        raise ValueError("step must be an int from 1 on")
+    scale_ptr = None if grad_scale is None else _device_word(grad_scale, "grad_scale", torch.float32, dev)
+    shapes = states._shapes
+    if any(g is None for g in grads):
+        given = [g for g in grads if g is not None]
+        shapes = [s for s, g in zip(shapes, grads) if g is not None]
+        if not given:
+            return
+    else:
+        given = grads
+    if _dense_list(given, "grads") != dev:
+        raise ValueError(f"grads must be on {dev}")
+    if list(map(_shape_of, given)) != shapes:
+        raise ValueError("every gradient must have its parameter's shape")
+    states._place()
+    if given is grads:
+        ptrs, codes = _pointers(grads), _dtype_codes(grads)
+    else:
+        ptrs = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+        codes = array("i", [0 if g is None else _DT[g.dtype] for g in grads])
+    with _on_device(dev):
+        _lib.call("frag_adamw_update", states._table, _address(ptrs), _address(codes), n, *states._held(), float(lr),
+                  lr_ptr, float(b1), float(b2), float(eps), step, step_ptr, scale_ptr, _stream(dev))

@@ -185,3 +185,54 @@ def test_smoke_has_no_matrix_for_pairs_of_blocks():
     assert "SMOKE_MATRICES" in inspect.getsource(entry.smoke)
     for m, n in entry.SMOKE_MATRICES:
         assert 4 * -(-m // 256) * -(-n // 256) < 3 * 74
+
+
+def test_layernorm_rejects_bad_arguments_on_the_host():
+    lib = _lib.load()
+    fwd = lambda M, N, dt=0, wdt=0, x=None, y=None, h=None: lib.frag_layernorm_fwd(  # noqa: E731
+        x, N, None, 0, None, None, y, h, None, None, M, N, 1e-5, dt, wdt, None)
+    assert fwd(4, 64) == 1 and fwd(-1, 64) == 1 and fwd(4, 64, dt=2) == 1 and fwd(4, 64, wdt=3) == 1
+    assert fwd(4, 0) == 2 and fwd(1 << 31, 8) == 2 and fwd(0, 64) == 0
+    assert fwd(4, 64, x=16, y=64, h=128) == 1  # h without a residual
+    assert fwd(4, 64, x=17, y=64) == 3 and fwd(4, 64, dt=1, x=16, y=66) == 3
+    bwd = lambda M, N, dt=0, dw=None, p=None, x=None: lib.frag_layernorm_bwd(  # noqa: E731
+        p, N, x or p, N, p, p, None, None, 0, p, dw, None, M, N, dt, 0, None, 0, None)
+    assert bwd(4, 64) == 1 and bwd(-1, 64) == 1 and bwd(4, 64, dt=2) == 1
+    assert bwd(4, 0) == 2 and bwd(0, 64) == 0 and bwd(4, 64, dw=64, p=64) == 4 and bwd(4, 64, p=64, x=65) == 3
+    assert lib.frag_layernorm_bwd_workspace_bytes(0, 64) == 0
+    assert lib.frag_layernorm_bwd_workspace_bytes(4, 64) >= 2 * 4 * 64
+
+
+def test_lists_of_tensors_are_checked_on_the_host():
+    lib = _lib.load()
+    one = lambda kind, v: (kind * 1)(v)  # noqa: E731
+    ptr, num, code = one(C.c_void_p, 64), one(C.c_int64, 10), one(C.c_int32, 1)
+    norm = lambda p=ptr, n=num, c=code, count=1, top=1.0, out=64, scale=None, ws=None, size=0: lib.frag_grad_norm(  # noqa: E731
+        p, n, c, count, top, out, scale, ws, size, None)
+    assert norm() == 4 and norm(ws=8, size=1 << 20) == 3  # workspace missing, not aligned
+    assert norm(count=-1) == 1 and norm(p=None) == 1 and norm(out=None) == 1 and norm(scale=64, top=0.0) == 1
+    assert norm(scale=64, top=float("nan")) == 1 and norm(n=one(C.c_int64, -1)) == 1 and norm(c=one(C.c_int32, 5)) == 1
+    assert norm(p=one(C.c_void_p, 66)) == 3 and norm(p=one(C.c_void_p, None)) == 1
+    assert lib.frag_grad_norm_workspace_bytes(1) > 0
+
+    def adamw(t=None, grads=ptr, codes=code, count=1, m=64, v=64, ms=None, vs=None, lr=1e-3, b1=0.9, b2=0.9, eps=1e-8, step=1):
+        table = (_lib.AdamWTensor * 1)(t or _lib.AdamWTensor(64, None, 10, 0, 1.0, 0.0, 1))
+        return lib.frag_adamw_update(table, grads, codes, count, m, v, ms, vs, lr, None, b1, b2, eps, step, None, None, None)
+    T = _lib.AdamWTensor
+    assert adamw(count=-1) == 1 and adamw(grads=None) == 1 and adamw(b1=1.0) == 1 and adamw(b2=-0.1) == 1
+    assert adamw(eps=-1.0) == 1 and adamw(lr=float("nan")) == 1 and adamw(step=0) == 1 and adamw(ms=64) == 1
+    assert adamw(m=None) == 1 and adamw(m=68) == 3 and adamw(codes=one(C.c_int32, 2)) == 1
+    assert adamw(T(None, None, 10, 0, 1.0, 0.0, 1)) == 1 and adamw(T(64, None, -1, 0, 1.0, 0.0, 1)) == 1
+    assert adamw(T(64, None, 10, 64, 1.0, 0.0, 1)) == 3 and adamw(T(66, None, 10, 0, 1.0, 0.0, 1)) == 3
+    assert adamw(T(64, 65, 10, 0, 1.0, 0.0, 1)) == 3 and adamw(T(64, None, 10, 0, float("inf"), 0.0, 1)) == 1
+    assert adamw(T(64, None, 10, 0, 1.0, 0.0, 7)) == 1 and adamw(T(64, None, 0, 0, 1.0, 0.0, 1)) == 0 and adamw(count=0) == 0
+
+
+def test_states_need_cuda_tensors():
+    for bad in ([], [torch.zeros(8)], [torch.zeros(8).half()], [1.0]):
+        with pytest.raises((ValueError, TypeError)):
+            ops.AdamWStates(bad)
+    with pytest.raises(ValueError):
+        ops.grad_norm([torch.zeros(8)])
+    with pytest.raises(ValueError):
+        ops.layernorm_fwd(torch.zeros(2, 8))
