@@ -1,0 +1,474 @@
+// layernorm_bwd.cu — the gradient of layer norm, with the sums over the rows for
+// weight and bias.
+#include "layernorm.cuh"
+
+namespace frag {
+namespace {
+
+template <class T>
+struct BwdP {
+  const T* dy;
+  const T* x;
+  const T* dres;
+  T* dx;
+  Vector w;
+  const float* mean;
+  const float* rstd;
+  float* partials;  // [G, vectors, N]: dw, db, as far as wanted
+  int64_t ys, xs, rs;
+  int64_t N;
+  int want_dw, want_db;
+};
+
+// --------------------------------------------------------------- gradient
+
+// A chunk: x becomes x - mean, and its part of (sum of g, sum of g (x - mean)),
+// g = dy w, is added.
+template <class T>
+__device__ __forceinline__ void chunk_sums(const float2* dy, float2* x, const float2* w, float mean, float2& s1,
+                                           float2& s2) {
+#pragma unroll
+  for (int q = 0; q < kP<T>; ++q) {
+    x[q] = __fadd2_rn(x[q], twice(-mean));
+    const float2 g = __fmul2_rn(dy[q], w[q]);
+    s1 = __fadd2_rn(s1, g);
+    s2 = __ffma2_rn(g, x[q], s2);
+  }
+}
+
+// What a row's second pass needs of its sums: dx = r g + a + b (x - mean).
+struct RowTerms {
+  float2 r, a, b;
+  __device__ __forceinline__ RowTerms(float rstd, float s1, float s2, float invN) {
+    r = twice(rstd);
+    a = twice(-s1 * invN * rstd);                           // mean(g) rstd
+    b = twice(-((s2 * rstd) * invN) * rstd * rstd);         // mean(xhat g) rstd, of xhat = (x - mean) rstd
+  }
+};
+
+// A chunk's dx (on top of dres, where there is one), and its part of dw and db.
+template <class T, bool RES>
+__device__ __forceinline__ void chunk_grad(const float2* dy, const float2* far, const float2* w, const RowTerms& t,
+                                           float2* o, float2* dw, float2* db) {
+#pragma unroll
+  for (int q = 0; q < kP<T>; ++q) {
+    float2 e = __ffma2_rn(far[q], t.b, t.a);
+    e = __ffma2_rn(__fmul2_rn(dy[q], w[q]), t.r, e);
+    o[q] = RES ? __fadd2_rn(o[q], e) : e;
+    dw[q] = __ffma2_rn(dy[q], __fmul2_rn(far[q], t.r), dw[q]);
+    db[q] = __fadd2_rn(dy[q], db[q]);
+  }
+}
+
+// Rows of up to 512 values, as fwd_lanes; the columns' sums stay in registers,
+// and at the end a block's groups add theirs in shared memory, one after the other.
+template <class T, int V, int L, Mode MODE, bool RES>
+__global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const BwdP<T> p, const Rows rows) {
+  constexpr int E = kE<T>, P = kP<T>, K = V / E, ROW = (RES ? 3 : 2) * K;
+  extern __shared__ __align__(16) uint4 held[];  // [kAhead][ROW][256], [kAhead][2][256] of float
+  float* stats = reinterpret_cast<float*>(held + kAhead * ROW * 256);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int N = static_cast<int>(p.N);
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (256 / L);  // a multiple of the classes
+  int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int off = MODE == EDGE ? static_cast<int>((rows.off + row % rows.classes * N) % E) : 0;
+  const int t = threadIdx.x % L;
+  const Places<T, MODE> at = {t, L, off};
+  auto ask = [&](int64_t r, int s) {
+    uint4* to = held + s * (ROW * 256) + threadIdx.x;
+    if (r < rows.M) {
+      ask_row<T, K, MODE>({p.dy, p.ys}, r, rows.M, at, N, to);
+      ask_row<T, K, MODE>({p.x, p.xs}, r, rows.M, at, N, to + K * 256);
+      if (RES) ask_row<T, K, MODE>({p.dres, p.rs}, r, rows.M, at, N, to + 2 * K * 256);
+      copy_async4(stats + s * 512 + threadIdx.x, p.mean + r);
+      copy_async4(stats + s * 512 + 256 + threadIdx.x, p.rstd + r);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead - 1; ++s) ask(row + s * groups, s);
+  float2 w[V / 2], dw[V / 2], db[V / 2];
+#pragma unroll
+  for (int k = 0; k < K; ++k) load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
+#pragma unroll
+  for (int q = 0; q < V / 2; ++q) dw[q] = db[q] = twice(0.f);
+  const float invN = 1.0f / static_cast<float>(N);
+  int s = 0;
+  // (the lanes of a warp stay together: shuffles are the whole warp's)
+  for (int64_t lead = row - (threadIdx.x & 31) / L; lead < rows.M; lead += groups, row += groups) {
+    ask(row + (kAhead - 1) * groups, (s + kAhead - 1) % kAhead);
+    copies_wait<kAhead - 1>();
+    const uint4* from = held + s * (ROW * 256) + threadIdx.x;
+    const float mean = stats[s * 512 + threadIdx.x], rstd = stats[s * 512 + 256 + threadIdx.x];
+    s = (s + 1) % kAhead;
+    float2 d[V / 2], x[V / 2], s1 = twice(0.f), s2 = s1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!at[k].some(N)) continue;
+      unpack<T>(from[k * 256], d + k * P);
+      unpack<T>(from[(K + k) * 256], x + k * P);
+      own_values<T, MODE>(at[k], N, 0.f, d + k * P);
+      own_values<T, MODE>(at[k], N, mean, x + k * P);
+      chunk_sums<T>(d + k * P, x + k * P, w + k * P, mean, s1, s2);
+    }
+    const float g1 = lanes_sum<L>(s1.x + s1.y), g2 = lanes_sum<L>(s2.x + s2.y);
+    if (row >= rows.M) continue;
+    const RowTerms terms(rstd, g1, g2, invN);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!at[k].some(N)) continue;
+      float2 o[P];
+      if (RES) unpack<T>(from[(2 * K + k) * 256], o);
+      chunk_grad<T, RES>(d + k * P, x + k * P, w + k * P, terms, o, dw + k * P, db + k * P);
+      store_chunk<T, MODE>(p.dx + row * p.N, at[k], N, o);
+    }
+  }
+  if (!p.want_dw && !p.want_db) return;
+  copies_wait<0>();
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(held);  // [2][512]
+  for (int i = threadIdx.x; i < 2 * 512; i += 256) sums[i] = 0.f;
+  for (int q = 0; q < 256 / L; ++q) {
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) / L != q) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (at[k].some(N) && at[k].has(i, N)) {
+          sums[at[k].n0 + i] += part(dw[k * P + i / 2], i & 1);
+          sums[512 + at[k].n0 + i] += part(db[k * P + i / 2], i & 1);
+        }
+  }
+  __syncthreads();
+  float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * N;
+  for (int n = threadIdx.x; n < N; n += 256) {
+    if (p.want_dw) to[n] = sums[n];
+    if (p.want_db) to[(p.want_dw ? N : 0) + n] = sums[512 + n];
+  }
+}
+
+// A chunk's sums into a row of partials.
+template <class T, Mode MODE>
+__device__ __forceinline__ void store_sums(float* row, const Place<T, MODE>& at, int N, float2* f) {
+  if (MODE != EDGE && at.some(N)) {
+#pragma unroll
+    for (int q = 0; q < kP<T>; q += 2)
+      *reinterpret_cast<float4*>(row + at.n0 + 2 * q) = make_float4(f[q].x, f[q].y, f[q + 1].x, f[q + 1].y);
+  } else if (MODE == EDGE && at.some(N)) {
+#pragma unroll
+    for (int i = 0; i < kE<T>; ++i)
+      if (at.has(i, N)) row[at.n0 + i] = part(f[i / 2], i & 1);
+  }
+}
+
+// Two sums over a block of up to 512 threads, in a fixed order, for every thread.
+// After one exchange the lower half of a warp's lanes add the first and the upper
+// half the second, so that both take one shuffle a level.
+__device__ __forceinline__ float2 block_pair(float a, float b, float (*slots)[32], int parity) {
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  const bool upper = lane & 16;
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((lane & 15) == 0) slots[parity][(threadIdx.x >> 5) + (upper ? 16 : 0)] = v;
+  __syncthreads();
+  v = (lane & 15) < nw ? slots[parity][lane] : 0.f;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+}
+
+// Wider rows: a block stays for `each` rows of a class, 16 values a thread, the
+// next rows in the ring.  A thread keeps the weights at its columns, their two
+// sums, and a row's dy and x - mean from the first pass to the second, at most 112
+// registers: two blocks of 256 threads an SM, whose barriers overlap.  WIDE (more
+// than 512 threads a block): 64 registers, the row is read from its stage twice
+// and the weights come from L1.
+template <class T, Mode MODE, bool RES, bool WIDE>
+__device__ __forceinline__ void bwd_ring_body(const BwdP<T>& p, const Rows& rows, const RingShape& shape, int* err) {
+  constexpr int P = kP<T>, V = 16, K = V / kE<T>, INPUTS = RES ? 3 : 2;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float2 slots2[WIDE ? 2 : 1][32];
+  __shared__ float slots[2][32];
+  __shared__ int s_abort;
+  const int N = static_cast<int>(p.N);
+  Ring<T, INPUTS, MODE> ring;
+  ring.in[0] = {p.dy, p.ys};
+  ring.in[1] = {p.x, p.xs};
+  if (RES) ring.in[INPUTS - 1] = {p.dres, p.rs};
+  deal(ring, rows, shape, smem, N);
+  const Places<T, MODE> at = {static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), ring.off};
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    ring.begin();
+  }
+  __syncthreads();
+  // A stage is free again when every thread is in the next row: S - 1 rows ahead.
+  if (threadIdx.x == 0)
+    for (int i = 0; i < max(1, ring.S - 1); ++i) ring.issue(i);
+  float2 w[WIDE ? 1 : V / 2], dw[V / 2], db[V / 2];
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
+  }
+#pragma unroll
+  for (int q = 0; q < V / 2; ++q) dw[q] = db[q] = twice(0.f);
+  const float invN = 1.0f / static_cast<float>(N);
+  int i = 0;
+  for (; i < ring.count; ++i) {
+    const int64_t row = ring.row(i);
+    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+    if (!ring.wait(i, err)) s_abort = 1;
+    float2 d[WIDE ? P : V / 2], x[WIDE ? P : V / 2], wk[P], s1 = twice(0.f), s2 = s1;
+    // A chunk's dy, x - mean and weights, and its part of the sums.
+    auto take = [&](int k, float2* dk, float2* xk) {
+      const int c = threadIdx.x + k * blockDim.x;
+      unpack<T>(ring.chunk(i, 0, c), dk);
+      unpack<T>(ring.chunk(i, 1, c), xk);
+      own_values<T, MODE>(at[k], N, 0.f, dk);
+      own_values<T, MODE>(at[k], N, mean, xk);
+      if constexpr (WIDE) load_vector<T, MODE>(p.w, at[k], N, 1.f, wk);
+      chunk_sums<T>(dk, xk, WIDE ? wk : w + (WIDE ? 0 : k * P), mean, s1, s2);
+    };
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (at[k].some(N)) take(k, d + (WIDE ? 0 : k * P), x + (WIDE ? 0 : k * P));
+    const float2 tot = WIDE ? block_sum2(make_float2(s1.x + s1.y, s2.x + s2.y), slots2, i & 1)
+                            : block_pair(s1.x + s1.y, s2.x + s2.y, slots, i & 1);
+    if (s_abort) break;
+    if (threadIdx.x == 0 && ring.S > 1) ring.issue(i + ring.S - 1);
+    const RowTerms terms(rstd, tot.x, tot.y, invN);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!at[k].some(N)) continue;
+      if (WIDE) take(k, d, x);
+      float2 o[P];
+      if (RES) unpack<T>(ring.chunk(i, INPUTS - 1, threadIdx.x + k * blockDim.x), o);
+      const int j = WIDE ? 0 : k * P;
+      chunk_grad<T, RES>(d + j, x + j, WIDE ? wk : w + j, terms, o, dw + k * P, db + k * P);
+      store_chunk<T, MODE>(p.dx + row * p.N, at[k], N, o);
+    }
+    if (ring.S == 1) {
+      __syncthreads();
+      if (threadIdx.x == 0) ring.issue(i + 1);
+    }
+  }
+  if (threadIdx.x == 0 && s_abort) ring.drain(i);
+  if (!p.want_dw && !p.want_db) return;
+  float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * N;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (p.want_dw) store_sums<T, MODE>(to, at[k], N, dw + k * P);
+    if (p.want_db) store_sums<T, MODE>(to + (p.want_dw ? N : 0), at[k], N, db + k * P);
+  }
+}
+
+template <class T, Mode MODE, bool RES>
+__global__ void __maxnreg__(112) bwd_ring(const BwdP<T> p, const Rows rows, const RingShape shape, int* err) {
+  bwd_ring_body<T, MODE, RES, false>(p, rows, shape, err);
+}
+template <class T, Mode MODE, bool RES>
+__global__ void __launch_bounds__(1024) bwd_ring_wide(const BwdP<T> p, const Rows rows, const RingShape shape, int* err) {
+  bwd_ring_body<T, MODE, RES, true>(p, rows, shape, err);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) bwd_any_dx(const BwdP<T> p) {
+  __shared__ float2 slots[2][32];
+  const int64_t row = blockIdx.x;
+  const T* dy = p.dy + row * p.ys;
+  const T* x = p.x + row * p.xs;
+  const float mean = p.mean[row], r = p.rstd[row];
+  float2 s = make_float2(0.f, 0.f);
+  for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
+    const float g = get(dy + n) * vector_at(p.w, n, 1.f);
+    s.x += g;
+    s.y = fmaf((get(x + n) - mean) * r, g, s.y);
+  }
+  s = block_sum2(s, slots, 0);
+  const float invN = 1.0f / static_cast<float>(p.N);
+  const float mg = s.x * invN, mx = s.y * invN;
+  for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
+    const float g = get(dy + n) * vector_at(p.w, n, 1.f), xhat = (get(x + n) - mean) * r;
+    const float d = (g - mg - xhat * mx) * r;
+    put(p.dx + row * p.N + n, p.dres ? get(p.dres + row * p.rs + n) + d : d);
+  }
+}
+
+// Columns of a block of rows, a thread each.
+template <class T>
+__global__ void __launch_bounds__(256) bwd_any_columns(const BwdP<T> p, int64_t M, int64_t R) {
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (n >= p.N) return;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * R, r1 = min(M, r0 + R);
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = r0; row < r1; ++row) {
+    const float g = get(p.dy + row * p.ys + n);
+    dw = fmaf(g, (get(p.x + row * p.xs + n) - p.mean[row]) * p.rstd[row], dw);
+    db += g;
+  }
+  float* to = p.partials + static_cast<int64_t>(blockIdx.y) * (p.want_dw + p.want_db) * p.N;
+  if (p.want_dw) to[n] = dw;
+  if (p.want_db) to[(p.want_dw ? p.N : 0) + n] = db;
+}
+
+// The G rows of [G, columns] partials added in a fixed order: 32 columns a
+// block, warp w adds the rows w, w + 32, ..., then the warps' sums in order.  The
+// first N columns go to `first`, the others to `second`.
+__global__ void __launch_bounds__(1024) add_partials(const float* __restrict__ partials, int64_t G, int64_t columns,
+                                                      int64_t N, float* first, float* second) {
+  __shared__ float red[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float a = 0.f;
+  if (col < columns) {
+    for (int64_t g0 = warp; g0 < G; g0 += 32 * 16) {
+      float v[16];  // one round trip for up to 512 rows
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = g0 + 32 * j < G ? partials[(g0 + 32 * j) * columns + col] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) a += v[j];
+    }
+  }
+  red[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && col < columns) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) s += red[w][lane];
+    if (col < N) first[col] = s;
+    else second[col - N] = s;
+  }
+}
+
+int launch_add_partials(const float* partials, int64_t G, int64_t N, float* dw, float* db, cudaStream_t s) {
+  const int64_t columns = ((dw ? 1 : 0) + (db ? 1 : 0)) * N;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(columns, 32)));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, add_partials, partials, G, columns, N, dw ? dw : db, db));
+}
+
+// Blocks of rows that the columns' sums are split over, at most.
+int64_t row_blocks(int64_t M, int64_t N) {
+  const int sms = sm_count();
+  const int64_t per_sm = std::max(4, N <= kHeld ? ring_blocks(ring_threads(N), 112) : 0);
+  return std::min(M + 8, (sms > 0 ? sms : 148) * per_sm);
+}
+
+template <class T, int V, int L, Mode MODE, bool RES>
+int launch_bwd_lanes(const BwdP<T>& p, const Rows& rows, int64_t* G, cudaStream_t s) {
+  const int per = 256 / L;  // a multiple of 8, as the classes are a divisor of 8
+  const int smem = kAhead * 256 * ((RES ? 3 : 2) * V * static_cast<int>(sizeof(T)) + 8);
+  auto kernel = bwd_lanes<T, V, L, MODE, RES>;
+  if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;
+  const int64_t resident = static_cast<int64_t>(sm_count()) * std::min(lane_blocks(V, MODE, 3), kSmem / (smem + 1024));
+  *G = std::min(ceil_div(rows.M, per), resident);
+  kernel<<<dim3(static_cast<unsigned>(*G)), 256, smem, s>>>(p, rows);
+  return check_launch();
+}
+
+template <class T, Mode MODE, bool RES>
+int launch_bwd(const BwdP<T>& p, Rows rows, int64_t held, int64_t* G, cudaStream_t s) {
+  if (held <= 64) return launch_bwd_lanes<T, 8, 8, EDGE, RES>(p, rows, G, s);
+  if (held <= 128) return launch_bwd_lanes<T, 8, 16, EDGE, RES>(p, rows, G, s);
+  if (held <= 256) return launch_bwd_lanes<T, 8, 32, EDGE, RES>(p, rows, G, s);
+  if (held <= kLanes) return launch_bwd_lanes<T, 16, 32, EDGE, RES>(p, rows, G, s);
+  const int threads = ring_threads(held);
+  auto kernel = threads > 512 ? bwd_ring_wide<T, MODE, RES> : bwd_ring<T, MODE, RES>;
+  RingShape shape;
+  int smem = 0;
+  *G = plan_ring(rows, shape, &smem, RES ? 3 : 2, static_cast<int>(ceil_div(held, kE<T>)) * 16,
+                 ring_blocks(threads, threads > 512 ? 64 : 112));
+  if (!*G) return FRAG_ERR_SHAPE;
+  if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;
+  kernel<<<dim3(static_cast<unsigned>(*G)), threads, smem, s>>>(p, rows, shape, device_error_word());
+  return check_launch();
+}
+
+template <class T>
+int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) {
+  Layout lay(p.N, sizeof(T));
+  lay.add(p.dy, p.ys);
+  lay.add(p.x, p.xs);
+  lay.add(p.dres, p.rs);
+  lay.add(p.dx, p.N);
+  const bool edge = lay.off || lay.residue;
+  const int64_t held = p.N + (edge ? kE<T> - 1 : 0);
+  const Rows rows = {M, lay.off, lay.classes(), 1};
+  int64_t G = 0;
+  int st;
+  if (!lay.alike || held > kHeld) {
+    bwd_any_dx<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
+    if (st = check_launch(); st != FRAG_OK || (!dw && !db)) return st;
+    const int64_t R = ceil_div(M, std::min(M, static_cast<int64_t>(sm_count()) * 4));
+    G = ceil_div(M, R);
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 256)), static_cast<unsigned>(G));
+    bwd_any_columns<T><<<grid, 256, 0, s>>>(p, M, R);
+    st = check_launch();
+  } else {
+    const bool full = p.N == 64 || p.N == 128 || p.N == 256 || p.N % 512 == 0;
+    st = by_mode(edge, full, [&](auto mode) {
+      constexpr Mode MODE = decltype(mode)::value;
+      return p.dres ? launch_bwd<T, MODE, true>(p, rows, held, &G, s) : launch_bwd<T, MODE, false>(p, rows, held, &G, s);
+    });
+  }
+  if (st != FRAG_OK || (!dw && !db)) return st;
+  return launch_add_partials(p.partials, G, p.N, dw, db, s);
+}
+
+}  // namespace
+}  // namespace frag
+
+using namespace frag;
+
+extern "C" {
+
+size_t frag_layernorm_bwd_workspace_bytes(int64_t M, int64_t N) {
+  if (M <= 0 || N <= 0) return 0;
+  return align_up(static_cast<size_t>(row_blocks(M, N)) * 2 * N * sizeof(float), 256);
+}
+
+int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
+                       const float* rstd, const void* w, const void* dres, int64_t dres_stride, void* dx, float* dw,
+                       float* db, int64_t M, int64_t N, int dtype, int wdtype, void* workspace,
+                       size_t workspace_bytes, frag_stream_t stream) {
+  if (M < 0 || N < 0 || !known(dtype) || !known(wdtype)) return FRAG_ERR_INVALID_ARG;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    cudaError_t e = cudaSuccess;
+    if (dw && N) e = cudaMemsetAsync(dw, 0, N * sizeof(float), s);
+    if (db && N && e == cudaSuccess) e = cudaMemsetAsync(db, 0, N * sizeof(float), s);
+    return cuda_status(e);
+  }
+  if (N == 0 || M > 0x7fffffffLL || N > (1LL << 31)) return FRAG_ERR_SHAPE;
+  if (!dy || !x || !mean || !rstd || !dx) return FRAG_ERR_INVALID_ARG;
+  if (!whole(dy, dtype) || !whole(x, dtype) || !whole(dres, dtype) || !whole(dx, dtype) || !whole(w, wdtype))
+    return FRAG_ERR_ALIGN;
+  if (dw || db) {
+    if (!workspace || workspace_bytes < frag_layernorm_bwd_workspace_bytes(M, N)) return FRAG_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
+  }
+  const Vector wv = {w, wdtype == FRAG_DT_F32, aligned16(w)};
+  float* ws = static_cast<float*>(workspace);
+  if (dtype == FRAG_DT_F32)
+    return backward<float>({static_cast<const float*>(dy), static_cast<const float*>(x),
+                            static_cast<const float*>(dres), static_cast<float*>(dx), wv, mean, rstd, ws, dy_stride,
+                            x_stride, dres_stride, N, dw != nullptr, db != nullptr},
+                           M, dw, db, s);
+  return backward<uint16_t>({static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(x),
+                             static_cast<const uint16_t*>(dres), static_cast<uint16_t*>(dx), wv, mean, rstd, ws,
+                             dy_stride, x_stride, dres_stride, N, dw != nullptr, db != nullptr},
+                            M, dw, db, s);
+}
+
+}  // extern "C"
