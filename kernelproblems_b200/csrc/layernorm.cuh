@@ -42,10 +42,6 @@ __device__ __forceinline__ float vector_at(const Vector& v, int64_t n, float non
   return v.f32 ? static_cast<const float*>(v.p)[n] : bf16_to_f(static_cast<const uint16_t*>(v.p)[n]);
 }
 
-#ifndef FWD_V
-#define FWD_V 32
-#define FWD_REGS 128
-#endif
 // ------------------------------------------------------- rows in 16-byte chunks
 //
 // A row is cut at the 16-byte boundaries of memory into chunks of E values.  Its
@@ -121,7 +117,7 @@ __device__ __forceinline__ void own_values(const Place<T, MODE>& at, int N, floa
 template <class T, Mode MODE>
 __device__ __forceinline__ void store_chunk(T* row, const Place<T, MODE>& at, int N, float2* f) {
   if (at.all(N)) {
-    st_global(row + at.n0, pack<T>(f));
+    st_stream(row + at.n0, pack<T>(f));
   } else if (MODE == EDGE && at.some(N)) {
 #pragma unroll
     for (int i = 0; i < kE<T>; ++i)
@@ -150,16 +146,20 @@ __device__ __forceinline__ void load_vector(const Vector& v, const Place<T, MODE
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kE<T>; ++i)
-    part(f[i / 2], i & 1) = at.some(N) && at.has(i, N) ? vector_at(v, at.n0 + i, none) : 0.f;
+  for (int i = 0; i < kE<T>; ++i) {
+    const bool in = at.some(N) && at.has(i, N);
+    const int n = in ? at.n0 + i : 0;
+    float x = none;
+    if (v.p) x = v.f32 ? __ldg(static_cast<const float*>(v.p) + n) : bf16_to_f(__ldg(static_cast<const uint16_t*>(v.p) + n));
+    part(f[i / 2], i & 1) = in ? x : 0.f;
+  }
 }
 
 // How a launch's rows are dealt out.
 struct Rows {
   int64_t M;
-  int off;       // of row 0
-  int classes;   // P
-  int64_t each;  // rows of a class that a block takes
+  int off;      // of row 0
+  int classes;  // P
 };
 
 // One of a call's inputs: rows of N values, `stride` apart.
@@ -214,103 +214,174 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// ------------------------------------------- a block's ring: a row a stage
+// ------------------------------------------- wider rows: groups of a block's warps
 
-// Thread 0 streams the windows (a row's chunks, whole) of a block's rows of up
-// to three inputs into a ring of S stages by bulk copies, one mbarrier a stage.
+// A block fills an SM.  Its threads make groups, each with rows of its own: 32
+// values a thread, a named barrier, and a ring of S stages that the group's first
+// thread streams its next rows' windows (their chunks, whole) of up to three
+// inputs into by bulk copies.  All rows of a block are of one class, so the groups
+// share the weights at their columns in shared memory.  Groups that
+// wait for nothing but their own rows fill one another's latencies, and the
+// gradient's sums over rows leave an SM as one row of partials.
+//
 // A window reaches up to 15 bytes past its row on either side.  Where that is not
 // the tensor's own memory (before its first value, behind its last) the chunk is
-// left out of the copy and its own values are written by thread 0.
-struct RingShape {
-  int stages, slot;  // bytes of a row's window
+// left out of the copy and its own values are written by the first thread.
+constexpr int kV = 32;
+struct Shape {
+  int groups, threads;  // of a block, of a group
+  int stages, slot;     // bytes of a row's window
+};
+
+// A group's threads, and a barrier of theirs.
+struct Group {
+  int index, t, threads;
+  __device__ __forceinline__ explicit Group(int n) : threads(n) {
+    index = threadIdx.x / n;
+    t = threadIdx.x - index * n;
+  }
+  __device__ __forceinline__ void sync() const {
+    if (threads == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(threads) : "memory");
+  }
 };
 
 template <class T, int INPUTS, Mode MODE>
 struct Ring {
   unsigned char* smem;
   uint64_t* bars;
-  int S, slot, count, off, N, issued;
+  int S, slot, count, off, N;
   int64_t r0, step, M;
   Input<T> in[INPUTS];
+  int cur, phase;    // the row that every thread is at: its stage, the barrier's parity
+  int issued, into;  // thread 0: rows asked for, the next one's stage
+  uint32_t bytes;    // of a row's windows
 
-  __device__ __forceinline__ unsigned char* stage(int i) const {
-    return smem + static_cast<size_t>(i % S) * (INPUTS * slot);
+  __device__ __forceinline__ unsigned char* stage(int s) const { return smem + s * (INPUTS * slot); }
+  // Chunk c of the current row.
+  __device__ __forceinline__ uint4 chunk(int input, int c) const {
+    return *reinterpret_cast<const uint4*>(stage(cur) + input * slot + c * 16);
   }
-  __device__ __forceinline__ uint4 chunk(int i, int input, int c) const {
-    return *reinterpret_cast<const uint4*>(stage(i) + input * slot + c * 16);
-  }
-  __device__ __forceinline__ int64_t row(int i) const { return r0 + i * step; }
 
   __device__ __forceinline__ void begin() {  // thread 0
     for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
     mbar_init_fence();
   }
 
-  // Row i into its stage (thread 0).
-  __device__ __forceinline__ void issue(int i) {
-    if (i >= count) return;
-    uint64_t* bar = &bars[i % S];
-    unsigned char* to = stage(i);
-    const int64_t r = row(i);
-    if (MODE != EDGE) {
-      mbar_arrive_expect_tx(bar, INPUTS * slot);
+  // The next row into the next stage (thread 0).
+  __device__ __forceinline__ void issue() {
+    if (issued >= count) return;
+    uint64_t* bar = &bars[into];
+    unsigned char* to = stage(into);
+    const int64_t r = r0 + issued * step;
+    // (rows a whole chunk or more apart: only the first and the last row's windows
+    // can reach out of a tensor)
+    bool inner = true;
+    if (MODE == EDGE) {
+      inner = r > 0 && r < M - 1;
 #pragma unroll
-      for (int k = 0; k < INPUTS; ++k) bulk_g2s(to + k * slot, in[k].p + r * in[k].stride, slot, bar);
-    } else {
-      constexpr int E = kE<T>;
-      const int chunks = (off + N + E - 1) / E, over = chunks * E - off - N;
-      uint32_t bytes = 0;
-#pragma unroll
-      for (int k = 0; k < INPUTS; ++k) bytes += 16 * (chunks - ends(k, r, over, false) - ends(k, r, over, true));
-      // (a thread's own writes come before its arrival, the bytes are expected
-      // before any can come in)
-      asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                   : "memory");
-#pragma unroll
-      for (int k = 0; k < INPUTS; ++k) {
-        const int first = ends(k, r, over, false), last = chunks - ends(k, r, over, true);
-        const T* from = in[k].p + r * in[k].stride - off;  // the window's begin
-        T* own = reinterpret_cast<T*>(to + k * slot);
-        if (first)
-          for (int n = off; n < E; ++n) own[n] = from[n];
-        if (last < chunks)
-          for (int n = last * E; n < off + N; ++n) own[n] = from[n];
-        bulk_g2s(to + k * slot + first * 16, from + first * E, (last - first) * 16, bar);
-      }
-      mbar_arrive(bar);
+      for (int k = 0; k < INPUTS; ++k) inner = inner && in[k].stride >= kE<T>;
     }
-    issued = i + 1;
+    if (inner) {
+      mbar_arrive_expect_tx(bar, INPUTS * bytes);
+#pragma unroll
+      for (int k = 0; k < INPUTS; ++k)
+        bulk_g2s_hint(to + k * slot, in[k].p + r * in[k].stride - off, bytes, bar, l2_policy_evict_first());
+    } else {
+      issue_parts(*this, bar, to, r);
+    }
+    ++issued;
+    into = into + 1 == S ? 0 : into + 1;
   }
-  // Whether the window's first (or last) chunk is left out of the copy.
-  __device__ __forceinline__ int ends(int k, int64_t r, int over, bool last) const {
-    return last ? (M - 1 - r) * in[k].stride < over : r * in[k].stride < off;
+  // (by value: the members of the ring that the rows go by stay in registers)
+  static __device__ __noinline__ void issue_parts(const Ring ring, uint64_t* bar, unsigned char* to, int64_t r) {
+    constexpr int E = kE<T>;
+    const int chunks = static_cast<int>(ring.bytes / 16), over = chunks * E - ring.off - ring.N;
+    uint32_t expect = 0;
+    for (int k = 0; k < INPUTS; ++k) expect += 16 * (chunks - ring.before(k, r) - ring.behind(k, r, over));
+    // (a thread's own writes come before its arrival, the bytes are expected
+    // before any can come in)
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(expect)
+                 : "memory");
+    for (int k = 0; k < INPUTS; ++k) {
+      const int first = ring.before(k, r), last = chunks - ring.behind(k, r, over);
+      const T* from = ring.in[k].p + r * ring.in[k].stride - ring.off;  // the window's begin
+      T* own = reinterpret_cast<T*>(to + k * ring.slot);
+      if (first)
+        for (int n = ring.off; n < E; ++n) own[n] = from[n];
+      if (last < chunks)
+        for (int n = last * E; n < ring.off + ring.N; ++n) own[n] = from[n];
+      bulk_g2s(to + k * ring.slot + first * 16, from + first * E, (last - first) * 16, bar);
+    }
+    mbar_arrive(bar);
   }
+  // Whether the window's first, or last, chunk is left out of the copy.
+  __device__ __forceinline__ int before(int k, int64_t r) const { return r * in[k].stride < off; }
+  __device__ __forceinline__ int behind(int k, int64_t r, int over) const { return (M - 1 - r) * in[k].stride < over; }
 
-  // Waits for row i (every thread).
-  __device__ __forceinline__ bool wait(int i, int* err) { return mbar_wait(&bars[i % S], (i / S) & 1, err); }
-  // Waits for what is in flight from row i on (thread 0, after a wait ran out).
+  // Waits for the current row (every thread).
+  __device__ __forceinline__ bool wait(int* err) { return mbar_wait(&bars[cur], phase, err); }
+  __device__ __forceinline__ void next() {
+    if (++cur == S) {
+      cur = 0;
+      phase ^= 1;
+    }
+  }
+  // Waits for what is in flight from row i, the current one, on (thread 0, after a
+  // wait ran out).
   __device__ __forceinline__ void drain(int i) {
-    for (; i < issued; ++i) mbar_wait(&bars[i % S], (i / S) & 1, nullptr);
+    for (; i < issued; ++i, next()) mbar_wait(&bars[cur], phase, nullptr);
   }
 };
 
-// A block's share of the rows: `each` of one class.
+// A group's share of the rows: every n-th of the class, so that what the groups
+// are at lies together in memory.
 template <class T, int INPUTS, Mode MODE>
-__device__ __forceinline__ void deal(Ring<T, INPUTS, MODE>& ring, const Rows& rows, const RingShape& shape,
+__device__ __forceinline__ void deal(Ring<T, INPUTS, MODE>& ring, const Rows& rows, const Shape& shape, int group,
                                      unsigned char* smem, int N) {
-  const int cls = MODE == EDGE ? blockIdx.x % rows.classes : 0;
-  ring.smem = smem;
+  const int P = MODE == EDGE ? rows.classes : 1, cls = MODE == EDGE ? blockIdx.x % P : 0;
+  const int stage = INPUTS * shape.slot;
   ring.S = shape.stages;
   ring.slot = shape.slot;
-  ring.bars = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(shape.stages) * (INPUTS * shape.slot));
+  ring.smem = smem + group * (shape.stages * stage);
+  ring.bars = reinterpret_cast<uint64_t*>(smem + shape.groups * (shape.stages * stage)) + group * shape.stages;
   ring.off = MODE == EDGE ? static_cast<int>((rows.off + static_cast<int64_t>(cls) * N) % kE<T>) : 0;
   ring.N = N;
   ring.M = rows.M;
-  ring.step = rows.classes;
-  ring.r0 = blockIdx.x / rows.classes * rows.each * rows.classes + cls;
-  ring.count = ring.r0 < rows.M
-                   ? static_cast<int>(min(rows.each, (rows.M - ring.r0 + rows.classes - 1) / rows.classes)) : 0;
-  ring.issued = 0;
+  ring.step = static_cast<int64_t>(gridDim.x) * shape.groups;  // (the grid is a multiple of P)
+  ring.r0 = cls + static_cast<int64_t>(P) * (group * (gridDim.x / P) + blockIdx.x / P);
+  ring.count = ring.r0 < rows.M ? static_cast<int>((rows.M - ring.r0 + ring.step - 1) / ring.step) : 0;
+  ring.bytes = (ring.off + N + kE<T> - 1) / kE<T> * 16;
+  ring.cur = ring.phase = ring.issued = ring.into = 0;
+}
+
+// A vector at the block's columns, `count` of them, into shared memory; 0 outside
+// the row.  W: as fp32, or as bf16 where it is (half the space and accesses, for a
+// conversion each time); fp32 values of an 8-value chunk lie in two planes, so that
+// neighbouring threads read neighbouring 16 bytes.
+template <class T, class W, Mode MODE>
+__device__ __forceinline__ void share_vector(const Vector& v, float none, W* to, int count, int off, int N) {
+  for (int c = threadIdx.x; c < count / kE<T>; c += blockDim.x) {
+    float2 f[kP<T>];
+    load_vector<T, MODE == FULL ? PART : MODE>(v, {c, off}, N, none, f);
+    uint4* at = reinterpret_cast<uint4*>(to) + c;
+    if constexpr (sizeof(W) == 2) {
+      *at = pack<T>(f);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kP<T>; q += 2) at[q / 2 * (count / kE<T>)] = pack<float>(f + q);
+    }
+  }
+}
+template <class T, class W>
+__device__ __forceinline__ void shared_chunk(const W* vector, int count, int c, float2* f) {
+  const uint4* at = reinterpret_cast<const uint4*>(vector) + c;
+  if constexpr (sizeof(W) == 2) {
+    unpack<T>(*at, f);
+  } else {
+#pragma unroll
+    for (int q = 0; q < kP<T>; q += 2) unpack<float>(at[q / 2 * (count / kE<T>)], f + q);
+  }
 }
 
 // Rows that a thread's own ring holds.
@@ -322,25 +393,29 @@ constexpr int lane_blocks(int V, Mode mode, int most) { return most - (V == 8 &&
 constexpr int64_t kLanes = 512, kHeld = 16384;
 constexpr int kSmem = 232448;  // of an SM, for its blocks
 
-int ring_threads(int64_t held) { return static_cast<int>(ceil_div(held, 512) * 32); }
-// Blocks of a ring kernel that an SM's registers hold.
-int ring_blocks(int threads, int registers) { return std::max(1, std::min(12, 65536 / (registers * threads))); }
+int group_threads(int64_t held) { return static_cast<int>(ceil_div(held, 32 * kV) * 32); }
 
-// The ring of a launch and its blocks: as many an SM as leave each two stages, and
-// then as many stages as fit.  Returns the blocks, 0 where not one stage fits.
-int64_t plan_ring(Rows& rows, RingShape& shape, int* smem, int inputs, int slot, int per_sm) {
-  const int stage = slot * inputs;
-  shape.slot = slot;
-  for (;; --per_sm) {
-    shape.stages = std::min(8, (kSmem / per_sm - 2048) / stage);  // (1 KB is the system's, 1 the rest of the block's)
-    if (shape.stages >= 2 || per_sm == 1) break;
+// The groups of a launch's blocks, at most `most` threads: as many as leave each
+// `least` stages, and then as many stages as fit beside `vectors` shared ones.
+// Returns the blocks, 0 where not one stage fits.
+int64_t plan_groups(const Rows& rows, int64_t held, int size, int inputs, int vectors, int vector_size, int most,
+                    int least, Shape& shape, int* smem) {
+  const int E = 16 / size;
+  shape.threads = group_threads(held);
+  shape.slot = static_cast<int>(ceil_div(held, E)) * 16;
+  const int shared = vectors * shape.threads * kV * vector_size, stage = shape.slot * inputs;
+  const int64_t sms = sm_count() / rows.classes * rows.classes;
+  // (15 named barriers; rows fewer than groups leave some without)
+  int groups = std::min(most / shape.threads, shape.threads == 32 ? 32 : 15);
+  groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, ceil_div(rows.M, sms))));
+  for (;; --groups) {
+    shape.stages = std::min(8, (kSmem - 2048 - shared) / (stage * groups));
+    if (shape.stages >= least || groups == 1) break;
   }
   if (shape.stages < 1) return 0;
-  *smem = shape.stages * stage + 8 * shape.stages;
-  const int64_t of_class = ceil_div(rows.M, rows.classes);
-  const int64_t resident = std::max(1, sm_count() * per_sm / rows.classes);
-  rows.each = ceil_div(of_class, std::min(of_class, resident));
-  return ceil_div(of_class, rows.each) * rows.classes;
+  shape.groups = groups;
+  *smem = shared + groups * shape.stages * (stage + 8);
+  return std::min(ceil_div(rows.M, rows.classes) * rows.classes, sms);
 }
 
 // Whether rows of all of a call's tensors lie alike (the same off, row for row),
@@ -368,6 +443,15 @@ struct Layout {
  private:
   int size_;
 };
+
+// The type that a call's weights are kept in, as a constant: bf16 only beside bf16
+// rows (of all ones, where there are none).
+template <class T, class F>
+int by_weight(const Vector& w, const Vector& b, F&& f) {
+  if constexpr (sizeof(T) == 2)
+    if (!(w.p && w.f32) && !(b.p && b.f32)) return f(uint16_t{});
+  return f(float{});
+}
 
 // The templates' mode, as a constant.
 template <class F>

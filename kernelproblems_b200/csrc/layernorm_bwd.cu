@@ -162,116 +162,144 @@ __device__ __forceinline__ void store_sums(float* row, const Place<T, MODE>& at,
   }
 }
 
-// Two sums over a block of up to 512 threads, in a fixed order, for every thread.
+// Two sums over a group of up to 16 warps, in a fixed order, for every thread.
 // After one exchange the lower half of a warp's lanes add the first and the upper
-// half the second, so that both take one shuffle a level.
-__device__ __forceinline__ float2 block_pair(float a, float b, float (*slots)[32], int parity) {
-  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  const bool upper = lane & 16;
+// half the second, so that both take one shuffle a level.  slots: [2][16][2],
+// the group's at `first`.
+__device__ __forceinline__ float2 group_pair(const Group& g, float a, float b, float (*slots)[2], int first) {
+  const int lane = threadIdx.x & 31, nw = g.threads >> 5;
+  const int upper = lane >> 4;
   float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((lane & 15) == 0) slots[parity][(threadIdx.x >> 5) + (upper ? 16 : 0)] = v;
-  __syncthreads();
-  v = (lane & 15) < nw ? slots[parity][lane] : 0.f;
+  if ((lane & 15) == 0) slots[first + (g.t >> 5)][upper] = v;
+  g.sync();
+  if (nw > 1) {
+    v = (lane & 15) < nw ? slots[first + (lane & 15)][upper] : 0.f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
 }
 
-// Wider rows: a block stays for `each` rows of a class, 16 values a thread, the
-// next rows in the ring.  A thread keeps the weights at its columns, their two
-// sums, and a row's dy and x - mean from the first pass to the second, at most 112
-// registers: two blocks of 256 threads an SM, whose barriers overlap.  WIDE (more
-// than 512 threads a block): 64 registers, the row is read from its stage twice
-// and the weights come from L1.
-template <class T, Mode MODE, bool RES, bool WIDE>
-__device__ __forceinline__ void bwd_ring_body(const BwdP<T>& p, const Rows& rows, const RingShape& shape, int* err) {
-  constexpr int P = kP<T>, V = 16, K = V / kE<T>, INPUTS = RES ? 3 : 2;
+// Wider rows, a group a row at a time.  A thread keeps its columns' two sums (64
+// registers); a row is read from its stage twice, for its sums and for its results.
+template <class T, class W, Mode MODE, bool RES>
+__global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows rows, const Shape shape, int* err) {
+  constexpr int E = kE<T>, P = kP<T>, V = kV, K = V / E, INPUTS = RES ? 3 : 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float2 slots2[WIDE ? 2 : 1][32];
-  __shared__ float slots[2][32];
-  __shared__ int s_abort;
+  extern __shared__ __align__(128) unsigned char smem[];  // w, the rings; at the end dw, db
+  __shared__ float slots[2][16][2];
+  __shared__ int s_abort[16];
   const int N = static_cast<int>(p.N);
+  const Group g(shape.threads);
+  const int apart = shape.threads * V;
+  W* w = reinterpret_cast<W*>(smem);
   Ring<T, INPUTS, MODE> ring;
   ring.in[0] = {p.dy, p.ys};
   ring.in[1] = {p.x, p.xs};
   if (RES) ring.in[INPUTS - 1] = {p.dres, p.rs};
-  deal(ring, rows, shape, smem, N);
-  const Places<T, MODE> at = {static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), ring.off};
-  if (threadIdx.x == 0) {
-    s_abort = 0;
+  deal(ring, rows, shape, g.index, smem + sizeof(W) * apart, N);
+  const Places<T, MODE> at = {g.t, g.threads, ring.off};
+  if (g.t == 0) {
+    s_abort[g.index] = 0;
     ring.begin();
+    // A stage is free again when every thread is in the next row: S - 1 rows ahead.
+    for (int i = 0; i < max(1, ring.S - 1); ++i) ring.issue();
   }
-  __syncthreads();
-  // A stage is free again when every thread is in the next row: S - 1 rows ahead.
-  if (threadIdx.x == 0)
-    for (int i = 0; i < max(1, ring.S - 1); ++i) ring.issue(i);
-  float2 w[WIDE ? 1 : V / 2], dw[V / 2], db[V / 2];
-  if constexpr (!WIDE) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
-  }
+  share_vector<T, W, MODE>(p.w, 1.f, w, apart, ring.off, N);
+  float2 dw[V / 2], db[V / 2];
 #pragma unroll
   for (int q = 0; q < V / 2; ++q) dw[q] = db[q] = twice(0.f);
+  int64_t row = ring.r0;
+  float mean = 0.f, rstd = 0.f;
+  if (ring.count) {
+    mean = __ldg(p.mean + row);
+    rstd = __ldg(p.rstd + row);
+  }
+  __syncthreads();
   const float invN = 1.0f / static_cast<float>(N);
+  const int first = g.index * (g.threads >> 5);
   int i = 0;
-  for (; i < ring.count; ++i) {
-    const int64_t row = ring.row(i);
-    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
-    if (!ring.wait(i, err)) s_abort = 1;
-    float2 d[WIDE ? P : V / 2], x[WIDE ? P : V / 2], wk[P], s1 = twice(0.f), s2 = s1;
-    // A chunk's dy, x - mean and weights, and its part of the sums.
-    auto take = [&](int k, float2* dk, float2* xk) {
-      const int c = threadIdx.x + k * blockDim.x;
-      unpack<T>(ring.chunk(i, 0, c), dk);
-      unpack<T>(ring.chunk(i, 1, c), xk);
-      own_values<T, MODE>(at[k], N, 0.f, dk);
-      own_values<T, MODE>(at[k], N, mean, xk);
-      if constexpr (WIDE) load_vector<T, MODE>(p.w, at[k], N, 1.f, wk);
-      chunk_sums<T>(dk, xk, WIDE ? wk : w + (WIDE ? 0 : k * P), mean, s1, s2);
+  for (; i < ring.count; ++i, row += ring.step) {
+    if (!ring.wait(err)) s_abort[g.index] = 1;
+    // A chunk's dy, x and weights.
+    auto take = [&](int k, float2* d, float2* x, float2* wk) {
+      const int c = g.t + k * g.threads;
+      unpack<T>(ring.chunk(0, c), d);
+      unpack<T>(ring.chunk(1, c), x);
+      own_values<T, MODE>(at[k], N, 0.f, d);
+      own_values<T, MODE>(at[k], N, mean, x);
+      shared_chunk<T, W>(w, apart, c, wk);
     };
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (at[k].some(N)) take(k, d + (WIDE ? 0 : k * P), x + (WIDE ? 0 : k * P));
-    const float2 tot = WIDE ? block_sum2(make_float2(s1.x + s1.y, s2.x + s2.y), slots2, i & 1)
-                            : block_pair(s1.x + s1.y, s2.x + s2.y, slots, i & 1);
-    if (s_abort) break;
-    if (threadIdx.x == 0 && ring.S > 1) ring.issue(i + ring.S - 1);
-    const RowTerms terms(rstd, tot.x, tot.y, invN);
+    float2 s1 = twice(0.f), s2 = s1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!at[k].some(N)) continue;
-      if (WIDE) take(k, d, x);
-      float2 o[P];
-      if (RES) unpack<T>(ring.chunk(i, INPUTS - 1, threadIdx.x + k * blockDim.x), o);
-      const int j = WIDE ? 0 : k * P;
-      chunk_grad<T, RES>(d + j, x + j, WIDE ? wk : w + j, terms, o, dw + k * P, db + k * P);
+      float2 d[P], x[P], wk[P];
+      take(k, d, x, wk);
+      chunk_sums<T>(d, x, wk, mean, s1, s2);
+    }
+    const float2 tot = group_pair(g, s1.x + s1.y, s2.x + s2.y, slots[i & 1], first);
+    if (s_abort[g.index]) break;
+    if (g.t == 0 && ring.S > 1) ring.issue();
+    const RowTerms terms(rstd, tot.x, tot.y, invN);
+    float next_mean = 0.f, next_rstd = 0.f;
+    if (i + 1 < ring.count) {
+      next_mean = __ldg(p.mean + row + ring.step);
+      next_rstd = __ldg(p.rstd + row + ring.step);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!at[k].some(N)) continue;
+      float2 d[P], x[P], wk[P], o[P];
+      take(k, d, x, wk);
+#pragma unroll
+      for (int q = 0; q < P; ++q) x[q] = __fadd2_rn(x[q], twice(-mean));
+      if (RES) unpack<T>(ring.chunk(INPUTS - 1, g.t + k * g.threads), o);
+      chunk_grad<T, RES>(d, x, wk, terms, o, dw + k * P, db + k * P);
       store_chunk<T, MODE>(p.dx + row * p.N, at[k], N, o);
     }
+    mean = next_mean;
+    rstd = next_rstd;
     if (ring.S == 1) {
-      __syncthreads();
-      if (threadIdx.x == 0) ring.issue(i + 1);
+      g.sync();
+      if (g.t == 0) ring.issue();
     }
+    ring.next();
   }
-  if (threadIdx.x == 0 && s_abort) ring.drain(i);
+  if (g.t == 0 && s_abort[g.index]) ring.drain(i);
   if (!p.want_dw && !p.want_db) return;
   float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * N;
+  if (shape.groups == 1) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (p.want_dw) store_sums<T, MODE>(to, at[k], N, dw + k * P);
-    if (p.want_db) store_sums<T, MODE>(to + (p.want_dw ? N : 0), at[k], N, db + k * P);
+    for (int k = 0; k < K; ++k) {
+      if (p.want_dw) store_sums<T, MODE>(to, at[k], N, dw + k * P);
+      if (p.want_db) store_sums<T, MODE>(to + (p.want_dw ? N : 0), at[k], N, db + k * P);
+    }
+    return;
   }
-}
-
-template <class T, Mode MODE, bool RES>
-__global__ void __maxnreg__(112) bwd_ring(const BwdP<T> p, const Rows rows, const RingShape shape, int* err) {
-  bwd_ring_body<T, MODE, RES, false>(p, rows, shape, err);
-}
-template <class T, Mode MODE, bool RES>
-__global__ void __launch_bounds__(1024) bwd_ring_wide(const BwdP<T> p, const Rows rows, const RingShape shape, int* err) {
-  bwd_ring_body<T, MODE, RES, true>(p, rows, shape, err);
+  // All groups' sums into shared memory, a column's added in the groups' order.
+  __syncthreads();
+  float2* sums = reinterpret_cast<float2*>(smem) + g.index * (V * g.threads) + g.t;
+#pragma unroll
+  for (int q = 0; q < V / 2; ++q) {
+    sums[q * g.threads] = dw[q];
+    sums[(V / 2 + q) * g.threads] = db[q];
+  }
+  __syncthreads();
+  for (int n = threadIdx.x; n < N; n += blockDim.x) {
+    const int at_row = n + ring.off, c = at_row / E, k = c / g.threads;
+    const float* from = reinterpret_cast<const float*>(smem) +
+                        2 * ((k * P + at_row % E / 2) * g.threads + c - k * g.threads) + (at_row & 1);
+    float sw = 0.f, sb = 0.f;
+    for (int q = 0; q < shape.groups; ++q) {
+      sw += from[q * (2 * V * g.threads)];
+      sb += from[q * (2 * V * g.threads) + V * g.threads];
+    }
+    if (p.want_dw) to[n] = sw;
+    if (p.want_db) to[(p.want_dw ? N : 0) + n] = sb;
+  }
 }
 
 template <class T>
@@ -359,10 +387,9 @@ int launch_add_partials(const float* partials, int64_t G, int64_t N, float* dw, 
 }
 
 // Blocks of rows that the columns' sums are split over, at most.
-int64_t row_blocks(int64_t M, int64_t N) {
+int64_t row_blocks(int64_t M) {
   const int sms = sm_count();
-  const int64_t per_sm = std::max(4, N <= kHeld ? ring_blocks(ring_threads(N), 112) : 0);
-  return std::min(M + 8, (sms > 0 ? sms : 148) * per_sm);
+  return std::min<int64_t>(M + 8, (sms > 0 ? sms : 148) * 4);
 }
 
 template <class T, int V, int L, Mode MODE, bool RES>
@@ -377,22 +404,29 @@ int launch_bwd_lanes(const BwdP<T>& p, const Rows& rows, int64_t* G, cudaStream_
   return check_launch();
 }
 
-template <class T, Mode MODE, bool RES>
-int launch_bwd(const BwdP<T>& p, Rows rows, int64_t held, int64_t* G, cudaStream_t s) {
-  if (held <= 64) return launch_bwd_lanes<T, 8, 8, EDGE, RES>(p, rows, G, s);
-  if (held <= 128) return launch_bwd_lanes<T, 8, 16, EDGE, RES>(p, rows, G, s);
-  if (held <= 256) return launch_bwd_lanes<T, 8, 32, EDGE, RES>(p, rows, G, s);
-  if (held <= kLanes) return launch_bwd_lanes<T, 16, 32, EDGE, RES>(p, rows, G, s);
-  const int threads = ring_threads(held);
-  auto kernel = threads > 512 ? bwd_ring_wide<T, MODE, RES> : bwd_ring<T, MODE, RES>;
-  RingShape shape;
+// Returns -1, nothing launched, where a row's stage does not fit in shared memory.
+template <class T, class W, Mode MODE, bool RES>
+int launch_bwd_groups(const BwdP<T>& p, const Rows& rows, int64_t held, int64_t* G, cudaStream_t s) {
+  auto kernel = bwd_groups<T, W, MODE, RES>;
+  Shape shape;
   int smem = 0;
-  *G = plan_ring(rows, shape, &smem, RES ? 3 : 2, static_cast<int>(ceil_div(held, kE<T>)) * 16,
-                 ring_blocks(threads, threads > 512 ? 64 : 112));
-  if (!*G) return FRAG_ERR_SHAPE;
+  *G = plan_groups(rows, held, sizeof(T), RES ? 3 : 2, 1, sizeof(W), 512, 2, shape, &smem);
+  if (!*G) return -1;
+  if (shape.groups > 1) smem = std::max(smem, shape.groups * shape.threads * kV * 8);  // the sums at the end
   if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;
-  kernel<<<dim3(static_cast<unsigned>(*G)), threads, smem, s>>>(p, rows, shape, device_error_word());
+  kernel<<<dim3(static_cast<unsigned>(*G)), shape.groups * shape.threads, smem, s>>>(p, rows, shape,
+                                                                                      device_error_word());
   return check_launch();
+}
+
+template <class T, Mode MODE, bool RES>
+int launch_bwd(const BwdP<T>& p, const Rows& rows, int64_t held, int64_t* G, cudaStream_t s) {
+  constexpr Mode LANES = MODE == FULL ? PART : MODE;
+  if (held <= 64) return launch_bwd_lanes<T, 8, 8, LANES, RES>(p, rows, G, s);
+  if (held <= 128) return launch_bwd_lanes<T, 8, 16, LANES, RES>(p, rows, G, s);
+  if (held <= 256) return launch_bwd_lanes<T, 8, 32, LANES, RES>(p, rows, G, s);
+  if (held <= kLanes) return launch_bwd_lanes<T, 16, 32, LANES, RES>(p, rows, G, s);
+  return by_weight<T>(p.w, {}, [&](auto w) { return launch_bwd_groups<T, decltype(w), MODE, RES>(p, rows, held, G, s); });
 }
 
 template <class T>
@@ -404,10 +438,16 @@ int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) 
   lay.add(p.dx, p.N);
   const bool edge = lay.off || lay.residue;
   const int64_t held = p.N + (edge ? kE<T> - 1 : 0);
-  const Rows rows = {M, lay.off, lay.classes(), 1};
   int64_t G = 0;
-  int st;
-  if (!lay.alike || held > kHeld) {
+  int st = -1;
+  if (lay.alike && held <= kHeld) {
+    const Rows rows = {M, lay.off, lay.classes()};
+    st = by_mode(edge, p.N % (32 * kV) == 0, [&](auto mode) {
+      constexpr Mode MODE = decltype(mode)::value;
+      return p.dres ? launch_bwd<T, MODE, true>(p, rows, held, &G, s) : launch_bwd<T, MODE, false>(p, rows, held, &G, s);
+    });
+  }
+  if (st < 0) {
     bwd_any_dx<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
     if (st = check_launch(); st != FRAG_OK || (!dw && !db)) return st;
     const int64_t R = ceil_div(M, std::min(M, static_cast<int64_t>(sm_count()) * 4));
@@ -415,12 +455,6 @@ int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) 
     const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 256)), static_cast<unsigned>(G));
     bwd_any_columns<T><<<grid, 256, 0, s>>>(p, M, R);
     st = check_launch();
-  } else {
-    const bool full = p.N == 64 || p.N == 128 || p.N == 256 || p.N % 512 == 0;
-    st = by_mode(edge, full, [&](auto mode) {
-      constexpr Mode MODE = decltype(mode)::value;
-      return p.dres ? launch_bwd<T, MODE, true>(p, rows, held, &G, s) : launch_bwd<T, MODE, false>(p, rows, held, &G, s);
-    });
   }
   if (st != FRAG_OK || (!dw && !db)) return st;
   return launch_add_partials(p.partials, G, p.N, dw, db, s);
@@ -435,7 +469,7 @@ extern "C" {
 
 size_t frag_layernorm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
-  return align_up(static_cast<size_t>(row_blocks(M, N)) * 2 * N * sizeof(float), 256);
+  return align_up(static_cast<size_t>(row_blocks(M)) * 2 * N * sizeof(float), 256);
 }
 
 int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,

@@ -37,7 +37,7 @@ __device__ __forceinline__ void input_chunk(const uint4& x, const uint4& res, fl
 // Sum of the squared distances from `mean` of the values inside the row.
 template <class T, int V, Mode MODE>
 __device__ __forceinline__ float row_squares(const Places<T, MODE>& at, int N, const float2 (&v)[V / 2], float mean) {
-  float2 s = twice(0.f);
+  float2 s = twice(0.f), s2 = s;
   const float2 m = twice(-mean);
 #pragma unroll
   for (int k = 0; k < V / kE<T>; ++k) {
@@ -47,8 +47,12 @@ __device__ __forceinline__ float row_squares(const Places<T, MODE>& at, int N, c
     for (int q = 0; q < kP<T>; ++q) d[q] = __fadd2_rn(v[k * kP<T> + q], m);
     own_values<T, MODE>(at[k], N, 0.f, d);
 #pragma unroll
-    for (int q = 0; q < kP<T>; ++q) s = __ffma2_rn(d[q], d[q], s);
+    for (int q = 0; q < kP<T>; q += 2) {
+      s = __ffma2_rn(d[q], d[q], s);
+      s2 = __ffma2_rn(d[q + 1], d[q + 1], s2);
+    }
   }
+  s = __fadd2_rn(s, s2);
   return s.x + s.y;
 }
 
@@ -129,109 +133,111 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
   }
 }
 
-// How many of a row's values each warp holds.
-template <class T, int V>
-__device__ __forceinline__ float warp_holds(int w, int off, int N) {
+// How many of a row's values warp w of a group holds.
+template <class T>
+__device__ __forceinline__ float warp_holds(int w, int threads, int off, int N) {
   int n = 0;
 #pragma unroll
-  for (int k = 0; k < V / kE<T>; ++k) {
-    const int from = (k * static_cast<int>(blockDim.x) + w * 32) * kE<T>;
+  for (int k = 0; k < kV / kE<T>; ++k) {
+    const int from = (k * threads + w * 32) * kE<T>;
     n += max(0, min(from + 32 * kE<T>, off + N) - max(from, off));
   }
   return static_cast<float>(n);
 }
 
-// Wider rows: a block a row at a time, V = 16 values a thread, the next rows in
-// the ring.  A row's mean and 1 / deviation behind one barrier: each warp takes
-// its own mean and squares about it, and the warps' (count, sum, squares) are
-// joined,
+// Threads of a block: 80 registers each.
+constexpr int kMost = 768;
+
+// Wider rows, a group a row at a time.  A row's mean and 1 / deviation behind one
+// barrier: each warp takes its own mean and squares about it, and the warps'
+// (count, sum, squares) are joined,
 //   squares = sum over warps of squares_w + n_w (mean_w - mean)^2
-// where two sums over the block, one after the other, would need two.  The weights
-// stay in registers (at most 80, so that three blocks of 256 threads share an SM);
-// WIDE, with more than 768 threads a block and 64 registers, they come from L1.
-template <class T, int V, Mode MODE, bool RES, bool WIDE>
-__device__ __forceinline__ void fwd_ring_body(const FwdP<T>& p, const Rows& rows, const RingShape& shape, int* err) {
-  constexpr int P = kP<T>, K = V / kE<T>, INPUTS = RES ? 2 : 1;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float2 slots[2][32];
-  __shared__ int s_abort;
-  const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+// where two sums over the group, one after the other, would need two.
+template <class T, class W, Mode MODE, bool RES>
+__global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows rows, const Shape shape, int* err) {
+  constexpr int P = kP<T>, V = kV, K = V / kE<T>, INPUTS = RES ? 2 : 1;
+  extern __shared__ __align__(128) unsigned char smem[];  // w, b, the rings
+  __shared__ float2 slots[2][32], counts[16];             // (sum, squares) and (n, 1 / n) of each warp
+  __shared__ int s_abort[32];
+  const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, nw = shape.threads >> 5;
+  const Group g(shape.threads);
+  const int apart = shape.threads * V, warp = g.t >> 5;
+  W *w = reinterpret_cast<W*>(smem), *b = w + apart;
   Ring<T, INPUTS, MODE> ring;
   ring.in[0] = {p.x, p.xs};
   if (RES) ring.in[INPUTS - 1] = {p.res, p.rs};
-  deal(ring, rows, shape, smem, N);
-  const Places<T, MODE> at = {static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), ring.off};
-  if (threadIdx.x == 0) {
-    s_abort = 0;
+  deal(ring, rows, shape, g.index, smem + 2 * sizeof(W) * apart, N);
+  const Places<T, MODE> at = {g.t, g.threads, ring.off};
+  if (g.t == 0) {
+    s_abort[g.index] = 0;
     ring.begin();
+    for (int i = 0; i < ring.S; ++i) ring.issue();
   }
+  if (static_cast<int>(threadIdx.x) < nw) {
+    const float n = warp_holds<T>(threadIdx.x, g.threads, ring.off, N);
+    counts[threadIdx.x] = make_float2(n, n > 0.f ? 1.0f / n : 0.f);
+  }
+  share_vector<T, W, MODE>(p.w, 1.f, w, apart, ring.off, N);
+  share_vector<T, W, MODE>(p.b, 0.f, b, apart, ring.off, N);
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int i = 0; i < ring.S; ++i) ring.issue(i);
-  float2 w[WIDE ? 1 : V / 2], b[WIDE ? 1 : V / 2];
-  if constexpr (!WIDE) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
-      load_vector<T, MODE>(p.b, at[k], N, 0.f, b + k * P);
-    }
-  }
-  const float invN = 1.0f / static_cast<float>(N);
-  const float mine = warp_holds<T, V>(warp, ring.off, N), of_lane = lane < nw ? warp_holds<T, V>(lane, ring.off, N) : 0.f;
-  const float inv_mine = mine > 0.f ? 1.0f / mine : 0.f, inv_lane = of_lane > 0.f ? 1.0f / of_lane : 0.f;
+  const float invN = 1.0f / static_cast<float>(N), inv_mine = counts[warp].y;
+  const int first = g.index * nw;  // the group's slots
+  int64_t row = ring.r0;
   int i = 0;
-  for (; i < ring.count; ++i) {
-    const int64_t row = ring.row(i);
-    if (!ring.wait(i, err)) s_abort = 1;
-    float2 v[V / 2], sum = twice(0.f);
+  for (; i < ring.count; ++i, row += ring.step) {
+    if (!ring.wait(err)) s_abort[g.index] = 1;
+    float2 v[V / 2], sum = twice(0.f), sum2 = sum;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = threadIdx.x + k * blockDim.x;
+      const int c = g.t + k * g.threads;
       if (!at[k].some(N)) {
 #pragma unroll
         for (int q = 0; q < P; ++q) v[k * P + q] = twice(0.f);
         continue;
       }
       const uint4 none = make_uint4(0, 0, 0, 0);
-      input_chunk<T, RES>(ring.chunk(i, 0, c), RES ? ring.chunk(i, INPUTS - 1, c) : none, v + k * P);
+      input_chunk<T, RES>(ring.chunk(0, c), RES ? ring.chunk(INPUTS - 1, c) : none, v + k * P);
       own_values<T, MODE>(at[k], N, 0.f, v + k * P);
 #pragma unroll
-      for (int q = 0; q < P; ++q) sum = __fadd2_rn(sum, v[k * P + q]);
+      for (int q = 0; q < P; q += 2) {
+        sum = __fadd2_rn(sum, v[k * P + q]);
+        sum2 = __fadd2_rn(sum2, v[k * P + q + 1]);
+      }
       if (RES && p.h) store_chunk<T, MODE>(p.h + row * p.N, at[k], N, v + k * P);
     }
+    sum = __fadd2_rn(sum, sum2);
     const float ws = warp_sum(sum.x + sum.y);
     const float wq = warp_sum(row_squares<T, V, MODE>(at, N, v, ws * inv_mine));
-    if (lane == 0) slots[i & 1][warp] = make_float2(ws, wq);
-    __syncthreads();
-    if (s_abort) break;
-    if (threadIdx.x == 0) ring.issue(i + ring.S);  // every thread has its values of stage i % S
-    const float2 o = lane < nw ? slots[i & 1][lane] : twice(0.f);
-    const float mean = warp_sum(o.x) * invN;
-    const float d = fmaf(o.x, inv_lane, -mean);
-    const float r = rsqrtf(fmaf(warp_sum(fmaf(of_lane * d, d, o.y)), invN, p.eps));
-    if (threadIdx.x == 0) {
+    if (lane == 0) slots[i & 1][first + warp] = make_float2(ws, wq);
+    g.sync();
+    if (s_abort[g.index]) break;
+    if (g.t == 0) ring.issue();  // every thread has its values of this stage
+    float mean = ws * invN, var = wq * invN;
+    if (nw > 1) {  // (16 lanes take a warp each, the upper half the same again)
+      const int of = lane & 15;
+      const float2 o = of < nw ? slots[i & 1][first + of] : twice(0.f), n = of < nw ? counts[of] : twice(0.f);
+      mean = lanes_sum<16>(o.x) * invN;
+      const float d = fmaf(o.x, n.y, -mean);
+      var = lanes_sum<16>(fmaf(n.x * d, d, o.y)) * invN;
+    }
+    const float r = rsqrtf(var + p.eps);
+    if (g.t == 0) {
       if (p.mean) p.mean[row] = mean;
       if (p.rstd) p.rstd[row] = r;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if constexpr (WIDE) {
-        float2 wk[P], bk[P];
-        load_vector<T, MODE>(p.w, at[k], N, 1.f, wk);
-        load_vector<T, MODE>(p.b, at[k], N, 0.f, bk);
-        write_chunk<T, MODE>(p.y + row * p.N, at[k], N, v + k * P, mean, r, wk, bk);
-      } else {
-        write_chunk<T, MODE>(p.y + row * p.N, at[k], N, v + k * P, mean, r, w + k * P, b + k * P);
-      }
+      if (!at[k].some(N)) continue;
+      float2 wk[P], bk[P];
+      shared_chunk<T, W>(w, apart, g.t + k * g.threads, wk);
+      shared_chunk<T, W>(b, apart, g.t + k * g.threads, bk);
+      write_chunk<T, MODE>(p.y + row * p.N, at[k], N, v + k * P, mean, r, wk, bk);
     }
+    ring.next();
   }
-  if (threadIdx.x == 0 && s_abort) ring.drain(i);
+  if (g.t == 0 && s_abort[g.index]) ring.drain(i);
 }
 
-template <class T, Mode MODE, bool RES>
-__global__ void __maxnreg__(FWD_REGS) fwd_ring(const FwdP<T> p, const Rows rows, const RingShape shape, int* err) {
-  fwd_ring_body<T, FWD_V, MODE, RES, false>(p, rows, shape, err);
-}
 // Any width, any alignment: a block a row, the row read once for each pass
 // (the later passes from L2).
 template <class T>
@@ -273,27 +279,28 @@ int launch_fwd_lanes(const FwdP<T>& p, const Rows& rows, cudaStream_t s) {
   return check_launch();
 }
 
-template <class T, int V, Mode MODE, bool RES>
-int launch_fwd_ring(const FwdP<T>& p, Rows rows, int64_t held, cudaStream_t s) {
-  auto kernel = fwd_ring<T, MODE, RES>;
-  const int threads = static_cast<int>(ceil_div(held, 32 * V) * 32);
-  RingShape shape;
+// Returns -1, nothing launched, where a row's stage does not fit in shared memory.
+template <class T, class W, Mode MODE, bool RES>
+int launch_fwd_groups(const FwdP<T>& p, const Rows& rows, int64_t held, cudaStream_t s) {
+  auto kernel = fwd_groups<T, W, MODE, RES>;
+  Shape shape;
   int smem = 0;
-  const int64_t blocks = plan_ring(rows, shape, &smem, RES ? 2 : 1, static_cast<int>(ceil_div(held, kE<T>)) * 16,
-                                   ring_blocks(threads, FWD_REGS));
-  if (!blocks) return FRAG_ERR_SHAPE;
+  const int64_t blocks = plan_groups(rows, held, sizeof(T), RES ? 2 : 1, 2, sizeof(W), kMost, 1, shape, &smem);
+  if (!blocks) return -1;
   if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;
-  kernel<<<dim3(static_cast<unsigned>(blocks)), threads, smem, s>>>(p, rows, shape, device_error_word());
+  kernel<<<dim3(static_cast<unsigned>(blocks)), shape.groups * shape.threads, smem, s>>>(p, rows, shape,
+                                                                                          device_error_word());
   return check_launch();
 }
 
 template <class T, Mode MODE, bool RES>
 int launch_fwd(const FwdP<T>& p, const Rows& rows, int64_t held, cudaStream_t s) {
-  if (held <= 64) return launch_fwd_lanes<T, 8, 8, MODE, RES>(p, rows, s);
-  if (held <= 128) return launch_fwd_lanes<T, 8, 16, MODE, RES>(p, rows, s);
-  if (held <= 256) return launch_fwd_lanes<T, 8, 32, MODE, RES>(p, rows, s);
-  if (held <= kLanes) return launch_fwd_lanes<T, 16, 32, MODE, RES>(p, rows, s);
-  return launch_fwd_ring<T, FWD_V, MODE, RES>(p, rows, held, s);
+  constexpr Mode LANES = MODE == FULL ? PART : MODE;
+  if (held <= 64) return launch_fwd_lanes<T, 8, 8, LANES, RES>(p, rows, s);
+  if (held <= 128) return launch_fwd_lanes<T, 8, 16, LANES, RES>(p, rows, s);
+  if (held <= 256) return launch_fwd_lanes<T, 8, 32, LANES, RES>(p, rows, s);
+  if (held <= kLanes) return launch_fwd_lanes<T, 16, 32, LANES, RES>(p, rows, s);
+  return by_weight<T>(p.w, p.b, [&](auto w) { return launch_fwd_groups<T, decltype(w), MODE, RES>(p, rows, held, s); });
 }
 
 template <class T>
@@ -305,16 +312,16 @@ int forward(const FwdP<T>& p, int64_t M, cudaStream_t s) {
   lay.add(p.h, p.N);
   const bool edge = lay.off || lay.residue;
   const int64_t held = p.N + (edge ? kE<T> - 1 : 0);  // values of a row's chunks, at most
-  if (!lay.alike || held > kHeld) {
-    fwd_any<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
-    return check_launch();
+  if (lay.alike && held <= kHeld) {
+    const Rows rows = {M, lay.off, lay.classes()};
+    const int st = by_mode(edge, p.N % (32 * kV) == 0, [&](auto mode) {
+      constexpr Mode MODE = decltype(mode)::value;
+      return p.res ? launch_fwd<T, MODE, true>(p, rows, held, s) : launch_fwd<T, MODE, false>(p, rows, held, s);
+    });
+    if (st >= 0) return st;
   }
-  const Rows rows = {M, lay.off, lay.classes(), 1};
-  const bool full = p.N == 64 || p.N == 128 || p.N == 256 || p.N == 512 || (p.N > 512 && p.N % (32 * FWD_V) == 0);
-  return by_mode(edge, full, [&](auto mode) {
-    constexpr Mode MODE = decltype(mode)::value;
-    return p.res ? launch_fwd<T, MODE, true>(p, rows, held, s) : launch_fwd<T, MODE, false>(p, rows, held, s);
-  });
+  fwd_any<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
+  return check_launch();
 }
 
 }  // namespace
