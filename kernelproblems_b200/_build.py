@@ -23,6 +23,8 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 BUILD_DIR = REPO_DIR / "_build"
 LIB_PATH = PKG_DIR / "libfrag.so"
+BINDING_SRC = CSRC / "binding.cpp"
+BINDING_PATH = PKG_DIR / "_binding.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -68,8 +70,36 @@ def _compile(src: Path, verbose: bool, ptxas_verbose: bool) -> Path:
     return obj
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile csrc/binding.cpp, the Python extension module beside libfrag.so,
+    against the installed torch's headers."""
+    import sysconfig
+
+    import torch
+
+    newest = max(f.stat().st_mtime for f in (BINDING_SRC, INCLUDE / "frag.h", Path(torch.__file__), Path(__file__)))
+    if not force and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest:
+        return BINDING_PATH
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DUSE_CUDA",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
-    """Compile every csrc/*.cu for sm_100a and link libfrag.so.  Returns its path."""
+    """Compile every csrc/*.cu for sm_100a and link libfrag.so, and the binding
+    beside it.  Returns libfrag.so's path."""
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sources()
     dep_t = _deps_mtime()
@@ -78,8 +108,10 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         obj = BUILD_DIR / (s.stem + ".o")
         if force or ptxas_verbose or not obj.exists() or obj.stat().st_mtime < max(s.stat().st_mtime, dep_t):
             stale.append(s)
-    with cf.ThreadPoolExecutor(max_workers=max(1, min(len(stale), os.cpu_count() or 1))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=max(1, min(len(stale) + 1, os.cpu_count() or 1))) as ex:
+        binding = ex.submit(build_binding, force, verbose)
         list(ex.map(lambda s: _compile(s, verbose, ptxas_verbose), stale))
+        binding.result()
     objs = [BUILD_DIR / (s.stem + ".o") for s in srcs]
     if stale or not LIB_PATH.exists() or LIB_PATH.stat().st_mtime < max(o.stat().st_mtime for o in objs):
         tmp = LIB_PATH.with_suffix(".so.tmp")

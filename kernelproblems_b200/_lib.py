@@ -221,15 +221,42 @@ def load() -> C.CDLL:
         return lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled binding (csrc/binding.cpp), loaded once and given libfrag.so's
+    entry points."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib = load()
+    with _lock:
+        if _binding is None:
+            path = LIB_PATH.with_name("_binding.so")
+            if not path.exists():
+                raise FileNotFoundError(f"{path} is missing: build it with `python -m kernelproblems_b200._build`")
+            import importlib.util
+
+            spec = importlib.util.spec_from_file_location("_binding", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind(*(C.cast(getattr(lib, name), _vp).value for name in (
+                "frag_layernorm_fwd", "frag_layernorm_bwd", "frag_layernorm_bwd_workspace_bytes", "frag_grad_norm",
+                "frag_grad_norm_workspace_bytes", "frag_adamw_update")))
+            _binding = module
+    return _binding
+
+
+def check(name: str, status: int) -> None:
+    """Raise FragError for a non-zero status."""
+    if status != FRAG_OK:
+        raise FragError(name, status, f"cudaError {load().frag_last_cuda_error()}" if status == 5 else "")
+
+
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise FragError on failure."""
-    lib = load()
-    st = getattr(lib, name)(*args)
-    if st != FRAG_OK:
-        detail = ""
-        if st == 5:
-            detail = f"cudaError {lib.frag_last_cuda_error()}"
-        raise FragError(name, st, detail)
+    check(name, getattr(load(), name)(*args))
 
 
 def version() -> str:

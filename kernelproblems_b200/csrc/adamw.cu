@@ -12,9 +12,7 @@
 //
 // Bound: HBM.  28 bytes a value in 32 bits (30 with a bf16 copy), 10.1 for a bf16
 // tensor with states in 8.  Everything is read and written once, nothing is kept on
-// chip, so the kernel only has to keep enough loads in flight: eight
-// neighbouring values a thread, 16-byte accesses, all of a chunk's loads before its
-// arithmetic.
+// chip, so the kernel only has to keep enough loads in flight.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -26,9 +24,13 @@
 namespace frag {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kGroup = 128;                  // values of a scale
-constexpr int64_t kChunk = 2 * 8 * kThreads;  // values
+// A block takes one chunk, a thread eight values of it: twelve blocks an SM (42
+// registers) have 12 KB of bf16 values and their states in flight.  218 million
+// bf16 values with states in 8 bits: 372 us; blocks of 256 threads 379, of 512 463;
+// two chunks a thread 588 at four blocks of 256 an SM, 446 one.
+constexpr int kThreads = 128, kResident = 12;
+constexpr int kGroup = 128;                // values of a scale
+constexpr int64_t kChunk = 8 * kThreads;  // values
 
 struct Entry {
   void* p;
@@ -55,41 +57,51 @@ struct Step {
   const float* grad_scale;  // or nullptr
   const float* lr_dev;      // or nullptr: lr
   const int64_t* step_dev;  // or nullptr: c1, root
-  double lr, beta1, beta2;
-  double log1, log2;  // of the betas
-  double c1, root;    // 1 - beta1^step, 1 / sqrt(1 - beta2^step)
+  double log1, log2;        // of the betas
+  float lr;
+  float b1, a1, b2, a2;     // beta, 1 - beta
+  float c1, root;           // 1 / (1 - beta1^step), 1 / sqrt(1 - beta2^step)
   float eps;
 };
 
 // What all values of a tensor share.
 struct Factors {
-  float b1, a1, b2, a2;  // beta, 1 - beta
-  float keep;            // 1 - lr wd
-  float rate;            // lr / c1
-  float root;            // 1 / sqrt(c2)
-  float eps;
-  float g;               // gradient's scale
+  float keep;  // 1 - lr wd
+  float rate;  // lr / (1 - beta1^step)
+  float root;  // 1 / sqrt(1 - beta2^step)
+  float g;     // the gradient's scale
 };
 
-// The products and sums of the moments are rounded one by one: fused, they would
-// differ in the last bit from the same formula elsewhere, and the 8 bits
-// that follow would then round differently at ties.
-__device__ __forceinline__ void update(float p, float g, float& m, float& v, float& r, float& out,
-                                       const Factors& f) {
-  g = __fmul_rn(g, f.g);
-  m = __fadd_rn(__fmul_rn(f.b1, m), __fmul_rn(f.a1, g));
-  v = __fadd_rn(__fmul_rn(f.b2, v), __fmul_rn(__fmul_rn(f.a2, g), g));
-  r = __fsqrt_rn(v);
-  // (the quotient's 2 ulp are 2^-22 of the step)
-  out = fmaf(p, f.keep, -__fdividef(f.rate * m, fmaf(r, f.root, f.eps)));
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// m' of m = m_code m_scale, with b1s = beta1 m_scale (states in 32 bits: scale 1).
+__device__ __forceinline__ float2 first_moment(float2 m, float2 g, float b1s, const Step& s) {
+  return __ffma2_rn(m, twice(b1s), __fmul2_rn(g, twice(s.a1)));
+}
+// v' of a gradient and beta2 v.
+__device__ __forceinline__ float2 second_moment(float2 b2v, float2 g, const Step& s) {
+  return __ffma2_rn(__fmul2_rn(g, twice(s.a2)), g, b2v);
+}
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float inverse(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// p' from m' and r = sqrt(v').  Root, reciprocal and product are off by some 2^-22
+// of the step, which is small beside p.
+__device__ __forceinline__ float2 parameter(float2 p, float2 m, float2 r, const Factors& f, const Step& s) {
+  const float2 d = __ffma2_rn(r, twice(f.root), twice(s.eps));
+  const float2 u = __fmul2_rn(__fmul2_rn(m, twice(-f.rate)), make_float2(inverse(d.x), inverse(d.y)));
+  return __ffma2_rn(p, twice(f.keep), u);
 }
 
-__device__ __forceinline__ float e4m3_to_f(uint8_t b) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(b, __NV_E4M3);
-  return __half2float(__half(h));
-}
-__device__ __forceinline__ float2 e4m3x2_to_f2(uint16_t b) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3);
+__device__ __forceinline__ float2 e4m3x2_to_f2(uint32_t b) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(b), __NV_E4M3);
   return __half22float2(__half2(h));
 }
 
@@ -97,12 +109,24 @@ __device__ __forceinline__ float2 e4m3x2_to_f2(uint16_t b) {
 __device__ __forceinline__ float state_scale(float most, float& inv) {
   float s = most * (1.0f / 448.0f);
   if (s < 1.17549435e-38f) s = most == 0.f ? 1.0f : 1.17549435e-38f;
-  inv = __frcp_rn(s);
+  inv = inverse(s);
   return s;
 }
 
 // A root's multiple of the scale: what is not zero stays so.
 __device__ __forceinline__ float at_least_smallest(float r, float q) { return r > 0.f ? fmaxf(q, 0x1p-9f) : q; }
+
+// Four values' codes, of factor inv.
+__device__ __forceinline__ uint32_t codes(float2 a, float2 b, float inv) {
+  a = __fmul2_rn(a, twice(inv));
+  b = __fmul2_rn(b, twice(inv));
+  return to_fp8x2<false>(a.x, a.y) | static_cast<uint32_t>(to_fp8x2<false>(b.x, b.y)) << 16;
+}
+__device__ __forceinline__ uint32_t root_codes(float2 a, float2 b, float inv) {
+  const float2 x = __fmul2_rn(a, twice(inv)), y = __fmul2_rn(b, twice(inv));
+  return to_fp8x2<false>(at_least_smallest(a.x, x.x), at_least_smallest(a.y, x.y)) |
+         static_cast<uint32_t>(to_fp8x2<false>(at_least_smallest(b.x, y.x), at_least_smallest(b.y, y.y))) << 16;
+}
 
 template <class T>
 __device__ __forceinline__ float value(const T* p) {
@@ -113,204 +137,213 @@ __device__ __forceinline__ void set_value(T* p, float f) {
   if (sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p) = f_to_bf16(f);
   else *reinterpret_cast<float*>(p) = f;
 }
+__device__ __forceinline__ float& part(float2& v, int i) { return i ? v.y : v.x; }
 
-// Eight neighbouring values from a 16-byte boundary, n of them (any n >= 8: all).
-// RO: nothing writes them in this launch.
-template <bool RO, class T>
-__device__ __forceinline__ void load8(const T* p, int64_t n, float (&f)[8]) {
-  if (n >= 8) {
-    if (sizeof(T) == 2) {
-      unpack8(RO ? ld_stream(p) : ld_plain(p), f);
-    } else {
-      float4 a, b;
-      if (RO) {
-        a = ld_stream_f4(p);
-        b = ld_stream_f4(p + 4);
-      } else {
-        a = *reinterpret_cast<const float4*>(p);
-        b = *reinterpret_cast<const float4*>(p + 4);
-      }
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? value(p + i) : 0.f;
-  }
-}
+// Eight neighbouring values as they lie in memory, from a 16-byte boundary.
 template <class T>
-__device__ __forceinline__ void store8(T* p, int64_t n, const float (&f)[8]) {
-  if (n >= 8) {
-    if (sizeof(T) == 2) {
-      st_global(p, pack8(f));
-    } else {
-      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) set_value(p + i, f[i]);
-  }
-}
+struct Eight {
+  uint4 raw[sizeof(T) / 2];
 
-// States of a tensor: whole groups.
-__device__ __forceinline__ int64_t held_by(const Entry& e) { return (e.numel + kGroup - 1) / kGroup * kGroup; }
+  // n of them (8 or more: all).  RO: nothing writes them in this launch.
+  template <bool RO>
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= 8) {
+#pragma unroll
+      for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q)
+        raw[q] = RO ? ld_stream(reinterpret_cast<const uint4*>(p) + q) : ld_plain(reinterpret_cast<const uint4*>(p) + q);
+    } else {
+      float2 f[4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part(f[i / 2], i & 1) = i < n ? value(p + i) : 0.f;
+      set(f);
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (sizeof(T) == 2) return bf16x2_to_f2(u4_word(raw[0], i));
+    else return make_float2(__uint_as_float(u4_word(raw[i / 2], 2 * (i & 1))),
+                            __uint_as_float(u4_word(raw[i / 2], 2 * (i & 1) + 1)));
+  }
+  __device__ __forceinline__ void set(const float2 (&f)[4]) {
+    if constexpr (sizeof(T) == 2) {
+      raw[0] = make_uint4(f2_to_bf16x2(f[0]), f2_to_bf16x2(f[1]), f2_to_bf16x2(f[2]), f2_to_bf16x2(f[3]));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        raw[q] = make_uint4(__float_as_uint(f[2 * q].x), __float_as_uint(f[2 * q].y), __float_as_uint(f[2 * q + 1].x),
+                            __float_as_uint(f[2 * q + 1].y));
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n) const {
+    if (n >= 8) {
+#pragma unroll
+      for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) st_global(reinterpret_cast<uint4*>(p) + q, raw[q]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) {
+          float2 f = pair(i / 2);
+          set_value(p + i, part(f, i & 1));
+        }
+    }
+  }
+};
+
+// The largest of 16 neighbouring lanes' a and b.  After one exchange lanes without
+// bit 3 go on with a and the others with b, so that both take one shuffle a level.
+__device__ __forceinline__ void largest_pair(float& a, float& b) {
+  const bool second = threadIdx.x & 8;
+  float v = max_mag(second ? b : a, __shfl_xor_sync(0xffffffffu, second ? a : b, 8));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = max_mag(v, __shfl_xor_sync(0xffffffffu, v, o));
+  const float w = __shfl_xor_sync(0xffffffffu, v, 8);
+  a = second ? w : v;
+  b = second ? v : w;
+}
 
 // A chunk of a tensor whose pointers are 16-byte aligned: thread t has eight
 // neighbouring values, a group is 16 neighbouring lanes.  The states behind a
 // tensor's end belong to its last group and stay zero (their p and g read as
-// zero), so they are moved whole.
+// zero), so they are moved whole.  `n`: the chunk's values.
 template <bool EIGHT, class P, class G>
-__device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, const Factors& f, int64_t from) {
-#pragma unroll
-  for (int k = 0; k < kChunk / (8 * kThreads); ++k) {
-    const int64_t at = from + (k * kThreads + threadIdx.x) * 8;
-    const int64_t left = e.numel - at;
-    if (left + (threadIdx.x & 31) * 8 <= 0) return;  // the whole warp is behind the end
-    const int64_t st = e.state + at;
-    P* p = static_cast<P*>(e.p) + at;
-    float pv[8], gv[8], m[8], v[8], r[8];
-    const bool in_group = at < held_by(e);
-    load8<false>(p, left, pv);
-    load8<true>(static_cast<const G*>(e.g) + at, left, gv);
-    float ms = 0.f, vs = 0.f;
-    if (EIGHT) {
-      uint2 mq = make_uint2(0, 0), vq = make_uint2(0, 0);
-      if (in_group) {
-        mq = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.m) + st);
-        vq = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.v) + st);
-        ms = s.m_scale[st / kGroup];
-        vs = s.v_scale[st / kGroup];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = e4m3x2_to_f2(static_cast<uint16_t>((i < 2 ? mq.x : mq.y) >> (16 * (i & 1))));
-        const float2 b = e4m3x2_to_f2(static_cast<uint16_t>((i < 2 ? vq.x : vq.y) >> (16 * (i & 1))));
-        m[2 * i] = __fmul_rn(a.x, ms);
-        m[2 * i + 1] = __fmul_rn(a.y, ms);
-        const float x = __fmul_rn(b.x, vs), y = __fmul_rn(b.y, vs);
-        v[2 * i] = __fmul_rn(x, x);
-        v[2 * i + 1] = __fmul_rn(y, y);
-      }
-    } else {
-      load8<false>(static_cast<const float*>(s.m) + st, in_group ? 8 : 0, m);
-      load8<false>(static_cast<const float*>(s.v) + st, in_group ? 8 : 0, v);
+__device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
+  const int at = threadIdx.x * 8;
+  if ((at & ~255) >= n) return;  // the whole warp
+  P* p0 = static_cast<P*>(e.p) + from + at;
+  const int64_t st = e.state + from + at;
+  const bool in = at < (n + kGroup - 1) / kGroup * kGroup;
+  Eight<P> p;
+  Eight<G> g;
+  p.template load<false>(p0, n - at);
+  g.template load<true>(static_cast<const G*>(e.g) + from + at, n - at);
+  float2 pv[4];
+  if constexpr (EIGHT) {
+    uint2 *m0 = reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + st),
+          *v0 = reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + st);
+    float *ms = s.m_scale + st / kGroup, *vs = s.v_scale + st / kGroup;
+    uint2 mq = make_uint2(0, 0), vq = make_uint2(0, 0);
+    float mb = 0.f, vb = 0.f;
+    if (in) {
+      mq = *m0;
+      vq = *v0;
+      mb = *ms * s.b1;
+      vb = *vs;
     }
+    float2 m[4], r[4];
+    float mm = 0.f, rm = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) update(pv[i], gv[i], m[i], v[i], r[i], pv[i], f);
-    store8(p, left, pv);
-    if (e.copy) store8(e.copy + at, left, pv);
-    if (EIGHT) {
-      float mm = 0.f, rm = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mm = max_mag(mm, m[i]);
-        rm = max_mag(rm, r[i]);
-      }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        mm = max_mag(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-        rm = max_mag(rm, __shfl_xor_sync(0xffffffffu, rm, o));
-      }
-      float mi, ri;
-      ms = state_scale(mm, mi);
-      vs = state_scale(rm, ri);
-      if (in_group) {
-        uint32_t a[4], b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = to_fp8x2<false>(__fmul_rn(m[2 * i], mi), __fmul_rn(m[2 * i + 1], mi));
-          b[i] = to_fp8x2<false>(at_least_smallest(r[2 * i], __fmul_rn(r[2 * i], ri)),
-                                 at_least_smallest(r[2 * i + 1], __fmul_rn(r[2 * i + 1], ri)));
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + st) = make_uint2(a[0] | a[1] << 16, a[2] | a[3] << 16);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + st) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-        if ((threadIdx.x & 15) == 0) {
-          s.m_scale[st / kGroup] = ms;
-          s.v_scale[st / kGroup] = vs;
-        }
-      }
-    } else if (in_group) {
-      store8(static_cast<float*>(s.m) + st, 8, m);
-      store8(static_cast<float*>(s.v) + st, 8, v);
+    for (int i = 0; i < 4; ++i) {
+      const float2 gi = __fmul2_rn(g.pair(i), twice(f.g));
+      m[i] = first_moment(e4m3x2_to_f2((i < 2 ? mq.x : mq.y) >> (16 * (i & 1)) & 0xffff), gi, mb, s);
+      const float2 root = __fmul2_rn(e4m3x2_to_f2((i < 2 ? vq.x : vq.y) >> (16 * (i & 1)) & 0xffff), twice(vb));
+      const float2 v = second_moment(__fmul2_rn(__fmul2_rn(root, twice(s.b2)), root), gi, s);
+      r[i] = make_float2(root_of(v.x), root_of(v.y));
+      pv[i] = parameter(p.pair(i), m[i], r[i], f, s);
+      mm = max_mag2(mm, m[i]);
+      rm = max_mag2(rm, r[i]);
     }
+    largest_pair(mm, rm);
+    float mi, ri;
+    const float mscale = state_scale(mm, mi), rscale = state_scale(rm, ri);
+    if (in) {
+      *m0 = make_uint2(codes(m[0], m[1], mi), codes(m[2], m[3], mi));
+      *v0 = make_uint2(root_codes(r[0], r[1], ri), root_codes(r[2], r[3], ri));
+      if ((threadIdx.x & 15) == 0) {
+        *ms = mscale;
+        *vs = rscale;
+      }
+    }
+  } else {
+    float *m0 = static_cast<float*>(s.m) + st, *v0 = static_cast<float*>(s.v) + st;
+    Eight<float> m, v;
+    m.template load<false>(m0, in ? 8 : 0);
+    v.template load<false>(v0, in ? 8 : 0);
+    float2 mn[4], vn[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 gi = __fmul2_rn(g.pair(i), twice(f.g));
+      mn[i] = first_moment(m.pair(i), gi, s.b1, s);
+      vn[i] = second_moment(__fmul2_rn(v.pair(i), twice(s.b2)), gi, s);
+      pv[i] = parameter(p.pair(i), mn[i], make_float2(root_of(vn[i].x), root_of(vn[i].y)), f, s);
+    }
+    if (in) {
+      m.set(mn);
+      m.store(m0, 8);
+      v.set(vn);
+      v.store(v0, 8);
+    }
+  }
+  p.set(pv);
+  p.store(p0, n - at);
+  if (e.copy) {
+    Eight<uint16_t> c;
+    c.set(pv);
+    c.store(e.copy + from + at, n - at);
   }
 }
 
-// The same where some pointer is not aligned: lane l of a warp has every 32nd
-// of 256 values, single accesses that a warp makes to neighbouring addresses; a
-// group is four of its rows.
+// The same where some pointer is not aligned: a warp takes a group of 128 at a
+// time, lane l every 32nd of them, in single accesses that a warp makes to
+// neighbouring addresses.
 template <bool EIGHT, class P, class G>
-__device__ __forceinline__ void chunk_any(const Entry& e, const Step& s, const Factors& f, int64_t from) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void chunk_any(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
+  P* p0 = static_cast<P*>(e.p) + from;
+  const G* g0 = static_cast<const G*>(e.g) + from;
+  const int64_t st = e.state + from;
+  const int lane = threadIdx.x & 31;
 #pragma unroll 1
-  for (int k = 0; k < kChunk / (8 * kThreads); ++k) {
-    const int64_t at = from + (k * (kThreads / 32) + warp) * 256 + lane;
-    if (at - lane >= e.numel) return;
-    const int64_t st = e.state + at;
-    P* p = static_cast<P*>(e.p) + at;
-    const G* g = static_cast<const G*>(e.g) + at;
-    const int64_t held = held_by(e);
-    float pv[8], gv[8], m[8], v[8], r[8];
-    float ms[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
+  for (int at = (threadIdx.x >> 5) * kGroup; at < n && at < kChunk; at += kThreads / 32 * kGroup) {
+    float pv[4], gv[4], mv[4], rv[4];
+    float mb = s.b1, vb = 1.f;
+    if (EIGHT) {
+      mb *= s.m_scale[(st + at) / kGroup];
+      vb = s.v_scale[(st + at) / kGroup];
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool in = at + 32 * i < e.numel, st_in = at + 32 * i < held;
-      pv[i] = in ? value(p + 32 * i) : 0.f;
-      gv[i] = in ? value(g + 32 * i) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int j = at + lane + 32 * i;
+      pv[i] = j < n ? value(p0 + j) : 0.f;
+      gv[i] = j < n ? value(g0 + j) : 0.f;
+      mv[i] = EIGHT ? e4m3x2_to_f2(static_cast<const uint8_t*>(s.m)[st + j]).x : static_cast<const float*>(s.m)[st + j];
+      rv[i] = EIGHT ? e4m3x2_to_f2(static_cast<const uint8_t*>(s.v)[st + j]).x : static_cast<const float*>(s.v)[st + j];
+    }
+    float2 m[2], v[2], r[2];
+    float mm = 0.f, rm = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 gi = __fmul2_rn(make_float2(gv[2 * i], gv[2 * i + 1]), twice(f.g));
+      m[i] = first_moment(make_float2(mv[2 * i], mv[2 * i + 1]), gi, mb, s);
+      const float2 x = __fmul2_rn(make_float2(rv[2 * i], rv[2 * i + 1]), twice(vb));
+      const float2 y = __fmul2_rn(x, twice(s.b2));
+      v[i] = second_moment(EIGHT ? __fmul2_rn(y, x) : y, gi, s);
+      r[i] = make_float2(root_of(v[i].x), root_of(v[i].y));
+      const float2 q = parameter(make_float2(pv[2 * i], pv[2 * i + 1]), m[i], r[i], f, s);
+      pv[2 * i] = q.x;
+      pv[2 * i + 1] = q.y;
+      mm = max_mag2(mm, m[i]);
+      rm = max_mag2(rm, r[i]);
+    }
+    float mi = 1.f, ri = 1.f;
+    if (EIGHT) {
+      const float mscale = state_scale(warp_max_mag(mm), mi), rscale = state_scale(warp_max_mag(rm), ri);
+      if (lane == 0) {
+        s.m_scale[(st + at) / kGroup] = mscale;
+        s.v_scale[(st + at) / kGroup] = rscale;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = at + lane + 32 * i;
+      if (j < n) {
+        set_value(p0 + j, pv[i]);
+        if (e.copy) set_value(e.copy + from + j, pv[i]);
+      }
+      const float mn = part(m[i / 2], i & 1), rn = part(r[i / 2], i & 1);
       if (EIGHT) {
-        if (i % 4 == 0 && st_in) {
-          ms[i / 4] = s.m_scale[(st + 32 * i) / kGroup];
-          vs[i / 4] = s.v_scale[(st + 32 * i) / kGroup];
-        }
-        m[i] = st_in ? e4m3_to_f(static_cast<const uint8_t*>(s.m)[st + 32 * i]) : 0.f;
-        v[i] = st_in ? e4m3_to_f(static_cast<const uint8_t*>(s.v)[st + 32 * i]) : 0.f;
+        static_cast<uint8_t*>(s.m)[st + j] = to_fp8<false>(mn * mi);
+        static_cast<uint8_t*>(s.v)[st + j] = to_fp8<false>(at_least_smallest(rn, rn * ri));
       } else {
-        m[i] = st_in ? static_cast<const float*>(s.m)[st + 32 * i] : 0.f;
-        v[i] = st_in ? static_cast<const float*>(s.v)[st + 32 * i] : 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (EIGHT) {
-        m[i] = __fmul_rn(m[i], ms[i / 4]);
-        v[i] = __fmul_rn(v[i], vs[i / 4]);
-        v[i] = __fmul_rn(v[i], v[i]);
-      }
-      update(pv[i], gv[i], m[i], v[i], r[i], pv[i], f);
-      if (at + 32 * i < e.numel) {
-        set_value(p + 32 * i, pv[i]);
-        if (e.copy) set_value(e.copy + at + 32 * i, pv[i]);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float mi = 0.f, ri = 0.f;
-      if (EIGHT) {
-        float mm = 0.f, rm = 0.f;
-#pragma unroll
-        for (int i = 4 * h; i < 4 * h + 4; ++i) {
-          mm = max_mag(mm, m[i]);
-          rm = max_mag(rm, r[i]);
-        }
-        ms[h] = state_scale(warp_max_mag(mm), mi);
-        vs[h] = state_scale(warp_max_mag(rm), ri);
-        if (lane == 0 && at + 128 * h < held) {
-          s.m_scale[(st + 128 * h) / kGroup] = ms[h];
-          s.v_scale[(st + 128 * h) / kGroup] = vs[h];
-        }
-      }
-#pragma unroll
-      for (int i = 4 * h; i < 4 * h + 4; ++i) {
-        if (at + 32 * i >= held) continue;
-        if (EIGHT) {
-          static_cast<uint8_t*>(s.m)[st + 32 * i] = to_fp8<false>(__fmul_rn(m[i], mi));
-          static_cast<uint8_t*>(s.v)[st + 32 * i] = to_fp8<false>(at_least_smallest(r[i], __fmul_rn(r[i], ri)));
-        } else {
-          static_cast<float*>(s.m)[st + 32 * i] = m[i];
-          static_cast<float*>(s.v)[st + 32 * i] = v[i];
-        }
+        static_cast<float*>(s.m)[st + j] = mn;
+        static_cast<float*>(s.v)[st + j] = part(v[i / 2], i & 1);
       }
     }
   }
@@ -318,40 +351,35 @@ __device__ __forceinline__ void chunk_any(const Entry& e, const Step& s, const F
 
 template <bool EIGHT, class P, class G>
 __device__ __forceinline__ void chunk(bool aligned, const Entry& e, const Step& s, const Factors& f, int64_t from) {
-  if (aligned) chunk_aligned<EIGHT, P, G>(e, s, f, from);
-  else chunk_any<EIGHT, P, G>(e, s, f, from);
+  const int n = static_cast<int>(min(e.numel - from, kChunk));
+  if (aligned) chunk_aligned<EIGHT, P, G>(e, s, f, from, n);
+  else chunk_any<EIGHT, P, G>(e, s, f, from, n);
 }
 
 template <int CAP, bool EIGHT>
-__global__ void __launch_bounds__(kThreads) adamw(const __grid_constant__ List<CAP> L, const __grid_constant__ Step s) {
+__global__ void __launch_bounds__(kThreads, kResident) adamw(const __grid_constant__ List<CAP> L, const __grid_constant__ Step s) {
   const int i = find_tensor(L.first, L.count, blockIdx.x);
   const Entry& e = L.t[i];
-  const double lr = s.lr_dev ? static_cast<double>(*s.lr_dev) : s.lr;
-  const float scale = s.grad_scale ? *s.grad_scale : 1.0f;
-  double c1 = s.c1, root = s.root;
+  const float lr = (s.lr_dev ? *s.lr_dev : s.lr) * e.lr_scale;
+  Factors f;
+  f.g = s.grad_scale ? *s.grad_scale : 1.0f;
+  float c1 = s.c1;
+  f.root = s.root;
   if (s.step_dev) {
-    __shared__ double c[2];
+    __shared__ float c[2];
     const int64_t step = *s.step_dev;
     if (step < 1) return;
     if (threadIdx.x == 0) {
-      c[0] = -expm1(static_cast<double>(step) * s.log1);
-      c[1] = 1.0 / sqrt(-expm1(static_cast<double>(step) * s.log2));
+      c[0] = static_cast<float>(-1.0 / expm1(static_cast<double>(step) * s.log1));
+      c[1] = static_cast<float>(1.0 / sqrt(-expm1(static_cast<double>(step) * s.log2)));
     }
     __syncthreads();
     c1 = c[0];
-    root = c[1];
+    f.root = c[1];
   }
-  if (!isfinite(scale) || !isfinite(lr)) return;
-  Factors f;
-  f.b1 = static_cast<float>(s.beta1);
-  f.a1 = static_cast<float>(1.0 - s.beta1);
-  f.b2 = static_cast<float>(s.beta2);
-  f.a2 = static_cast<float>(1.0 - s.beta2);
-  f.keep = static_cast<float>(1.0 - lr * static_cast<double>(e.lr_scale) * static_cast<double>(e.decay));
-  f.rate = static_cast<float>(lr * static_cast<double>(e.lr_scale) / c1);
-  f.root = static_cast<float>(root);
-  f.eps = s.eps;
-  f.g = scale;
+  if (!isfinite(f.g) || !isfinite(lr)) return;
+  f.keep = fmaf(-lr, e.decay, 1.0f);
+  f.rate = lr * c1;
   const int64_t from = static_cast<int64_t>(blockIdx.x - L.first[i]) * kChunk;
   const bool aligned = L.kind[i] & 4;
   switch (L.kind[i] & 3) {
@@ -434,11 +462,25 @@ int frag_adamw_update(const frag_adamw_tensor* tensors, const void* const* grads
   if (values == 0) return FRAG_OK;
   if (!exp_avg || !exp_avg_sq) return FRAG_ERR_INVALID_ARG;
   if (!aligned16(exp_avg) || !aligned16(exp_avg_sq)) return FRAG_ERR_ALIGN;
-  Step p = {exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, grad_scale, lr_device, step_device, lr, beta1, beta2,
-            std::log(beta1), std::log(beta2), 1.0, 1.0, static_cast<float>(eps)};
+  Step p = {};
+  p.m = exp_avg;
+  p.v = exp_avg_sq;
+  p.m_scale = exp_avg_scale;
+  p.v_scale = exp_avg_sq_scale;
+  p.grad_scale = grad_scale;
+  p.lr_dev = lr_device;
+  p.step_dev = step_device;
+  p.log1 = std::log(beta1);
+  p.log2 = std::log(beta2);
+  p.lr = static_cast<float>(lr);
+  p.b1 = static_cast<float>(beta1);
+  p.a1 = static_cast<float>(1.0 - beta1);
+  p.b2 = static_cast<float>(beta2);
+  p.a2 = static_cast<float>(1.0 - beta2);
+  p.eps = static_cast<float>(eps);
   if (!step_device) {
-    p.c1 = -std::expm1(static_cast<double>(step) * p.log1);
-    p.root = 1.0 / std::sqrt(-std::expm1(static_cast<double>(step) * p.log2));
+    p.c1 = static_cast<float>(-1.0 / std::expm1(static_cast<double>(step) * p.log1));
+    p.root = static_cast<float>(1.0 / std::sqrt(-std::expm1(static_cast<double>(step) * p.log2)));
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return eight ? launch_lists<true>(tensors, grads, grad_dtypes, count, p, s)

@@ -1282,6 +1282,19 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum_buffer: torch.
 
 # ------------------------------------------------------------------ layer norm
 
+# The ordinary call of these operators goes through the compiled binding: it
+# checks, makes the outputs and launches in a third of the time.  What it does not
+# take (None: strided rows, another device, anything to be refused) goes on in
+# Python, to the same kernels.
+
+def _taken(name: str, status) -> bool:
+    """Whether the binding made the call; raises where the call failed."""
+    if status is None:
+        return False
+    _lib.check(name, status)
+    return True
+
+
 def _norm_input(x: torch.Tensor, name: str):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -1331,6 +1344,10 @@ def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: tor
 
     x and residual: bf16 or fp32, rows of contiguous values, any row stride.
     weight, bias: bf16 or fp32 (both the same), or None for 1 and 0."""
+    out = _lib.binding().layernorm_fwd(x, weight, bias, eps, residual, write_h, save_stats)
+    if out.__class__ is tuple:
+        return out
+    _taken("frag_layernorm_fwd", out)
     N, dtype, dev = _norm_input(x, "x")
     M = _row_count(x, N)
     x2, xs = _strided_rows(x, "x", N, dev, None, dtype)
@@ -1361,6 +1378,11 @@ def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
     db     fp32 [N], sum over the rows of dy in a fixed order; None with compute_db=False
 
     dy, x and dres: of one type, rows of contiguous values, any row stride."""
+    if workspace is None:
+        out = _lib.binding().layernorm_bwd(dy, x, mean, rstd, weight, dres, compute_dw, compute_db)
+        if out.__class__ is tuple:
+            return out
+        _taken("frag_layernorm_bwd", out)
     N, dtype, dev = _norm_input(x, "x")
     M = _row_count(x, N)
     x2, xs = _strided_rows(x, "x", N, dev, None, dtype)
@@ -1436,6 +1458,12 @@ def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor |
 
     grads: contiguous bf16 and fp32 tensors on one device, |g| up to 1e18; None
     entries are left out."""
+    grads = list(grads)
+    if workspace is None:
+        out = _lib.binding().grad_norm(grads, max_norm)
+        if out.__class__ is tuple:
+            return out
+        _taken("frag_grad_norm", out)
     grads = [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
@@ -1494,7 +1522,7 @@ class AdamWStates:
     GROUP = 128
 
     def __init__(self, params, *, dtype: torch.dtype = torch.float32, weight_decay=0.0, lr_scale=1.0, copies=None):
-        self.params = list(params)
+        self.params = tuple(params)
         n = len(self.params)
         if not n:
             raise ValueError("AdamWStates needs at least one parameter")
@@ -1502,7 +1530,7 @@ class AdamWStates:
             raise TypeError("dtype must be float32 or float8_e4m3fn")
         decay, lr_scale = _each(weight_decay, n, "weight_decay"), _each(lr_scale, n, "lr_scale")
         self.device = _dense_list(self.params, "params")
-        self.copies = [None] * n if copies is None else list(copies)
+        self.copies = (None,) * n if copies is None else tuple(copies)
         if len(self.copies) != n:
             raise ValueError(f"copies: {len(self.copies)} for {n} parameters")
         for p, c in zip(self.params, self.copies):
@@ -1510,7 +1538,7 @@ class AdamWStates:
                 _check_out(c, "a copy", torch.bfloat16, self.device, shape=p.shape)
         self.dtype = dtype
         self._shapes = list(map(_shape_of, self.params))
-        self._written = self.params + [c for c in self.copies if c is not None]
+        self._written = [*self.params, *(c for c in self.copies if c is not None)]
         self._kinds = list(map(_dtype_of, self._written))
         self._numel = list(map(torch.Tensor.numel, self._written))
         _disjoint(self._written, "parameters and copies")
@@ -1529,6 +1557,7 @@ class AdamWStates:
         for i, e in enumerate(self._table):
             e.numel, e.state_offset = self._numel[i], self.offsets[i]
             e.lr_scale, e.weight_decay, e.param_dtype = lr_scale[i], decay[i], _DT[self._kinds[i]]
+        self._codes, self._counts = _dtype_codes(self._written), array("q", self._numel)
         self._places = None
         self._place()
 
@@ -1553,6 +1582,8 @@ class AdamWStates:
                 e.copy = places[at]
                 at += 1
         self._places = places
+        # what the binding compares the tensors with: addresses of the three arrays, and the table's
+        self._known = (written, _address(places), _address(self._codes), _address(self._counts)), C.addressof(self._table)
 
     def _held(self):
         """The states' addresses; refused where one is not what it was made as."""
@@ -1638,15 +1669,22 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
         raise ValueError("betas must be in [0, 1)")
     if not (eps >= 0 and math.isfinite(eps)):
         raise ValueError("eps must be finite and not negative")
-    lr_ptr = step_ptr = None
+    lr_t = step_t = None
     if isinstance(lr, torch.Tensor):
-        lr_ptr, lr = _device_word(lr, "lr", torch.float32, dev), 0.0
+        lr_t, lr = lr, 0.0
     elif not math.isfinite(lr):
         raise ValueError("lr must be finite")
     if isinstance(step, torch.Tensor):
-        step_ptr, step = _device_word(step, "step", torch.int64, dev), 0
+        step_t, step = step, 0
     elif not isinstance(step, int) or step < 1:
         raise ValueError("step must be an int from 1 on")
+    known, table = states._known
+    if _taken("frag_adamw_update", _lib.binding().adamw(
+            *known, grads, table, states.exp_avg, states.exp_avg_sq, states.exp_avg_scale, states.exp_avg_sq_scale,
+            states._total, lr, lr_t, b1, b2, eps, step, step_t, grad_scale)):
+        return
+    lr_ptr = None if lr_t is None else _device_word(lr_t, "lr", torch.float32, dev)
+    step_ptr = None if step_t is None else _device_word(step_t, "step", torch.int64, dev)
     scale_ptr = None if grad_scale is None else _device_word(grad_scale, "grad_scale", torch.float32, dev)
     shapes = states._shapes
     if any(g is None for g in grads):

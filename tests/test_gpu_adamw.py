@@ -160,7 +160,7 @@ def run_and_check(sizes, dtype, gdtype, state, *, copies=False, shift=0, gap=0, 
         m = m64.view(-1, 128)
         check_cancelling(states.exp_avg.view(-1, 128)[at], states.exp_avg_scale[at], m[at], m_off[at])
         check_eight(states.exp_avg_sq.view(-1, 128)[at].view(-1), states.exp_avg_sq_scale[at],
-                    v64.sqrt().view(-1, 128)[at].reshape(-1), 4 * U, True)
+                    v64.sqrt().view(-1, 128)[at].reshape(-1), 5 * U, True)  # half of v's 6, and the root's 2^-23
     # what no tensor of the step holds is as it was: states without a gradient, and memory around the parameters
     wide = 4 if state == F32 else 1
     now = [states.exp_avg.view(torch.uint8), states.exp_avg_sq.view(torch.uint8)]
