@@ -169,13 +169,6 @@ struct Input {
   int64_t stride;
 };
 
-// Whether a row's chunk c is memory of the tensor from its first value to its
-// last (the chunk may be shared with the row before or behind): 0 yes, otherwise
-// it is not read as a whole.
-__device__ __forceinline__ bool outside(int64_t row, int64_t stride, int64_t M, int before, int behind) {
-  return row * stride < before || (M - 1 - row) * stride < behind;
-}
-
 // ------------------------------------------- a thread's own ring: short rows
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
@@ -188,23 +181,48 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Asks for a thread's K chunks of a row, to `to`, 256 threads' chunks apart.
+// Asks for a thread's K chunks of a row, to `to`, 256 threads' chunks apart.  A
+// chunk that the row shares with another is read whole, except where it reaches out
+// of the tensor: rows a whole chunk or more apart, only the first and the last row
+// can.
 template <class T, int K, Mode MODE>
 __device__ __forceinline__ void ask_row(const Input<T>& in, int64_t row, int64_t M, const Places<T, MODE>& at, int N,
                                         uint4* to) {
   const T* from = in.p + row * in.stride;
+  const bool inner = MODE != EDGE || (row > 0 && row < M - 1 && in.stride >= kE<T>);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const Place<T, MODE> a = at[k];
     if (!a.some(N)) continue;
-    if (MODE == EDGE && !a.all(N) && outside(row, in.stride, M, max(0, -a.n0), max(0, a.n0 + kE<T> - N))) {
+    if (inner || a.all(N)) {
+      copy_async16(to + k * 256, from + a.n0);
+    } else {
       for (int i = 0; i < kE<T>; ++i)
         if (a.has(i, N)) reinterpret_cast<T*>(to + k * 256)[i] = from[a.n0 + i];
-    } else {
-      copy_async16(to + k * 256, from + a.n0);
     }
   }
 }
+
+// The bits of a chunk that are its row's, for a thread whose columns stay.
+template <class T, Mode MODE>
+struct Bits {
+  uint4 mask;
+  __device__ __forceinline__ void set(const Place<T, MODE>& at, int N) {
+    if constexpr (MODE == EDGE) {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kE<T>; ++i)
+        if (at.has(i, N)) w[i * static_cast<int>(sizeof(T)) / 4] |= sizeof(T) == 4 ? ~0u : 0xffffu << (16 * (i & 1));
+      mask = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  // Zeros for the values of another row.
+  __device__ __forceinline__ uint4 operator()(const uint4& v) const {
+    if constexpr (MODE == EDGE)
+      return make_uint4(v.x & mask.x, v.y & mask.y, v.z & mask.z, v.w & mask.w);
+    else return v;
+  }
+};
 
 // Sum over groups of L neighbouring lanes.
 template <int L>
@@ -385,7 +403,7 @@ __device__ __forceinline__ void shared_chunk(const W* vector, int count, int c, 
 }
 
 // Rows that a thread's own ring holds.
-constexpr int kAhead = 4;
+constexpr int kAhead = 3;
 // Blocks an SM, as far as registers go: `most` of eight values a lane.
 constexpr int lane_blocks(int V, Mode mode, int most) { return most - (V == 8 && mode != EDGE ? 0 : 1); }
 
@@ -395,11 +413,12 @@ constexpr int kSmem = 232448;  // of an SM, for its blocks
 
 int group_threads(int64_t held) { return static_cast<int>(ceil_div(held, 32 * kV) * 32); }
 
-// The groups of a launch's blocks, at most `most` threads: as many as leave each
-// `least` stages, and then as many stages as fit beside `vectors` shared ones.
-// Returns the blocks, 0 where not one stage fits.
+// The groups of a launch's blocks, and their stages: as many groups as `most`
+// threads are that leave each `least`
+// stages beside `vectors` shared ones, and then as many stages as `flight` bytes
+// are.  Returns the blocks, 0 where not one stage fits.
 int64_t plan_groups(const Rows& rows, int64_t held, int size, int inputs, int vectors, int vector_size, int most,
-                    int least, Shape& shape, int* smem) {
+                    int least, int flight, Shape& shape, int* smem) {
   const int E = 16 / size;
   shape.threads = group_threads(held);
   shape.slot = static_cast<int>(ceil_div(held, E)) * 16;
@@ -409,7 +428,7 @@ int64_t plan_groups(const Rows& rows, int64_t held, int size, int inputs, int ve
   int groups = std::min(most / shape.threads, shape.threads == 32 ? 32 : 15);
   groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, ceil_div(rows.M, sms))));
   for (;; --groups) {
-    shape.stages = std::min(8, (kSmem - 2048 - shared) / (stage * groups));
+    shape.stages = std::min({8, (kSmem - 2048 - shared) / (stage * groups), std::max(least, flight / (stage * groups))});
     if (shape.stages >= least || groups == 1) break;
   }
   if (shape.stages < 1) return 0;

@@ -74,6 +74,9 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
   const int off = MODE == EDGE ? static_cast<int>((rows.off + row % rows.classes * N) % E) : 0;
   const int t = threadIdx.x % L;
   const Places<T, MODE> at = {t, L, off};
+  Bits<T, MODE> own[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) own[k].set(at[k], N);
   auto ask = [&](int64_t r, int s) {
     uint4* to = held + s * (ROW * 256) + threadIdx.x;
     if (r < rows.M) {
@@ -105,10 +108,9 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!at[k].some(N)) continue;
-      unpack<T>(from[k * 256], d + k * P);
-      unpack<T>(from[(K + k) * 256], x + k * P);
-      own_values<T, MODE>(at[k], N, 0.f, d + k * P);
-      own_values<T, MODE>(at[k], N, mean, x + k * P);
+      // (of another row's values dy is 0, and so is all that x is multiplied with)
+      unpack<T>(own[k](from[k * 256]), d + k * P);
+      unpack<T>(own[k](from[(K + k) * 256]), x + k * P);
       chunk_sums<T>(d + k * P, x + k * P, w + k * P, mean, s1, s2);
     }
     const float g1 = lanes_sum<L>(s1.x + s1.y), g2 = lanes_sum<L>(s2.x + s2.y);
@@ -410,7 +412,7 @@ int launch_bwd_groups(const BwdP<T>& p, const Rows& rows, int64_t held, int64_t*
   auto kernel = bwd_groups<T, W, MODE, RES>;
   Shape shape;
   int smem = 0;
-  *G = plan_groups(rows, held, sizeof(T), RES ? 3 : 2, 1, sizeof(W), 512, 2, shape, &smem);
+  *G = plan_groups(rows, held, sizeof(T), RES ? 3 : 2, 1, sizeof(W), 512, 2, 1 << 20, shape, &smem);
   if (!*G) return -1;
   if (shape.groups > 1) smem = std::max(smem, shape.groups * shape.threads * kV * 8);  // the sums at the end
   if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;

@@ -82,6 +82,9 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
   const int off = MODE == EDGE ? static_cast<int>((rows.off + row % rows.classes * N) % E) : 0;
   const int t = threadIdx.x % L;
   const Places<T, MODE> at = {t, L, off};
+  Bits<T, MODE> own[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) own[k].set(at[k], N);
   auto ask = [&](int64_t r, int s) {
     uint4* to = held + s * (ROW * 256) + threadIdx.x;
     if (r < rows.M) {
@@ -116,8 +119,7 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
         continue;
       }
       const uint4 none = make_uint4(0, 0, 0, 0);
-      input_chunk<T, RES>(from[k * 256], RES ? from[(K + k) * 256] : none, v + k * P);
-      own_values<T, MODE>(at[k], N, 0.f, v + k * P);
+      input_chunk<T, RES>(own[k](from[k * 256]), RES ? own[k](from[(K + k) * 256]) : none, v + k * P);
 #pragma unroll
       for (int q = 0; q < P; ++q) sum = __fadd2_rn(sum, v[k * P + q]);
       if (RES && p.h && in) store_chunk<T, MODE>(p.h + row * p.N, at[k], N, v + k * P);
@@ -145,8 +147,12 @@ __device__ __forceinline__ float warp_holds(int w, int threads, int off, int N) 
   return static_cast<float>(n);
 }
 
-// Threads of a block: 80 registers each.
+// Threads of a block (80 registers each): 512, and where that is one group only, 768.
 constexpr int kMost = 768;
+// Bytes of rows in flight on an SM.  More of them are slower, as the reads then hold
+// up the writes: 32768 rows of 8192 in bf16 168 us with 64 KB, 194 with 96 and
+// more; with the residual 335 with 64 KB, 370 with 128 and more.
+constexpr int kFlight = 65536;
 
 // Wider rows, a group a row at a time.  A row's mean and 1 / deviation behind one
 // barrier: each warp takes its own mean and squares about it, and the warps'
@@ -285,7 +291,8 @@ int launch_fwd_groups(const FwdP<T>& p, const Rows& rows, int64_t held, cudaStre
   auto kernel = fwd_groups<T, W, MODE, RES>;
   Shape shape;
   int smem = 0;
-  const int64_t blocks = plan_groups(rows, held, sizeof(T), RES ? 2 : 1, 2, sizeof(W), kMost, 1, shape, &smem);
+  const int64_t blocks = plan_groups(rows, held, sizeof(T), RES ? 2 : 1, 2, sizeof(W), held > 8 * 32 * kV ? kMost : 512, 1,
+                                     kFlight, shape, &smem);
   if (!blocks) return -1;
   if (!allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return FRAG_ERR_CUDA;
   kernel<<<dim3(static_cast<unsigned>(blocks)), shape.groups * shape.threads, smem, s>>>(p, rows, shape,
