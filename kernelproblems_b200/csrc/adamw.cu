@@ -116,18 +116,6 @@ __device__ __forceinline__ float state_scale(float most, float& inv) {
 // A root's multiple of the scale: what is not zero stays so.
 __device__ __forceinline__ float at_least_smallest(float r, float q) { return r > 0.f ? fmaxf(q, 0x1p-9f) : q; }
 
-// Four values' codes, of factor inv.
-__device__ __forceinline__ uint32_t codes(float2 a, float2 b, float inv) {
-  a = __fmul2_rn(a, twice(inv));
-  b = __fmul2_rn(b, twice(inv));
-  return to_fp8x2<false>(a.x, a.y) | static_cast<uint32_t>(to_fp8x2<false>(b.x, b.y)) << 16;
-}
-__device__ __forceinline__ uint32_t root_codes(float2 a, float2 b, float inv) {
-  const float2 x = __fmul2_rn(a, twice(inv)), y = __fmul2_rn(b, twice(inv));
-  return to_fp8x2<false>(at_least_smallest(a.x, x.x), at_least_smallest(a.y, x.y)) |
-         static_cast<uint32_t>(to_fp8x2<false>(at_least_smallest(b.x, y.x), at_least_smallest(b.y, y.y))) << 16;
-}
-
 template <class T>
 __device__ __forceinline__ float value(const T* p) {
   return sizeof(T) == 2 ? bf16_to_f(*reinterpret_cast<const uint16_t*>(p)) : *reinterpret_cast<const float*>(p);
@@ -203,30 +191,31 @@ __device__ __forceinline__ void largest_pair(float& a, float& b) {
 // A chunk of a tensor whose pointers are 16-byte aligned: thread t has eight
 // neighbouring values, a group is 16 neighbouring lanes.  The states behind a
 // tensor's end belong to its last group and stay zero (their p and g read as
-// zero), so they are moved whole.  `n`: the chunk's values.
+// zero), so they are moved whole.  `n`: the tensor's values from the chunk on.
 template <bool EIGHT, class P, class G>
 __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
+  P* p0 = static_cast<P*>(e.p) + from;
+  const G* g0 = static_cast<const G*>(e.g) + from;
+  const int64_t st = e.state + from;
+  const int held = (n + kGroup - 1) / kGroup * kGroup;
   const int at = threadIdx.x * 8;
-  if ((at & ~255) >= n) return;  // the whole warp
-  P* p0 = static_cast<P*>(e.p) + from + at;
-  const int64_t st = e.state + from + at;
-  const bool in = at < (n + kGroup - 1) / kGroup * kGroup;
+  if (at - (threadIdx.x & 31) * 8 >= n) return;  // the whole warp
+  const bool in = at < held;
   Eight<P> p;
   Eight<G> g;
-  p.template load<false>(p0, n - at);
-  g.template load<true>(static_cast<const G*>(e.g) + from + at, n - at);
+  p.template load<false>(p0 + at, n - at);
+  g.template load<true>(g0 + at, n - at);
   float2 pv[4];
   if constexpr (EIGHT) {
-    uint2 *m0 = reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + st),
-          *v0 = reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + st);
+    uint8_t *m0 = static_cast<uint8_t*>(s.m) + st, *v0 = static_cast<uint8_t*>(s.v) + st;
     float *ms = s.m_scale + st / kGroup, *vs = s.v_scale + st / kGroup;
     uint2 mq = make_uint2(0, 0), vq = make_uint2(0, 0);
     float mb = 0.f, vb = 0.f;
     if (in) {
-      mq = *m0;
-      vq = *v0;
-      mb = *ms * s.b1;
-      vb = *vs;
+      mq = *reinterpret_cast<const uint2*>(m0 + at);
+      vq = *reinterpret_cast<const uint2*>(v0 + at);
+      mb = ms[at / kGroup] * s.b1;
+      vb = vs[at / kGroup];
     }
     float2 m[4], r[4];
     float mm = 0.f, rm = 0.f;
@@ -245,15 +234,22 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
     float mi, ri;
     const float mscale = state_scale(mm, mi), rscale = state_scale(rm, ri);
     if (in) {
-      *m0 = make_uint2(codes(m[0], m[1], mi), codes(m[2], m[3], mi));
-      *v0 = make_uint2(root_codes(r[0], r[1], ri), root_codes(r[2], r[3], ri));
+      uint32_t a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = __fmul2_rn(m[i], twice(mi)), y = __fmul2_rn(r[i], twice(ri));
+        a[i] = to_fp8x2<false>(x.x, x.y);
+        b[i] = to_fp8x2<false>(at_least_smallest(r[i].x, y.x), at_least_smallest(r[i].y, y.y));
+      }
+      *reinterpret_cast<uint2*>(m0 + at) = make_uint2(a[0] | a[1] << 16, a[2] | a[3] << 16);
+      *reinterpret_cast<uint2*>(v0 + at) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
       if ((threadIdx.x & 15) == 0) {
-        *ms = mscale;
-        *vs = rscale;
+        ms[at / kGroup] = mscale;
+        vs[at / kGroup] = rscale;
       }
     }
   } else {
-    float *m0 = static_cast<float*>(s.m) + st, *v0 = static_cast<float*>(s.v) + st;
+    float *m0 = static_cast<float*>(s.m) + st + at, *v0 = static_cast<float*>(s.v) + st + at;
     Eight<float> m, v;
     m.template load<false>(m0, in ? 8 : 0);
     v.template load<false>(v0, in ? 8 : 0);
@@ -273,7 +269,7 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
     }
   }
   p.set(pv);
-  p.store(p0, n - at);
+  p.store(p0 + at, n - at);
   if (e.copy) {
     Eight<uint16_t> c;
     c.set(pv);

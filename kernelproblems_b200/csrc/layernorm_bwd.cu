@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
       shared_chunk<T, W>(w, apart, c, wk);
     };
     float2 s1 = twice(0.f), s2 = s1;
-#pragma unroll
+    constexpr int AT_ONCE = sizeof(T) == 4 ? 2 : K;
+#pragma unroll AT_ONCE
     for (int k = 0; k < K; ++k) {
       if (!at[k].some(N)) continue;
       float2 d[P], x[P], wk[P];
