@@ -236,3 +236,25 @@ def test_states_need_cuda_tensors():
         ops.grad_norm([torch.zeros(8)])
     with pytest.raises(ValueError):
         ops.layernorm_fwd(torch.zeros(2, 8))
+
+
+def test_the_binding_leaves_what_it_does_not_take():
+    """CPU tensors, lists of other things, wrong counts: None, and the Python path's errors."""
+    b = _lib.binding()
+    x = torch.zeros(2, 8)
+    assert b.layernorm_fwd(x, None, None, 1e-5, None, True, True) is None
+    assert b.layernorm_fwd("x", None, None, 1e-5, None, True, True) is None and b.layernorm_fwd(x) is None
+    assert b.layernorm_bwd(x, x, x, x, None, None, True, True) is None
+    assert b.grad_norm([x], 1.0) is None and b.grad_norm([], None) is None and b.grad_norm(x, None) is None
+    assert b.grad_norm([None, x], float("nan")) is None and b.grad_norm([x, 3], 1.0) is None
+    assert b.adamw(*[None] * 19) is None and b.adamw() is None
+    assert b.adamw([x], 0, 0, 0, [x], 0, x, x, None, None, 0, 0.0, None, 0.9, 0.9, 1e-8, 1, None, None) is None
+    with pytest.raises(TypeError):
+        b.bind(1)
+
+
+def test_a_missing_binding_fails_loudly(tmp_path, monkeypatch):
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "libfrag.so")
+    with pytest.raises(FileNotFoundError):
+        _lib.binding()
