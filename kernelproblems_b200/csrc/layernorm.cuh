@@ -181,27 +181,33 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Asks for a thread's K chunks of a row, to `to`, 256 threads' chunks apart.  A
-// chunk that the row shares with another is read whole, except where it reaches out
-// of the tensor: rows a whole chunk or more apart, only the first and the last row
-// can.
-template <class T, int K, Mode MODE>
-__device__ __forceinline__ void ask_row(const Input<T>& in, int64_t row, int64_t M, const Places<T, MODE>& at, int N,
-                                        uint4* to) {
-  const T* from = in.p + row * in.stride;
-  const bool inner = MODE != EDGE || (row > 0 && row < M - 1 && in.stride >= kE<T>);
+// A thread's way down its rows of one input, every `jump`-th value of it: asks for
+// the K chunks of a row, to `to`, 256 threads' chunks apart.  A chunk that the row
+// shares with another is read whole, except where it reaches out of the tensor:
+// rows a whole chunk or more apart, only the first and the last row (`end`) can.
+template <class T>
+struct Walk {
+  const T* next;
+  int64_t jump;
+  bool apart;
+  __device__ __forceinline__ Walk(const Input<T>& in, int64_t row, int64_t rows)
+      : next(in.p + row * in.stride), jump(rows * in.stride), apart(in.stride >= kE<T>) {}
+  template <int K, Mode MODE>
+  __device__ __forceinline__ void ask(const Places<T, MODE>& at, int N, bool end, uint4* to) const {
+    const bool inner = MODE != EDGE || (apart && !end);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Place<T, MODE> a = at[k];
-    if (!a.some(N)) continue;
-    if (inner || a.all(N)) {
-      copy_async16(to + k * 256, from + a.n0);
-    } else {
-      for (int i = 0; i < kE<T>; ++i)
-        if (a.has(i, N)) reinterpret_cast<T*>(to + k * 256)[i] = from[a.n0 + i];
+    for (int k = 0; k < K; ++k) {
+      const Place<T, MODE> a = at[k];
+      if (!a.some(N)) continue;
+      if (inner || a.all(N)) {
+        copy_async16(to + k * 256, next + a.n0);
+      } else {
+        for (int i = 0; i < kE<T>; ++i)
+          if (a.has(i, N)) reinterpret_cast<T*>(to + k * 256)[i] = next[a.n0 + i];
+      }
     }
   }
-}
+};
 
 // The bits of a chunk that are its row's, for a thread whose columns stay.
 template <class T, Mode MODE>

@@ -65,7 +65,7 @@ __device__ __forceinline__ void chunk_grad(const float2* dy, const float2* far, 
 template <class T, int V, int L, Mode MODE, bool RES>
 __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const BwdP<T> p, const Rows rows) {
   constexpr int E = kE<T>, P = kP<T>, K = V / E, ROW = (RES ? 3 : 2) * K;
-  extern __shared__ __align__(16) uint4 held[];  // [kAhead][ROW][256], [kAhead][2][256] of float
+  extern __shared__ __align__(16) uint4 held[];  // [kAhead][ROW][256], and (mean, rstd) of each row
   float* stats = reinterpret_cast<float*>(held + kAhead * ROW * 256);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int N = static_cast<int>(p.N);
@@ -77,19 +77,29 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
   Bits<T, MODE> own[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) own[k].set(at[k], N);
-  auto ask = [&](int64_t r, int s) {
+  Walk<T> dy({p.dy, p.ys}, row, groups), x({p.x, p.xs}, row, groups), res({RES ? p.dres : p.x, p.rs}, row, groups);
+  int64_t asked = row;
+  auto ask = [&](int s) {
     uint4* to = held + s * (ROW * 256) + threadIdx.x;
-    if (r < rows.M) {
-      ask_row<T, K, MODE>({p.dy, p.ys}, r, rows.M, at, N, to);
-      ask_row<T, K, MODE>({p.x, p.xs}, r, rows.M, at, N, to + K * 256);
-      if (RES) ask_row<T, K, MODE>({p.dres, p.rs}, r, rows.M, at, N, to + 2 * K * 256);
-      copy_async4(stats + s * 512 + threadIdx.x, p.mean + r);
-      copy_async4(stats + s * 512 + 256 + threadIdx.x, p.rstd + r);
+    if (asked < rows.M) {
+      const bool end = asked == 0 || asked == rows.M - 1;
+      dy.template ask<K, MODE>(at, N, end, to);
+      x.template ask<K, MODE>(at, N, end, to + K * 256);
+      if (RES) res.template ask<K, MODE>(at, N, end, to + 2 * K * 256);
+      if (t == 0) {  // (for all lanes of the row)
+        float* st = stats + (s * 256 + threadIdx.x) / L * 2;
+        copy_async4(st, p.mean + asked);
+        copy_async4(st + 1, p.rstd + asked);
+      }
     }
     copies_commit();
+    asked += groups;
+    dy.next += dy.jump;
+    x.next += x.jump;
+    if (RES) res.next += res.jump;
   };
 #pragma unroll
-  for (int s = 0; s < kAhead - 1; ++s) ask(row + s * groups, s);
+  for (int s = 0; s < kAhead - 1; ++s) ask(s);
   float2 w[V / 2], dw[V / 2], db[V / 2];
 #pragma unroll
   for (int k = 0; k < K; ++k) load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
@@ -97,21 +107,26 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
   for (int q = 0; q < V / 2; ++q) dw[q] = db[q] = twice(0.f);
   const float invN = 1.0f / static_cast<float>(N);
   int s = 0;
+  T* dx = p.dx + row * p.N;
+  const int64_t jump = groups * p.N;
   // (the lanes of a warp stay together: shuffles are the whole warp's)
-  for (int64_t lead = row - (threadIdx.x & 31) / L; lead < rows.M; lead += groups, row += groups) {
-    ask(row + (kAhead - 1) * groups, (s + kAhead - 1) % kAhead);
+  for (int64_t lead = row - (threadIdx.x & 31) / L; lead < rows.M; lead += groups, row += groups, dx += jump) {
+    __syncwarp();  // (every lane has the mean and deviation that the next ones replace)
+    ask(s == 0 ? kAhead - 1 : s - 1);
     copies_wait<kAhead - 1>();
+    __syncwarp();  // (the first lane's copies too)
     const uint4* from = held + s * (ROW * 256) + threadIdx.x;
-    const float mean = stats[s * 512 + threadIdx.x], rstd = stats[s * 512 + 256 + threadIdx.x];
-    s = (s + 1) % kAhead;
-    float2 d[V / 2], x[V / 2], s1 = twice(0.f), s2 = s1;
+    const float2 st = reinterpret_cast<const float2*>(stats)[(s * 256 + threadIdx.x) / L];
+    const float mean = st.x, rstd = st.y;
+    s = s == kAhead - 1 ? 0 : s + 1;
+    float2 d[V / 2], xv[V / 2], s1 = twice(0.f), s2 = s1;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!at[k].some(N)) continue;
       // (of another row's values dy is 0, and so is all that x is multiplied with)
       unpack<T>(own[k](from[k * 256]), d + k * P);
-      unpack<T>(own[k](from[(K + k) * 256]), x + k * P);
-      chunk_sums<T>(d + k * P, x + k * P, w + k * P, mean, s1, s2);
+      unpack<T>(own[k](from[(K + k) * 256]), xv + k * P);
+      chunk_sums<T>(d + k * P, xv + k * P, w + k * P, mean, s1, s2);
     }
     const float g1 = lanes_sum<L>(s1.x + s1.y), g2 = lanes_sum<L>(s2.x + s2.y);
     if (row >= rows.M) continue;
@@ -121,8 +136,8 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
       if (!at[k].some(N)) continue;
       float2 o[P];
       if (RES) unpack<T>(from[(2 * K + k) * 256], o);
-      chunk_grad<T, RES>(d + k * P, x + k * P, w + k * P, terms, o, dw + k * P, db + k * P);
-      store_chunk<T, MODE>(p.dx + row * p.N, at[k], N, o);
+      chunk_grad<T, RES>(d + k * P, xv + k * P, w + k * P, terms, o, dw + k * P, db + k * P);
+      store_chunk<T, MODE>(dx, at[k], N, o);
     }
   }
   if (!p.want_dw && !p.want_db) return;

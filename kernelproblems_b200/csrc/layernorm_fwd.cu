@@ -85,16 +85,22 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
   Bits<T, MODE> own[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) own[k].set(at[k], N);
-  auto ask = [&](int64_t r, int s) {
+  Walk<T> x({p.x, p.xs}, row, groups), res({RES ? p.res : p.x, p.rs}, row, groups);
+  int64_t asked = row;
+  auto ask = [&](int s) {
     uint4* to = held + s * (ROW * 256) + threadIdx.x;
-    if (r < rows.M) {
-      ask_row<T, K, MODE>({p.x, p.xs}, r, rows.M, at, N, to);
-      if (RES) ask_row<T, K, MODE>({p.res, p.rs}, r, rows.M, at, N, to + K * 256);
+    if (asked < rows.M) {
+      const bool end = asked == 0 || asked == rows.M - 1;
+      x.template ask<K, MODE>(at, N, end, to);
+      if (RES) res.template ask<K, MODE>(at, N, end, to + K * 256);
     }
     copies_commit();
+    asked += groups;
+    x.next += x.jump;
+    if (RES) res.next += res.jump;
   };
 #pragma unroll
-  for (int s = 0; s < kAhead - 1; ++s) ask(row + s * groups, s);
+  for (int s = 0; s < kAhead - 1; ++s) ask(s);
   float2 w[V / 2], b[V / 2];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -103,12 +109,14 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
   }
   const float invN = 1.0f / static_cast<float>(N);
   int s = 0;
+  T *y = p.y + row * p.N, *h = p.h + row * p.N;
+  const int64_t jump = groups * p.N;
   // (the lanes of a warp stay together: shuffles are the whole warp's)
-  for (int64_t lead = row - (threadIdx.x & 31) / L; lead < rows.M; lead += groups, row += groups) {
-    ask(row + (kAhead - 1) * groups, (s + kAhead - 1) % kAhead);
+  for (int64_t lead = row - (threadIdx.x & 31) / L; lead < rows.M; lead += groups, row += groups, y += jump, h += jump) {
+    ask(s == 0 ? kAhead - 1 : s - 1);
     copies_wait<kAhead - 1>();
     const uint4* from = held + s * (ROW * 256) + threadIdx.x;
-    s = (s + 1) % kAhead;
+    s = s == kAhead - 1 ? 0 : s + 1;
     const bool in = row < rows.M;
     float2 v[V / 2], sum = twice(0.f);
 #pragma unroll
@@ -122,7 +130,7 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
       input_chunk<T, RES>(own[k](from[k * 256]), RES ? own[k](from[(K + k) * 256]) : none, v + k * P);
 #pragma unroll
       for (int q = 0; q < P; ++q) sum = __fadd2_rn(sum, v[k * P + q]);
-      if (RES && p.h && in) store_chunk<T, MODE>(p.h + row * p.N, at[k], N, v + k * P);
+      if (RES && p.h && in) store_chunk<T, MODE>(h, at[k], N, v + k * P);
     }
     const float mean = lanes_sum<L>(sum.x + sum.y) * invN;
     const float r = rsqrtf(fmaf(lanes_sum<L>(row_squares<T, V, MODE>(at, N, v, mean)), invN, p.eps));
@@ -131,7 +139,7 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
     if (t == 0 && p.rstd) p.rstd[row] = r;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      write_chunk<T, MODE>(p.y + row * p.N, at[k], N, v + k * P, mean, r, w + k * P, b + k * P);
+      write_chunk<T, MODE>(y, at[k], N, v + k * P, mean, r, w + k * P, b + k * P);
   }
 }
 
