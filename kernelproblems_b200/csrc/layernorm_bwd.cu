@@ -14,7 +14,8 @@ struct BwdP {
   Vector w;
   const float* mean;
   const float* rstd;
-  float* partials;  // [G, vectors, N]: dw, db, as far as wanted
+  float* partials;  // [G, vectors, width]: dw, db, as far as wanted
+  int64_t width;    // N, or a row's chunks: a column then lies off places further on
   int64_t ys, xs, rs;
   int64_t N;
   int want_dw, want_db;
@@ -165,18 +166,12 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 3)) bwd_lanes(const 
   }
 }
 
-// A chunk's sums into a row of partials.
-template <class T, Mode MODE>
-__device__ __forceinline__ void store_sums(float* row, const Place<T, MODE>& at, int N, float2* f) {
-  if (MODE != EDGE && at.some(N)) {
+// A chunk's sums into a row of partials, by their places in the row's chunks.
+template <class T>
+__device__ __forceinline__ void store_sums(float* row, int c, const float2* f) {
 #pragma unroll
-    for (int q = 0; q < kP<T>; q += 2)
-      *reinterpret_cast<float4*>(row + at.n0 + 2 * q) = make_float4(f[q].x, f[q].y, f[q + 1].x, f[q + 1].y);
-  } else if (MODE == EDGE && at.some(N)) {
-#pragma unroll
-    for (int i = 0; i < kE<T>; ++i)
-      if (at.has(i, N)) row[at.n0 + i] = part(f[i / 2], i & 1);
-  }
+  for (int q = 0; q < kP<T>; q += 2)
+    *reinterpret_cast<float4*>(row + c * kE<T> + 2 * q) = make_float4(f[q].x, f[q].y, f[q + 1].x, f[q + 1].y);
 }
 
 // Two sums over a group of up to 16 warps, in a fixed order, for every thread.
@@ -288,12 +283,14 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
   }
   if (g.t == 0 && s_abort[g.index]) ring.drain(i);
   if (!p.want_dw && !p.want_db) return;
-  float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * N;
+  float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * p.width;
+  float* to_db = to + (p.want_dw ? p.width : 0);
   if (shape.groups == 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (p.want_dw) store_sums<T, MODE>(to, at[k], N, dw + k * P);
-      if (p.want_db) store_sums<T, MODE>(to + (p.want_dw ? N : 0), at[k], N, db + k * P);
+      if (!at[k].some(N)) continue;
+      if (p.want_dw) store_sums<T>(to, g.t + k * g.threads, dw + k * P);
+      if (p.want_db) store_sums<T>(to_db, g.t + k * g.threads, db + k * P);
     }
     return;
   }
@@ -308,6 +305,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
   __syncthreads();
   sums = reinterpret_cast<float2*>(smem) + g.t;
   for (int k = g.index; k < K; k += shape.groups) {
+    if (!at[k].some(N)) continue;
     float2 sw[P], sb[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) sw[j] = sb[j] = twice(0.f);
@@ -317,8 +315,8 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
         sw[j] = __fadd2_rn(sw[j], sums[(i * V + k * P + j) * g.threads]);
         sb[j] = __fadd2_rn(sb[j], sums[(i * V + V / 2 + k * P + j) * g.threads]);
       }
-    if (p.want_dw) store_sums<T, MODE>(to, at[k], N, sw);
-    if (p.want_db) store_sums<T, MODE>(to + (p.want_dw ? N : 0), at[k], N, sb);
+    if (p.want_dw) store_sums<T>(to, g.t + k * g.threads, sw);
+    if (p.want_db) store_sums<T>(to_db, g.t + k * g.threads, sb);
   }
 }
 
@@ -362,44 +360,56 @@ __global__ void __launch_bounds__(256) bwd_any_columns(const BwdP<T> p, int64_t 
   if (p.want_db) to[(p.want_dw ? p.N : 0) + n] = db;
 }
 
-// The G rows of [G, columns] partials added in a fixed order: 32 columns a
-// block, warp w adds the rows w, w + WARPS, ..., AT_ONCE in flight, then the warps'
-// sums in order.  The first N columns go to `first`, the others to `second`.
+// How the partials lie: row g's column n at n + (off + g N) % E of `width` places
+// (E = 1: at n).
+struct Partials {
+  const float* p;
+  int64_t G, N, width;
+  int vectors, off, E;
+};
+
+// The G rows of partials added in a fixed order: 32 columns a block, warp w adds the
+// rows w, w + WARPS, ..., AT_ONCE in flight, then the warps' sums in order.  The
+// first N columns go to `first`, the others to `second`.
 template <int WARPS, int AT_ONCE>
-__global__ void __launch_bounds__(32 * WARPS) add_partials(const float* __restrict__ partials, int64_t G,
-                                                           int64_t columns, int64_t N, float* first, float* second) {
+__global__ void __launch_bounds__(32 * WARPS) add_partials(const Partials in, float* first, float* second) {
   __shared__ float red[WARPS][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane, n = col < in.N ? col : col - in.N;
+  const bool is = col < in.vectors * in.N;
+  const float* from = in.p + (col < in.N ? 0 : in.width) + n;
+  const int step = static_cast<int>(in.N % in.E), G = static_cast<int>(in.G);
+  const int64_t apart = in.vectors * in.width;
   float a = 0.f;
-  if (col < columns) {
-    for (int64_t g0 = warp; g0 < G; g0 += WARPS * AT_ONCE) {
+  if (is) {
+    for (int g0 = warp; g0 < G; g0 += WARPS * AT_ONCE) {
+      const float* row = from + g0 * apart;
       float v[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) v[j] = g0 + WARPS * j < G ? partials[(g0 + WARPS * j) * columns + col] : 0.f;
+      for (int j = 0; j < AT_ONCE; ++j, row += WARPS * apart)
+        v[j] = g0 + WARPS * j < G ? row[(in.off + (g0 + WARPS * j) * step) & (in.E - 1)] : 0.f;
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) a += v[j];
     }
   }
   red[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && col < columns) {
+  if (warp == 0 && is) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) s += red[w][lane];
-    if (col < N) first[col] = s;
-    else second[col - N] = s;
+    if (col < in.N) first[n] = s;
+    else second[n] = s;
   }
 }
 
-int launch_add_partials(const float* partials, int64_t G, int64_t N, float* dw, float* db, cudaStream_t s) {
-  const int64_t columns = ((dw ? 1 : 0) + (db ? 1 : 0)) * N;
+int launch_add_partials(const Partials& in, float* dw, float* db, cudaStream_t s) {
+  const int64_t columns = in.vectors * in.N;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(columns, 32)));
   // A block of 32 warps fills an SM's registers.  Columns for more than one round of
-  // such blocks (and then the partials are a row an SM) take half as large ones:
-  // 8192 columns of 148 rows 5 us less, where 256 columns of 444 rows take 5 more.
+  // such blocks (the partials are then a row an SM) take half as large ones.
   const bool many = columns > 32LL * sm_count();
   cfg.blockDim = dim3(many ? 512 : 1024);
   cfg.stream = s;
@@ -408,8 +418,7 @@ int launch_add_partials(const float* partials, int64_t G, int64_t N, float* dw, 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, many ? add_partials<16, 10> : add_partials<32, 16>, partials, G, columns, N,
-                                        dw ? dw : db, db));
+  return cuda_status(cudaLaunchKernelEx(&cfg, many ? add_partials<16, 10> : add_partials<32, 16>, in, dw ? dw : db, db));
 }
 
 // Blocks of rows that the columns' sums are split over, at most.
@@ -456,7 +465,8 @@ int launch_bwd(const BwdP<T>& p, const Rows& rows, int64_t held, int64_t* G, cud
 }
 
 template <class T>
-int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) {
+int backward(BwdP<T> p, int64_t M, float* dw, float* db, cudaStream_t s) {
+  Partials sums = {p.partials, 0, p.N, p.N, p.want_dw + p.want_db, 0, 1};
   Layout lay(p.N, sizeof(T));
   lay.add(p.dy, p.ys);
   lay.add(p.x, p.xs);
@@ -468,12 +478,19 @@ int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) 
   int st = -1;
   if (lay.alike && held <= kHeld) {
     const Rows rows = {M, lay.off, lay.classes()};
+    if (edge && held > kLanes) {  // (the groups write their partials by chunks)
+      sums.width = p.width = ceil_div(held, kE<T>) * kE<T>;
+      sums.off = lay.off;
+      sums.E = kE<T>;
+    }
     st = by_mode(edge, p.N % (32 * kV) == 0, [&](auto mode) {
       constexpr Mode MODE = decltype(mode)::value;
       return p.dres ? launch_bwd<T, MODE, true>(p, rows, held, &G, s) : launch_bwd<T, MODE, false>(p, rows, held, &G, s);
     });
   }
   if (st < 0) {
+    sums.width = p.N;
+    sums.E = 1;
     bwd_any_dx<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
     if (st = check_launch(); st != FRAG_OK || (!dw && !db)) return st;
     const int64_t R = ceil_div(M, std::min(M, static_cast<int64_t>(sm_count()) * 4));
@@ -483,7 +500,8 @@ int backward(const BwdP<T>& p, int64_t M, float* dw, float* db, cudaStream_t s) 
     st = check_launch();
   }
   if (st != FRAG_OK || (!dw && !db)) return st;
-  return launch_add_partials(p.partials, G, p.N, dw, db, s);
+  sums.G = G;
+  return launch_add_partials(sums, dw, db, s);
 }
 
 }  // namespace
@@ -495,7 +513,7 @@ extern "C" {
 
 size_t frag_layernorm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
-  return align_up(static_cast<size_t>(row_blocks(M)) * 2 * N * sizeof(float), 256);
+  return align_up(static_cast<size_t>(row_blocks(M)) * 2 * (N + 16) * sizeof(float), 256);
 }
 
 int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
@@ -522,11 +540,11 @@ int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t
   float* ws = static_cast<float*>(workspace);
   if (dtype == FRAG_DT_F32)
     return backward<float>({static_cast<const float*>(dy), static_cast<const float*>(x),
-                            static_cast<const float*>(dres), static_cast<float*>(dx), wv, mean, rstd, ws, dy_stride,
+                            static_cast<const float*>(dres), static_cast<float*>(dx), wv, mean, rstd, ws, N, dy_stride,
                             x_stride, dres_stride, N, dw != nullptr, db != nullptr},
                            M, dw, db, s);
   return backward<uint16_t>({static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(x),
-                             static_cast<const uint16_t*>(dres), static_cast<uint16_t*>(dx), wv, mean, rstd, ws,
+                             static_cast<const uint16_t*>(dres), static_cast<uint16_t*>(dx), wv, mean, rstd, ws, N,
                              dy_stride, x_stride, dres_stride, N, dw != nullptr, db != nullptr},
                             M, dw, db, s);
 }
