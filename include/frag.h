@@ -622,7 +622,7 @@ FRAG_API int frag_grad_norm(const void* const* grads, const int64_t* numel, cons
  * v in fp32.  Given: exp_avg = m and exp_avg_sq = sqrt(v) in E4M3, each 128 values
  * times the fp32 scale [state / 128]; a scale is the largest magnitude / 448 (1
  * where all are zero), and what is not zero of sqrt(v) stays at least 2^-9 scale.
- * step counts from 1; step_device, lr_device (device words) replace step and lr
+ * eps >= 2^-126.  step counts from 1; step_device, lr_device (device words) replace step and lr
  * when given, for steps that are captured once and replayed.  With a grad_scale
  * (device word, or NULL) or a device lr that is not finite, or a device step below
  * 1, nothing is changed.  No counterpart in the reference.

@@ -434,7 +434,8 @@ int frag_adamw_update(const frag_adamw_tensor* tensors, const void* const* grads
                       const int64_t* step_device, const float* grad_scale, frag_stream_t stream) {
   if (count < 0 || (count > 0 && (!tensors || !grads || !grad_dtypes))) return FRAG_ERR_INVALID_ARG;
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return FRAG_ERR_INVALID_ARG;
-  if (!std::isfinite(eps) || eps < 0.0) return FRAG_ERR_INVALID_ARG;
+  // (a normal number in 32 bits: the reciprocal takes what lies below for 0)
+  if (!std::isfinite(eps) || eps < 0x1p-126) return FRAG_ERR_INVALID_ARG;
   if (!lr_device && !std::isfinite(lr)) return FRAG_ERR_INVALID_ARG;
   if (!step_device && step < 1) return FRAG_ERR_INVALID_ARG;
   const bool eight = exp_avg_scale != nullptr;

@@ -244,9 +244,9 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // values a thread, a named barrier, and a ring of S stages that the group's first
 // thread streams its next rows' windows (their chunks, whole) of up to three
 // inputs into by bulk copies.  All rows of a block are of one class, so the groups
-// share the weights at their columns in shared memory.  Groups that
-// wait for nothing but their own rows fill one another's latencies, and the
-// gradient's sums over rows leave an SM as one row of partials.
+// share the weights at their columns in shared memory.  Groups that wait for
+// nothing but their own rows fill one another's latencies, and the gradient's sums
+// over rows leave an SM as one row of partials.
 //
 // A window reaches up to 15 bytes past its row on either side.  Where that is not
 // the tensor's own memory (before its first value, behind its last) the chunk is
@@ -420,16 +420,16 @@ constexpr int kSmem = 232448;  // of an SM, for its blocks
 int group_threads(int64_t held) { return static_cast<int>(ceil_div(held, 32 * kV) * 32); }
 
 // The groups of a launch's blocks, and their stages: as many groups as `most`
-// threads are that leave each `least`
-// stages beside `vectors` shared ones, and then as many stages as `flight` bytes
-// are.  Returns the blocks, 0 where not one stage fits.
+// threads are that leave each `least` stages beside `vectors` shared ones, and then
+// as many stages as `flight` bytes are.  Returns the blocks, 0 where not one stage
+// fits.
 int64_t plan_groups(const Rows& rows, int64_t held, int size, int inputs, int vectors, int vector_size, int most,
                     int least, int flight, Shape& shape, int* smem) {
   const int E = 16 / size;
   shape.threads = group_threads(held);
   shape.slot = static_cast<int>(ceil_div(held, E)) * 16;
   const int shared = vectors * shape.threads * kV * vector_size, stage = shape.slot * inputs;
-  const int64_t sms = sm_count() / rows.classes * rows.classes;
+  const int64_t sms = std::max(1, sm_count() / rows.classes) * rows.classes;  // (blocks: a multiple of the classes)
   // (15 named barriers; rows fewer than groups leave some without)
   int groups = std::min(most / shape.threads, shape.threads == 32 ? 32 : 15);
   groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, ceil_div(rows.M, sms))));

@@ -536,6 +536,7 @@ int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t
     if (!workspace || workspace_bytes < frag_layernorm_bwd_workspace_bytes(M, N)) return FRAG_ERR_WORKSPACE;
     if (!aligned16(workspace)) return FRAG_ERR_ALIGN;
   }
+  if (sm_count() <= 0) return FRAG_ERR_NO_DEVICE;
   const Vector wv = {w, wdtype == FRAG_DT_F32, aligned16(w)};
   float* ws = static_cast<float*>(workspace);
   if (dtype == FRAG_DT_F32)

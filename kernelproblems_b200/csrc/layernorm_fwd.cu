@@ -357,6 +357,7 @@ int frag_layernorm_fwd(const void* x, int64_t x_stride, const void* res, int64_t
       !whole(b, wdtype))
     return FRAG_ERR_ALIGN;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (sm_count() <= 0) return FRAG_ERR_NO_DEVICE;
   const Vector wv = {w, wdtype == FRAG_DT_F32, aligned16(w)}, bv = {b, wdtype == FRAG_DT_F32, aligned16(b)};
   if (dtype == FRAG_DT_F32)
     return forward<float>({static_cast<const float*>(x), static_cast<const float*>(res), static_cast<float*>(y),

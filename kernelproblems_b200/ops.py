@@ -1667,8 +1667,8 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
     b1, b2 = betas
     if not (0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError("betas must be in [0, 1)")
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError("eps must be finite and not negative")
+    if not (eps >= 2.0 ** -126 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and at least 2^-126, the least normal number of 32 bits")
     lr_t = step_t = None
     if isinstance(lr, torch.Tensor):
         lr_t, lr = lr, 0.0

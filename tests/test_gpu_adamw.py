@@ -215,15 +215,15 @@ def test_types_and_alignments(dtype, gdtype, state, shift, gap, gshift):
 
 @pytest.mark.parametrize("state", [F32, E4])
 @pytest.mark.parametrize("kw", [dict(step=1), dict(step=100000), dict(betas=(0.0, 0.0)), dict(betas=(0.0, 0.999)),
-                                dict(betas=(0.99, 0.5)), dict(lr=0.0), dict(lr=1.0, decay=0.5), dict(eps=1e-3),
+                                dict(betas=(0.99, 0.5)), dict(lr=0.0), dict(lr=1.0, decay=0.5), dict(eps=1e-3), dict(eps=2.0 ** -126),
                                 dict(skip=(0,)), dict(skip=(1, 2)), dict(skip=(0, 1, 2))])
 def test_constants_and_missing_gradients(state, kw):
     run_and_check([1000, 4096, 300], F32, BF, state, **kw)
 
 
 def test_a_large_tensor():
-    """Sizes past 2^31 bytes of each kind, and a tensor behind it."""
-    n = (1 << 29) + 1000
+    """Values past 2^31, and a tensor behind them."""
+    n = (1 << 31) + 1000
     p = torch.zeros(n, dtype=BF, device=DEV)
     q = torch.ones(300, dtype=BF, device=DEV)
     g = torch.zeros(n, dtype=BF, device=DEV)
@@ -445,7 +445,7 @@ def test_refusals():
            (TypeError, lambda: up([g[0], g[1].half()])), (ValueError, lambda: up([g[0], g[1].cpu()])),
            (ValueError, lambda: up([g[0], torch.empty(1000, device=DEV)[::2]])), (ValueError, lambda: up(step=0)),
            (ValueError, lambda: up(step=1.0)), (ValueError, lambda: up(lr=float("inf"))), (ValueError, lambda: up(betas=(1.0, 0.9))),
-           (ValueError, lambda: up(betas=(0.9, -0.1))), (ValueError, lambda: up(eps=-1.0)),
+           (ValueError, lambda: up(betas=(0.9, -0.1))), (ValueError, lambda: up(eps=-1.0)), (ValueError, lambda: up(eps=0.0)), (ValueError, lambda: up(eps=1e-40)),
            (TypeError, lambda: up(grad_scale=torch.ones((), dtype=torch.float64, device=DEV))),
            (ValueError, lambda: up(grad_scale=torch.ones(()))), (ValueError, lambda: up(grad_scale=torch.ones(2, device=DEV))),
            (TypeError, lambda: up(step=torch.ones((), device=DEV))),

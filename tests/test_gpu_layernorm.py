@@ -255,6 +255,22 @@ def test_gradient_against_differences(N):
         assert abs(diff - want) <= bound, f"{name}: {diff.item()} {want.item()} {bound.item()}"
 
 
+def test_values_past_2_31():
+    """The last rows lie beyond what 32 bits count."""
+    M, N = (1 << 18) + 5, 8192
+    x = torch.zeros(M, N, dtype=BF, device=DEV)
+    dy = torch.zeros(M, N, dtype=BF, device=DEV)
+    at = torch.tensor([0, 1, 262143, 262144, M - 1], device=DEV)
+    x[at], dy[at] = rand(5, N, seed=1, mean=0.5), rand(5, N, seed=2)
+    w = weight(N)
+    y, _, mean, rstd = ops.layernorm_fwd(x, w, None, EPS)
+    check_fwd(x[at], w, None, None, (y[at], None, mean[at], rstd[at]))
+    assert bool((y[2:1000] == 0).all()) and bool((y[-1000:-10] == 0).all())
+    del y
+    dx, dw, db = ops.layernorm_bwd(dy, x, mean, rstd, w)
+    check_bwd(dy[at], x[at], mean[at], rstd[at], w, None, (dx[at], dw, db))
+
+
 def test_streams_and_graphs():
     x, w, b, dy = rand(64, 4096, seed=1), weight(4096), rand(4096, seed=5), rand(64, 4096, seed=2)
     want = ops.layernorm_fwd(x, w, b)

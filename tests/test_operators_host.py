@@ -220,7 +220,7 @@ def test_lists_of_tensors_are_checked_on_the_host():
         return lib.frag_adamw_update(table, grads, codes, count, m, v, ms, vs, lr, None, b1, b2, eps, step, None, None, None)
     T = _lib.AdamWTensor
     assert adamw(count=-1) == 1 and adamw(grads=None) == 1 and adamw(b1=1.0) == 1 and adamw(b2=-0.1) == 1
-    assert adamw(eps=-1.0) == 1 and adamw(lr=float("nan")) == 1 and adamw(step=0) == 1 and adamw(ms=64) == 1
+    assert adamw(eps=-1.0) == 1 and adamw(eps=0.0) == 1 and adamw(eps=1e-39) == 1 and adamw(lr=float("nan")) == 1 and adamw(step=0) == 1 and adamw(ms=64) == 1
     assert adamw(m=None) == 1 and adamw(m=68) == 3 and adamw(codes=one(C.c_int32, 2)) == 1
     assert adamw(T(None, None, 10, 0, 1.0, 0.0, 1)) == 1 and adamw(T(64, None, -1, 0, 1.0, 0.0, 1)) == 1
     assert adamw(T(64, None, 10, 64, 1.0, 0.0, 1)) == 3 and adamw(T(66, None, 10, 0, 1.0, 0.0, 1)) == 3
@@ -258,3 +258,11 @@ def test_a_missing_binding_fails_loudly(tmp_path, monkeypatch):
     monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "libfrag.so")
     with pytest.raises(FileNotFoundError):
         _lib.binding()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no memory")
+@pytest.mark.parametrize("N", [64, 4096, 4097, 20000])
+def test_no_device_is_a_status(N):
+    lib = _lib.load()
+    assert lib.frag_layernorm_fwd(64, N, None, 0, None, None, 64, None, None, None, 8, N, 1e-5, 0, 0, None) == 6
+    assert lib.frag_layernorm_bwd(64, N, 64, N, 64, 64, None, None, 0, 64, None, None, 8, N, 0, 0, None, 0, None) == 6
