@@ -15,8 +15,9 @@
 // chip, so the kernel only has to keep enough loads in flight.  218 million values
 // in 9 tensors: fp32 throughout 888 us (6.9 TB/s, above a copy's 6.5 as more is read
 // than written), with a bf16 copy 960; fp32 parameters, bf16 gradients and copies,
-// states in 8 bits 520; bf16 with states in 8 bits 371 (5.9 TB/s), where 81% of the
-// issue slots are busy.  Off 16-byte boundaries 900, 746 and 634 (chunk_any).
+// states in 8 bits 524; bf16 with states in 8 bits 374 (5.9 TB/s), where 81% of the
+// issue slots are busy.  Off 16-byte boundaries 889, 616 and 503: shifts and the
+// warps' ends; loads and stores of single values took 900, 746 and 634.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -30,9 +31,12 @@ namespace {
 
 // A block takes one chunk, a thread eight values of it: twelve blocks an SM (40
 // registers) have 12 KB of bf16 values and their states in flight.  218 million
-// bf16 values with states in 8 bits: 371 us; blocks of 256 threads 379, of 512 463;
-// two chunks a thread 588 at four blocks of 256 an SM, 446 one.
-constexpr int kThreads = 128, kResident = 12;
+// bf16 values with states in 8 bits: 374 us; blocks of 256 threads 379, of 512 463;
+// two chunks a thread 588 at four blocks of 256 an SM, 446 one.  States in 32 bits:
+// nine blocks, where twelve spill off 16-byte boundaries (1003 us against 889, at
+// them 887 both); nine are slower with states in 8 (549 against 503 off them).
+constexpr int kThreads = 128;
+constexpr int resident(bool eight) { return eight ? 12 : 9; }
 constexpr int kGroup = 128;                // values of a scale
 constexpr int64_t kChunk = 8 * kThreads;  // values
 
@@ -131,23 +135,68 @@ __device__ __forceinline__ void set_value(T* p, float f) {
 }
 __device__ __forceinline__ float& part(float2& v, int i) { return i ? v.y : v.x; }
 
-// Eight neighbouring values as they lie in memory, from a 16-byte boundary.
-template <class T>
-struct Eight {
-  uint4 raw[sizeof(T) / 2];
-
-  // n of them (8 or more: all).  RO: nothing writes them in this launch.
-  template <bool RO>
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if (n >= 8) {
+// The first W of W + 4 words from `bytes` on (even, below 16; the same for a warp).
+template <int W>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[W + 4], int bytes) {
+  const int bits = 8 * (bytes & 2);
+  auto from = [&](int q) {
 #pragma unroll
-      for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q)
-        raw[q] = RO ? ld_stream(reinterpret_cast<const uint4*>(p) + q) : ld_plain(reinterpret_cast<const uint4*>(p) + q);
+    for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(w[i + q], w[i + q + 1], bits);
+  };
+  switch (bytes >> 2) {
+    case 0: from(0); break;
+    case 1: from(1); break;
+    case 2: from(2); break;
+    default: from(3);
+  }
+}
+
+// Eight neighbouring values as they lie in memory.  ANY: from any address, all else
+// from a 16-byte boundary.
+template <class T, bool ANY>
+struct Eight {
+  static constexpr int E = 16 / sizeof(T), K = 8 / E, W = 4 * K;  // values of a 16-byte chunk, chunks, words
+  uint4 raw[K], last;  // ANY: `last`, the chunk behind
+  int shift;           // ANY: bytes that raw begins before the values
+
+  static __device__ __forceinline__ int bytes_off(const T* p) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u);
+  }
+
+  // Asks for n of them (8 or more: all); settle() then makes them the values.  RO:
+  // nothing writes them in this launch.  ANY: the chunks that they lie in, whole,
+  // where those are the tensor's own (what neighbours write meanwhile is shifted
+  // out); `first`: the tensor's first values.
+  template <bool RO>
+  __device__ __forceinline__ void load(const T* p, int n, bool first) {
+    auto chunk = [](const T* a) {
+      return RO ? ld_stream(reinterpret_cast<const uint4*>(a)) : ld_plain(reinterpret_cast<const uint4*>(a));
+    };
+    shift = ANY ? bytes_off(p) : 0;
+    const int off = shift / static_cast<int>(sizeof(T));
+    if (!shift ? n >= 8 : !first && n >= 8 + E - off) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[k] = chunk(p - off + k * E);
+      if (ANY && shift) last = chunk(p - off + 8);
     } else {
       float2 f[4];
 #pragma unroll
       for (int i = 0; i < 8; ++i) part(f[i / 2], i & 1) = i < n ? value(p + i) : 0.f;
       set(f);
+      shift = 0;
+    }
+  }
+  __device__ __forceinline__ void settle() {
+    if constexpr (ANY) {
+      if (!shift) return;
+      uint32_t w[W + 4];
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = u4_word(raw[i / 4], i & 3);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[W + i] = u4_word(last, i);
+      shift_words<W>(w, shift);
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
     }
   }
   __device__ __forceinline__ float2 pair(int i) const {
@@ -165,17 +214,50 @@ struct Eight {
                             __float_as_uint(f[2 * q + 1].y));
     }
   }
+  // n of them; by whole warps, whose lanes' values lie one behind the other.  ANY: a
+  // chunk is written whole by the lane that has its last value, with the lane before's
+  // part of it; value by value where it reaches out of the warp's values.
   __device__ __forceinline__ void store(T* p, int n) const {
-    if (n >= 8) {
+    const int bytes = ANY ? bytes_off(p) : 0;
+    if (!ANY || !bytes) {
+      if (n >= 8) {
 #pragma unroll
-      for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q) st_global(reinterpret_cast<uint4*>(p) + q, raw[q]);
-    } else {
+        for (int k = 0; k < K; ++k) st_global(reinterpret_cast<uint4*>(p) + k, raw[k]);
+      } else {
+        store_some(p, n, 0xff);
+      }
+      return;
+    }
+    const int off = bytes / static_cast<int>(sizeof(T)), lane = threadIdx.x & 31;
+    uint32_t w[W + 4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) {
-          float2 f = pair(i / 2);
-          set_value(p + i, part(f, i & 1));
-        }
+    for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xffffffffu, u4_word(raw[K - 1], i), 1);
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[4 + i] = u4_word(raw[i / 4], i & 3);
+    shift_words<W>(w, 16 - bytes);
+    uint32_t single = 0;  // the values of chunks that are not written whole
+#pragma unroll
+    for (int k = 0; k <= K; ++k) {
+      // chunk k: values k E - off to (k + 1) E - off - 1; the last is the next lane's first
+      const bool whole = n >= (k + 1) * E - off && (k > 0 || lane > 0) && (k < K || lane < 31);
+      const int i = 4 * k % W;
+      if (whole && k < K) st_global(reinterpret_cast<uint4*>(p - off) + k, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+      if (!whole) single |= ((1u << E) - 1) << (k * E) >> off;
+    }
+    store_some(p, n, single);
+  }
+
+ private:
+  // Those of the first n (or 8) whose bit is set, one by one.
+  __device__ __forceinline__ void store_some(T* p, int n, uint32_t which) const {
+    which &= n >= 8 ? 0xffu : (1u << max(n, 0)) - 1;
+    if (!which) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!(which >> i & 1)) continue;
+      const uint32_t word = u4_word(raw[i / E], i % E * static_cast<int>(sizeof(T)) / 4);
+      if constexpr (sizeof(T) == 2) p[i] = static_cast<uint16_t>(i & 1 ? word >> 16 : word);
+      else p[i] = __uint_as_float(word);
     }
   }
 };
@@ -192,12 +274,11 @@ __device__ __forceinline__ void largest_pair(float& a, float& b) {
   b = second ? v : w;
 }
 
-// A chunk of a tensor whose pointers are 16-byte aligned: thread t has eight
-// neighbouring values, a group is 16 neighbouring lanes.  The states behind a
+// A chunk of a tensor: thread t has eight neighbouring values, a group is 16 neighbouring lanes.  The states behind a
 // tensor's end belong to its last group and stay zero (their p and g read as
 // zero), so they are moved whole.  `n`: the tensor's values from the chunk on.
-template <bool EIGHT, class P, class G>
-__device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
+template <bool EIGHT, bool ANY, class P, class G>
+__device__ __forceinline__ void chunk(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
   P* p0 = static_cast<P*>(e.p) + from;
   const G* g0 = static_cast<const G*>(e.g) + from;
   const int64_t st = e.state + from;
@@ -205,10 +286,10 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
   const int at = threadIdx.x * 8;
   if (at - (threadIdx.x & 31) * 8 >= n) return;  // the whole warp
   const bool in = at < held;
-  Eight<P> p;
-  Eight<G> g;
-  p.template load<false>(p0 + at, n - at);
-  g.template load<true>(g0 + at, n - at);
+  Eight<P, ANY> p;
+  Eight<G, ANY> g;
+  p.template load<false>(p0 + at, n - at, from + at == 0);
+  g.template load<true>(g0 + at, n - at, from + at == 0);
   float2 pv[4];
   if constexpr (EIGHT) {
     uint8_t *m0 = static_cast<uint8_t*>(s.m) + st, *v0 = static_cast<uint8_t*>(s.v) + st;
@@ -221,6 +302,8 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
       mb = ms[at / kGroup] * s.b1;
       vb = vs[at / kGroup];
     }
+    p.settle();
+    g.settle();
     float2 m[4], r[4];
     float mm = 0.f, rm = 0.f;
 #pragma unroll
@@ -254,9 +337,11 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
     }
   } else {
     float *m0 = static_cast<float*>(s.m) + st + at, *v0 = static_cast<float*>(s.v) + st + at;
-    Eight<float> m, v;
-    m.template load<false>(m0, in ? 8 : 0);
-    v.template load<false>(v0, in ? 8 : 0);
+    Eight<float, false> m, v;
+    m.template load<false>(m0, in ? 8 : 0, false);
+    v.template load<false>(v0, in ? 8 : 0, false);
+    p.settle();
+    g.settle();
     float2 mn[4], vn[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -275,89 +360,15 @@ __device__ __forceinline__ void chunk_aligned(const Entry& e, const Step& s, con
   p.set(pv);
   p.store(p0 + at, n - at);
   if (e.copy) {
-    Eight<uint16_t> c;
+    Eight<uint16_t, ANY> c;
     c.set(pv);
     c.store(e.copy + from + at, n - at);
   }
 }
 
-// The same where some pointer is not aligned: a warp takes a group of 128 at a
-// time, lane l every 32nd of them, in single accesses that a warp makes to
-// neighbouring addresses.
-template <bool EIGHT, class P, class G>
-__device__ __forceinline__ void chunk_any(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
-  P* p0 = static_cast<P*>(e.p) + from;
-  const G* g0 = static_cast<const G*>(e.g) + from;
-  const int64_t st = e.state + from;
-  const int lane = threadIdx.x & 31;
-#pragma unroll 1
-  for (int at = (threadIdx.x >> 5) * kGroup; at < n && at < kChunk; at += kThreads / 32 * kGroup) {
-    float pv[4], gv[4], mv[4], rv[4];
-    float mb = s.b1, vb = 1.f;
-    if (EIGHT) {
-      mb *= s.m_scale[(st + at) / kGroup];
-      vb = s.v_scale[(st + at) / kGroup];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = at + lane + 32 * i;
-      pv[i] = j < n ? value(p0 + j) : 0.f;
-      gv[i] = j < n ? value(g0 + j) : 0.f;
-      mv[i] = EIGHT ? e4m3x2_to_f2(static_cast<const uint8_t*>(s.m)[st + j]).x : static_cast<const float*>(s.m)[st + j];
-      rv[i] = EIGHT ? e4m3x2_to_f2(static_cast<const uint8_t*>(s.v)[st + j]).x : static_cast<const float*>(s.v)[st + j];
-    }
-    float2 m[2], v[2], r[2];
-    float mm = 0.f, rm = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 gi = __fmul2_rn(make_float2(gv[2 * i], gv[2 * i + 1]), twice(f.g));
-      m[i] = first_moment(make_float2(mv[2 * i], mv[2 * i + 1]), gi, mb, s);
-      const float2 x = __fmul2_rn(make_float2(rv[2 * i], rv[2 * i + 1]), twice(vb));
-      const float2 y = __fmul2_rn(x, twice(s.b2));
-      v[i] = second_moment(EIGHT ? __fmul2_rn(y, x) : y, gi, s);
-      r[i] = make_float2(root_of(v[i].x), root_of(v[i].y));
-      const float2 q = parameter(make_float2(pv[2 * i], pv[2 * i + 1]), m[i], r[i], f, s);
-      pv[2 * i] = q.x;
-      pv[2 * i + 1] = q.y;
-      mm = max_mag2(mm, m[i]);
-      rm = max_mag2(rm, r[i]);
-    }
-    float mi = 1.f, ri = 1.f;
-    if (EIGHT) {
-      const float mscale = state_scale(warp_max_mag(mm), mi), rscale = state_scale(warp_max_mag(rm), ri);
-      if (lane == 0) {
-        s.m_scale[(st + at) / kGroup] = mscale;
-        s.v_scale[(st + at) / kGroup] = rscale;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = at + lane + 32 * i;
-      if (j < n) {
-        set_value(p0 + j, pv[i]);
-        if (e.copy) set_value(e.copy + from + j, pv[i]);
-      }
-      const float mn = part(m[i / 2], i & 1), rn = part(r[i / 2], i & 1);
-      if (EIGHT) {
-        static_cast<uint8_t*>(s.m)[st + j] = to_fp8<false>(mn * mi);
-        static_cast<uint8_t*>(s.v)[st + j] = to_fp8<false>(at_least_smallest(rn, rn * ri));
-      } else {
-        static_cast<float*>(s.m)[st + j] = mn;
-        static_cast<float*>(s.v)[st + j] = part(v[i / 2], i & 1);
-      }
-    }
-  }
-}
-
-template <bool EIGHT, class P, class G>
-__device__ __forceinline__ void chunk(bool aligned, const Entry& e, const Step& s, const Factors& f, int64_t from) {
-  const int n = static_cast<int>(min(e.numel - from, kChunk));
-  if (aligned) chunk_aligned<EIGHT, P, G>(e, s, f, from, n);
-  else chunk_any<EIGHT, P, G>(e, s, f, from, n);
-}
-
 template <int CAP, bool EIGHT>
-__global__ void __launch_bounds__(kThreads, kResident) adamw(const __grid_constant__ List<CAP> L, const __grid_constant__ Step s) {
+__global__ void __launch_bounds__(kThreads, resident(EIGHT)) adamw(const __grid_constant__ List<CAP> L,
+                                                                   const __grid_constant__ Step s) {
   const int i = find_tensor(L.first, L.count, blockIdx.x);
   const Entry& e = L.t[i];
   const float lr = (s.lr_dev ? *s.lr_dev : s.lr) * e.lr_scale;
@@ -381,12 +392,16 @@ __global__ void __launch_bounds__(kThreads, kResident) adamw(const __grid_consta
   f.keep = fmaf(-lr, e.decay, 1.0f);
   f.rate = lr * c1;
   const int64_t from = static_cast<int64_t>(blockIdx.x - L.first[i]) * kChunk;
-  const bool aligned = L.kind[i] & 4;
-  switch (L.kind[i] & 3) {
-    case 0: chunk<EIGHT, uint16_t, uint16_t>(aligned, e, s, f, from); break;
-    case 1: chunk<EIGHT, float, uint16_t>(aligned, e, s, f, from); break;
-    case 2: chunk<EIGHT, uint16_t, float>(aligned, e, s, f, from); break;
-    default: chunk<EIGHT, float, float>(aligned, e, s, f, from);
+  const int n = static_cast<int>(min(e.numel - from, kChunk));
+  switch (L.kind[i]) {
+    case 0: chunk<EIGHT, true, uint16_t, uint16_t>(e, s, f, from, n); break;
+    case 1: chunk<EIGHT, true, float, uint16_t>(e, s, f, from, n); break;
+    case 2: chunk<EIGHT, true, uint16_t, float>(e, s, f, from, n); break;
+    case 3: chunk<EIGHT, true, float, float>(e, s, f, from, n); break;
+    case 4: chunk<EIGHT, false, uint16_t, uint16_t>(e, s, f, from, n); break;
+    case 5: chunk<EIGHT, false, float, uint16_t>(e, s, f, from, n); break;
+    case 6: chunk<EIGHT, false, uint16_t, float>(e, s, f, from, n); break;
+    default: chunk<EIGHT, false, float, float>(e, s, f, from, n);
   }
 }
 

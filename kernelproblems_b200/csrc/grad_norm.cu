@@ -5,13 +5,13 @@
 // word to leave everything as it is.
 //
 // One pass over the data.  Block b of G owns the chunks [b C / G, (b + 1) C / G)
-// of all tensors' C, so the order of the sums depends on sizes alone.  A thread
-// adds the 32 squares that it has of a chunk in 32 bits and everything beyond in
-// 64 (a long run of equal gradients would round the same way every time); a
-// second, one-block launch adds the blocks' sums and starts while the first ends.
+// of all tensors' C, so the order of the sums depends on sizes and alignment alone.
+// A thread adds the 32 squares that it has of a chunk in 32 bits and everything
+// beyond in 64 (a long run of equal gradients would round the same way every time);
+// a second, one-block launch adds the blocks' sums and starts while the first ends.
 //
 // Bound: HBM.  218 million values in 9 tensors: 75 us in bf16 (5.8 TB/s; 67 at a
-// copy's rate), 139 in fp32 (6.3); from addresses off 16 bytes 91 and 159.  Tensors
+// copy's rate), 139 in fp32 (6.3), from addresses off 16 bytes too.  Tensors
 // of a few thousand values are a chunk each, and the two launches' latency.
 #include <algorithm>
 #include <cmath>
@@ -100,8 +100,11 @@ __global__ void __launch_bounds__(kThreads) squares(const __grid_constant__ Norm
   int i = find_tensor(L.first, L.count, c);
   for (; c < end; ++c) {
     while (c >= L.first[i + 1]) ++i;
-    const int64_t from = static_cast<int64_t>(c - L.first[i]) * kChunk;
-    const int64_t n = min(kChunk, L.numel[i] - from);
+    // Chunks end at 16-byte boundaries: only a tensor's first and last have values
+    // beside them.
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(L.ptr[i]) & 15u) >> (L.f32[i] ? 2 : 1));
+    const int64_t at = static_cast<int64_t>(c - L.first[i]) * kChunk - off, from = max(at, static_cast<int64_t>(0));
+    const int64_t n = (c + 1 == L.first[i + 1] ? L.numel[i] : at + kChunk) - from;
     a += L.f32[i] ? chunk_squares(static_cast<const float*>(L.ptr[i]) + from, n)
                   : chunk_squares(static_cast<const uint16_t*>(L.ptr[i]) + from, n);
   }

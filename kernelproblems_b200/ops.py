@@ -1451,7 +1451,7 @@ def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor |
     without a look from the host.  Returns (norm, scale), fp32 tensors of no
     dimension:
 
-    norm   sqrt(sum of all squares), in an order that the sizes alone decide
+    norm   sqrt(sum of all squares), in an order that sizes and alignment alone decide
     scale  max_norm / max(norm, max_norm), which adamw_update takes as its
            grad_scale; NaN where norm is not finite (the update then changes
            nothing); None without max_norm

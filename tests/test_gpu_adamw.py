@@ -221,6 +221,17 @@ def test_constants_and_missing_gradients(state, kw):
     run_and_check([1000, 4096, 300], F32, BF, state, **kw)
 
 
+@pytest.mark.parametrize("state", [F32, E4])
+@pytest.mark.parametrize("shift", [1, 2, 3, 4, 5, 6, 7])
+def test_every_place_between_boundaries(shift, state):
+    """Ends of tensors, of a warp's 256 values and of a block's 1024 at every place
+    between two 16-byte boundaries, of parameters and gradients apart."""
+    sizes = [1, 7, 9, 255, 256, 257, 264, 511, 1023, 1024, 1025, 1288, 2048, 2055]
+    run_and_check(sizes, BF, BF, state, shift=shift, gap=16 - shift, gshift=8 - shift)
+    run_and_check(sizes, F32, BF, state, shift=shift, gap=shift, gshift=shift, copies=True)
+    run_and_check(sizes, BF, F32, state, shift=0, gap=8, gshift=shift)
+
+
 def test_a_large_tensor():
     """Values past 2^31, and a tensor behind them."""
     n = (1 << 31) + 1000
