@@ -15,9 +15,9 @@
 // chip, so the kernel only has to keep enough loads in flight.  218 million values
 // in 9 tensors: fp32 throughout 888 us (6.9 TB/s, above a copy's 6.5 as more is read
 // than written), with a bf16 copy 960; fp32 parameters, bf16 gradients and copies,
-// states in 8 bits 524; bf16 with states in 8 bits 374 (5.9 TB/s), where 81% of the
-// issue slots are busy.  Off 16-byte boundaries 889, 616 and 503: shifts and the
-// warps' ends; loads and stores of single values took 900, 746 and 634.
+// states in 8 bits 525; bf16 with states in 8 bits 397 (5.6 TB/s), where four fifths
+// of the issue slots are busy.  Off 16-byte boundaries 884, 624 and 523: shifts and
+// the warps' ends; loads and stores of single values took 900, 746 and 634.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -31,10 +31,10 @@ namespace {
 
 // A block takes one chunk, a thread eight values of it: twelve blocks an SM (40
 // registers) have 12 KB of bf16 values and their states in flight.  218 million
-// bf16 values with states in 8 bits: 374 us; blocks of 256 threads 379, of 512 463;
-// two chunks a thread 588 at four blocks of 256 an SM, 446 one.  States in 32 bits:
-// nine blocks, where twelve spill off 16-byte boundaries (1003 us against 889, at
-// them 887 both); nine are slower with states in 8 (549 against 503 off them).
+// bf16 values with states in 8 bits: 397 us; with ten blocks 510.  (Before the roots'
+// rounding 372; blocks of 256 threads 379, of 512 463; two chunks a thread 588 at four
+// blocks of 256 an SM, 446 one.)  States in 32 bits: nine blocks, where twelve spill
+// off 16-byte boundaries (1003 us against 884, at them 887 both).
 constexpr int kThreads = 128;
 constexpr int resident(bool eight) { return eight ? 12 : 9; }
 constexpr int kGroup = 128;                // values of a scale
@@ -82,18 +82,53 @@ struct Factors {
 
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 
-// m' of m = m_code m_scale, with b1s = beta1 m_scale (states in 32 bits: scale 1).
-__device__ __forceinline__ float2 first_moment(float2 m, float2 g, float b1s, const Step& s) {
-  return __ffma2_rn(m, twice(b1s), __fmul2_rn(g, twice(s.a1)));
+// A product that no sum is contracted with (which happens to __fmul2_rn's).
+__device__ __forceinline__ float2 product(float2 a, float2 b) { return __ffma2_rn(a, b, twice(0.f)); }
+// m' and v', each operation rounded by itself, as elementary 32-bit operations have
+// them, and roots rounded correctly below: states in 8 bits are then those of the
+// formula in 32 bits to the last bit.  (Contracted, one of 400000 codes is its
+// neighbour, a sixteenth off, and where |m| / r is large that shows in the next step.)
+__device__ __forceinline__ float2 first_moment(float2 m, float2 g, const Step& s) {
+  return __fadd2_rn(product(m, twice(s.b1)), product(g, twice(s.a1)));
 }
-// v' of a gradient and beta2 v.
-__device__ __forceinline__ float2 second_moment(float2 b2v, float2 g, const Step& s) {
-  return __ffma2_rn(__fmul2_rn(g, twice(s.a2)), g, b2v);
+__device__ __forceinline__ float2 second_moment(float2 v, float2 g, const Step& s) {
+  return __fadd2_rn(product(v, twice(s.b2)), product(product(g, twice(s.a2)), g));
 }
 __device__ __forceinline__ float root_of(float v) {
   float r;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+__device__ __forceinline__ float least_of(float a, float b, float c) {
+  float m;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// Square roots rounded to nearest: an approximate one, s = v y of y near 1 / sqrt(v),
+// and one step of Newton's iteration, s + (v - s^2) y / 2, with the residual exact
+// in an FMA; a thread with values that this does not hold for (0, what underflows,
+// infinity) takes all by themselves.  218 million bf16 values: 397 us, with all by
+// themselves 411, with an approximation's last bit 375.
+__device__ __forceinline__ void roots(const float2 (&v)[4], float2 (&r)[4]) {
+  float least = v[0].x, most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    least = least_of(least, v[i].x, v[i].y);
+    most = max_mag2(most, v[i]);
+  }
+  if (least >= 0x1p-96f && most <= 0x1p+120f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 y;
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v[i].x));
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v[i].y));
+      const float2 s = __fmul2_rn(v[i], y);
+      r[i] = __ffma2_rn(__ffma2_rn(make_float2(-s.x, -s.y), s, v[i]), __fmul2_rn(y, twice(0.5f)), s);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = make_float2(__fsqrt_rn(v[i].x), __fsqrt_rn(v[i].y));
+  }
 }
 __device__ __forceinline__ float inverse(float v) {
   float r;
@@ -117,7 +152,7 @@ __device__ __forceinline__ float2 e4m3x2_to_f2(uint32_t b) {
 __device__ __forceinline__ float state_scale(float most, float& inv) {
   float s = most * (1.0f / 448.0f);
   if (s < 1.17549435e-38f) s = most == 0.f ? 1.0f : 1.17549435e-38f;
-  inv = inverse(s);
+  inv = __frcp_rn(s);
   return s;
 }
 
@@ -262,16 +297,20 @@ struct Eight {
   }
 };
 
-// The largest of 16 neighbouring lanes' a and b.  After one exchange lanes without
-// bit 3 go on with a and the others with b, so that both take one shuffle a level.
-__device__ __forceinline__ void largest_pair(float& a, float& b) {
+// The scales of a group, 16 neighbouring lanes, by its lanes' largest first moments
+// and roots: 1 / scale of both, and the scale that the lane is for.  After one exchange
+// lanes without bit 3 go on with the moments and the others with the roots, so that
+// both take one shuffle a level and one division.
+__device__ __forceinline__ float group_scales(float m, float r, float& m_inv, float& r_inv) {
   const bool second = threadIdx.x & 8;
-  float v = max_mag(second ? b : a, __shfl_xor_sync(0xffffffffu, second ? a : b, 8));
+  float v = max_mag(second ? r : m, __shfl_xor_sync(0xffffffffu, second ? m : r, 8));
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) v = max_mag(v, __shfl_xor_sync(0xffffffffu, v, o));
-  const float w = __shfl_xor_sync(0xffffffffu, v, 8);
-  a = second ? w : v;
-  b = second ? v : w;
+  float inv;
+  const float scale = state_scale(v, inv), other = __shfl_xor_sync(0xffffffffu, inv, 8);
+  m_inv = second ? other : inv;
+  r_inv = second ? inv : other;
+  return scale;
 }
 
 // A chunk of a tensor: thread t has eight neighbouring values, a group is 16 neighbouring lanes.  The states behind a
@@ -299,27 +338,30 @@ __device__ __forceinline__ void chunk(const Entry& e, const Step& s, const Facto
     if (in) {
       mq = *reinterpret_cast<const uint2*>(m0 + at);
       vq = *reinterpret_cast<const uint2*>(v0 + at);
-      mb = ms[at / kGroup] * s.b1;
+      mb = ms[at / kGroup];
       vb = vs[at / kGroup];
     }
     p.settle();
     g.settle();
-    float2 m[4], r[4];
+    float2 m[4], v[4], r[4];
     float mm = 0.f, rm = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 gi = __fmul2_rn(g.pair(i), twice(f.g));
-      m[i] = first_moment(e4m3x2_to_f2((i < 2 ? mq.x : mq.y) >> (16 * (i & 1)) & 0xffff), gi, mb, s);
-      const float2 root = __fmul2_rn(e4m3x2_to_f2((i < 2 ? vq.x : vq.y) >> (16 * (i & 1)) & 0xffff), twice(vb));
-      const float2 v = second_moment(__fmul2_rn(__fmul2_rn(root, twice(s.b2)), root), gi, s);
-      r[i] = make_float2(root_of(v.x), root_of(v.y));
-      pv[i] = parameter(p.pair(i), m[i], r[i], f, s);
+      const float2 mo = e4m3x2_to_f2((i < 2 ? mq.x : mq.y) >> (16 * (i & 1)) & 0xffff);
+      const float2 ro = product(e4m3x2_to_f2((i < 2 ? vq.x : vq.y) >> (16 * (i & 1)) & 0xffff), twice(vb));
+      m[i] = first_moment(product(mo, twice(mb)), gi, s);
+      v[i] = second_moment(product(ro, ro), gi, s);
       mm = max_mag2(mm, m[i]);
+    }
+    roots(v, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pv[i] = parameter(p.pair(i), m[i], r[i], f, s);
       rm = max_mag2(rm, r[i]);
     }
-    largest_pair(mm, rm);
     float mi, ri;
-    const float mscale = state_scale(mm, mi), rscale = state_scale(rm, ri);
+    const float scale = group_scales(mm, rm, mi, ri);
     if (in) {
       uint32_t a[4], b[4];
 #pragma unroll
@@ -330,10 +372,7 @@ __device__ __forceinline__ void chunk(const Entry& e, const Step& s, const Facto
       }
       *reinterpret_cast<uint2*>(m0 + at) = make_uint2(a[0] | a[1] << 16, a[2] | a[3] << 16);
       *reinterpret_cast<uint2*>(v0 + at) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-      if ((threadIdx.x & 15) == 0) {
-        ms[at / kGroup] = mscale;
-        vs[at / kGroup] = rscale;
-      }
+      if ((threadIdx.x & 7) == 0) (threadIdx.x & 8 ? vs : ms)[at / kGroup] = scale;
     }
   } else {
     float *m0 = static_cast<float*>(s.m) + st + at, *v0 = static_cast<float*>(s.v) + st + at;
@@ -346,8 +385,8 @@ __device__ __forceinline__ void chunk(const Entry& e, const Step& s, const Facto
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 gi = __fmul2_rn(g.pair(i), twice(f.g));
-      mn[i] = first_moment(m.pair(i), gi, s.b1, s);
-      vn[i] = second_moment(__fmul2_rn(v.pair(i), twice(s.b2)), gi, s);
+      mn[i] = first_moment(m.pair(i), gi, s);
+      vn[i] = second_moment(v.pair(i), gi, s);
       pv[i] = parameter(p.pair(i), mn[i], make_float2(root_of(vn[i].x), root_of(vn[i].y)), f, s);
     }
     if (in) {

@@ -232,6 +232,38 @@ def test_every_place_between_boundaries(shift, state):
     run_and_check(sizes, BF, F32, state, shift=0, gap=8, gshift=shift)
 
 
+@pytest.mark.parametrize("shift", [0, 3])
+def test_states_in_8_bits_are_the_formulas_in_32(shift):
+    """Codes as elementary 32-bit operations give them, each rounded, over several
+    steps; their scales to one last place (the roots' step of Newton's iteration is
+    rounded to nearest but where 2^-21 of all arguments lie by a midpoint)."""
+    n, (b1, b2) = 300000, (0.9, 0.95)
+    (p,), _ = make([n], F32, 0, shift=shift)
+    s = ops.AdamWStates([p], dtype=E4)
+    pad = s.exp_avg.numel() - n
+    m = torch.zeros(n + pad, device=DEV).view(-1, 128)
+    r = torch.zeros_like(m)
+    for step in range(1, 5):
+        (g,), _ = make([n], BF, step, std=1e-3, shift=shift)
+        g = g * torch.exp(2 * torch.randn(n, device=DEV, generator=gen(step + 10))).bfloat16()
+        g[1000:3000] = 0
+        ops.adamw_update(s, [g], lr=1e-4, step=step, betas=(b1, b2))
+        g32 = torch.nn.functional.pad(g.float(), (0, pad)).view(-1, 128)
+        m = b1 * m + (1 - b1) * g32
+        r = torch.sqrt(b2 * (r * r) + (1 - b2) * g32 * g32)
+        held = []
+        for y, codes, scale in ((m, s.exp_avg, s.exp_avg_scale), (r, s.exp_avg_sq, s.exp_avg_sq_scale)):
+            most = y.abs().amax(-1)
+            want = torch.where(most > 0, (most * (1.0 / 448)).clamp_min(2.0 ** -126), 1.0)
+            q = y * (1.0 / want)[:, None]
+            q = torch.where(y > 0, q.clamp_min(2.0 ** -9), q) if y is r else q
+            q = q.clamp(-448, 448).to(E4)
+            assert torch.equal(q.view(-1).float(), codes.float())
+            assert ((scale - want).abs() <= 2.0 ** -23 * want).all()
+            held.append(codes.float().view(-1, 128) * scale[:, None])
+        m, r = held
+
+
 def test_a_large_tensor():
     """Values past 2^31, and a tensor behind them."""
     n = (1 << 31) + 1000
