@@ -15,8 +15,8 @@
 // chip, so the kernel only has to keep enough loads in flight.  218 million values
 // in 9 tensors: fp32 throughout 888 us (6.9 TB/s, above a copy's 6.5 as more is read
 // than written), with a bf16 copy 960; fp32 parameters, bf16 gradients and copies,
-// states in 8 bits 525; bf16 with states in 8 bits 397 (5.6 TB/s), where four fifths
-// of the issue slots are busy.  Off 16-byte boundaries 884, 624 and 523: shifts and
+// states in 8 bits 524; bf16 with states in 8 bits 395 (5.6 TB/s), where four fifths
+// of the issue slots are busy.  Off 16-byte boundaries 884, 627 and 519: shifts and
 // the warps' ends; loads and stores of single values took 900, 746 and 634.
 #include <cuda_fp8.h>
 
@@ -31,7 +31,7 @@ namespace {
 
 // A block takes one chunk, a thread eight values of it: twelve blocks an SM (40
 // registers) have 12 KB of bf16 values and their states in flight.  218 million
-// bf16 values with states in 8 bits: 397 us; with ten blocks 510.  (Before the roots'
+// bf16 values with states in 8 bits: 395 us; with ten blocks 510.  (Before the roots'
 // rounding 372; blocks of 256 threads 379, of 512 463; two chunks a thread 588 at four
 // blocks of 256 an SM, 446 one.)  States in 32 bits: nine blocks, where twelve spill
 // off 16-byte boundaries (1003 us against 884, at them 887 both).
@@ -106,9 +106,10 @@ __device__ __forceinline__ float least_of(float a, float b, float c) {
 }
 // Square roots rounded to nearest: an approximate one, s = v y of y near 1 / sqrt(v),
 // and one step of Newton's iteration, s + (v - s^2) y / 2, with the residual exact
-// in an FMA; a thread with values that this does not hold for (0, what underflows,
-// infinity) takes all by themselves.  218 million bf16 values: 397 us, with all by
-// themselves 411, with an approximation's last bit 375.
+// in an FMA.  A thread with values that this does not hold for (what underflows,
+// infinity, single zeros; not all zeros, as of rows that no gradient came by) takes
+// all by themselves.  218 million bf16 values: 395 us, with all by themselves 411,
+// with an approximation's last bit 375.
 __device__ __forceinline__ void roots(const float2 (&v)[4], float2 (&r)[4]) {
   float least = v[0].x, most = 0.f;
 #pragma unroll
@@ -116,12 +117,13 @@ __device__ __forceinline__ void roots(const float2 (&v)[4], float2 (&r)[4]) {
     least = least_of(least, v[i].x, v[i].y);
     most = max_mag2(most, v[i]);
   }
-  if (least >= 0x1p-96f && most <= 0x1p+120f) {
+  if ((least >= 0x1p-90f && most <= 0x1p+120f) || most == 0.f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 y;
-      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v[i].x));
-      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v[i].y));
+      const float2 a = __fadd2_rn(v[i], twice(0x1p-120f));  // (v itself, but of zeros)
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(a.x));
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(a.y));
       const float2 s = __fmul2_rn(v[i], y);
       r[i] = __ffma2_rn(__ffma2_rn(make_float2(-s.x, -s.y), s, v[i]), __fmul2_rn(y, twice(0.5f)), s);
     }

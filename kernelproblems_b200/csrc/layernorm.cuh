@@ -416,9 +416,9 @@ constexpr int lane_blocks(int V, Mode mode, int most) { return most - (V == 8 &&
 // Rows of up to so many values are a few lanes' (16 values a lane, what registers
 // hold beside weights and sums), and of up to so many a group's (512 threads of 32).
 // 65536 rows in bf16, us by lanes and by groups: of 512 27 and 42 (gradient 39 and
-// 56), of 300 36 and 58 (52 and 75); in fp32 of 512 48 and 50 (71 and 72).  Rows
-// above a group's: 4096 of 16001 83 (gradient 111); the kernels for any row read
-// 4096 of 20000 two and three times.
+// 56), of 300 36 and 58 (52 and 75); in fp32 of 512 48 and 50 (71 and 72).  4096 rows
+// of 16384 by groups 50 (gradient 81), of 20000 by the kernels for any row 200 (388);
+// 8192 of 4096 26 and 88 (41 and 139).
 constexpr int64_t kLanes = 512, kHeld = 16384;
 constexpr int kSmem = 232448;  // of an SM, for its blocks
 
