@@ -165,11 +165,6 @@ template <class T>
 __device__ __forceinline__ float value(const T* p) {
   return sizeof(T) == 2 ? bf16_to_f(*reinterpret_cast<const uint16_t*>(p)) : *reinterpret_cast<const float*>(p);
 }
-template <class T>
-__device__ __forceinline__ void set_value(T* p, float f) {
-  if (sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p) = f_to_bf16(f);
-  else *reinterpret_cast<float*>(p) = f;
-}
 __device__ __forceinline__ float& part(float2& v, int i) { return i ? v.y : v.x; }
 
 // The first W of W + 4 words from `bytes` on (even, below 16; the same for a warp).
@@ -315,9 +310,11 @@ __device__ __forceinline__ float group_scales(float m, float r, float& m_inv, fl
   return scale;
 }
 
-// A chunk of a tensor: thread t has eight neighbouring values, a group is 16 neighbouring lanes.  The states behind a
-// tensor's end belong to its last group and stay zero (their p and g read as
-// zero), so they are moved whole.  `n`: the tensor's values from the chunk on.
+// A chunk of a tensor: thread t has eight neighbouring values, a group is 16
+// neighbouring lanes.  ANY: parameters, gradients or copies off 16-byte boundaries
+// (states never are).  The states behind a tensor's end belong to its last group and
+// stay zero (their p and g read as zero), so they are moved whole.  `n`: the chunk's
+// values.
 template <bool EIGHT, bool ANY, class P, class G>
 __device__ __forceinline__ void chunk(const Entry& e, const Step& s, const Factors& f, int64_t from, int n) {
   P* p0 = static_cast<P*>(e.p) + from;
