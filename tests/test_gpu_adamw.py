@@ -264,6 +264,67 @@ def test_states_in_8_bits_are_the_formulas_in_32(shift):
         m, r = held
 
 
+def first_scales(g, r, betas):
+    """The scales of the roots that one step leaves of groups whose values are all
+    alike: gradient g, root r before.  A group's scale is its root times 1 / 448."""
+    grad = g[:, None].expand(-1, 128).reshape(-1).contiguous()
+    s = ops.AdamWStates([torch.zeros(grad.numel(), device=DEV)], dtype=E4)
+    s.exp_avg_sq.copy_(torch.full_like(s.exp_avg_sq, 256.0, dtype=F32))
+    s.exp_avg_sq_scale.copy_(r / 256)
+    ops.adamw_update(s, [grad], lr=1e-4, step=1, betas=betas)
+    return s.exp_avg_sq_scale
+
+
+def scales_of(v):
+    """sqrt(v) rounded to 32 bits once (a 64-bit root holds twice the digits and two
+    more, so rounding it again is rounding the root), times 1 / 448."""
+    s = v.double().sqrt().float() * (1.0 / 448)
+    return torch.where(v > 0, s.clamp_min(2.0 ** -126), 1.0)
+
+
+def test_roots_of_every_mantissa_are_rounded_to_nearest():
+    """All 2^24 numbers of two binades, the second moments v = a + 0.75 g^2 of a = r^2 / 4."""
+    b2 = 0.25
+    for lo in range(0, 1 << 24, 1 << 18):
+        at = torch.arange(lo, lo + (1 << 18), device=DEV)
+        v = ((at % (1 << 23)).float() * 2.0 ** -23 + 1) * (1.0 if lo < 1 << 23 else 2.0)
+        k = (16 * v.sqrt()).floor() - 1  # a = (k / 16)^2 is exact, and v - a at least 1 / 16
+        a, r = (k / 16).square(), k / 8
+        g = ((v.double() - a.double()) / (1 - b2)).sqrt().float()
+        for step in (1, -1, 2, -2, 3, -3):  # the gradient near it with which the rounded operations meet v
+            near = (g.view(torch.int32) + step).view(F32)
+            g = torch.where(a + (g * (1 - b2)) * g == v, g, torch.where(a + (near * (1 - b2)) * near == v, near, g))
+        assert bool((a + (g * (1 - b2)) * g == v).all())
+        assert torch.equal(first_scales(g, r, (0.9, b2)), scales_of(v))
+
+
+def test_roots_of_all_sizes_are_rounded_to_nearest():
+    """From what underflows to what overflows nearly; and of nothing."""
+    e = torch.rand(1 << 15, generator=gen(1), device=DEV) * 144 - 80
+    g = (1 + torch.rand(1 << 15, generator=gen(2), device=DEV)) * e.floor().exp2()
+    g[:100] = 0
+    want = scales_of((g * 0.5) * g)
+    assert torch.equal(first_scales(g, torch.zeros_like(g), (0.9, 0.5)), want) and bool((want == 1).any())
+
+
+@pytest.mark.parametrize("shift", [1, 3])
+def test_states_in_8_bits_of_shifted_gradients_are_the_aligned_ones(shift):
+    """Gradients, parameters and copies off 16-byte boundaries leave the same bits."""
+    sizes, held = [70001, 130, 4096], []
+    for by in (0, shift):
+        params, _ = make(sizes, F32, 0, shift=by, gap=by)
+        grads, _ = make(sizes, BF, 1, std=1e-3, shift=by, gap=by)
+        assert by == 0 or all(g.data_ptr() % 16 for g in grads)
+        copies, _ = make(sizes, BF, 2, shift=by, gap=by)
+        s = ops.AdamWStates(params, dtype=E4, copies=copies)
+        for step in range(1, 5):
+            for i, g in enumerate(grads):
+                g.mul_(torch.exp(torch.randn(g.shape, generator=gen(10 * step + i), device=DEV)).bfloat16())
+            ops.adamw_update(s, grads, lr=1e-3, step=step)
+        held.append([*params, *copies, s.exp_avg.float(), s.exp_avg_sq.float(), s.exp_avg_scale, s.exp_avg_sq_scale])
+    assert all(torch.equal(a, b) for a, b in zip(*held))
+
+
 def test_a_large_tensor():
     """Values past 2^31, and a tensor behind them."""
     n = (1 << 31) + 1000
