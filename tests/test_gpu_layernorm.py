@@ -271,6 +271,27 @@ def test_values_past_2_31():
     check_bwd(dy[at], x[at], mean[at], rstd[at], w, None, (dx[at], dw, db))
 
 
+@pytest.mark.parametrize("M,N,dtype,by", [(262144, 8192, F32, 0), (1 << 24, 64, F32, 0), (1 << 23, 96, BF, 0), (1 << 20, 64, F32, 1),
+                                          (1 << 20, 1000, BF, 0), (70000, 16000, BF, 0), (300000, 1001, F32, 0)])
+def test_long_sums_of_rows_that_are_alike(M, N, dtype, by):
+    """Every row the same, so that the roundings of a column's sum all go one way; over
+    hundreds and thousands of rows for a thread.  by: dy lies unlike x."""
+    x, w = rand(1, N, seed=1, mean=0.5, dtype=dtype), weight(N, dtype)
+    dy = rand(1, N, seed=3, dtype=dtype)
+    dy[0, 0], dy[0, 1] = 0.3, 0.1
+    one = lambda t: t.expand(M, N)  # noqa: E731
+    mean, rstd = stats(x)
+    dx, dw, db = ops.layernorm_bwd(one(shifted(dy, by) if by else dy), one(x), mean.expand(M).contiguous(),
+                                   rstd.expand(M).contiguous(), w)
+    assert all(torch.equal(dx[i], dx[0]) for i in (1, M // 2, M - 1))
+    del dx
+    term = dy[0].double()
+    within(db, M * term, REL * M * term.abs(), "db")
+    term = term * (x[0].double() - mean.double()) * rstd.double()
+    # (and each term's own two roundings)
+    within(dw, M * term, (REL + 2.0 ** -23) * M * term.abs(), "dw")
+
+
 def test_streams_and_graphs():
     x, w, b, dy = rand(64, 4096, seed=1), weight(4096), rand(4096, seed=5), rand(64, 4096, seed=2)
     want = ops.layernorm_fwd(x, w, b)
