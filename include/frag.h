@@ -575,8 +575,10 @@ FRAG_API int frag_muon_update(const frag_matrix* param, const frag_matrix* grad,
  * T (dtype): FRAG_DT_BF16 or FRAG_DT_F32, of x, res, h, y, dy, dres and dx alike;
  * w, b: [N] of wdtype, NULL for 1 and 0.  x, res, dy, dres: rows of N values
  * *_stride values apart; h, y, dx: dense [M,N].  mean, rstd: fp32 [M].  NULL: res,
- * h (only with res), mean and rstd of the forward, dres, dw, db.  A row's sums are
- * taken about its mean, so a mean far from zero costs no digits.  y and h may not
+ * h (only with res), mean and rstd of the forward, dres, dw, db.  Squares are
+ * taken about the mean, so a mean far from zero costs rstd none; the mean is one fp32
+ * number, rounded once where it is more than 8 deviations, so that y may be off by
+ * |mean| 2^-24 rstd w on top of its own roundings.  y and h may not
  * share memory with x or res, nor dx with dy, x or dres.  Workspace:
  * frag_layernorm_bwd_workspace_bytes(M, N), 16-byte aligned.  The reference's
  * graphs have RMSNorm only; these stand beside frag_rmsnorm_fwd and

@@ -56,6 +56,59 @@ __device__ __forceinline__ float row_squares(const Places<T, MODE>& at, int N, c
   return s.x + s.y;
 }
 
+// 1 / N as a number and what that leaves out, so that a quotient is rounded once: sum / N
+// is not off by a place where it is a number of 32 bits, as in a row of equal values.
+// (Of an infinity the quotient is NaN, as the row's outputs are; as_stored is what its mean
+// is.)  Bf16 rows without a residual pay for it: 32768 of 8192 174 us, by the product with
+// 1 / N alone 168.
+struct Count {
+  float inverse, rest;
+  __device__ __forceinline__ explicit Count(int N) {
+    inverse = 1.0f / static_cast<float>(N);
+    rest = fmaf(-inverse, static_cast<float>(N), 1.0f) * inverse;
+  }
+  __device__ __forceinline__ float mean(float sum) const { return fmaf(sum, inverse, sum * rest); }
+  __device__ __forceinline__ float as_stored(float mean, float sum) const {
+    return isfinite(mean) ? mean : sum * inverse;
+  }
+};
+
+// A mean that is many deviations is off by some of them if its sum is rounded: fp32 rows
+// of 1001 values 1000.3 had deviations of 1.2e-4 in place of none.  So an fp32 row whose
+// mean is more than 8 deviations adds up its distances from it, which have no digits to
+// lose, and the mean becomes the true one but for its own rounding.  (8192 rows of 1001:
+// 25 us, all of them far from zero 29; 32768 of 8192 332 both.)  The sum of bf16 values that
+// lie about a mean so far from zero is exact: 8 binary digits each and those of their
+// count, at most 15, are less than 24.
+template <class T>
+__device__ __forceinline__ bool far_from_zero(float mean, float var) {
+  return sizeof(T) == 4 && mean * mean > 64.f * var;
+}
+__device__ __forceinline__ void correct(float& mean, float& var, float distances, float squares, float invN) {
+  const float off = distances * invN;
+  var = fmaxf(fmaf(squares, invN, -off * off), 0.f);
+  mean += off;
+}
+// Sums of the distances from `mean`, and of their squares, of the values inside the row.
+template <class T, int V, Mode MODE>
+__device__ __forceinline__ float2 row_distances(const Places<T, MODE>& at, int N, const float2 (&v)[V / 2], float mean) {
+  float2 a = twice(0.f), s = a;
+#pragma unroll
+  for (int k = 0; k < V / kE<T>; ++k) {
+    if (!at[k].some(N)) continue;
+    float2 d[kP<T>];
+#pragma unroll
+    for (int q = 0; q < kP<T>; ++q) d[q] = __fadd2_rn(v[k * kP<T> + q], twice(-mean));
+    own_values<T, MODE>(at[k], N, 0.f, d);
+#pragma unroll
+    for (int q = 0; q < kP<T>; ++q) {
+      a = __fadd2_rn(a, d[q]);
+      s = __ffma2_rn(d[q], d[q], s);
+    }
+  }
+  return make_float2(a.x + a.y, s.x + s.y);
+}
+
 // A chunk of y.
 template <class T, Mode MODE>
 __device__ __forceinline__ void write_chunk(T* row, const Place<T, MODE>& at, int N, const float2* v, float mean,
@@ -71,8 +124,8 @@ __device__ __forceinline__ void write_chunk(T* row, const Place<T, MODE>& at, in
 // of lanes stay within a class, with the weights in registers; each thread keeps
 // its own chunks of the next rows in flight, kAhead of them, into its own places in
 // shared memory, so nothing has to be waited for but its own copies.  Issue bounds
-// them (two thirds of the slots): 262144 rows of 128 in bf16 26.6 us, 5.0 TB/s, of
-// a million 94, 5.7.  Odd widths (129: 77 us) pay
+// them (two thirds of the slots): 262144 rows of 128 in bf16 27.9 us, 4.8 TB/s, of
+// a million 98, 5.5.  Odd widths (129: 78 us) pay
 // for shifts, for masks, and at a row's ends for stores of single values.
 template <class T, int V, int L, Mode MODE, bool RES>
 __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const FwdP<T> p, const Rows rows) {
@@ -109,7 +162,8 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
     load_vector<T, MODE>(p.w, at[k], N, 1.f, w + k * P);
     load_vector<T, MODE>(p.b, at[k], N, 0.f, b + k * P);
   }
-  const float invN = 1.0f / static_cast<float>(N);
+  const Count count(N);
+  const float invN = count.inverse;
   int s = 0;
   T *y = p.y + row * p.N, *h = p.h + row * p.N;
   const int64_t jump = groups * p.N;
@@ -134,10 +188,20 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
       for (int q = 0; q < P; ++q) sum = __fadd2_rn(sum, v[k * P + q]);
       if (RES && p.h && in) store_chunk<T, MODE>(h, at[k], N, v + k * P);
     }
-    const float mean = lanes_sum<L>(sum.x + sum.y) * invN;
-    const float r = rsqrtf(fmaf(lanes_sum<L>(row_squares<T, V, MODE>(at, N, v, mean)), invN, p.eps));
+    const float all = lanes_sum<L>(sum.x + sum.y);
+    float mean = count.mean(all);
+    float var = lanes_sum<L>(row_squares<T, V, MODE>(at, N, v, mean)) * invN;
+    if constexpr (sizeof(T) == 4) {
+      const bool far = far_from_zero<T>(mean, var);
+      if (__any_sync(0xffffffffu, far)) {  // (shuffles are the whole warp's)
+        float2 d = row_distances<T, V, MODE>(at, N, v, mean);
+        d = make_float2(lanes_sum<L>(d.x), lanes_sum<L>(d.y));
+        if (far) correct(mean, var, d.x, d.y, invN);
+      }
+    }
+    const float r = rsqrtf(var + p.eps);
     if (!in) continue;
-    if (t == 0 && p.mean) p.mean[row] = mean;
+    if (t == 0 && p.mean) p.mean[row] = count.as_stored(mean, all);
     if (t == 0 && p.rstd) p.rstd[row] = r;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -173,7 +237,7 @@ constexpr int kFlight = 65536;
 // where two sums over the group, one after the other, would need two.
 //
 // Bound: HBM, beside some 5 us to start and to end.  In bf16 8192 rows of 4096 take
-// 26.2 us (5.1 TB/s) and 32768 of 8192 168 (6.4, 0.98 of a copy's rate), with the
+// 26.5 us (5.1 TB/s) and 32768 of 8192 174 (6.2, 0.94 of a copy's rate), with the
 // residual 46 and 335.  A block for each row, its weights read again from L2 each
 // time, took 382 for the last; 1024 threads with 64 registers
 // were slower too.
@@ -182,6 +246,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
   constexpr int P = kP<T>, V = kV, K = V / kE<T>, INPUTS = RES ? 2 : 1;
   extern __shared__ __align__(128) unsigned char smem[];  // w, b, the rings
   __shared__ float2 slots[2][32], counts[16];             // (sum, squares) and (n, 1 / n) of each warp
+  __shared__ float2 distances[32];                        // of each warp, where a row is far from zero
   __shared__ int s_abort[32];
   const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, nw = shape.threads >> 5;
   const Group g(shape.threads);
@@ -204,7 +269,8 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
   share_vector<T, W, MODE>(p.w, 1.f, w, apart, ring.off, N);
   share_vector<T, W, MODE>(p.b, 0.f, b, apart, ring.off, N);
   __syncthreads();
-  const float invN = 1.0f / static_cast<float>(N), inv_mine = counts[warp].y;
+  const Count count(N);
+  const float invN = count.inverse, inv_mine = counts[warp].y;
   const int first = g.index * nw;  // the group's slots
   int64_t row = ring.r0;
   int i = 0;
@@ -236,17 +302,26 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
     g.sync();
     if (s_abort[g.index]) break;
     if (g.t == 0) ring.issue();  // every thread has its values of this stage
-    float mean = ws * invN, var = wq * invN;
+    float all = ws, var = wq * invN;
     if (nw > 1) {  // (16 lanes take a warp each, the upper half the same again)
       const int of = lane & 15;
       const float2 o = of < nw ? slots[i & 1][first + of] : twice(0.f), n = of < nw ? counts[of] : twice(0.f);
-      mean = lanes_sum<16>(o.x) * invN;
-      const float d = fmaf(o.x, n.y, -mean);
+      all = lanes_sum<16>(o.x);
+      const float d = fmaf(o.x, n.y, -all * invN);
       var = lanes_sum<16>(fmaf(n.x * d, d, o.y)) * invN;
+    }
+    float mean = count.mean(all);
+    if (far_from_zero<T>(mean, var)) {  // (the whole group: its warps have the same sums)
+      const float2 d = warp_sum2(row_distances<T, V, MODE>(at, N, v, mean));
+      if (lane == 0) distances[first + warp] = d;
+      g.sync();
+      const int of = lane & 15;
+      const float2 o = of < nw ? distances[first + of] : twice(0.f);
+      correct(mean, var, lanes_sum<16>(o.x), lanes_sum<16>(o.y), invN);
     }
     const float r = rsqrtf(var + p.eps);
     if (g.t == 0) {
-      if (p.mean) p.mean[row] = mean;
+      if (p.mean) p.mean[row] = count.as_stored(mean, all);
       if (p.rstd) p.rstd[row] = r;
     }
 #pragma unroll
@@ -268,6 +343,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
 template <class T>
 __global__ void __launch_bounds__(256) fwd_any(const FwdP<T> p) {
   __shared__ float slots[2][32];
+  __shared__ float2 distances[1][32];
   const int64_t row = blockIdx.x;
   const T* x = p.x + row * p.xs;
   const T* res = p.res ? p.res + row * p.rs : nullptr;
@@ -278,13 +354,24 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdP<T> p) {
     if (p.h) put(p.h + row * p.N + n, v);
     s += v;
   }
-  const float mean = block_sum(s, slots, 0) / static_cast<float>(p.N);
+  float mean = block_sum(s, slots, 0) / static_cast<float>(p.N);
   s = 0.f;
   for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
     const float v = h(n) - mean;
     s = fmaf(v, v, s);
   }
-  const float r = rsqrtf(block_sum(s, slots, 1) / static_cast<float>(p.N) + p.eps);
+  float var = block_sum(s, slots, 1) / static_cast<float>(p.N);
+  if (far_from_zero<T>(mean, var)) {
+    float2 d = make_float2(0.f, 0.f);
+    for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
+      const float v = h(n) - mean;
+      d.x += v;
+      d.y = fmaf(v, v, d.y);
+    }
+    d = block_sum2(d, distances, 0);
+    correct(mean, var, d.x, d.y, 1.0f / static_cast<float>(p.N));
+  }
+  const float r = rsqrtf(var + p.eps);
   if (threadIdx.x == 0) {
     if (p.mean) p.mean[row] = mean;
     if (p.rstd) p.rstd[row] = r;

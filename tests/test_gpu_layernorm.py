@@ -13,6 +13,7 @@ EPS = 1e-5
 # A row's sums: up to 130 terms one after the other and a tree of ten levels, in
 # 32 bits: 140 * 2^-24, and a handful of single roundings behind them.
 REL = 1e-5
+U = 2.0 ** -24  # half a step of 32 bits
 
 
 def rand(*shape, seed=0, std=1.0, mean=0.0, dtype=BF):
@@ -236,6 +237,59 @@ def test_a_mean_far_from_zero(N):
     """A thousand deviations from zero: the deviations keep the digits that 32 bits leave them."""
     x = rand(40, N, seed=1, mean=1000.0, dtype=F32)
     check_fwd(x, weight(N, F32), None, None, ops.layernorm_fwd(x, weight(N, F32), None, EPS))
+
+
+FAR = [1, 3, 7, 64, 100, 129, 500, 1000, 1001, 4096, 4099, 8192, 12288, 16384, 20000]
+
+
+@pytest.mark.parametrize("N", FAR)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rows_of_one_value(N, dtype, residual):
+    """Any value, not whole numbers alone: the mean is that value, y the bias, to the last bit."""
+    values = torch.tensor([1000.3, -0.1, 3e-3, 12345.678, 0.0, -7e4], device=DEV)
+    x = values[:, None].expand(6, N).to(dtype).contiguous()
+    w, b = weight(N, dtype), rand(N, seed=5, dtype=dtype)
+    y, h, mean, rstd = ops.layernorm_fwd(x, w, b, EPS, residual=0.5 * x if residual else None)
+    h = h if residual else x
+    assert torch.equal(mean, h[:, 0].float())
+    assert torch.equal(y, b.expand(6, N))
+    # distances from a mean of some roundings, of the row and of parts of it
+    var = (4 * U * h[:, 0].double()).square() + 8 * U * (REL * h[:, 0].double()).square()
+    within(rstd, torch.full_like(var, EPS ** -0.5), EPS ** -0.5 * (var / EPS + 8 * U), "rstd")
+
+
+@pytest.mark.parametrize("N", FAR[3:])
+@pytest.mark.parametrize("far", [1e3, -1e4])
+def test_a_mean_far_from_zero_is_off_by_its_last_place(N, far):
+    x, w = rand(40, N, seed=1, mean=far, dtype=F32), weight(N, F32)
+    y, _, mean, rstd = ops.layernorm_fwd(x, w, None, EPS)
+    m64 = x.double().mean(-1)
+    d = x.double() - m64[:, None]
+    var = d.square().mean(-1)
+    r64 = (var + EPS).rsqrt()
+    # its own rounding; the distances' sums, of the deviations and of what the first mean is off by
+    off = U * m64.abs() * 1.001 + REL * (d.abs().mean(-1) + REL * m64.abs())
+    rel = REL + 8 * U * (REL * m64).square() / (var + EPS)
+    within(mean, m64, off, "mean")
+    within(rstd, r64, rel * r64, "rstd")
+    y64 = d * r64[:, None] * w.double()
+    slack = (off[:, None] + d.abs() * (rel + 4 * U)[:, None]) * r64[:, None] * w.double().abs()
+    within(y, y64, slack, "y")
+
+
+@pytest.mark.parametrize("N", FAR)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_mean_of_a_row_with_infinities(N, dtype):
+    """Is infinite, or not a number where two of them have two signs; the rows beside it are as they were."""
+    x = rand(4, N, seed=1, dtype=dtype)
+    clean = ops.layernorm_fwd(x, None, None, EPS)
+    x[1, N // 2], x[2, N - 1], x[2, 0] = float("inf"), float("-inf"), float("inf") if N > 1 else float("-inf")
+    y, _, mean, rstd = ops.layernorm_fwd(x, None, None, EPS)
+    assert mean[1] == float("inf") and (bool(torch.isnan(mean[2])) if N > 1 else mean[2] == float("-inf"))
+    assert bool(torch.isnan(y[1:3]).all()) and bool(torch.isnan(rstd[1:3]).all())
+    for i in (0, 3):
+        assert torch.equal(y[i], clean[0][i]) and mean[i] == clean[2][i] and rstd[i] == clean[3][i]
 
 
 @pytest.mark.parametrize("N", [48, 129, 1024, 2567])
