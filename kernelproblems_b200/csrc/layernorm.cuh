@@ -337,6 +337,8 @@ struct Ring {
         for (int n = last * E; n < ring.off + ring.N; ++n) own[n] = from[n];
       bulk_g2s(to + k * ring.slot + first * 16, from + first * E, (last - first) * 16, bar);
     }
+    // (the copy of a row S later goes over what was written here)
+    proxy_fence_shared();
     mbar_arrive(bar);
   }
   // Whether the window's first, or last, chunk is left out of the copy.

@@ -60,9 +60,8 @@ template <int N>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 template <int N>
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
-// Orders ordinary accesses and those of bulk copies; in shared memory only.
+// Orders ordinary accesses and those of bulk copies.
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
-__device__ __forceinline__ void proxy_fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, int columns) {

@@ -4,7 +4,7 @@ NaN, the gradient against the formula and against differences, refusals."""
 import pytest
 import torch
 
-from kernelproblems_b200 import ops
+from kernelproblems_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -344,6 +344,39 @@ def test_long_sums_of_rows_that_are_alike(M, N, dtype, by):
     term = term * (x[0].double() - mean.double()) * rstd.double()
     # (and each term's own two roundings)
     within(dw, M * term, (REL + 2.0 ** -23) * M * term.abs(), "dw")
+
+
+@pytest.mark.parametrize("N", [40, 129, 600, 1001, 2570, 4099, 8192, 16001])
+@pytest.mark.parametrize("by", [1, 3, 4])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_all_tensors_alike_off_a_boundary(N, by, dtype):
+    """The C ABI with outputs, too, `by` values behind a boundary.  The first row's begin and
+    the last one's end are then not copied but written into their place in the ring, which
+    the rows behind go over: the same, right results in several runs, and nothing beside them."""
+    M = 6000 if N < 2000 else 2500
+    code = _lib.FRAG_DT_BF16 if dtype == BF else _lib.FRAG_DT_F32
+    ptr = lambda t: t.data_ptr()  # noqa: E731
+    x, dy, w, b = rand(M, N, seed=1, mean=0.5, dtype=dtype), rand(M, N, seed=3, dtype=dtype), weight(N, dtype), rand(N, dtype=dtype)
+    xs, ds = shifted(x, by), shifted(dy, by)
+    mean, rstd = torch.empty(M, device=DEV), torch.empty(M, device=DEV)
+    dw, db = torch.empty(N, device=DEV), torch.empty(N, device=DEV)
+    need = _lib.load().frag_layernorm_bwd_workspace_bytes(M, N)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    held = []
+    for _ in range(10):
+        y, h, dx = (shifted(torch.zeros_like(x), by) for _ in range(3))
+        _lib.call("frag_layernorm_fwd", ptr(xs), N, ptr(ds), N, ptr(w), ptr(b), ptr(y), ptr(h), ptr(mean), ptr(rstd),
+                  M, N, EPS, code, code, torch.cuda.current_stream().cuda_stream)
+        _lib.call("frag_layernorm_bwd", ptr(ds), N, ptr(h), N, ptr(mean), ptr(rstd), ptr(w), ptr(xs), N, ptr(dx),
+                  ptr(dw), ptr(db), M, N, code, code, ptr(ws), need, torch.cuda.current_stream().cuda_stream)
+        for t in (y, h, dx):
+            around = t.view(-1).as_strided((t.numel() + by + 8,), (1,), 0)
+            assert not bool(around[:by].any()) and not bool(around[by + t.numel():].any())
+        held.append([t.clone() for t in (y, h, mean, rstd, dx, dw, db)])
+    y, h, mean, rstd, dx, dw, db = held[0]
+    check_fwd(x, w, b, dy, (y, h, mean, rstd))
+    check_bwd(dy, h, mean, rstd, w, x, (dx, dw, db))
+    assert all(torch.equal(a, c) for again in held[1:] for a, c in zip(held[0], again))
 
 
 def test_streams_and_graphs():
