@@ -270,6 +270,19 @@ struct Group {
   }
 };
 
+// Whether a thread of a group gave up its wait for row i.  All of them leave the loop at
+// the same row, behind its barrier: a flag of its own for every other row, as one that is
+// already at the next row's wait (and gives up there) must not be heard at this one.  The
+// others would go, and it would wait at its barrier for good.
+struct Gave {
+  int flags[2][32];
+  __device__ __forceinline__ void begin(const Group& g) { flags[0][g.index] = flags[1][g.index] = 0; }
+  __device__ __forceinline__ void up(const Group& g, int i) { flags[i & 1][g.index] = 1; }
+  __device__ __forceinline__ bool is_up(const Group& g, int i) const {
+    return *static_cast<const volatile int*>(&flags[i & 1][g.index]);
+  }
+};
+
 template <class T, int INPUTS, Mode MODE>
 struct Ring {
   unsigned char* smem;

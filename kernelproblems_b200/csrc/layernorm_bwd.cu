@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) unsigned char smem[];  // w, the rings; at the end dw, db
   __shared__ float slots[2][16][2];
-  __shared__ int s_abort[16];
+  __shared__ Gave gave;
   const int N = static_cast<int>(p.N);
   const Group g(shape.threads);
   const int apart = shape.threads * V;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
   deal(ring, rows, shape, g.index, smem + sizeof(W) * apart, N);
   const Places<T, MODE> at = {g.t, g.threads, ring.off};
   if (g.t == 0) {
-    s_abort[g.index] = 0;
+    gave.begin(g);
     ring.begin();
     // A stage is free again when every thread is in the next row: S - 1 rows ahead.
     for (int i = 0; i < max(1, ring.S - 1); ++i) ring.issue();
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
   const int first = g.index * (g.threads >> 5);
   int i = 0;
   for (; i < ring.count; ++i, row += ring.step) {
-    if (!ring.wait(err)) s_abort[g.index] = 1;
+    if (!ring.wait(err)) gave.up(g, i);
     // A chunk's dy, x and weights.
     auto take = [&](int k, float2* d, float2* x, float2* wk) {
       const int c = g.t + k * g.threads;
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
       chunk_sums<T>(d, x, wk, mean, s1, s2);
     }
     const float2 tot = group_pair(g, s1.x + s1.y, s2.x + s2.y, slots[i & 1], first);
-    if (s_abort[g.index]) break;
+    if (gave.is_up(g, i)) break;
     if (g.t == 0 && ring.S > 1) ring.issue();
     const RowTerms terms(rstd, tot.x, tot.y, invN);
     float next_mean = 0.f, next_rstd = 0.f;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(512) bwd_groups(const BwdP<T> p, const Rows ro
     }
     ring.next();
   }
-  if (g.t == 0 && s_abort[g.index]) ring.drain(i);
+  if (g.t == 0 && i < ring.count) ring.drain(i);
   if (!p.want_dw && !p.want_db) return;
   float* to = p.partials + static_cast<int64_t>(blockIdx.x) * (p.want_dw + p.want_db) * p.width;
   float* to_db = to + (p.want_dw ? p.width : 0);

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
   extern __shared__ __align__(128) unsigned char smem[];  // w, b, the rings
   __shared__ float2 slots[2][32], counts[16];             // (sum, squares) and (n, 1 / n) of each warp
   __shared__ float2 distances[32];                        // of each warp, where a row is far from zero
-  __shared__ int s_abort[32];
+  __shared__ Gave gave;
   const int N = static_cast<int>(p.N), lane = threadIdx.x & 31, nw = shape.threads >> 5;
   const Group g(shape.threads);
   const int apart = shape.threads * V, warp = g.t >> 5;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
   deal(ring, rows, shape, g.index, smem + 2 * sizeof(W) * apart, N);
   const Places<T, MODE> at = {g.t, g.threads, ring.off};
   if (g.t == 0) {
-    s_abort[g.index] = 0;
+    gave.begin(g);
     ring.begin();
     for (int i = 0; i < ring.S; ++i) ring.issue();
   }
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
   int64_t row = ring.r0;
   int i = 0;
   for (; i < ring.count; ++i, row += ring.step) {
-    if (!ring.wait(err)) s_abort[g.index] = 1;
+    if (!ring.wait(err)) gave.up(g, i);
     float2 v[V / 2], sum = twice(0.f), sum2 = sum;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
     const float wq = warp_sum(row_squares<T, V, MODE>(at, N, v, ws * inv_mine));
     if (lane == 0) slots[i & 1][first + warp] = make_float2(ws, wq);
     g.sync();
-    if (s_abort[g.index]) break;
+    if (gave.is_up(g, i)) break;
     if (g.t == 0) ring.issue();  // every thread has its values of this stage
     float all = ws, var = wq * invN;
     if (nw > 1) {  // (16 lanes take a warp each, the upper half the same again)
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
     }
     ring.next();
   }
-  if (g.t == 0 && s_abort[g.index]) ring.drain(i);
+  if (g.t == 0 && i < ring.count) ring.drain(i);
 }
 
 // Any width, any alignment (rows above 16384 values, or tensors whose rows begin at
