@@ -233,7 +233,9 @@ def binding():
     lib = load()
     with _lock:
         if _binding is None:
-            path = LIB_PATH.with_name("_binding.so")
+            from ._build import binding_name
+
+            path = LIB_PATH.with_name(binding_name())
             if not path.exists():
                 raise FileNotFoundError(f"{path} is missing: build it with `python -m kernelproblems_b200._build`")
             import importlib.util

@@ -1,11 +1,14 @@
 """RopeFrequencies on the CPU: the scaling rules at their ends, and refusals."""
 import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
-from kernelproblems_b200 import _lib, ops
+from kernelproblems_b200 import _build, _lib, ops
 
 
 def freq(plan):
@@ -258,6 +261,44 @@ def test_a_missing_binding_fails_loudly(tmp_path, monkeypatch):
     monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "libfrag.so")
     with pytest.raises(FileNotFoundError):
         _lib.binding()
+
+
+def test_the_binding_is_of_this_torch_and_python():
+    path = _lib.LIB_PATH.with_name(_build.binding_name())
+    assert path.exists() and torch.__version__ in path.name and f"{sys.version_info.major}{sys.version_info.minor}" in path.name
+    assert _lib.binding().__file__ == str(path)
+
+
+@pytest.fixture
+def build_in(tmp_path, monkeypatch):
+    """_build with its files under tmp_path and a compiler that only makes them."""
+    made = []
+
+    def run(cmd, **kw):
+        out = Path(cmd[cmd.index("-o") + 1])
+        out.write_text("")
+        made.append(out.name)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(_build, "BUILD_DIR", tmp_path / "objects")
+    monkeypatch.setattr(_build, "LIB_PATH", tmp_path / "libfrag.so")
+    monkeypatch.setattr(_build, "nvcc", lambda: "nvcc")
+    monkeypatch.setattr(_build.subprocess, "run", run)
+    return made
+
+
+def test_the_library_is_linked_where_the_binding_does_not_build(build_in, monkeypatch):
+    def fails(*a):
+        raise RuntimeError("no host compiler that fits")
+    monkeypatch.setattr(_build, "build_binding", fails)
+    with pytest.raises(RuntimeError, match="that fits"):
+        _build.build()
+    assert _build.LIB_PATH.exists() and "adamw.o" in build_in
+
+
+def test_the_library_is_built_without_torch(build_in, monkeypatch):
+    monkeypatch.setattr(_build.importlib.util, "find_spec", lambda name: None)
+    monkeypatch.setattr(_build, "build_binding", lambda *a: pytest.fail("torch is not there"))
+    assert _build.build() == _build.LIB_PATH and _build.LIB_PATH.exists()
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no memory")
