@@ -40,12 +40,12 @@ struct Entries {
 } entries;
 
 // A plain torch.Tensor (or Parameter) on the current device, contiguous, holding
-// its values as they are.
+// its values as they are (and holding them: what a function transform wraps does not).
 const at::Tensor* plain(PyObject* o, int device) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() ||
-      t.is_neg() || t.is_conj())
+  if (!t.defined() || !t.has_storage() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device ||
+      !t.is_contiguous() || t.is_neg() || t.is_conj())
     return nullptr;
   return &t;
 }
@@ -54,7 +54,7 @@ const at::Tensor* plain(PyObject* o, int device) {
 int device_of(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return -1;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || !t.is_cuda() || t.get_device() != c10::cuda::current_device()) return -1;
+  if (!t.defined() || !t.has_storage() || !t.is_cuda() || t.get_device() != c10::cuda::current_device()) return -1;
   return t.get_device();
 }
 int code(const at::Tensor& t) {
@@ -88,6 +88,8 @@ PyObject* tuple(const Ts&... ts) {
   }
   return out;
 }
+// (Pointers are asked for ahead of a call without the interpreter's lock: an exception
+// may not leave that.)
 void* data(const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const void* given(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 frag_stream_t stream_of(int device) {
@@ -131,11 +133,15 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     mean = like(*x, rows, at::kFloat);
     rstd = like(*x, rows, at::kFloat);
   }
+  const void *xp = x->const_data_ptr(), *rp = res ? res->const_data_ptr() : nullptr, *wp = given(w), *bp = given(b);
+  void *yp = data(y), *hp = data(h);
+  float *mp = static_cast<float*>(data(mean)), *sp = static_cast<float*>(data(rstd));
+  const int dtype = code(*x);
+  const frag_stream_t stream = stream_of(device);
   int st;
   Py_BEGIN_ALLOW_THREADS
-  st = entries.layernorm_fwd(x->const_data_ptr(), N, res ? res->const_data_ptr() : nullptr, N, given(w), given(b),
-                             data(y), data(h), static_cast<float*>(data(mean)), static_cast<float*>(data(rstd)), M, N,
-                             static_cast<float>(eps), code(*x), type < 0 ? FRAG_DT_F32 : type, stream_of(device));
+  st = entries.layernorm_fwd(xp, N, rp, N, wp, bp, yp, hp, mp, sp, M, N, static_cast<float>(eps), dtype,
+                             type < 0 ? FRAG_DT_F32 : type, stream);
   Py_END_ALLOW_THREADS
   return st ? PyLong_FromLong(st) : tuple(y, h, mean, rstd);
   END_HANDLE_TH_ERRORS
@@ -172,14 +178,18 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     bytes = entries.layernorm_bwd_workspace(M, N);
     ws = like(*x, {static_cast<int64_t>(bytes)}, at::kByte);
   }
+  const void *yp = dy->const_data_ptr(), *xp = x->const_data_ptr(), *wp = given(w),
+             *rp = dres ? dres->const_data_ptr() : nullptr;
+  const float *mp = static_cast<const float*>(mean->const_data_ptr()),
+              *sp = static_cast<const float*>(rstd->const_data_ptr());
+  void *dxp = data(dx), *wsp = data(ws);
+  float *dwp = static_cast<float*>(data(dw)), *dbp = static_cast<float*>(data(db));
+  const int dtype = code(*x);
+  const frag_stream_t stream = stream_of(device);
   int st;
   Py_BEGIN_ALLOW_THREADS
-  st = entries.layernorm_bwd(dy->const_data_ptr(), N, x->const_data_ptr(), N,
-                             static_cast<const float*>(mean->const_data_ptr()),
-                             static_cast<const float*>(rstd->const_data_ptr()), given(w),
-                             dres ? dres->const_data_ptr() : nullptr, N, data(dx), static_cast<float*>(data(dw)),
-                             static_cast<float*>(data(db)), M, N, code(*x), type < 0 ? FRAG_DT_F32 : type, data(ws),
-                             bytes, stream_of(device));
+  st = entries.layernorm_bwd(yp, N, xp, N, mp, sp, wp, rp, N, dxp, dwp, dbp, M, N, dtype, type < 0 ? FRAG_DT_F32 : type,
+                             wsp, bytes, stream);
   Py_END_ALLOW_THREADS
   return st ? PyLong_FromLong(st) : tuple(dx, dw, db);
   END_HANDLE_TH_ERRORS
@@ -231,11 +241,13 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!absent(a[1])) scale = like(*one, {}, at::kFloat);
   const int64_t bytes = static_cast<int64_t>(entries.grad_norm_workspace(ptrs.size()));
   const at::Tensor ws = like(norm, {bytes}, at::kByte);
+  float *np = static_cast<float*>(data(norm)), *sp = static_cast<float*>(data(scale));
+  void* wsp = data(ws);
+  const frag_stream_t stream = stream_of(device);
   int st;
   Py_BEGIN_ALLOW_THREADS
-  st = entries.grad_norm(ptrs.data(), numel.data(), codes.data(), ptrs.size(), static_cast<float>(top),
-                         static_cast<float*>(data(norm)), static_cast<float*>(data(scale)), data(ws), bytes,
-                         stream_of(device));
+  st = entries.grad_norm(ptrs.data(), numel.data(), codes.data(), ptrs.size(), static_cast<float>(top), np, sp, wsp,
+                         bytes, stream);
   Py_END_ALLOW_THREADS
   return st ? PyLong_FromLong(st) : tuple(norm, scale);
   END_HANDLE_TH_ERRORS
@@ -298,11 +310,12 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (word(a[12], device, at::kFloat, &lr_p) < 0 || word(a[17], device, at::kLong, &step_p) < 0 ||
       word(a[18], device, at::kFloat, &scale_p) < 0)
     Py_RETURN_NONE;
+  const frag_stream_t stream = stream_of(device);
   int st;
   Py_BEGIN_ALLOW_THREADS
   st = entries.adamw(table, ptrs.data(), codes.data(), count, held[0], held[1], static_cast<float*>(held[2]),
                      static_cast<float*>(held[3]), lr, static_cast<const float*>(lr_p), b1, b2, eps, step,
-                     static_cast<const int64_t*>(step_p), static_cast<const float*>(scale_p), stream_of(device));
+                     static_cast<const int64_t*>(step_p), static_cast<const float*>(scale_p), stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(st);
   END_HANDLE_TH_ERRORS

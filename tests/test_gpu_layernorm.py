@@ -414,6 +414,22 @@ def test_workspace():
         assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("N", [64, 4096])
+def test_tensors_that_hold_no_values_are_refused(N):
+    """What torch.func's transforms hand on has no memory of its own: an error, and the next call is as ever."""
+    x, w = rand(4, N, seed=1), weight(N)
+    want = ops.layernorm_fwd(x, w)
+    for call in (lambda: torch.func.grad(lambda t: ops.layernorm_fwd(t, w)[0].float().sum())(x),
+                 lambda: torch.func.vmap(lambda t: ops.layernorm_fwd(t, w)[0])(x[None]),
+                 lambda: torch.func.grad(lambda t: ops.layernorm_fwd(x, t)[0].float().sum())(w),
+                 lambda: torch.func.grad(lambda t: ops.layernorm_fwd(x, w, residual=t)[0].float().sum())(x),
+                 lambda: torch.func.vmap(lambda t: ops.layernorm_bwd(t, x, want[2], want[3], w)[0])(x[None]),
+                 lambda: torch.func.grad(lambda t: ops.grad_norm([x, t])[0])(x)):
+        with pytest.raises(RuntimeError):
+            call()
+        assert torch.equal(ops.layernorm_fwd(x, w)[0], want[0])
+
+
 def test_refusals():
     x, w = rand(4, 64), weight(64)
     mean, rstd = stats(x)
