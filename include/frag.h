@@ -626,8 +626,8 @@ FRAG_API int frag_grad_norm(const void* const* grads, const int64_t* numel, cons
  * where all are zero), and what is not zero of sqrt(v) stays at least 2^-9 scale.
  * eps >= 2^-126.  step counts from 1; step_device, lr_device (device words) replace step and lr
  * when given, for steps that are captured once and replayed.  With a grad_scale
- * (device word, or NULL) or a device lr that is not finite, or a device step below
- * 1, nothing is changed.  No counterpart in the reference.
+ * (device word, or NULL) or a device lr (times lr_scale) that is not finite, or a device
+ * step below 1, nothing is changed; an lr of the host's that is not is refused.  No counterpart in the reference.
  * ------------------------------------------------------------------------- */
 typedef struct frag_adamw_tensor {
   void* param;

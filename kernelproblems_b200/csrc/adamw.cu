@@ -496,7 +496,8 @@ int frag_adamw_update(const frag_adamw_tensor* tensors, const void* const* grads
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return FRAG_ERR_INVALID_ARG;
   // (a normal number in 32 bits: the reciprocal takes what lies below for 0)
   if (!std::isfinite(eps) || eps < 0x1p-126) return FRAG_ERR_INVALID_ARG;
-  if (!lr_device && !std::isfinite(lr)) return FRAG_ERR_INVALID_ARG;
+  // (in 32 bits, as the kernel takes it: there a rate that is not finite changes nothing)
+  if (!lr_device && !std::isfinite(static_cast<float>(lr))) return FRAG_ERR_INVALID_ARG;
   if (!step_device && step < 1) return FRAG_ERR_INVALID_ARG;
   const bool eight = exp_avg_scale != nullptr;
   if (eight != (exp_avg_sq_scale != nullptr)) return FRAG_ERR_INVALID_ARG;
@@ -508,6 +509,7 @@ int frag_adamw_update(const frag_adamw_tensor* tensors, const void* const* grads
         (grad_dtypes[i] != FRAG_DT_BF16 && grad_dtypes[i] != FRAG_DT_F32))
       return FRAG_ERR_INVALID_ARG;
     if (!std::isfinite(t.lr_scale) || !std::isfinite(t.weight_decay)) return FRAG_ERR_INVALID_ARG;
+    if (!lr_device && !std::isfinite(static_cast<float>(lr) * t.lr_scale)) return FRAG_ERR_INVALID_ARG;
     if (t.state_offset % kGroup) return FRAG_ERR_ALIGN;
     if (reinterpret_cast<uintptr_t>(t.param) % (t.param_dtype == FRAG_DT_F32 ? 4 : 2) ||
         reinterpret_cast<uintptr_t>(grads[i]) % (grad_dtypes[i] == FRAG_DT_F32 ? 4 : 2) ||

@@ -1481,12 +1481,17 @@ def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor |
     return norm, scale
 
 
+def _finite(v: float) -> bool:
+    """Whether a number is finite in 32 bits."""
+    return math.isfinite(C.c_float(v).value)
+
+
 def _each(v, n: int, name: str) -> list[float]:
     values = [float(v)] * n if isinstance(v, (int, float)) else [float(x) for x in v]
     if len(values) != n:
         raise ValueError(f"{name}: {len(values)} values for {n} tensors")
-    if not all(map(math.isfinite, values)):
-        raise ValueError(f"{name} must be finite")
+    if not all(map(_finite, values)):
+        raise ValueError(f"{name} must be finite, in 32 bits")
     return values
 
 
@@ -1529,6 +1534,7 @@ class AdamWStates:
         if dtype not in (torch.float32, torch.float8_e4m3fn):
             raise TypeError("dtype must be float32 or float8_e4m3fn")
         decay, lr_scale = _each(weight_decay, n, "weight_decay"), _each(lr_scale, n, "lr_scale")
+        self._most_scale = max(1.0, *map(abs, lr_scale))
         self.device = _dense_list(self.params, "params")
         self.copies = (None,) * n if copies is None else tuple(copies)
         if len(self.copies) != n:
@@ -1652,8 +1658,8 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
                 are what they were at capture)
     grad_scale  one-element fp32 CUDA tensor (grad_norm's scale), or None
 
-    Where grad_scale or a device lr is not finite, or a device step below 1, nothing
-    is changed.  Parameters are rounded to nearest: bf16 ones do not move by less than
+    Where grad_scale or a device lr is not finite (times a tensor's lr_scale, in 32 bits), or
+    a device step below 1, nothing is changed.  Parameters are rounded to nearest: bf16 ones do not move by less than
     2^-9 of their value, for which there are fp32 parameters with bf16 copies.  With
     states in 8 bits a gradient that is not finite makes its whole group of 128 NaN.
     Gradients must not share memory with parameters, copies or states."""
@@ -1672,8 +1678,8 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
     lr_t = step_t = None
     if isinstance(lr, torch.Tensor):
         lr_t, lr = lr, 0.0
-    elif not math.isfinite(lr):
-        raise ValueError("lr must be finite")
+    elif not _finite(lr * states._most_scale):
+        raise ValueError("lr must be finite, in 32 bits and times every lr_scale")
     if isinstance(step, torch.Tensor):
         step_t, step = step, 0
     elif not isinstance(step, int) or step < 1:

@@ -532,6 +532,22 @@ def test_norm_on_other_streams():
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
 
 
+def test_rates_beyond_32_bits_are_refused():
+    p, _ = make([300, 500], F32, 0)
+    g, _ = make([300, 500], F32, 1)
+    before = [t.clone() for t in p]
+    for lr, scale in ((1e39, 1.0), (-1e39, 1.0), (1e30, [1.0, 1e30]), (float("nan"), 1.0), (1e39, [0.5, 0.5])):
+        with pytest.raises(ValueError):
+            ops.adamw_update(ops.AdamWStates(p, lr_scale=scale), g, lr=lr, step=1)
+    with pytest.raises(ValueError):
+        ops.AdamWStates(p, lr_scale=1e39)
+    with pytest.raises(ValueError):
+        ops.AdamWStates(p, weight_decay=[0.0, -1e39])
+    assert all(torch.equal(a, b) for a, b in zip(before, p))
+    ops.adamw_update(ops.AdamWStates(p, lr_scale=[1e-30, 1e-30]), g, lr=1e30, step=1)
+    assert not any(torch.equal(a, b) for a, b in zip(before, p))
+
+
 def test_refusals():
     p, _ = make([300, 500], F32, 0)
     g, _ = make([300, 500], F32, 1)

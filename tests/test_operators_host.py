@@ -231,6 +231,23 @@ def test_lists_of_tensors_are_checked_on_the_host():
     assert adamw(T(64, None, 10, 0, 1.0, 0.0, 7)) == 1 and adamw(T(64, None, 0, 0, 1.0, 0.0, 1)) == 0 and adamw(count=0) == 0
 
 
+def test_rates_that_are_not_finite_in_32_bits_are_refused():
+    """The kernel leaves everything as it is for such a rate: from the host it is an error."""
+    lib, code = _lib.load(), (C.c_int32 * 1)(1)
+    ptr = (C.c_void_p * 1)(64)
+
+    def adamw(lr, lr_scale=1.0):
+        table = (_lib.AdamWTensor * 1)(_lib.AdamWTensor(64, None, 10, 0, lr_scale, 0.0, 1))
+        return lib.frag_adamw_update(table, ptr, code, 1, 68, 64, None, None, lr, None, 0.9, 0.9, 1e-8, 1, None, None, None)
+    # (states that are not aligned are the next refusal)
+    assert adamw(1e-3) == 3 and adamw(3e38) == 3 and adamw(1e30, 1e-30) == 3
+    assert adamw(1e39) == 1 and adamw(1e30, 1e30) == 1 and adamw(-1e39) == 1
+    for values in (1e39, [1e39], float("nan")):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops._each(values, 1, "lr_scale")
+    assert ops._each([3e38], 1, "lr_scale") == [3e38]
+
+
 def test_states_need_cuda_tensors():
     for bad in ([], [torch.zeros(8)], [torch.zeros(8).half()], [1.0]):
         with pytest.raises((ValueError, TypeError)):
