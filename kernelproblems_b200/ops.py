@@ -17,6 +17,7 @@ import functools
 import math
 import operator
 import os
+import warnings
 from array import array
 
 import torch
@@ -1509,7 +1510,7 @@ class AdamWStates:
 
     params        contiguous bf16 or fp32 CUDA tensors of one device, updated in place
     dtype         torch.float32, or torch.float8_e4m3fn: 8 bits and a scale for
-                  each 128 values of a tensor
+                  each 128 values of a tensor, for betas up to (0.95, 0.98)
     weight_decay  one for all, or one for each (0 for norms and biases)
     lr_scale      a factor on lr, one for all or one for each
     copies        bf16 tensors (or None) shaped like the parameters, which receive
@@ -1662,6 +1663,17 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
     a device step below 1, nothing is changed.  Parameters are rounded to nearest: bf16 ones do not move by less than
     2^-9 of their value, for which there are fp32 parameters with bf16 copies.  With
     states in 8 bits a gradient that is not finite makes its whole group of 128 NaN.
+
+    States in 8 bits are rounded to nearest, too: one moves by itself only where a step
+    moves it by over half of E4M3's step (3 to 6 percent), and else with its group, whose
+    scale is fp32.  What decays more slowly stays behind a value that holds the scale.
+    With a group's gradients fallen tenfold but for one value's, the others' roots of the
+    second moment are, 20 / (1 - beta2) steps later, 1.0 times what they should be at
+    beta2 = 0.95, 1.04 at 0.98, 5.9 at 0.99 and 7.7 at 0.999, and their steps as many times
+    too small.  Roots of values whose gradients end stay on at any beta2, which changes
+    nothing until they come again; first moments of such values go at beta1 = 0.9, and
+    beside a value that does not change up to a twentieth of them stays at 0.95, half at
+    0.97.  So above betas of (0.95, 0.98) there is a warning: those are for states in 32 bits.
     Gradients must not share memory with parameters, copies or states."""
     if not isinstance(states, AdamWStates):
         raise TypeError("states must be an AdamWStates")
@@ -1673,6 +1685,9 @@ def adamw_update(states: AdamWStates, grads, *, lr, step, betas=(0.9, 0.95), eps
     b1, b2 = betas
     if not (0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError("betas must be in [0, 1)")
+    if (b1 > 0.95 or b2 > 0.98) and states.dtype != torch.float32:
+        warnings.warn(f"states in 8 bits stay behind with betas of ({b1}, {b2}): above (0.95, 0.98) take float32",
+                      RuntimeWarning, stacklevel=2)
     if not (eps >= 2.0 ** -126 and math.isfinite(eps)):
         raise ValueError("eps must be finite and at least 2^-126, the least normal number of 32 bits")
     lr_t = step_t = None
