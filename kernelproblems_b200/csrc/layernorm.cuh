@@ -155,6 +155,34 @@ __device__ __forceinline__ void load_vector(const Vector& v, const Place<T, MODE
   }
 }
 
+// A thread's part of a row's two sums, for rows of any length: `term` gives value n's.
+// A row of a million values is 4096 a thread, whose squares in one sum would be off by
+// up to 1e-4; in runs of 64, added up in 64 bits, by 2e-6.  (4096 rows of 20000 in bf16:
+// forward 165 us, gradient 467; in one sum 200 and 385.)
+template <class F>
+__device__ __forceinline__ float2 long_sums(int64_t N, F&& term) {
+  constexpr int RUN = 64;
+  const int64_t apart = blockDim.x;
+  double a = 0.0, b = 0.0;
+  float2 s = make_float2(0.f, 0.f);
+  auto add = [&](int64_t n) {
+    const float2 t = term(n);
+    s.x += t.x;
+    s.y += t.y;
+  };
+  int64_t n = threadIdx.x;
+  for (; n + (RUN - 1) * apart < N; n += RUN * apart) {
+#pragma unroll 16
+    for (int i = 0; i < RUN; ++i) add(n + i * apart);
+    a += s.x;
+    b += s.y;
+    s = make_float2(0.f, 0.f);
+  }
+#pragma unroll 8
+  for (; n < N; n += apart) add(n);
+  return make_float2(static_cast<float>(a + s.x), static_cast<float>(b + s.y));
+}
+
 // How a launch's rows are dealt out.
 struct Rows {
   int64_t M;

@@ -350,12 +350,16 @@ __global__ void __launch_bounds__(256) bwd_any_dx(const BwdP<T> p) {
   const T* dy = p.dy + row * p.ys;
   const T* x = p.x + row * p.xs;
   const float mean = p.mean[row], r = p.rstd[row];
-  float2 s = make_float2(0.f, 0.f);
-  for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
-    const float g = get(dy + n) * vector_at(p.w, n, 1.f);
-    s.x += g;
-    s.y = fmaf((get(x + n) - mean) * r, g, s.y);
-  }
+  auto sums = [&](auto weight) {
+    return long_sums(p.N, [&](int64_t n) {
+      const float g = get(dy + n) * weight(n);
+      return make_float2(g, (get(x + n) - mean) * r * g);
+    });
+  };
+  float2 s;  // (what the weights are is asked once)
+  if (!p.w.p) s = sums([](int64_t) { return 1.f; });
+  else if (p.w.f32) s = sums([&](int64_t n) { return static_cast<const float*>(p.w.p)[n]; });
+  else s = sums([&](int64_t n) { return bf16_to_f(static_cast<const uint16_t*>(p.w.p)[n]); });
   s = block_sum2(s, slots, 0);
   const float invN = 1.0f / static_cast<float>(p.N);
   const float mg = s.x * invN, mx = s.y * invN;

@@ -340,37 +340,26 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
 // Any width, any alignment (rows above 16384 values, or tensors whose rows begin at
 // different places between 16-byte boundaries): a block a row, the row read once
 // for each pass, the later ones from L2.
-template <class T>
+template <class T, bool RES>
 __global__ void __launch_bounds__(256) fwd_any(const FwdP<T> p) {
-  __shared__ float slots[2][32];
-  __shared__ float2 distances[1][32];
+  __shared__ float2 slots[2][32];
   const int64_t row = blockIdx.x;
   const T* x = p.x + row * p.xs;
-  const T* res = p.res ? p.res + row * p.rs : nullptr;
-  auto h = [&](int64_t n) { return res ? rounded<T>(get(res + n) + get(x + n)) : get(x + n); };
-  float s = 0.f;
-  for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
-    const float v = h(n);
-    if (p.h) put(p.h + row * p.N + n, v);
-    s += v;
-  }
-  float mean = block_sum(s, slots, 0) / static_cast<float>(p.N);
-  s = 0.f;
-  for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
+  const T* res = RES ? p.res + row * p.rs : nullptr;
+  auto h = [&](int64_t n) { return RES ? rounded<T>(get(res + n) + get(x + n)) : get(x + n); };
+  const float N = static_cast<float>(p.N);
+  float mean = block_sum2(long_sums(p.N, [&](int64_t n) {
+                            const float v = h(n);
+                            if (RES && p.h) put(p.h + row * p.N + n, v);
+                            return make_float2(v, 0.f);
+                          }), slots, 0).x / N;
+  auto distances = [&](int64_t n) {
     const float v = h(n) - mean;
-    s = fmaf(v, v, s);
-  }
-  float var = block_sum(s, slots, 1) / static_cast<float>(p.N);
-  if (far_from_zero<T>(mean, var)) {
-    float2 d = make_float2(0.f, 0.f);
-    for (int64_t n = threadIdx.x; n < p.N; n += blockDim.x) {
-      const float v = h(n) - mean;
-      d.x += v;
-      d.y = fmaf(v, v, d.y);
-    }
-    d = block_sum2(d, distances, 0);
-    correct(mean, var, d.x, d.y, 1.0f / static_cast<float>(p.N));
-  }
+    return make_float2(v, v * v);
+  };
+  float2 d = block_sum2(long_sums(p.N, distances), slots, 1);
+  float var = d.y / N;
+  if (far_from_zero<T>(mean, var)) correct(mean, var, d.x, d.y, 1.0f / N);
   const float r = rsqrtf(var + p.eps);
   if (threadIdx.x == 0) {
     if (p.mean) p.mean[row] = mean;
@@ -433,7 +422,8 @@ int forward(const FwdP<T>& p, int64_t M, cudaStream_t s) {
     });
     if (st >= 0) return st;
   }
-  fwd_any<T><<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
+  auto any = p.res ? fwd_any<T, true> : fwd_any<T, false>;
+  any<<<dim3(static_cast<unsigned>(M)), 256, 0, s>>>(p);
   return check_launch();
 }
 

@@ -379,6 +379,24 @@ def test_all_tensors_alike_off_a_boundary(N, by, dtype):
     assert all(torch.equal(a, c) for again in held[1:] for a, c in zip(held[0], again))
 
 
+@pytest.mark.parametrize("N", [16385, 1 << 20, 3_000_001])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_long_rows_of_values_that_are_alike(N, dtype):
+    """Thousands of terms for a thread, whose roundings all go one way: the squares of
+    values of one magnitude, and gradients that are equal."""
+    x = torch.full((3, N), 0.3, device=DEV)
+    x[:, ::2] *= -1
+    x[1] += 0.7  # (and a mean that is not zero)
+    x, w = x.to(dtype), weight(N, dtype)
+    dy = torch.full((3, N), 0.1, device=DEV).to(dtype)
+    dy[2] += rand(N, seed=1, dtype=dtype)
+    out = ops.layernorm_fwd(x, w, None, EPS)
+    check_fwd(x, w, None, None, out)
+    check_fwd(x, None, None, 2 * x, ops.layernorm_fwd(x, None, None, EPS, residual=2 * x))
+    check_bwd(dy, x, out[2], out[3], w, None, ops.layernorm_bwd(dy, x, out[2], out[3], w))
+    check_bwd(dy, x, out[2], out[3], None, None, ops.layernorm_bwd(dy, x, out[2], out[3], None))
+
+
 def test_streams_and_graphs():
     x, w, b, dy = rand(64, 4096, seed=1), weight(4096), rand(4096, seed=5), rand(64, 4096, seed=2)
     want = ops.layernorm_fwd(x, w, b)
