@@ -57,30 +57,32 @@ int* device_error_word() {
 }
 
 bool allow_dynamic_smem(const void* kernel, int bytes) {
-  // Largest dynamic shared memory size set so far, per device and kernel.
+  // Largest dynamic shared memory size set so far, per device and kernel.  The table
+  // holds several times the library's kernels: one that found no place would have its
+  // size set again by each call, and lowered under another thread's launch.
+  constexpr size_t kPlaces = 1024;
+  struct Held {
+    const void* kernel;
+    int bytes;
+  };
   static std::mutex mu;
-  static const void* kern[64][128] = {};
-  static int set_bytes[64][128] = {};
+  static Held held[64][kPlaces] = {};
   const int d = current_device();
   if (d < 0 || d >= 64) return false;
   std::lock_guard<std::mutex> lk(mu);
-  int slot = -1;
-  for (int i = 0; i < 128; ++i) {
-    if (kern[d][i] == kernel) {
-      if (set_bytes[d][i] >= bytes) return true;
-      slot = i;
-      break;
-    }
-    if (kern[d][i] == nullptr && slot < 0) slot = i;
+  size_t i = reinterpret_cast<uintptr_t>(kernel) / 16 * 0x9E3779B97F4A7C15ull >> 54;
+  size_t tried = 0;
+  while (held[d][i].kernel && held[d][i].kernel != kernel && tried < kPlaces) {
+    i = (i + 1) % kPlaces;
+    ++tried;
   }
+  if (tried == kPlaces) return false;
+  if (held[d][i].kernel == kernel && held[d][i].bytes >= bytes) return true;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return false;
   }
-  if (slot >= 0) {
-    kern[d][slot] = kernel;
-    set_bytes[d][slot] = bytes;
-  }
+  held[d][i] = {kernel, bytes};
   return true;
 }
 

@@ -1,6 +1,8 @@
 """layernorm_fwd / layernorm_bwd against 64 bits: types, widths, alignments and
 strides, rows of one value, of equal values and far from zero, infinities and
 NaN, the gradient against the formula and against differences, refusals."""
+import threading
+
 import pytest
 import torch
 
@@ -419,6 +421,45 @@ def test_streams_and_graphs():
     want = ops.layernorm_fwd(x, w, b)
     grads = ops.layernorm_bwd(dy, x, want[2], want[3], w)
     assert torch.equal(held[0], want[0]) and all(torch.equal(a, c) for a, c in zip(hg, grads))
+
+
+def test_two_threads_behind_every_variant():
+    """A kernel's largest shared memory is remembered for each of more than a hundred
+    kernels: where one found no place, two threads' calls of it with different widths
+    would lower it under each other's launches."""
+    for dtype in (BF, F32):
+        for N in (48, 120, 248, 504, 1000, 1024, 49, 121, 249, 499, 1001, 2049):
+            x = rand(5, N, seed=N, dtype=dtype)
+            mean, rstd = stats(x)
+            for w in (weight(N, BF), weight(N, F32)):
+                for res in (None, x):
+                    check_fwd(x, w, None, res, ops.layernorm_fwd(x, w, None, EPS, residual=res))
+                    check_bwd(x, x, mean, rstd, w, res, ops.layernorm_bwd(x, x, mean, rstd, w, dres=res))
+    for N in (64, 512, 1000, 1024, 2048, 4096, 5120, 8192, 12288, 16384):
+        x, w = rand(64, N, seed=N), weight(N)
+        ops.rmsnorm_fwd(x, w)
+        ops.add_rmsnorm_fwd(x, x, w)
+    errors = []
+
+    def run(N, M, stream):
+        with torch.cuda.stream(stream):
+            x, w = rand(M, N, seed=N), weight(N)
+            want = ops.layernorm_fwd(x, w, None, EPS)
+            grads = ops.layernorm_bwd(x, x, want[2], want[3], w)
+            try:
+                for _ in range(300):
+                    out = ops.layernorm_fwd(x, w, None, EPS)
+                    assert torch.equal(out[0], want[0])
+                    assert all(torch.equal(a, b) for a, b in zip(ops.layernorm_bwd(x, x, want[2], want[3], w), grads))
+            except Exception as e:  # noqa: BLE001
+                errors.append(e)
+    threads = [threading.Thread(target=run, args=(N, M, torch.cuda.Stream())) for N, M in ((1032, 4), (16376, 2000), (8200, 300))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
 
 
 def test_workspace():
