@@ -457,11 +457,12 @@ int launch_add_partials(const Partials& in, float* dw, float* db, cudaStream_t s
   return cuda_status(cudaLaunchKernelEx(&cfg, many ? add_partials<16, 10> : add_partials<32, 16>, in, dw ? dw : db, db));
 }
 
-// Blocks of rows that the columns' sums are split over, at most (blocks_for: at_once, and
-// one for each kRun rows and more).
-int64_t row_blocks(int64_t M) {
+// Blocks of rows that the columns' sums are split over, at most: blocks_for's at_once and
+// one for each kRun rows of a group, or of a block of 8 rows at once; for any row 4 an SM.
+int64_t row_blocks(int64_t M, int64_t N) {
   const int sms = sm_count();
-  return std::min<int64_t>(M + 8, (sms > 0 ? sms : 148) * 4 + M / kRun);
+  const int64_t more = N > kHeld ? 0 : M / (N <= kLanes - 7 ? 8 * kRun : kRun);
+  return std::min<int64_t>(M + 8, (sms > 0 ? sms : 148) * 4 + more);
 }
 
 template <class T, int V, int L, Mode MODE, bool RES>
@@ -551,7 +552,7 @@ extern "C" {
 
 size_t frag_layernorm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
-  return align_up(static_cast<size_t>(row_blocks(M)) * 2 * (N + 16) * sizeof(float), 256);
+  return align_up(static_cast<size_t>(row_blocks(M, N)) * 2 * (N + 16) * sizeof(float), 256);
 }
 
 int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,

@@ -423,6 +423,26 @@ def test_streams_and_graphs():
     assert torch.equal(held[0], want[0]) and all(torch.equal(a, c) for a, c in zip(hg, grads))
 
 
+@pytest.mark.parametrize("M,N", [(1, 64), (9, 513), (1000, 129), (1 << 20, 64), (1 << 20, 121), (200001, 505), (300000, 520),
+                                 (100003, 1001), (60000, 8192), (40001, 16001), (4000, 20000)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_workspace_is_enough(M, N, dtype):
+    """Nothing is written behind the bytes that the gradient asks for."""
+    x, w = rand(1, N, seed=1, mean=0.5, dtype=dtype), weight(N, dtype)
+    mean, rstd = (t.expand(M).contiguous() for t in stats(x))
+    dy = rand(1, N, seed=2, dtype=dtype)
+    need = _lib.load().frag_layernorm_bwd_workspace_bytes(M, N)
+    ws = torch.full((need + (8 << 20),), 77, dtype=torch.uint8, device=DEV)
+    dx, dw, db = torch.empty(M, N, dtype=dtype, device=DEV), torch.empty(N, device=DEV), torch.empty(N, device=DEV)
+    code = _lib.FRAG_DT_BF16 if dtype == BF else _lib.FRAG_DT_F32
+    for dres in (None, x.data_ptr()):
+        _lib.call("frag_layernorm_bwd", dy.data_ptr(), 0, x.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+                  dres, 0, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), M, N, code, code, ws.data_ptr(), need,
+                  torch.cuda.current_stream().cuda_stream)
+        assert bool((ws[need:] == 77).all())
+        within(db, M * dy[0].double(), REL * M * dy[0].double().abs(), "db")
+
+
 def test_two_threads_behind_every_variant():
     """A kernel's largest shared memory is remembered for each of more than a hundred
     kernels: where one found no place, two threads' calls of it with different widths
