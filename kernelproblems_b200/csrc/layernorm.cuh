@@ -158,7 +158,8 @@ __device__ __forceinline__ void load_vector(const Vector& v, const Place<T, MODE
 // A thread's part of a row's two sums, for rows of any length: `term` gives value n's.
 // A row of a million values is 4096 a thread, whose squares in one sum would be off by
 // up to 1e-4; in runs of 64, added up in 64 bits, by 2e-6.  (4096 rows of 20000 in bf16:
-// forward 165 us, gradient 467; in one sum 200 and 385.)
+// forward 190 us, gradient 419, with the residual 611 and 471; all in one sum 200, 385, 633
+// and 489.)
 template <class F>
 __device__ __forceinline__ float2 long_sums(int64_t N, F&& term) {
   constexpr int RUN = 64;
@@ -171,14 +172,15 @@ __device__ __forceinline__ float2 long_sums(int64_t N, F&& term) {
     s.y += t.y;
   };
   int64_t n = threadIdx.x;
-  for (; n + (RUN - 1) * apart < N; n += RUN * apart) {
+  if (N > 2 * RUN * apart) {  // (else one run of both)
+    for (; n + (RUN - 1) * apart < N; n += RUN * apart) {
 #pragma unroll 16
-    for (int i = 0; i < RUN; ++i) add(n + i * apart);
-    a += s.x;
-    b += s.y;
-    s = make_float2(0.f, 0.f);
+      for (int i = 0; i < RUN; ++i) add(n + i * apart);
+      a += s.x;
+      b += s.y;
+      s = make_float2(0.f, 0.f);
+    }
   }
-#pragma unroll 8
   for (; n < N; n += apart) add(n);
   return make_float2(static_cast<float>(a + s.x), static_cast<float>(b + s.y));
 }

@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(256) bwd_any_columns(const BwdP<T> p, int64_t 
   float dw = 0.f, db = 0.f;
   for (int64_t row = r0; row < r1;) {
     float rw = 0.f, rb = 0.f;
+#pragma unroll 4
     for (const int64_t end = min(r1, row + kRun); row < end; ++row) {
       const float g = get(p.dy + row * p.ys + n);
       rw = fmaf(g, (get(p.x + row * p.xs + n) - p.mean[row]) * p.rstd[row], rw);
