@@ -600,7 +600,8 @@ FRAG_API int frag_layernorm_bwd(const void* dy, int64_t dy_stride, const void* x
  * grads, numel, dtypes: HOST arrays of device pointers, counts and FRAG_DT_BF16 /
  * FRAG_DT_F32; any alignment of whole values.  norm, scale (or NULL): fp32 device
  * words.  Squares are added in 32 bits within a thread's 32 values and in 64
- * beyond, in an order that the sizes fix: |g| up to 1e18.  Workspace:
+ * beyond, in an order that the sizes fix: |g| up to 1e18, and from 1e-18 on (squares
+ * of smaller ones lose digits, and below 1e-22 count nothing).  Workspace:
  * frag_grad_norm_workspace_bytes(count), 16-byte aligned.  No counterpart in the
  * reference, whose graphs end at the weights' gradients.
  * ------------------------------------------------------------------------- */

@@ -11,7 +11,7 @@
 // a second, one-block launch adds the blocks' sums and starts while the first ends.
 //
 // Bound: HBM.  218 million values in 9 tensors: 75 us in bf16 (5.8 TB/s; 67 at a
-// copy's rate), 139 in fp32 (6.3), from addresses off 16 bytes too.  Tensors
+// copy's rate; 70 among other calls), 140 in fp32 (6.3), from addresses off 16 bytes too.  Tensors
 // of a few thousand values are a chunk each, and the two launches' latency.
 #include <algorithm>
 #include <cmath>

@@ -462,8 +462,8 @@ constexpr int lane_blocks(int V, Mode mode, int most) { return most - (V == 8 &&
 // hold beside weights and sums), and of up to so many a group's (512 threads of 32).
 // 65536 rows in bf16, us by lanes and by groups: of 512 27 and 42 (gradient 39 and
 // 56), of 300 36 and 58 (52 and 75); in fp32 of 512 48 and 50 (71 and 72).  4096 rows
-// of 16384 by groups 50 (gradient 81), of 20000 by the kernels for any row 200 (388);
-// 8192 of 4096 26 and 88 (41 and 139).
+// of 16384 by groups 52 (gradient 83), of 20000 by the kernels for any row 190 (419);
+// 8192 of 4096 27 and 84 (42 and 152).
 constexpr int64_t kLanes = 512, kHeld = 16384;
 constexpr int kSmem = 232448;  // of an SM, for its blocks
 

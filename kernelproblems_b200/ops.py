@@ -1344,7 +1344,13 @@ def layernorm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: tor
     rstd   1 / sqrt(mean((h - mean)^2) + eps), the same; None with save_stats=False
 
     x and residual: bf16 or fp32, rows of contiguous values, any row stride.
-    weight, bias: bf16 or fp32 (both the same), or None for 1 and 0."""
+    weight, bias: bf16 or fp32 (both the same), or None for 1 and 0.
+
+    Rows of up to 16384 values (14336 in fp32 with a residual) are read once, where those
+    of x, residual and outputs (which begin at a 16-byte boundary) lie alike between such
+    boundaries; any others two or three times, which takes up to four times as long.
+    The mean is one fp32 number: y is off by up to |mean| 2^-24 rstd weight beside its
+    own roundings."""
     out = _lib.binding().layernorm_fwd(x, weight, bias, eps, residual, write_h, save_stats)
     if out.__class__ is tuple:
         return out
@@ -1378,7 +1384,8 @@ def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
            None with compute_dw=False or without a weight
     db     fp32 [N], sum over the rows of dy in a fixed order; None with compute_db=False
 
-    dy, x and dres: of one type, rows of contiguous values, any row stride."""
+    dy, x and dres: of one type, rows of contiguous values, any row stride; what
+    layernorm_fwd says of rows that are read once holds here, with dres for residual."""
     if workspace is None:
         out = _lib.binding().layernorm_bwd(dy, x, mean, rstd, weight, dres, compute_dw, compute_db)
         if out.__class__ is tuple:
@@ -1457,8 +1464,9 @@ def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor |
            grad_scale; NaN where norm is not finite (the update then changes
            nothing); None without max_norm
 
-    grads: contiguous bf16 and fp32 tensors on one device, |g| up to 1e18; None
-    entries are left out."""
+    grads: contiguous bf16 and fp32 tensors on one device, |g| up to 1e18 (and from 1e-18
+    on: squares of smaller ones lose digits, and below 1e-22 count nothing); None entries
+    are left out."""
     grads = list(grads)
     if workspace is None:
         out = _lib.binding().grad_norm(grads, max_norm)
