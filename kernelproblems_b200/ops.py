@@ -1490,9 +1490,12 @@ def grad_norm(grads, *, max_norm: float | None = None, workspace: torch.Tensor |
     return norm, scale
 
 
+_F32_END = 2.0 ** 128 - 2.0 ** 103  # the least that 32 bits round to infinity
+
+
 def _finite(v: float) -> bool:
     """Whether a number is finite in 32 bits."""
-    return math.isfinite(C.c_float(v).value)
+    return -_F32_END < v < _F32_END
 
 
 def _each(v, n: int, name: str) -> list[float]:

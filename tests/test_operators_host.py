@@ -246,6 +246,9 @@ def test_rates_that_are_not_finite_in_32_bits_are_refused():
         with pytest.raises(ValueError, match="32 bits"):
             ops._each(values, 1, "lr_scale")
     assert ops._each([3e38], 1, "lr_scale") == [3e38]
+    end = 2.0 ** 128 - 2.0 ** 103
+    for v in (end, -end, math.nextafter(end, 0), -math.nextafter(end, 0), float("inf"), float("nan"), 0.0, 2.0 ** -200):
+        assert ops._finite(v) == math.isfinite(C.c_float(v).value)
 
 
 def test_states_need_cuda_tensors():
