@@ -77,13 +77,10 @@ struct Count {
 // of 1001 values 1000.3 had deviations of 1.2e-4 in place of none.  So an fp32 row whose
 // mean is more than 8 deviations adds up its distances from it, which have no digits to
 // lose, and the mean becomes the true one but for its own rounding.  (8192 rows of 1001:
-// 25 us, all of them far from zero 29; 32768 of 8192 332 both.)  The sum of bf16 values that
-// lie about a mean so far from zero is exact: 8 binary digits each and those of their
-// count, at most 15, are less than 24.
-template <class T>
-__device__ __forceinline__ bool far_from_zero(float mean, float var) {
-  return sizeof(T) == 4 && mean * mean > 64.f * var;
-}
+// 25 us, all of them far from zero 29; 32768 of 8192 332 both.)  The sum of up to 16384
+// bf16 values that lie about a mean so far from zero is exact: 8 binary digits each and
+// those of their count, 14, are less than 24.
+__device__ __forceinline__ bool far_from_zero(float mean, float var) { return mean * mean > 64.f * var; }
 __device__ __forceinline__ void correct(float& mean, float& var, float distances, float squares, float invN) {
   const float off = distances * invN;
   var = fmaxf(fmaf(squares, invN, -off * off), 0.f);
@@ -192,7 +189,7 @@ __global__ void __launch_bounds__(256, lane_blocks(V, MODE, 4)) fwd_lanes(const 
     float mean = count.mean(all);
     float var = lanes_sum<L>(row_squares<T, V, MODE>(at, N, v, mean)) * invN;
     if constexpr (sizeof(T) == 4) {
-      const bool far = far_from_zero<T>(mean, var);
+      const bool far = far_from_zero(mean, var);
       if (__any_sync(0xffffffffu, far)) {  // (shuffles are the whole warp's)
         float2 d = row_distances<T, V, MODE>(at, N, v, mean);
         d = make_float2(lanes_sum<L>(d.x), lanes_sum<L>(d.y));
@@ -311,7 +308,7 @@ __global__ void __launch_bounds__(kMost) fwd_groups(const FwdP<T> p, const Rows 
       var = lanes_sum<16>(fmaf(n.x * d, d, o.y)) * invN;
     }
     float mean = count.mean(all);
-    if (far_from_zero<T>(mean, var)) {  // (the whole group: its warps have the same sums)
+    if (sizeof(T) == 4 && far_from_zero(mean, var)) {  // (the whole group: its warps have the same sums)
       const float2 d = warp_sum2(row_distances<T, V, MODE>(at, N, v, mean));
       if (lane == 0) distances[first + warp] = d;
       g.sync();
@@ -359,7 +356,7 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdP<T> p) {
   };
   float2 d = block_sum2(long_sums(p.N, distances), slots, 1);
   float var = d.y / N;
-  if (far_from_zero<T>(mean, var)) correct(mean, var, d.x, d.y, 1.0f / N);
+  if (far_from_zero(mean, var)) correct(mean, var, d.x, d.y, 1.0f / N);
   const float r = rsqrtf(var + p.eps);
   if (threadIdx.x == 0) {
     if (p.mean) p.mean[row] = mean;

@@ -261,6 +261,15 @@ def test_rows_of_one_value(N, dtype, residual):
     within(rstd, torch.full_like(var, EPS ** -0.5), EPS ** -0.5 * (var / EPS + 8 * U), "rstd")
 
 
+@pytest.mark.parametrize("N", [16392, 100001, 3_000_001])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_long_rows_of_one_value(N, dtype):
+    x = torch.tensor([1000.3, -0.1, 12345.678], device=DEV)[:, None].expand(3, N).to(dtype).contiguous()
+    b = rand(N, seed=5, dtype=dtype)
+    y, _, mean, _ = ops.layernorm_fwd(x, weight(N, dtype), b, EPS)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, b.expand(3, N))
+
+
 @pytest.mark.parametrize("N", FAR[3:])
 @pytest.mark.parametrize("far", [1e3, -1e4])
 def test_a_mean_far_from_zero_is_off_by_its_last_place(N, far):
