@@ -452,6 +452,24 @@ def test_the_workspace_is_enough(M, N, dtype):
         within(db, M * dy[0].double(), REL * M * dy[0].double().abs(), "db")
 
 
+def test_more_blocks_than_an_sm_holds_in_a_graph():
+    """The pass that adds the partials starts beside the last of the gradient's blocks, and
+    waits for all of them: captured, and replayed on other values."""
+    M, N = 310000, 520
+    x, dy, w = rand(M, N, seed=1, mean=0.5), rand(M, N, seed=2), weight(N)
+    mean, rstd = stats(x)
+    ops.layernorm_bwd(dy, x, mean, rstd, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [ops.layernorm_bwd(dy, x, mean, rstd, w) for _ in range(2)]
+    for seed in (3, 4):
+        dy.copy_(rand(M, N, seed=seed))
+        graph.replay()
+        want = ops.layernorm_bwd(dy, x, mean, rstd, w)
+        assert all(torch.equal(a, b) for out in held for a, b in zip(out, want))
+    check_bwd(dy, x, mean, rstd, w, None, want)
+
+
 def test_two_threads_behind_every_variant():
     """A kernel's largest shared memory is remembered for each of more than a hundred
     kernels: where one found no place, two threads' calls of it with different widths
